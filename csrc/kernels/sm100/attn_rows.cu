@@ -4,70 +4,80 @@
 //
 //   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = 2^(scale log2(e) q_i.k_j - m_i)  over the j that row i sees; no such j: zeros
 //
-// One CTA = (16 query rows: the G heads of 16 / G tokens, one kv head, a share of the context). A producer warp brings tiles of
-// 64 tokens into a ring of shared memory by TMA; four warps take 16 tokens of each tile and keep (m, l, O) of their own; the four
-// are joined at the end, and the shares of one row, written as partials, by a second kernel (kern_attn_rows_merge).
+// One CTA = (8, 16 or 32 query rows: the G heads of some tokens, one kv head, a share of the context). A producer warp brings
+// tiles of tokens into a ring of shared memory by TMA; four or eight warps take 16 tokens of a tile at a time and keep (m, l, O) of
+// their own. They are joined at the end, then the shares of one row: over distributed shared memory in a cluster of up to 8 CTAs, and
+// where that is not enough as partials that a second kernel joins (kern_attn_rows_merge).
 //
-// The time goes to reading the cache, so the arithmetic has to stay well under the memory's rate with little shared-memory
-// traffic. Operands go from shared memory to registers in 16-byte loads and are not moved again: the order of the contraction
-// index and of the output columns inside an mma.sync fragment is free as long as both operands agree, so a lane takes whole
-// 16-byte pieces of a key row (Q's fragment is built in the same order), and whole pieces of value rows, of which it pairs two
-// tokens' bytes with PRMT. The same code then serves bf16 words and e4m3 bytes, which become f16 pairs, exactly, in one
-// instruction (cvt.rn.f16x2.e4m3x2). Tokens are dealt to lanes so that the 8 lanes of a shared-memory phase hit 8 different
-// 16-byte columns of the 128-byte swizzle.
+// The time goes to reading the cache, so a byte of it may cost few instructions. Products are turned around: S^T = K Q^T and
+// O^T = V^T P^T on mma.sync, so that the 16-row operand is the cache and the 8-column one the query rows, of which a single token
+// has 4 or 8. The order of the contraction index and of the operand rows inside a fragment is free as long as both operands agree,
+// so a lane takes whole 16-byte pieces of key and value rows from shared memory and nothing is moved again: of a value row's
+// pieces it pairs two tokens' bytes with PRMT, and P^T comes from S^T by movmatrix. The same code serves bf16 words and e4m3
+// bytes, which become f16 pairs, exactly, in one instruction (cvt.rn.f16x2.e4m3x2). Tokens are dealt to lanes so that the 8 lanes
+// of a shared-memory phase hit 8 different 16-byte columns of the swizzle. The references m (and R below) move only when a weight
+// has outgrown them by 2^15: most tiles need no maximum over lanes and no pass over O.
 //
 // 8-bit: Q goes to f16 with its row's power of two taken out; the scores of a key row are multiplied by its scale in f32; a value
-// row's scale goes into its weight, w_ij = p_ij 2^(e_j - c_i), where c_i follows the largest s_ij + e_j - m_i seen, so that the
-// f16 weights that matter are between 2^-14 and 1 whatever the sizes of the value rows. Rounding a weight to f16 (2^-11) is four
-// steps finer than the output's own rounding; bf16 caches take bf16 weights (2^-8 of each weight, as the value rows' own rounding).
+// row's scale goes into its weight, w_ij = 2^(s_ij + e_j - R_i). R follows the largest s_ij + e_j seen, less 7, so the largest weight
+// of a row is between 2^6 and 2^15 whatever the sizes of the value rows, and every weight down to 2^-20 of it keeps all of f16's
+// bits. Rounding a weight to f16 (2^-11) is three bits finer than the output's own rounding; bf16 caches take bf16 weights (2^-8 of
+// each weight, as the value rows' own rounding).
 //
-// Values that a row does not see do not reach it, whatever they are: tokens behind the sequence's end are cleared, and in the
-// tiles where rows see different tokens values that are not finite are taken out of the product and put back for the rows that
-// see them (a second pass of products over 0 / 1, only when there are any).
+// Values that a row does not see do not reach it, whatever they are: tokens behind the end are cleared, and in the tiles where
+// rows see different tokens values that are not finite are taken out of the product and put back for the rows that see them (a
+// second pass of products over 0 / 1, only when there are any).
 #include <cuda_fp8.h>
 
 #include "common.cuh"
 
 namespace kern {
 
-constexpr int kTile = 64;            // tokens per tile
-constexpr int kRowsThreads = 160;    // four warps of products, one producer
+constexpr float kUnset = -1e30f;     // a reference before its first score
+constexpr float kOutgrown = 32768.f; // the weight at which references move: f16 holds twice that
 
 struct RowsArgs {
   const __nv_bfloat16* q;
   __nv_bfloat16* out;
-  float* ws_o;               // partials [row][head][splits][D] (one split: none)
-  float* ws_ml;              // [row][head][splits][2]
+  float* ws_o;               // partials [row][head][groups][D] (one group: none)
+  float* ws_ml;              // [row][head][groups][2]
   const uint8_t* pool;       // (8-bit) scale bytes are read from here
   const int* block_table;
   const int* seq_lens;
   const int* cu_q;
   const long long* masks;    // (tree) [row][words]
   int* err;
-  int words, rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, splits, pool_pages;
+  int words, rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, cluster, pool_pages;
   float scale_log2;
 };
 
-template <int D, bool E4M3>
+// D, cache format, NT: columns of query rows in eights
+template <int D, bool E4M3, int NT>
 struct RowsCfg {
   static constexpr int kRowBytes = D * (E4M3 ? 1 : 2);
+    static constexpr int kTile = kRowBytes <= 128 ? 128 : 64;          // tokens: a stage of 32 KB where rows allow it
   static constexpr int kHalf = kTile * kRowBytes;                    // a tile of K or of V
   static constexpr int kStage = 2 * kHalf;
   static constexpr int kScaleBytes = E4M3 ? 2 * kTile : 0;
-  // about 96 KB of ring, so that two CTAs share an SM (one at 128 KB rows)
-  static constexpr int kStages = kStage >= 65536 ? 3 : (98304 / kStage > 8 ? 8 : 98304 / kStage);
-  static constexpr int kQBytes = D == 256 ? (D / 16) * 32 * 16 : 0;  // Q's fragments, where registers do not hold them
-  static constexpr int kSmem = 1024 + kStages * (kStage + kScaleBytes) + kQBytes + 256;
+  // 96 KB of ring, so that two CTAs share an SM; one where accumulators or 512-byte rows take the room of two
+  static constexpr int kPerSm = D == 256 || D * NT > 256 ? 1 : 2;
+  static constexpr int kStages = kStage >= 65536 ? 3 : (kPerSm == 1 ? 196608 : 98304) / kStage;
   static constexpr int kBox = kRowBytes < 128 ? kRowBytes : 128;     // bytes of a row in one box
+  // warps of products, 16 tokens of a tile at a time each (eight of them, at 96 registers, were 15 % slower: 75 us against 66 for
+  // 64 sequences of up to 4096 tokens)
+  static constexpr int kWarps = 4;
+  static constexpr int kThreads = 32 * (kWarps + 1);                 // and a producer
+  static constexpr bool kQShared = D == 256 && NT > 1;               // Q's fragments in shared memory: registers do not hold them
+  static constexpr int kQBytes = kQShared ? NT * (D / 16) * 32 * 8 : 0;
 };
 
-// byte offset of (token, 16-byte piece) in a tile of kRowBytes rows stored as 128-byte column blocks with the TMA's swizzle
-template <int RB>
+// byte offset of (token, 16-byte piece) in a tile of RB-byte rows stored as 128-byte column blocks with the TMA's swizzle
+template <int RB, int TILE>
 KERN_DEVICE uint32_t piece_off(int tok, int piece) {
   if constexpr (RB == 64) {
     return (uint32_t)(tok * 64 + ((piece ^ ((tok >> 1) & 3)) << 4));
   } else {
-    return (uint32_t)((piece >> 3) * (kTile * 128) + tok * 128 + (((piece & 7) ^ (tok & 7)) << 4));
+    return (uint32_t)((piece >> 3) * (TILE * 128) + tok * 128 + (((piece & 7) ^ (tok & 7)) << 4));
   }
 }
 
@@ -86,15 +96,20 @@ KERN_DEVICE uint32_t lds8(uint32_t a) {
   asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a));
   return v;
 }
-// two e4m3 codes (low 16 bits) -> two f16, exact
-KERN_DEVICE uint32_t codes_f16x2(uint32_t pair) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(pair));
-  return r;
+// four e4m3 codes -> two pairs of f16, exact
+KERN_DEVICE void codes_f16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
 }
 KERN_DEVICE uint32_t pack_f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <bool F16>
+KERN_DEVICE uint32_t pack_pair(float lo, float hi) {
+  if constexpr (F16) return pack_f16x2(lo, hi);
+  else return pack_bf16x2(lo, hi);
 }
 template <bool F16>
 KERN_DEVICE void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -110,12 +125,37 @@ KERN_DEVICE void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
 }
+// the 8 x 8 matrix of 16-bit values whose row lane / 4, columns 2 (lane % 4) and + 1 each lane holds, transposed
+KERN_DEVICE uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 // 4 bytes global -> shared, and an arrival on `bar` once this lane's copies so far have landed (counted by the barrier's setting)
 KERN_DEVICE void async_copy4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 KERN_DEVICE void async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// clusters: the same place in another CTA's shared memory, and a barrier over the CTAs that orders what they wrote there
+KERN_DEVICE uint32_t at_rank(uint32_t a, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  return r;
+}
+KERN_DEVICE float ld_rank(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+KERN_DEVICE float4 ld_rank4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
+}
+KERN_DEVICE void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // of the two 16-bit (f16 or bf16) halves of w: all ones where the half is not finite
@@ -130,23 +170,26 @@ KERN_DEVICE uint32_t not_finite(uint32_t w) {
 
 KERN_DEVICE float pow2i(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 
-// how many shares the context of `tiles` tiles is cut into: no share under four tiles
-KERN_DEVICE int rows_shares(int tiles, int splits) { return min(splits, max(1, (tiles + 3) / 4)); }
+// A context is dealt out in runs of whole 128-token units: how many shares `end` tokens are cut into, and the tokens
+// of each.
+KERN_DEVICE int rows_shares(int end, int splits) { return min(splits, max(1, (end + 127) / 128)); }
+KERN_DEVICE int rows_share_len(int end, int shares) { return ((end + 127) / 128 + shares - 1) / shares * 128; }
 
-template <int D, bool E4M3, bool TREE>
+template <int D, bool E4M3, bool TREE, int NT>
 KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
-  using Cfg = RowsCfg<D, E4M3>;
-  constexpr int RB = Cfg::kRowBytes, kStages = Cfg::kStages;
+  using Cfg = RowsCfg<D, E4M3, NT>;
+  constexpr int RB = Cfg::kRowBytes, kStages = Cfg::kStages, kTile = Cfg::kTile;
   constexpr int KP = RB / 64;              // 16-byte pieces of a key row per lane
   constexpr int VB = RB / 8;               // bytes of a value row per lane: D / 8 columns
-  constexpr int NC = D / 8;                // value columns per lane = n-tiles of O
-  constexpr int KS = D / 16;               // k-steps of Q K^T
-  constexpr bool kQShared = D == 256;
+  constexpr int MI = D / 16;               // 16-row tiles of O^T
+  constexpr int KS = D / 16;               // k-steps of K Q^T
+  constexpr int kRows = 8 * NT, kWarps = Cfg::kWarps, kThreads = Cfg::kThreads;
+  constexpr bool kQShared = Cfg::kQShared;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* stages = smem;
   uint8_t* scales = smem + kStages * Cfg::kStage;
-  uint4* q_frag = reinterpret_cast<uint4*>(scales + kStages * Cfg::kScaleBytes);
+  uint2* q_frag = reinterpret_cast<uint2*>(scales + kStages * Cfg::kScaleBytes);
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(q_frag) + Cfg::kQBytes);
   uint64_t* empty_bar = full_bar + kStages;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(empty_bar + kStages);
@@ -158,7 +201,7 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full_bar[s], E4M3 ? 33 : 1);
-      mbar_init(&empty_bar[s], 4);
+      mbar_init(&empty_bar[s], kWarps);
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -170,164 +213,191 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
   const int L = max(a.seq_lens[seq], 0);
   const int row0 = a.cu_q ? a.cu_q[seq] : seq * a.rows_per_seq;
   const int R = a.cu_q ? a.cu_q[seq + 1] - row0 : a.rows_per_seq;
-  const int toks = 16 / G > 0 ? 16 / G : 1;
+  const int toks = kRows / G;
   const int tok_lo = blk * toks;
-  if (tok_lo >= R) return;                                   // uniform per CTA
+  if (tok_lo >= R) return;                                   // uniform over the cluster
   const int valid = min(toks, R - tok_lo) * G;
   const int past = L - R;                                    // what the sequence had before this call's rows
   // causal: the last row of the block decides how far the walk goes
   const int end = TREE ? L : max(0, past + tok_lo + min(toks, R - tok_lo));
-  const int tiles_all = (end + kTile - 1) / kTile;
-  const int shares = rows_shares(tiles_all, a.splits);
-  const int split = blockIdx.z;
-  if (split >= shares) return;
-  const int per = (tiles_all + shares - 1) / shares;
-  const int tile_lo = split * per, ntiles = max(0, min(tiles_all, tile_lo + per) - tile_lo);
+  const int shares = rows_shares(end, gridDim.z);
+  const int share_len = rows_share_len(end, shares);
+  const int from = min(end, (int)blockIdx.z * share_len), to = (int)blockIdx.z < shares ? min(end, from + share_len) : from;
+  const int ntiles = (to - from + kTile - 1) / kTile;
 
-  // ---- Q's fragments, in the order in which a lane holds the keys ----
   const int g = lane >> 2, c = lane & 3;
-  const int rA = g, rB = g + 8;
-  uint32_t qf[KS][4];
-  float f_row[2] = {a.scale_log2, a.scale_log2};             // what turns a row's products into base-2 scores
-  if (warp < 4 && (!kQShared || warp == 0)) {
+  // of columns (query rows) 8 nt + 2 c + x; g = 2^(m - R)
+  float l_run[NT][2], m_run[NT][2], r_run[NT][2], g_run[NT][2];
+  float o[NT][MI][4];
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const int r = hh ? rB : rA;
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      l_run[nt][x] = 0.f;
+      m_run[nt][x] = r_run[nt][x] = kUnset;
+      g_run[nt][x] = 1.f;
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+  }
+
+  if (warp == kWarps) {
+    // ---------------- producer ----------------
+    const int box = a.page_size < 64 ? a.page_size : 64, box_bits = 31 - __clz(box);
+    const int* pages = a.block_table + (size_t)seq * a.max_pages;
+    // (page of the table, row in it) of the tile's first token; the table is read 32 pages at a time, a lane each
+    int pi0 = from / a.page_size, off0 = from - pi0 * a.page_size, first = pi0 - 32, id = 0;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int t = 0; t < ntiles; ++t) {
+      const int here = min(kTile, to - (from + t * kTile));
+      const int boxes = (here + box - 1) >> box_bits;
+      if (pi0 + (kTile >> 3) > first + 32) {                  // (a tile has 16 pages at most)
+        first = pi0;
+        const int pi = first + lane;
+        id = pi < a.max_pages ? pages[pi] : -1;
+        if (id < 0 || id >= a.pool_pages) {
+          if (pi * a.page_size < to) set_error(a.err, ERR_BOUNDS);
+          id = 0;
+        }
+      }
+      // box b of the tile
+      auto place = [&](int b, int& pi, int& off) {
+        pi = pi0;
+        off = off0 + (b << box_bits);
+        if (box == a.page_size) {
+          pi += b;
+          off = 0;
+        } else if (off >= a.page_size) {                      // (pages of 64 tokens and more: two to a tile at most)
+          ++pi;
+          off -= a.page_size;
+        }
+      };
+      if (!mbar_wait_ns(&empty_bar[stage], phase ^ 1, abort_flag)) {
+        set_error(a.err, ERR_WAIT_EMPTY);
+        *abort_flag = 1;
+        break;
+      }
+      uint8_t* sk = stages + stage * Cfg::kStage;
+      // boxes behind the share's end are not brought: their tokens are masked and their values cleared
+      if (lane == 0) mbar_expect_tx(&full_bar[stage], boxes * box * RB * 2);
+      __syncwarp();
+      {
+        int pi, off;
+        place(lane >> 1, pi, off);
+        const int page = __shfl_sync(0xffffffffu, id, (pi - first) & 31);
+        const int b = lane >> 1, which = lane & 1;            // a lane to each box of K and of V
+        if (b < boxes) {
+#pragma unroll
+          for (int cb = 0; cb < RB / Cfg::kBox; ++cb)
+            tma_load_3d(sk + which * Cfg::kHalf + cb * (kTile * 128) + (b << box_bits) * Cfg::kBox, kv_map, cb * (Cfg::kBox * D / RB),
+                        (which * a.hk + kvh) * a.page_size + off, page, &full_bar[stage]);
+        }
+      }
+      if constexpr (E4M3) {
+        const size_t codes = (size_t)2 * a.hk * a.page_size * D;
+#pragma unroll
+        for (int i = 0; i < 2 * (kTile / 4); i += 32) {
+          const int which = (i + lane) / (kTile / 4), i4 = ((i + lane) % (kTile / 4)) * 4;
+          int pi, off;
+          place(i4 >> box_bits, pi, off);
+          const int page = __shfl_sync(0xffffffffu, id, (pi - first) & 31);
+          if (i4 < here) {
+            const uint8_t* src = a.pool + (size_t)page * (codes + 2 * a.hk * a.page_size) + codes + (size_t)(which * a.hk + kvh) * a.page_size + off + (i4 & (box - 1));
+            if (KERN_CHECK(src, 4, SITE_KV_ROW)) async_copy4(smem_u32(scales + stage * Cfg::kScaleBytes + which * kTile + i4), src);
+          }
+        }
+        async_arrive(&full_bar[stage]);
+      }
+      if (box == a.page_size) {
+        pi0 += kTile >> box_bits;
+      } else {
+        off0 += kTile;
+        while (off0 >= a.page_size) {
+          off0 -= a.page_size;
+          ++pi0;
+        }
+      }
+      if (++stage == kStages) { stage = 0; phase ^= 1; }
+    }
+  } else {
+    // ---------------- Q's fragments, in the order in which a lane holds the keys ----------------
+    uint32_t qf[NT][KS][2];
+    float f_col[NT][2];                                      // what turns a column's products into base-2 scores
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = nt * 8 + g;
       const bool ok = r < valid;
       const __nv_bfloat16* src = a.q + (size_t)(row0 + tok_lo + (ok ? r / G : 0)) * a.q_stride + (size_t)(kvh * G + (ok ? r % G : 0)) * D;
+      float f = a.scale_log2;
       if constexpr (E4M3) {
-        // 16 values to a piece: words w of the piece make k-step 4 i + w
+        // 16 values to a piece: word w of the piece makes k-step 4 i + w
         float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < KP; ++i) {
+        for (int i = 0; i < KP; ++i)
 #pragma unroll
           for (int h2 = 0; h2 < 2; ++h2) {
             const uint4 v = ok ? *reinterpret_cast<const uint4*>(src + (c + 4 * i) * 16 + h2 * 8) : make_uint4(0, 0, 0, 0);
-            qf[4 * i + 2 * h2][hh] = v.x;
-            qf[4 * i + 2 * h2][2 + hh] = v.y;
-            qf[4 * i + 2 * h2 + 1][hh] = v.z;
-            qf[4 * i + 2 * h2 + 1][2 + hh] = v.w;
+            qf[nt][4 * i + 2 * h2][0] = v.x;
+            qf[nt][4 * i + 2 * h2][1] = v.y;
+            qf[nt][4 * i + 2 * h2 + 1][0] = v.z;
+            qf[nt][4 * i + 2 * h2 + 1][1] = v.w;
           }
-        }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          const float2 u = unpack_bf16x2(qf[s][hh]), v = unpack_bf16x2(qf[s][2 + hh]);
+          const float2 u = unpack_bf16x2(qf[nt][s][0]), v = unpack_bf16x2(qf[nt][s][1]);
           top = fmaxf(top, fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(v.x), fabsf(v.y))));
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int x = min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100), 100);
         const float inv = pow2i(-x);
-        f_row[hh] = a.scale_log2 * pow2i(x);
+        f *= pow2i(x);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          const float2 u = unpack_bf16x2(qf[s][hh]), v = unpack_bf16x2(qf[s][2 + hh]);
-          qf[s][hh] = pack_f16x2(u.x * inv, u.y * inv);
-          qf[s][2 + hh] = pack_f16x2(v.x * inv, v.y * inv);
+          const float2 u = unpack_bf16x2(qf[nt][s][0]), v = unpack_bf16x2(qf[nt][s][1]);
+          qf[nt][s][0] = pack_f16x2(u.x * inv, u.y * inv);
+          qf[nt][s][1] = pack_f16x2(v.x * inv, v.y * inv);
         }
       } else {
         // 8 values to a piece: its words make k-steps 2 i and 2 i + 1
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
           const uint4 v = ok ? *reinterpret_cast<const uint4*>(src + (c + 4 * i) * 8) : make_uint4(0, 0, 0, 0);
-          qf[2 * i][hh] = v.x;
-          qf[2 * i][2 + hh] = v.y;
-          qf[2 * i + 1][hh] = v.z;
-          qf[2 * i + 1][2 + hh] = v.w;
+          qf[nt][2 * i][0] = v.x;
+          qf[nt][2 * i][1] = v.y;
+          qf[nt][2 * i + 1][0] = v.z;
+          qf[nt][2 * i + 1][1] = v.w;
         }
       }
-    }
-  }
-  if constexpr (kQShared) {
-    float* f_s = reinterpret_cast<float*>(const_cast<int*>(abort_flag) + 1);
-    if (warp == 0) {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) q_frag[s * 32 + lane] = make_uint4(qf[s][0], qf[s][1], qf[s][2], qf[s][3]);
-      if (c == 0) {
-        f_s[rA] = f_row[0];
-        f_s[rB] = f_row[1];
+      for (int x = 0; x < 2; ++x) f_col[nt][x] = __shfl_sync(0xffffffffu, f, (2 * c + x) * 4);
+      if constexpr (kQShared) {
+        // (the warps write the same values)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q_frag[(nt * KS + s) * 32 + lane] = make_uint2(qf[nt][s][0], qf[nt][s][1]);
       }
     }
-    __syncthreads();
-    f_row[0] = f_s[rA];
-    f_row[1] = f_s[rB];
-  }
+    __syncwarp();
 
-  float o[NC][4];
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f}, w_run[2] = {-INFINITY, -INFINITY};
-  int c_run[2] = {-1000, -1000};
-#pragma unroll
-  for (int i = 0; i < NC; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-
-  if (warp == 4) {
-    // ---------------- producer ----------------
-    const int box = a.page_size < kTile ? a.page_size : kTile;
-    const int* pages = a.block_table + (size_t)seq * a.max_pages;
-    int stage = 0;
-    uint32_t phase = 0;
-    for (int t = 0; t < ntiles; ++t) {
-      if (!mbar_wait_ns(&empty_bar[stage], phase ^ 1, abort_flag)) {
-        set_error(a.err, ERR_WAIT_EMPTY);
-        *abort_flag = 1;
-        break;
-      }
-      const int tok0 = (tile_lo + t) * kTile;
-      uint8_t* sk = stages + stage * Cfg::kStage;
-      // (page, row in page) of a token; tokens behind the end read the pool's first page
-      auto place = [&](int tok, int& page, int& off) {
-        page = 0;
-        off = 0;
-        const int pi = tok / a.page_size;
-        if (tok < L && pi < a.max_pages) {
-          page = pages[pi];
-          off = tok - pi * a.page_size;
-        }
-        if (page < 0 || page >= a.pool_pages) {
-          set_error(a.err, ERR_BOUNDS);
-          page = 0;
-        }
-      };
-      if (lane == 0) mbar_expect_tx(&full_bar[stage], Cfg::kStage);
-      __syncwarp();
-      for (int b = lane; b < kTile / box; b += 32) {
-        int page, off;
-        place(tok0 + b * box, page, off);
-#pragma unroll
-        for (int which = 0; which < 2; ++which)
-#pragma unroll
-          for (int cb = 0; cb < RB / Cfg::kBox; ++cb)
-            tma_load_3d(sk + which * Cfg::kHalf + cb * (kTile * 128) + b * box * Cfg::kBox, kv_map, cb * (Cfg::kBox * D / RB),
-                        (which * a.hk + kvh) * a.page_size + off, page, &full_bar[stage]);
-      }
-      if constexpr (E4M3) {
-        const int which = lane >> 4, i4 = (lane & 15) * 4;
-        int page, off;
-        place(tok0 + i4, page, off);
-        const size_t codes = (size_t)2 * a.hk * a.page_size * D;
-        const uint8_t* src = a.pool + (size_t)page * (codes + 2 * a.hk * a.page_size) + codes + (size_t)(which * a.hk + kvh) * a.page_size + off;
-        if (KERN_CHECK(src, 4, SITE_KV_ROW)) async_copy4(smem_u32(scales + stage * Cfg::kScaleBytes + which * kTile + i4), src);
-        async_arrive(&full_bar[stage]);
-      }
-      if (++stage == kStages) { stage = 0; phase ^= 1; }
-    }
-  } else {
     // ---------------- products ----------------
-    const int posA = rA < valid ? past + tok_lo + rA / G : -1, posB = rB < valid ? past + tok_lo + rB / G : -1;
-    const long long* maskA = TREE ? a.masks + (size_t)(row0 + tok_lo + (rA < valid ? rA / G : 0)) * a.words : nullptr;
-    const long long* maskB = TREE ? a.masks + (size_t)(row0 + tok_lo + (rB < valid ? rB / G : 0)) * a.words : nullptr;
-    // whether a row of this block sees token j
-    auto sees = [&](int j, int pos, const long long* mask) -> bool {
+    // whether column r of this block sees token j
+    auto sees = [&](int j, int r) -> bool {
+      if (r >= valid || j >= to) return false;
+      const int tk = tok_lo + r / G;
       if constexpr (TREE) {
         if (j < past) return true;
         const int n = j - past;
-        return j < L && n < a.words * 64 && ((mask[n >> 6] >> (n & 63)) & 1);
+        return n < a.words * 64 && ((a.masks[(size_t)(row0 + tk) * a.words + (n >> 6)] >> (n & 63)) & 1);
       } else {
-        return j <= pos;
+        return j <= past + tk;
       }
     };
     // the first token that some row of the block may not see
-    const int clear = TREE ? past : past + tok_lo + 1;
-    const int wtok = warp * 16;
+    const int clear = min(to, TREE ? past : past + tok_lo + 1);
+    const int pg = (g & 1) << 2 | (g >> 1);                   // the key row of operand row g: 0, 4, 1, 5, 2, 6, 3, 7
+    // of a pair of value rows, which is loaded first: chosen so that a phase's 8 lanes hit different columns of the swizzle
+    const int swap = RB == 64 ? (c >> 1) & 1 : (RB == 512 ? 0 : g & 1);
     int stage = 0;
     uint32_t phase = 0;
     for (int t = 0; t < ntiles; ++t) {
@@ -337,190 +407,219 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
         break;
       }
       const uint32_t sk = smem_u32(stages + stage * Cfg::kStage), sv = sk + Cfg::kHalf;
-      const int tok0 = (tile_lo + t) * kTile + wtok;          // this warp's first token
-      if (tok0 < end) {
-        // ---- S = Q K^T: n-tile n holds tokens n * 8 + (0, 4, 1, 5, 2, 6, 3, 7), so that neighbouring rows of a load differ in
-        // the bit of the swizzle that a row's own pieces do not reach ----
-        float s[2][4];
+#pragma unroll 1
+      for (int part = 0; part < kTile / (16 * kWarps); ++part) {
+        const int wtok = (part * kWarps + warp) * 16;               // this warp's 16 tokens of the tile
+        const int tok0 = from + t * kTile + wtok;
+        if (tok0 >= to) break;
+        // ---- S^T = K Q^T: operand rows g and g + 8 are tokens pg and 8 + pg, so that neighbouring rows of a load differ in the
+        // bit of the swizzle that a row's own pieces do not reach ----
+        float s[NT][4], s2[NT][4];                            // two chains of sums: one would be D / 16 dependent products
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-          const int tok = wtok + n * 8 + ((g & 1) << 2 | (g >> 1));
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int i = 0; i < KP; ++i) {
-            const uint4 kv = lds128(sk + piece_off<RB>(tok, c + 4 * i));
-            const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
+          for (int k = 0; k < 4; ++k) s[nt][k] = s2[nt][k] = 0.f;
+#pragma unroll
+        for (int i = 0; i < KP; ++i) {
+          const uint4 ka = lds128(sk + piece_off<RB, kTile>(wtok + pg, c + 4 * i)), kb = lds128(sk + piece_off<RB, kTile>(wtok + 8 + pg, c + 4 * i));
+          const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+          constexpr int steps = E4M3 ? 4 : 2;
+#pragma unroll
+          for (int x = 0; x < steps; ++x) {
+            uint32_t a0, a1, a2, a3;
             if constexpr (E4M3) {
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                uint4 qv;
-                if constexpr (kQShared) qv = q_frag[(4 * i + x) * 32 + lane];
-                else qv = make_uint4(qf[4 * i + x][0], qf[4 * i + x][1], qf[4 * i + x][2], qf[4 * i + x][3]);
-                mma_16816<true>(s[n], qv.x, qv.y, qv.z, qv.w, codes_f16x2(w[x]), codes_f16x2(w[x] >> 16));
-              }
+              codes_f16x4(wa[x], a0, a2);
+              codes_f16x4(wb[x], a1, a3);
             } else {
+              a0 = wa[2 * x]; a2 = wa[2 * x + 1];
+              a1 = wb[2 * x]; a3 = wb[2 * x + 1];
+            }
 #pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                uint4 qv;
-                if constexpr (kQShared) qv = q_frag[(2 * i + x) * 32 + lane];
-                else qv = make_uint4(qf[2 * i + x][0], qf[2 * i + x][1], qf[2 * i + x][2], qf[2 * i + x][3]);
-                mma_16816<false>(s[n], qv.x, qv.y, qv.z, qv.w, w[2 * x], w[2 * x + 1]);
-              }
+            for (int nt = 0; nt < NT; ++nt) {
+              const int ks = steps * i + x;
+              uint2 qv;
+              if constexpr (kQShared) qv = q_frag[(nt * KS + ks) * 32 + lane];
+              else qv = make_uint2(qf[nt][ks][0], qf[nt][ks][1]);
+              mma_16816<E4M3>(x & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, qv.x, qv.y);
             }
           }
         }
-        // ---- scores, what the rows see, running maximum ----
+        // ---- scores of tokens pg and 8 + pg, columns 8 nt + 2 c + x ----
         const bool edge = tok0 + 16 > clear;                  // rows see different tokens, or some are behind the end
-        bool see[2][4];
-        float ev[2][2];                                       // (8-bit) exponents of this lane's value rows, tokens c and c + 4
-        float mx[2] = {-INFINITY, -INFINITY}, wx[2] = {-INFINITY, -INFINITY};
-        const uint32_t ss = smem_u32(scales + stage * Cfg::kScaleBytes) + wtok;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-#pragma unroll
-          for (int h2 = 0; h2 < 2; ++h2) {
-            const int off = n * 8 + h2 * 4 + c, j = tok0 + off;
-            float kscale = 1.f;
-            if constexpr (E4M3) {
-              kscale = __uint_as_float(lds8(ss + off) << 23);
-              ev[n][h2] = (float)((int)lds8(ss + kTile + off) - 127);
-            }
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-              float& x = s[n][hh * 2 + h2];
-              x *= f_row[hh] * kscale;
-              bool ok = true;
-              if (edge) {
-                ok = (hh ? rB : rA) < valid && sees(j, hh ? posB : posA, hh ? maskB : maskA);
-                if (!ok) x = -INFINITY;
-              }
-              see[n][hh * 2 + h2] = ok;
-              mx[hh] = fmaxf(mx[hh], x);
-              if constexpr (E4M3) wx[hh] = fmaxf(wx[hh], x + ev[n][h2]);
-            }
-          }
-        }
-        float p[2][4];
-        float corr[2];
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 1));
-          mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 2));
-          const float m = fmaxf(m_run[hh], mx[hh]), mu = m == -INFINITY ? 0.f : m;
-          corr[hh] = exp2f(m_run[hh] - mu);
-          l_run[hh] *= corr[hh];
-          float cf = 1.f;                                     // 2^-c of the weights of this tile
-          if constexpr (E4M3) {
-            wx[hh] = fmaxf(wx[hh], __shfl_xor_sync(0xffffffffu, wx[hh], 1));
-            wx[hh] = fmaxf(wx[hh], __shfl_xor_sync(0xffffffffu, wx[hh], 2));
-            w_run[hh] = fmaxf(w_run[hh], wx[hh]);
-            // both maxima are running ones, so c never lets a weight above 1
-            const float cw = ceilf(w_run[hh] - mu);
-            const int cn = cw > -120.f ? (int)fminf(cw, 120.f) : -120;
-            if (c_run[hh] != -1000) corr[hh] *= pow2i(c_run[hh] - cn);
-            c_run[hh] = cn;
-            cf = pow2i(-cn);
-          }
-          m_run[hh] = m;
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int h2 = 0; h2 < 2; ++h2) {
-              const float e = exp2f(s[n][hh * 2 + h2] - mu);
-              l_run[hh] += e;
-              if constexpr (E4M3) p[n][hh * 2 + h2] = e * pow2i((int)ev[n][h2]) * cf;
-              else p[n][hh * 2 + h2] = e;
-            }
-        }
-        if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
-#pragma unroll
-          for (int i = 0; i < NC; ++i) {
-            o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[1]; o[i][3] *= corr[1];
-          }
-        }
-        uint32_t pa[4];
+        float kscale[2] = {1.f, 1.f}, vscale[2] = {1.f, 1.f};
         if constexpr (E4M3) {
-          pa[0] = pack_f16x2(p[0][0], p[0][1]); pa[1] = pack_f16x2(p[0][2], p[0][3]);
-          pa[2] = pack_f16x2(p[1][0], p[1][1]); pa[3] = pack_f16x2(p[1][2], p[1][3]);
-        } else {
-          pa[0] = pack_bf16x2(p[0][0], p[0][1]); pa[1] = pack_bf16x2(p[0][2], p[0][3]);
-          pa[2] = pack_bf16x2(p[1][0], p[1][1]); pa[3] = pack_bf16x2(p[1][2], p[1][3]);
+          const uint32_t ss = smem_u32(scales + stage * Cfg::kScaleBytes) + wtok + pg;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            kscale[h] = __uint_as_float(lds8(ss + 8 * h) << 23);
+            vscale[h] = __uint_as_float(lds8(ss + kTile + 8 * h) << 23);
+          }
         }
-        // ---- O += P V: the lane's k indices are tokens c, c + 4, 8 + c, 12 + c; its columns g * D / 8 onward. Which of a pair of
-        // tokens is loaded first is chosen by the lane so that a phase's 8 lanes hit different columns of the swizzle. ----
+        uint32_t see = 0xffffffffu;                           // bit nt * 4 + h * 2 + x
+        if (edge) {
+          see = 0;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const bool ok = sees(tok0 + pg + 8 * (k >> 1), nt * 8 + 2 * c + (k & 1));
+              see |= (ok ? 1u : 0u) << (nt * 4 + k);
+            }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (tok0 + pg + 8 * h >= to) kscale[h] = vscale[h] = 1.f;      // (not brought: anything may lie there)
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            s[nt][k] = (s[nt][k] + s2[nt][k]) * (f_col[nt][k & 1] * kscale[k >> 1]);
+            if (edge && !(see >> (nt * 4 + k) & 1)) s[nt][k] = -INFINITY;
+          }
+        float e[NT][4], w[NT][4];
+        auto weigh = [&]() {
+          float top = 0.f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              e[nt][k] = exp2f(s[nt][k] - m_run[nt][k & 1]);
+              top = fmaxf(top, e[nt][k]);
+              if constexpr (E4M3) {
+                w[nt][k] = e[nt][k] * (g_run[nt][k & 1] * vscale[k >> 1]);
+                top = fmaxf(top, w[nt][k]);
+              } else {
+                w[nt][k] = e[nt][k];
+              }
+            }
+          return top;
+        };
+        if (__any_sync(0xffffffffu, weigh() > kOutgrown)) {
+          // a reference moves to its column's maximum (rounded up: factors stay powers of two), and what it scaled with it
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              float mx = fmaxf(s[nt][x], s[nt][2 + x]), rx = mx;
+              if constexpr (E4M3)
+                rx = fmaxf(s[nt][x] + (float)((int)(__float_as_uint(vscale[0]) >> 23) - 127), s[nt][2 + x] + (float)((int)(__float_as_uint(vscale[1]) >> 23) - 127));
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) {
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                if constexpr (E4M3) rx = fmaxf(rx, __shfl_xor_sync(0xffffffffu, rx, d));
+              }
+              const float m = fmaxf(m_run[nt][x], ceilf(mx));
+              float co = exp2f(m_run[nt][x] - m);
+              l_run[nt][x] *= co;
+              m_run[nt][x] = m;
+              if constexpr (E4M3) {
+                const float r = fmaxf(r_run[nt][x], ceilf(rx) - 7.f);
+                co = exp2f(r_run[nt][x] - r);
+                r_run[nt][x] = r;
+                g_run[nt][x] = exp2f(m - r);
+              }
+#pragma unroll
+              for (int i = 0; i < MI; ++i) {
+                o[nt][i][x] *= co;
+                o[nt][i][2 + x] *= co;
+              }
+            }
+          weigh();
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) l_run[nt][k & 1] += e[nt][k];
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          pb[nt][0] = transposed(pack_pair<E4M3>(w[nt][0], w[nt][1]));
+          pb[nt][1] = transposed(pack_pair<E4M3>(w[nt][2], w[nt][3]));
+        }
+        // ---- O^T += V^T P^T: the lane's contraction indices are tokens c, c + 4, 8 + c, 12 + c; its channels g * D / 8 onward, two
+        // to an operand's rows g and g + 8 ----
         constexpr int VP = VB >= 16 ? VB / 16 : 1;            // loads per token
-        const int swap = RB == 64 ? (c >> 1) & 1 : (RB == 512 ? 0 : g & 1);
+        constexpr int W = VB >= 16 ? 4 : 2;                   // words per load
 #pragma unroll
         for (int h = 0; h < VP; ++h) {
-          uint32_t v[2][2][4];                                // [n][first, second][words]
+          uint32_t v[2][2][4];                                // [token half][first, second][words]
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               const int tok = wtok + n * 8 + c + 4 * (x ^ swap);
               if constexpr (VB >= 16) {
-                const uint4 w = lds128(sv + piece_off<RB>(tok, g * VP + h));
-                v[n][x][0] = w.x; v[n][x][1] = w.y; v[n][x][2] = w.z; v[n][x][3] = w.w;
+                const uint4 q4 = lds128(sv + piece_off<RB, kTile>(tok, g * VP + h));
+                v[n][x][0] = q4.x; v[n][x][1] = q4.y; v[n][x][2] = q4.z; v[n][x][3] = q4.w;
               } else {
-                const uint2 w = lds64(sv + piece_off<RB>(tok, g >> 1) + (g & 1) * 8);
-                v[n][x][0] = w.x; v[n][x][1] = w.y; v[n][x][2] = 0; v[n][x][3] = 0;
+                const uint2 q2 = lds64(sv + piece_off<RB, kTile>(tok, g >> 1) + (g & 1) * 8);
+                v[n][x][0] = q2.x; v[n][x][1] = q2.y; v[n][x][2] = v[n][x][3] = 0;
               }
-              if (edge && tok0 - wtok + tok >= L) v[n][x][0] = v[n][x][1] = v[n][x][2] = v[n][x][3] = 0;
+              if (edge && tok0 - wtok + tok >= to) v[n][x][0] = v[n][x][1] = v[n][x][2] = v[n][x][3] = 0;
             }
-          constexpr int W = VB >= 16 ? 4 : 2;                 // words per load
-          // columns of one word: their operand pairs (first token low)
-          auto column = [&](int w, int col, uint32_t& b0, uint32_t& b1) {
+          // channels 2 p and 2 p + 1 of word wd: operand rows g and g + 8, the first token of a pair low
+          auto operand = [&](int wd, int p, uint32_t (&av)[4]) {
             if constexpr (E4M3) {
-              const uint32_t sel = col < 2 ? (swap ? 0x1504u : 0x5140u) : (swap ? 0x3726u : 0x7362u);
-              b0 = codes_f16x2(__byte_perm(v[0][0][w], v[0][1][w], sel) >> ((col & 1) * 16));
-              b1 = codes_f16x2(__byte_perm(v[1][0][w], v[1][1][w], sel) >> ((col & 1) * 16));
+              const uint32_t sel = p == 0 ? (swap ? 0x1504u : 0x5140u) : (swap ? 0x3726u : 0x7362u);
+              codes_f16x4(__byte_perm(v[0][0][wd], v[0][1][wd], sel), av[0], av[1]);
+              codes_f16x4(__byte_perm(v[1][0][wd], v[1][1][wd], sel), av[2], av[3]);
             } else {
-              const uint32_t sel = col == 0 ? (swap ? 0x1054u : 0x5410u) : (swap ? 0x3276u : 0x7632u);
-              b0 = __byte_perm(v[0][0][w], v[0][1][w], sel);
-              b1 = __byte_perm(v[1][0][w], v[1][1][w], sel);
+              const uint32_t lo = swap ? 0x1054u : 0x5410u, hi = swap ? 0x3276u : 0x7632u;
+              av[0] = __byte_perm(v[0][0][wd], v[0][1][wd], lo);
+              av[1] = __byte_perm(v[0][0][wd], v[0][1][wd], hi);
+              av[2] = __byte_perm(v[1][0][wd], v[1][1][wd], lo);
+              av[3] = __byte_perm(v[1][0][wd], v[1][1][wd], hi);
             }
           };
-          constexpr int CW = E4M3 ? 4 : 2;                    // columns per word
+          constexpr int PW = E4M3 ? 2 : 1;                    // channel pairs per word
           if (!edge) {
 #pragma unroll
-            for (int w = 0; w < W; ++w)
+            for (int wd = 0; wd < W; ++wd)
 #pragma unroll
-              for (int col = 0; col < CW; ++col) {
-                uint32_t b0, b1;
-                column(w, col, b0, b1);
-                mma_16816<E4M3>(o[h * W * CW + w * CW + col], pa[0], pa[1], pa[2], pa[3], b0, b1);
+              for (int p = 0; p < PW; ++p) {
+                uint32_t av[4];
+                operand(wd, p, av);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_16816<E4M3>(o[nt][(h * W + wd) * PW + p], av[0], av[1], av[2], av[3], pb[nt][0], pb[nt][1]);
               }
           } else {
-            constexpr uint32_t one = E4M3 ? 0x3c003c00u : 0x3f803f80u;
-            auto half_one = [](bool lo, bool hi) { return (lo ? (one & 0xffffu) : 0u) | (hi ? (one & 0xffff0000u) : 0u); };
-            const uint32_t a0 = half_one(see[0][0], see[0][1]), a1 = half_one(see[0][2], see[0][3]);
-            const uint32_t a2 = half_one(see[1][0], see[1][1]), a3 = half_one(see[1][2], see[1][3]);
+            constexpr uint32_t one = E4M3 ? 0x3c003c00u : 0x3f803f80u, inf = E4M3 ? 0x7c00u : 0x7f80u;
+            auto ones = [](uint32_t lo, uint32_t hi) { return (lo ? (one & 0xffffu) : 0u) | (hi ? (one & 0xffff0000u) : 0u); };
 #pragma unroll
-            for (int w = 0; w < W; ++w)
+            for (int wd = 0; wd < W; ++wd)
 #pragma unroll
-              for (int col = 0; col < CW; ++col) {
-                uint32_t b0, b1;
-                column(w, col, b0, b1);
-                float (&oo)[4] = o[h * W * CW + w * CW + col];
-                const uint32_t n0 = not_finite<E4M3>(b0), n1 = not_finite<E4M3>(b1);
-                if (__any_sync(0xffffffffu, (n0 | n1) != 0)) {
-                  // rows that see an infinity or a NaN here get it back: counts of those that pull up (+inf, NaN) and down
-                  constexpr uint32_t inf = E4M3 ? 0x7c00u : 0x7f80u;
-                  auto pulls = [](uint32_t w16, bool bad, uint32_t towards) { return bad && (w16 == towards || (w16 & 0x7fffu) > inf); };
-                  const uint32_t up0 = half_one(pulls(b0 & 0xffffu, n0 & 1u, inf), pulls(b0 >> 16, n0 >> 16, inf));
-                  const uint32_t up1 = half_one(pulls(b1 & 0xffffu, n1 & 1u, inf), pulls(b1 >> 16, n1 >> 16, inf));
-                  const uint32_t dn0 = half_one(pulls(b0 & 0xffffu, n0 & 1u, inf | 0x8000u), pulls(b0 >> 16, n0 >> 16, inf | 0x8000u));
-                  const uint32_t dn1 = half_one(pulls(b1 & 0xffffu, n1 & 1u, inf | 0x8000u), pulls(b1 >> 16, n1 >> 16, inf | 0x8000u));
-                  float up[4] = {0.f, 0.f, 0.f, 0.f}, dn[4] = {0.f, 0.f, 0.f, 0.f};
-                  mma_16816<E4M3>(up, a0, a1, a2, a3, up0, up1);
-                  mma_16816<E4M3>(dn, a0, a1, a2, a3, dn0, dn1);
+              for (int p = 0; p < PW; ++p) {
+                uint32_t av[4], bad[4];
+                operand(wd, p, av);
 #pragma unroll
-                  for (int x = 0; x < 4; ++x) {
-                    if (up[x] > 0.f) oo[x] += INFINITY;
-                    if (dn[x] > 0.f) oo[x] -= INFINITY;
+                for (int k = 0; k < 4; ++k) bad[k] = not_finite<E4M3>(av[k]);
+                if (__any_sync(0xffffffffu, (bad[0] | bad[1] | bad[2] | bad[3]) != 0)) {
+                  // columns that see an infinity or a NaN here get it back: counts of those that pull up (+inf, NaN) and down
+                  uint32_t up[4], dn[4];
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    auto pulls = [&](uint32_t half, uint32_t towards) { return half == towards || (half & 0x7fffu) > inf; };
+                    up[k] = ones((bad[k] & 1u) && pulls(av[k] & 0xffffu, inf), (bad[k] >> 16) && pulls(av[k] >> 16, inf));
+                    dn[k] = ones((bad[k] & 1u) && pulls(av[k] & 0xffffu, inf | 0x8000u), (bad[k] >> 16) && pulls(av[k] >> 16, inf | 0x8000u));
+                  }
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt) {
+                    const uint32_t sb = see >> (nt * 4);
+                    const uint32_t b0 = transposed(ones(sb & 1u, sb & 2u)), b1 = transposed(ones(sb & 4u, sb & 8u));
+                    float nu[4] = {0.f, 0.f, 0.f, 0.f}, nd[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_16816<E4M3>(nu, up[0], up[1], up[2], up[3], b0, b1);
+                    mma_16816<E4M3>(nd, dn[0], dn[1], dn[2], dn[3], b0, b1);
+                    float (&oo)[4] = o[nt][(h * W + wd) * PW + p];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                      if (nu[k] > 0.f) oo[k] += INFINITY;
+                      if (nd[k] > 0.f) oo[k] -= INFINITY;
+                    }
                   }
                 }
-                mma_16816<E4M3>(oo, pa[0], pa[1], pa[2], pa[3], b0 & ~n0, b1 & ~n1);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                  mma_16816<E4M3>(o[nt][(h * W + wd) * PW + p], av[0] & ~bad[0], av[1] & ~bad[1], av[2] & ~bad[2], av[3] & ~bad[3], pb[nt][0], pb[nt][1]);
               }
           }
         }
@@ -530,144 +629,197 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
       if (++stage == kStages) { stage = 0; phase ^= 1; }
     }
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      l_run[hh] += __shfl_xor_sync(0xffffffffu, l_run[hh], 1);
-      l_run[hh] += __shfl_xor_sync(0xffffffffu, l_run[hh], 2);
-    }
-    if constexpr (E4M3) {
-      const float fa = c_run[0] == -1000 ? 1.f : pow2i(c_run[0]), fb = c_run[1] == -1000 ? 1.f : pow2i(c_run[1]);
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < NC; ++i) { o[i][0] *= fa; o[i][1] *= fa; o[i][2] *= fb; o[i][3] *= fb; }
-    }
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l_run[nt][x] += __shfl_xor_sync(0xffffffffu, l_run[nt][x], d);
+        if constexpr (E4M3) {
+          const float f = 1.f / g_run[nt][x];                 // (a power of two)
+#pragma unroll
+          for (int i = 0; i < MI; ++i) {
+            o[nt][i][x] *= f;
+            o[nt][i][2 + x] *= f;
+          }
+        }
+      }
   }
 
-  // ---------------- the four warps' parts are joined: rows of floats in the ring's memory ----------------
+  // ---------------- the warps' parts are joined: rows of floats in the ring's memory ----------------
   pdl_launch_dependents();
   __syncthreads();
   if (*abort_flag != 0) {
     const uint64_t t0 = globaltimer_ns();       // let copies in flight land before the memory is used again or goes away
     while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
-    return;
   }
   constexpr int kPad = D + 4;
-  float* mo = reinterpret_cast<float*>(stages);               // [4][16][D + 4]
-  float* mm = mo + 4 * 16 * kPad;                             // [4][16] maxima
-  float* ml = mm + 64;                                        // [4][16] sums
-  if (warp < 4) {
-    if (c == 0) {
-      mm[warp * 16 + rA] = m_run[0]; mm[warp * 16 + rB] = m_run[1];
-      ml[warp * 16 + rA] = l_run[0]; ml[warp * 16 + rB] = l_run[1];
-    }
-    // the lane's columns: two runs of D / 8, from 2 c D / 8 and (2 c + 1) D / 8
+  float* mo = reinterpret_cast<float*>(stages);               // [warps][rows][D + 4]
+  float* mm = mo + kWarps * kRows * kPad;                     // [warps][rows] references
+  float* ml = mm + kWarps * kRows;                            // [warps][rows] sums
+  float* jm = ml + kWarps * kRows;                            // [rows] of the CTA
+  float* jl = jm + kRows;
+  __syncthreads();
+  if (warp < kWarps) {
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int par = 0; par < 2; ++par)
+      for (int x = 0; x < 2; ++x) {
+        const int r = nt * 8 + 2 * c + x;
+        if (g == 0) {
+          mm[warp * kRows + r] = m_run[nt][x];
+          ml[warp * kRows + r] = l_run[nt][x];
+        }
+        float* dst = mo + (warp * kRows + r) * kPad + g * (D / 8);
 #pragma unroll
-        for (int i = 0; i < NC; i += 4)
-          *reinterpret_cast<float4*>(mo + (warp * 16 + (hh ? rB : rA)) * kPad + (2 * c + par) * NC + i) =
-              make_float4(o[i][hh * 2 + par], o[i + 1][hh * 2 + par], o[i + 2][hh * 2 + par], o[i + 3][hh * 2 + par]);
+        for (int i = 0; i < MI; i += 2)
+          *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(o[nt][i][x], o[nt][i][2 + x], o[nt][i + 1][x], o[nt][i + 1][2 + x]);
+      }
   }
   __syncthreads();
-  const bool whole = shares == 1;
-  for (int i = threadIdx.x; i < valid * (D / 8); i += kRowsThreads) {
-    const int r = i / (D / 8), col = (i % (D / 8)) * 8;
-    const float m0 = mm[r], m1 = mm[16 + r], m2 = mm[32 + r], m3 = mm[48 + r];
-    const float m = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)), mu = m == -INFINITY ? 0.f : m;
-    float f[4] = {exp2f(m0 - mu), exp2f(m1 - mu), exp2f(m2 - mu), exp2f(m3 - mu)};
-    float l = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if (mm[w * 16 + r] == -INFINITY && ml[w * 16 + r] == 0.f) continue;       // a warp that saw nothing of this row
-      l += f[w] * ml[w * 16 + r];
-      const float* src = mo + (w * 16 + r) * kPad + col;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] += f[w] * src[k];
-    }
+  auto store = [&](int r, int col, float m, float l, const float (&y)[8], bool whole) {
     const int tk = row0 + tok_lo + r / G, head = kvh * G + r % G;
     if (whole) {
       const float inv = l == 0.f ? 0.f : 1.f / l;             // a row that sees nothing: zeros
       *reinterpret_cast<uint4*>(a.out + (size_t)tk * a.out_stride + (size_t)head * D + col) =
-          make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv), pack_bf16x2(x[4] * inv, x[5] * inv),
-                     pack_bf16x2(x[6] * inv, x[7] * inv));
+          make_uint4(pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv), pack_bf16x2(y[4] * inv, y[5] * inv),
+                     pack_bf16x2(y[6] * inv, y[7] * inv));
     } else {
-      const size_t at = ((size_t)tk * a.hq + head) * a.splits + split;
+      const int groups = gridDim.z / a.cluster;
+      const size_t at = ((size_t)tk * a.hq + head) * groups + blockIdx.z / a.cluster;
       float4* dst = reinterpret_cast<float4*>(a.ws_o + at * D + col);
-      dst[0] = make_float4(x[0], x[1], x[2], x[3]);
-      dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+      dst[0] = make_float4(y[0], y[1], y[2], y[3]);
+      dst[1] = make_float4(y[4], y[5], y[6], y[7]);
       if (col == 0) {
         a.ws_ml[at * 2] = m;
         a.ws_ml[at * 2 + 1] = l;
       }
     }
+  };
+  const bool whole = shares <= a.cluster;                     // this cluster has the whole context
+  for (int i = threadIdx.x; i < valid * (D / 8); i += kThreads) {
+    const int r = i / (D / 8), col = (i % (D / 8)) * 8;
+    float m = kUnset, l = 0.f, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, mm[w * kRows + r]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float lw = ml[w * kRows + r];
+      if (lw == 0.f) continue;                                // a warp that saw nothing of this row
+      const float f = exp2f(mm[w * kRows + r] - m);
+      l += f * lw;
+      const float4* src = reinterpret_cast<const float4*>(mo + (w * kRows + r) * kPad + col);
+      const float4 u = src[0], v = src[1];
+      y[0] += f * u.x; y[1] += f * u.y; y[2] += f * u.z; y[3] += f * u.w;
+      y[4] += f * v.x; y[5] += f * v.y; y[6] += f * v.z; y[7] += f * v.w;
+    }
+    if (a.cluster == 1) {
+      if (whole || (int)blockIdx.z < shares) store(r, col, m, l, y, whole);
+    } else {
+      float4* dst = reinterpret_cast<float4*>(mo + r * kPad + col);       // (in place of what this thread has read)
+      dst[0] = make_float4(y[0], y[1], y[2], y[3]);
+      dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+      if (col == 0) {
+        jm[r] = m;
+        jl[r] = l;
+      }
+    }
+  }
+  if (a.cluster > 1) {
+    // ---------------- and the cluster's: every CTA finishes a part of the rows ----------------
+    cluster_barrier();
+    const int rank = blockIdx.z % a.cluster, first = blockIdx.z - rank;
+    const int live = min(a.cluster, shares - first);          // CTAs of this cluster that had a share
+    for (int i = rank * kThreads + threadIdx.x; live > 0 && i < valid * (D / 8); i += a.cluster * kThreads) {
+      const int r = i / (D / 8), col = (i % (D / 8)) * 8;
+      const uint32_t am = smem_u32(jm + r), al = smem_u32(jl + r), ao = smem_u32(mo + r * kPad + col);
+      float m = kUnset, l = 0.f, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < live; ++k) m = fmaxf(m, ld_rank(at_rank(am, k)));
+#pragma unroll 4
+      for (int k = 0; k < live; ++k) {
+        const float lk = ld_rank(at_rank(al, k));
+        if (lk == 0.f) continue;
+        const float f = exp2f(ld_rank(at_rank(am, k)) - m);
+        l += f * lk;
+        const float4 u = ld_rank4(at_rank(ao, k)), v = ld_rank4(at_rank(ao, k) + 16);
+        y[0] += f * u.x; y[1] += f * u.y; y[2] += f * u.z; y[3] += f * u.w;
+        y[4] += f * v.x; y[5] += f * v.y; y[6] += f * v.z; y[7] += f * v.w;
+      }
+      store(r, col, m, l, y, whole);
+    }
+    cluster_barrier();                                        // no CTA's memory goes before the others have read it
   }
 }
 
-// Joins the shares of every row that was cut: a warp per (row, head), D / 32 columns a lane. grid (ceil(max_rows * hq / 8), seqs).
+// Joins the groups of shares of every row that was cut further than a cluster reaches: a warp per (row, head), D / 32 columns a
+// lane. grid (ceil(max_rows * hq / 8), seqs).
 template <int D, bool TREE>
 KERN_DEVICE void rows_merge(const float* ws_o, const float* ws_ml, __nv_bfloat16* out, const int* seq_lens, const int* cu_q, int rows_per_seq,
-                            int hq, int hk, int splits, int out_stride) {
+                            int hq, int toks, int splits, int cluster, int out_stride) {
   pdl_wait();
   const int lane = threadIdx.x & 31, seq = blockIdx.y;
   const int at = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int row0 = cu_q ? cu_q[seq] : seq * rows_per_seq, R = cu_q ? cu_q[seq + 1] - row0 : rows_per_seq;
   const int tok = at / hq, head = at % hq;
   if (tok >= R) return;
-  const int L = max(seq_lens[seq], 0), G = hq / hk, toks = 16 / G > 0 ? 16 / G : 1;
-  const int lo = tok / toks * toks;
+  const int L = max(seq_lens[seq], 0), lo = tok / toks * toks;
   const int end = TREE ? L : max(0, L - R + lo + min(toks, R - lo));
-  const int shares = rows_shares((end + kTile - 1) / kTile, splits);
-  if (shares == 1) return;                                    // written by its one CTA
-  const size_t base = ((size_t)(row0 + tok) * hq + head) * splits;
-  float m = -INFINITY;
-  for (int s = 0; s < shares; ++s) m = fmaxf(m, ws_ml[(base + s) * 2]);
-  const float mu = m == -INFINITY ? 0.f : m;
+  const int shares = rows_shares(end, splits);
+  if (shares <= cluster) return;                              // written by its one cluster
+  const int groups = splits / cluster, live = (shares + cluster - 1) / cluster;
+  const size_t base = ((size_t)(row0 + tok) * hq + head) * groups;
+  float m = kUnset;
+  for (int s = 0; s < live; ++s) m = fmaxf(m, ws_ml[(base + s) * 2]);
   constexpr int N = D / 32;
-  float x[N], l = 0.f;
+  float y[N], l = 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < shares; ++s) {
+  for (int i = 0; i < N; ++i) y[i] = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < live; ++s) {
     const float ms = ws_ml[(base + s) * 2], ls = ws_ml[(base + s) * 2 + 1];
-    if (ms == -INFINITY && ls == 0.f) continue;
-    const float f = exp2f(ms - mu);
+    const float f = ls == 0.f ? 0.f : exp2f(ms - m);
     l += f * ls;
     const float* src = ws_o + (base + s) * D + lane * N;
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] += f * src[i];
+    for (int i = 0; i < N; ++i) y[i] += f * src[i];
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   __nv_bfloat16* dst = out + (size_t)(row0 + tok) * out_stride + (size_t)head * D + lane * N;
 #pragma unroll
-  for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(x[i] * inv, x[i + 1] * inv);
+  for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(y[i] * inv, y[i + 1] * inv);
 }
 
 }  // namespace kern
 
 using namespace kern;
 
-#define KERN_ROWS_ENTRY(D, KIND, E4M3, FORM, TREE)                                                                                \
-  extern "C" __global__ void __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) kern_attn_rows_##KIND##_##FORM##_d##D(             \
-      const __grid_constant__ CUtensorMap kv_map, const __nv_bfloat16* q, __nv_bfloat16* out, float* ws_o, float* ws_ml,          \
-      const uint8_t* pool, const int* block_table, const int* seq_lens, const int* cu_q, const long long* masks, int words,       \
-      int rows_per_seq, int hq, int hk, int q_stride, int out_stride, int max_pages, int page_size, int splits, int pool_pages,   \
-      float scale_log2, int* err) {                                                                                               \
-    rows_body<D, E4M3, TREE>(&kv_map, RowsArgs{q, out, ws_o, ws_ml, pool, block_table, seq_lens, cu_q, masks, err, words,         \
-                                               rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, splits,          \
-                                               pool_pages, scale_log2});                                                          \
+#define KERN_ROWS_ENTRY(D, KIND, E4M3, FORM, TREE, NT)                                                                            \
+  extern "C" __global__ void __launch_bounds__(RowsCfg<D, E4M3, NT>::kThreads, RowsCfg<D, E4M3, NT>::kPerSm)                                        \
+      kern_attn_rows_##KIND##_##FORM##_d##D##_n##NT(                                                                              \
+          const __grid_constant__ CUtensorMap kv_map, const __nv_bfloat16* q, __nv_bfloat16* out, float* ws_o, float* ws_ml,      \
+          const uint8_t* pool, const int* block_table, const int* seq_lens, const int* cu_q, const long long* masks, int words,   \
+          int rows_per_seq, int hq, int hk, int q_stride, int out_stride, int max_pages, int page_size, int cluster,              \
+          int pool_pages, float scale_log2, int* err) {                                                                           \
+    rows_body<D, E4M3, TREE, NT>(&kv_map, RowsArgs{q, out, ws_o, ws_ml, pool, block_table, seq_lens, cu_q, masks, err, words,     \
+                                                   rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, cluster,     \
+                                                   pool_pages, scale_log2});                                                      \
   }
 #define KERN_ROWS_MERGE(D, FORM, TREE)                                                                                            \
   extern "C" __global__ void __launch_bounds__(256) kern_attn_rows_merge_##FORM##_d##D(                                           \
       const float* ws_o, const float* ws_ml, __nv_bfloat16* out, const int* seq_lens, const int* cu_q, int rows_per_seq, int hq,  \
-      int hk, int splits, int out_stride) {                                                                                       \
-    rows_merge<D, TREE>(ws_o, ws_ml, out, seq_lens, cu_q, rows_per_seq, hq, hk, splits, out_stride);                              \
+      int toks, int splits, int cluster, int out_stride) {                                                                        \
+    rows_merge<D, TREE>(ws_o, ws_ml, out, seq_lens, cu_q, rows_per_seq, hq, toks, splits, cluster, out_stride);                   \
   }
-#define KERN_ROWS(D)                           \
-  KERN_ROWS_ENTRY(D, e4m3, true, causal, false) \
-  KERN_ROWS_ENTRY(D, e4m3, true, tree, true)    \
-  KERN_ROWS_ENTRY(D, bf16, false, tree, true)   \
-  KERN_ROWS_MERGE(D, causal, false)             \
+#define KERN_ROWS_FORMS(D, NT)                      \
+  KERN_ROWS_ENTRY(D, e4m3, true, causal, false, NT) \
+  KERN_ROWS_ENTRY(D, e4m3, true, tree, true, NT)    \
+  KERN_ROWS_ENTRY(D, bf16, false, tree, true, NT)
+#define KERN_ROWS(D)      \
+  KERN_ROWS_FORMS(D, 1)   \
+  KERN_ROWS_FORMS(D, 2)   \
+  KERN_ROWS_MERGE(D, causal, false) \
   KERN_ROWS_MERGE(D, tree, true)
 KERN_ROWS(64)
 KERN_ROWS(128)
 KERN_ROWS(256)
+KERN_ROWS_FORMS(64, 4)
+KERN_ROWS_FORMS(128, 4)

@@ -44,10 +44,11 @@ KERN_DEVICE float group_max(float v) {
   return v;
 }
 
-// a cos - b sin with the rounding of b sin taken back: a code next to a border then falls where the exact value does
-KERN_DEVICE float turned(float a, float c, float b, float s) {
-  const float p = b * s;
-  return fmaf(a, c, -p) - fmaf(b, s, -p);
+// A double as a float that a later rounding to fewer bits takes where it would have taken the double: cut, and the last bit set
+// if anything was cut off. e4m3 has few borders, but one value in a million sits near enough to one for 24 bits to pick the wrong side.
+KERN_DEVICE float sticky_float(double x) {
+  const float f = __double2float_rz(x);
+  return __uint_as_float(__float_as_uint(f) | ((double)f != x && fabsf(f) <= 3.402823466e38f ? 1u : 0u));
 }
 
 struct AppendArgs {
@@ -103,7 +104,7 @@ KERN_DEVICE void append_body(const AppendArgs& a) {
     }
   }
   const long long page = slot >= 0 ? slot / a.page_size : 0;
-  const int off = slot >= 0 ? (int)(slot % a.page_size) : 0;
+  const int slot_off = slot >= 0 ? (int)(slot % a.page_size) : 0;
   const size_t codes = (size_t)2 * a.hk * a.page_size * D;
   uint8_t* const pg = a.pool + (size_t)page * (codes + 2 * a.hk * a.page_size);
   const int rows = a.hq + 2 * a.hk;
@@ -115,77 +116,143 @@ KERN_DEVICE void append_body(const AppendArgs& a) {
     const bool live = h < rows && (h < a.hq || slot >= 0);
     const bool is_q = h < a.hq, is_k = !is_q && h < a.hq + a.hk;
     float x[8];
+    uint32_t w0[4];
     {
       uint4 raw = make_uint4(0, 0, 0, 0);
       if (live) raw = *reinterpret_cast<const uint4*>(src + (size_t)h * D + i0);
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+      w0[0] = raw.x; w0[1] = raw.y; w0[2] = raw.z; w0[3] = raw.w;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack_bf16x2(w[i]);
+        const float2 f = unpack_bf16x2(w0[i]);
         x[2 * i] = f.x;
         x[2 * i + 1] = f.y;
       }
     }
+    // the partners' values, and with norms the weights of both
+    float y[8], wx[8], wy[8];
+    const int from = turns && !a.interleaved ? (upper ? lane - partner_lanes : lane + partner_lanes) : lane;
+    if (a.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack_bf16x2(__shfl_sync(0xffffffffu, w0[i], from, kLanes));
+        y[2 * i] = f.x;
+        y[2 * i + 1] = f.y;
+      }
+    }
     const __nv_bfloat16* nw = is_q ? a.q_norm : a.k_norm;
+    const bool norm = (is_q || is_k) && nw != nullptr, changed = norm || ((is_q || is_k) && turns);
+    float inv = 1.f;
     if (a.q_norm != nullptr || a.k_norm != nullptr) {        // uniform
       float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
       ss = group_sum<kLanes>(ss);
-      if (live && (is_q || is_k) && nw != nullptr) {
+      if (norm) {
         const float m = ss / (float)D + a.eps;
-        float inv = rsqrtf(m);
+        inv = rsqrtf(m);
         inv = inv * fmaf(-0.5f * m * inv, inv, 1.5f);        // one Newton step: the hardware's estimate is two units off
         const uint4 wv = *reinterpret_cast<const uint4*>(nw + i0);
-        const uint32_t w[4] = {wv.x, wv.y, wv.z, wv.w};
+        const uint4 pv = *reinterpret_cast<const uint4*>(nw + from * 8);
+        const uint32_t ww[4] = {wv.x, wv.y, wv.z, wv.w}, pw[4] = {pv.x, pv.y, pv.z, pv.w};
+        const float one = a.norm_plus_one ? 1.f : 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 f = unpack_bf16x2(w[i]);
-          x[2 * i] *= inv * (a.norm_plus_one ? f.x + 1.f : f.x);
-          x[2 * i + 1] *= inv * (a.norm_plus_one ? f.y + 1.f : f.y);
+          const float2 f = unpack_bf16x2(ww[i]), h2 = unpack_bf16x2(pw[i]);
+          wx[2 * i] = f.x + one;
+          wx[2 * i + 1] = f.y + one;
+          wy[2 * i] = a.interleaved ? f.y + one : h2.x + one;
+          wy[2 * i + 1] = a.interleaved ? f.x + one : h2.y + one;
         }
       }
     }
-    if (a.interleaved) {
-      if (turns && (is_q || is_k)) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float u = x[2 * i], v = x[2 * i + 1];
-          x[2 * i] = turned(u, cs[i], v, sn[i]);
-          x[2 * i + 1] = turned(v, cs[i], u, -sn[i]);
-        }
-      }
-    } else {
-      const int from = turns ? (upper ? lane - partner_lanes : lane + partner_lanes) : lane;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float y = __shfl_sync(0xffffffffu, x[i], from, kLanes);
-        if (turns && (is_q || is_k)) x[i] = turned(x[i], cs[i], y, upper ? -sn[i] : sn[i]);
-      }
-    }
-    if (is_q) {
-      if (live)
-        *reinterpret_cast<uint4*>(a.q_out + (size_t)t * a.q_stride + (size_t)h * D + i0) =
-            make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-    }
-    float top = 0.f;
+    // x becomes the row's values; off: how far they may be from the exact ones (several units of the 24 bits of both partners)
+    float off[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (!(fabsf(x[i]) <= 3.402823466e38f)) x[i] = __uint_as_float(0x7fffffffu);      // not finite: NaN
-      top = fmaxf(top, fabsf(x[i]));                                                  // (a NaN is not taken)
+      float u = x[i], v = y[i];
+      if (norm) {
+        u *= wx[i] * inv;
+        v *= wy[i] * inv;
+      }
+      off[i] = changed ? (fabsf(u) + fabsf(v)) * 4.76837158e-7f : 0.f;      // 2^-21
+      if (turns && (is_q || is_k)) {
+        const bool minus = a.interleaved ? (i & 1) == 0 : !upper;
+        u = fmaf(u, a.interleaved ? cs[i >> 1] : cs[i], (minus ? -v : v) * (a.interleaved ? sn[i >> 1] : sn[i]));
+      }
+      y[i] = u;
     }
-    top = group_max<kLanes>(top);
-    if (live && !is_q) {
-      const int e = row_exponent(top);
-      const float inv = pow2f(-e);
-      uint32_t c[2];
+    if (is_q && live)
+      *reinterpret_cast<uint4*>(a.q_out + (size_t)t * a.q_stride + (size_t)h * D + i0) =
+          make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+    const bool stored = live && !is_q;
+    if (!__any_sync(0xffffffffu, stored)) continue;
+    auto biggest = [&]() {
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (!(fabsf(y[i]) <= 3.402823466e38f)) y[i] = __uint_as_float(0x7fffffffu);    // not finite: NaN
+        top = fmaxf(top, fabsf(y[i]));                                                // (a NaN is not taken)
+      }
+      return group_max<kLanes>(top);
+    };
+    auto encode = [&](float scale, float by, uint32_t (&c)[2]) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i] * inv, x[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2] * inv, x[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(fmaf(off[4 * i], by, y[4 * i]) * scale, fmaf(off[4 * i + 1], by, y[4 * i + 1]) * scale), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(fmaf(off[4 * i + 2], by, y[4 * i + 2]) * scale, fmaf(off[4 * i + 3], by, y[4 * i + 3]) * scale), __NV_SATFINITE, __NV_E4M3);
         c[i] = lo | (hi << 16);
       }
-      const size_t row = ((size_t)(is_k ? 0 : a.hk) + (h - a.hq - (is_k ? 0 : a.hk))) * a.page_size + off;
+    };
+    float top = biggest();
+    int e = row_exponent(top);
+    uint32_t c[2], c2[2];
+    encode(pow2f(-e), 1.f, c);
+    encode(pow2f(-e), -1.f, c2);
+    const bool close = stored && changed && (c[0] != c2[0] || c[1] != c2[1] || row_exponent(top * 1.000001f) != row_exponent(top * 0.999999f));
+    if (__any_sync(0xffffffffu, close)) {
+      // a value, or the row's largest, sits next to a border: the warp's keys once more, in 64 bits
+      double dinv = 1.0;
+      if (a.k_norm != nullptr) {
+        double ss = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fma((double)x[i], (double)x[i], ss);
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const double m = ss / (double)D + (double)a.eps;
+        dinv = (double)rsqrtf((float)m);
+        dinv = dinv * fma(-0.5 * m * dinv, dinv, 1.5);       // 22 bits, doubled twice
+        dinv = dinv * fma(-0.5 * m * dinv, dinv, 1.5);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float pv;
+        if (a.interleaved) pv = x[i ^ 1];
+        else {
+          const float2 f = unpack_bf16x2(__shfl_sync(0xffffffffu, w0[i >> 1], from, kLanes));
+          pv = (i & 1) ? f.y : f.x;
+        }
+        if (is_k && changed) {
+          double u = x[i], v = pv;
+          if (norm) {
+            u *= (double)wx[i] * dinv;
+            v *= (double)wy[i] * dinv;
+          }
+          if (turns) {
+            const bool minus = a.interleaved ? (i & 1) == 0 : !upper;
+            u = fma(u, (double)(a.interleaved ? cs[i >> 1] : cs[i]), (minus ? -v : v) * (double)(a.interleaved ? sn[i >> 1] : sn[i]));
+          }
+          y[i] = sticky_float(u);
+        }
+      }
+      top = biggest();
+      e = row_exponent(top);
+      encode(pow2f(-e), 0.f, c);
+    }
+    if (stored) {
+      const size_t row = ((size_t)(is_k ? 0 : a.hk) + (h - a.hq - (is_k ? 0 : a.hk))) * a.page_size + slot_off;
       uint8_t* dst = pg + row * D + i0;
       if (KERN_CHECK(dst, 8, SITE_KV_APPEND)) {
         *reinterpret_cast<uint2*>(dst) = make_uint2(c[0], c[1]);
@@ -238,7 +305,7 @@ KERN_DEVICE void read_body(const uint8_t* pool, const long long* slots, __nv_bfl
 }  // namespace kern
 
 #define KERN_APPEND_ENTRY(D)                                                                                                      \
-  extern "C" __global__ void __launch_bounds__(256) kern_rope_kv_append_e4m3_d##D(                                                \
+  extern "C" __global__ void __launch_bounds__(256, 3) kern_rope_kv_append_e4m3_d##D(                                                \
       const __nv_bfloat16* qkv, __nv_bfloat16* q_out, uint8_t* pool, const long long* positions, const long long* slots,          \
       const float* cos_tab, const float* sin_tab, const __nv_bfloat16* q_norm, const __nv_bfloat16* k_norm, int tokens, int hq,   \
       int hk, int rot, int page_size, float eps, int norm_plus_one, int interleaved, long long kv_slots, int max_pos,             \

@@ -118,7 +118,8 @@ class Device {
     return out;
   }
 
-  void launch(CUfunction f, const LaunchDims& d, CUstream stream, void** params) {
+  // `image`: the whole parameter block as the kernel has it (every parameter at its natural alignment), instead of `params`
+  void launch(CUfunction f, const LaunchDims& d, CUstream stream, void** params, const void* image = nullptr, size_t image_bytes = 0) {
     if (d.grid[0] == 0 || d.grid[1] == 0 || d.grid[2] == 0) return;  // an empty grid is a no-op
     auto& cu = Cuda::get();
     if (d.shared_mem > 48 * 1024) {
@@ -151,7 +152,8 @@ class Device {
     }
     cfg.attrs = attrs;
     cfg.numAttrs = na;
-    cu_check(cu.cuLaunchKernelEx_(&cfg, f, params, nullptr), "cuLaunchKernelEx");
+    void* extra[] = {CU_LAUNCH_PARAM_BUFFER_POINTER, const_cast<void*>(image), CU_LAUNCH_PARAM_BUFFER_SIZE, &image_bytes, CU_LAUNCH_PARAM_END};
+    cu_check(cu.cuLaunchKernelEx_(&cfg, f, image ? nullptr : params, image ? extra : nullptr), "cuLaunchKernelEx");
   }
 
   // ---- TMA descriptors ----
