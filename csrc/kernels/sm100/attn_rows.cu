@@ -27,29 +27,9 @@
 // Values that a row does not see do not reach it, whatever they are: tokens behind the end are cleared, and in the tiles where
 // rows see different tokens values that are not finite are taken out of the product and put back for the rows that see them (a
 // second pass of products over 0 / 1, only when there are any).
-#include <cuda_fp8.h>
-
-#include "common.cuh"
+#include "attn_rows.cuh"
 
 namespace kern {
-
-constexpr float kUnset = -1e30f;     // a reference before its first score
-constexpr float kOutgrown = 32768.f; // the weight at which references move: f16 holds twice that
-
-struct RowsArgs {
-  const __nv_bfloat16* q;
-  __nv_bfloat16* out;
-  float* ws_o;               // partials [row][head][groups][D] (one group: none)
-  float* ws_ml;              // [row][head][groups][2]
-  const uint8_t* pool;       // (8-bit) scale bytes are read from here
-  const int* block_table;
-  const int* seq_lens;
-  const int* cu_q;
-  const long long* masks;    // (tree) [row][words]
-  int* err;
-  int words, rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, cluster, pool_pages;
-  float scale_log2;
-};
 
 // D, cache format, NT: columns of query rows in eights
 template <int D, bool E4M3, int NT>
@@ -95,21 +75,6 @@ KERN_DEVICE uint32_t lds8(uint32_t a) {
   uint32_t v;
   asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a));
   return v;
-}
-// four e4m3 codes -> two pairs of f16, exact
-KERN_DEVICE void codes_f16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-      : "=r"(lo), "=r"(hi)
-      : "r"(w));
-}
-KERN_DEVICE uint32_t pack_f16x2(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <bool F16>
-KERN_DEVICE uint32_t pack_pair(float lo, float hi) {
-  if constexpr (F16) return pack_f16x2(lo, hi);
-  else return pack_bf16x2(lo, hi);
 }
 template <bool F16>
 KERN_DEVICE void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -157,23 +122,6 @@ KERN_DEVICE float4 ld_rank4(uint32_t a) {
 KERN_DEVICE void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
-
-// of the two 16-bit (f16 or bf16) halves of w: all ones where the half is not finite
-template <bool F16>
-KERN_DEVICE uint32_t not_finite(uint32_t w) {
-  constexpr uint32_t lo = F16 ? 0x7c00u : 0x7f80u;
-  uint32_t r = 0;
-  if ((w & lo) == lo) r |= 0xffffu;
-  if ((w & (lo << 16)) == (lo << 16)) r |= 0xffff0000u;
-  return r;
-}
-
-KERN_DEVICE float pow2i(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
-
-// A context is dealt out in runs of whole 128-token units: how many shares `end` tokens are cut into, and the tokens
-// of each.
-KERN_DEVICE int rows_shares(int end, int splits) { return min(splits, max(1, (end + 127) / 128)); }
-KERN_DEVICE int rows_share_len(int end, int shares) { return ((end + 127) / 128 + shares - 1) / shares * 128; }
 
 template <int D, bool E4M3, bool TREE, int NT>
 KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {

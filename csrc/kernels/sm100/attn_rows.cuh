@@ -1,0 +1,60 @@
+// What the kernels of attention over a cache in either format share (attn_rows.cu: few query rows, attn_tile.cu: many): their
+// arguments, conversions, and how a context is dealt out.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace kern {
+
+constexpr float kUnset = -1e30f;     // a reference before its first score
+constexpr float kOutgrown = 32768.f; // the weight at which references move: f16 holds twice that
+
+struct RowsArgs {
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;
+  float* ws_o;               // partials [row][head][groups][D] (one group: none)
+  float* ws_ml;              // [row][head][groups][2]
+  const uint8_t* pool;       // (8-bit) scale bytes are read from here
+  const int* block_table;
+  const int* seq_lens;
+  const int* cu_q;
+  const long long* masks;    // (tree) [row][words]
+  int* err;
+  int words, rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, cluster, pool_pages;
+  float scale_log2;
+};
+
+// four e4m3 codes -> two pairs of f16, exact
+KERN_DEVICE void codes_f16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
+KERN_DEVICE uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <bool F16>
+KERN_DEVICE uint32_t pack_pair(float lo, float hi) {
+  if constexpr (F16) return pack_f16x2(lo, hi);
+  else return pack_bf16x2(lo, hi);
+}
+// of the two 16-bit (f16 or bf16) halves of w: all ones where the half is not finite
+template <bool F16>
+KERN_DEVICE uint32_t not_finite(uint32_t w) {
+  constexpr uint32_t lo = F16 ? 0x7c00u : 0x7f80u;
+  uint32_t r = 0;
+  if ((w & lo) == lo) r |= 0xffffu;
+  if ((w & (lo << 16)) == (lo << 16)) r |= 0xffff0000u;
+  return r;
+}
+
+KERN_DEVICE float pow2i(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
+
+// A context is dealt out in runs of whole 128-token units: how many shares `end` tokens are cut into, and the tokens
+// of each.
+KERN_DEVICE int rows_shares(int end, int splits) { return min(splits, max(1, (end + 127) / 128)); }
+KERN_DEVICE int rows_share_len(int end, int shares) { return ((end + 127) / 128 + shares - 1) / shares * 128; }
+
+}  // namespace kern

@@ -1,0 +1,698 @@
+// Attention of many query rows over a paged cache, bf16 or e4m3, on the 5th-generation tensor cores: prompt chunks (causal) and
+// trees of drafted tokens. The formulas, formats and what a row sees are those of attn_rows.cu, which has the few rows.
+//
+// One CTA = (256 query rows: the G heads of 256 / G tokens, one kv head, a share of the context), 16 warps:
+//
+//   warps 0..3, 4..7   softmax of one 128-row tile each, a thread to a row: scores out of TMEM, weights back into TMEM over them
+//   warps 8..11        bring key and value tiles of 128 tokens into shared memory, two stages of each. 8-bit codes come by plain
+//                      loads one tile ahead, become f16 and are stored in the swizzle that the tensor cores read; bf16 tiles come
+//                      by TMA, and only tiles in which rows see different tokens are looked through
+//   warp 12            issues the products:  S = Q K^T  and  O += P V  (P from TMEM), for the two tiles in turn
+//
+// The two tiles take turns on the tensor cores: while one's products run, the other's exponentials do. At most 128 rows (a small
+// tree): both tiles are the same rows, on alternate key tiles, and are added up at the end, so the turns remain. TMEM: S and O of
+// both tiles, 512 columns; P overwrites S.
+//
+// Bound: 2 * 128 * 128 * D multiply-adds a tile and side on 4096 a clock against 128 * 128 exponentials on 16 a clock, which at
+// D = 128 take as long as each other: the softmax is kept to a handful of instructions a score. The reference R of a row moves only
+// when a weight has outgrown it by 2^15 (found on the packed halves, one instruction for two), so one pass over the scores does:
+// scale and shift, exponential, sum, pack. No pass over O but then.
+//
+// 8-bit: a tile's rows are brought to one exponent, E = the largest of its scale bytes, as they become f16 (exact down to 2^-21 of
+// the tile's largest row, and to 2^-25 of one step beyond); 2^E of the keys is then part of the scores' scale, E of the values part
+// of the weights' exponent, w_ij = 2^(s_ij + E_t - R_i): no work per score.
+#include "attn_rows.cuh"
+
+namespace kern {
+
+constexpr int kQ = 128, kT = 128;    // query rows of a tile, tokens of a tile
+constexpr int kTileThreads = 512;
+
+template <int D>
+struct TileCfg {
+  static constexpr int kQBytes = 2 * kQ * D * 2;
+  static constexpr int kHalf = kT * D * 2;                  // a tile of K or of V
+  static constexpr int kRing = 4 * kHalf;                   // two stages of each
+  static constexpr int kSmem = 1024 + kQBytes + kRing + 2 * kQ * 4 + 512;
+};
+
+// Shared-memory descriptor of an MN-major operand tile with the 128-byte swizzle: rows are the contraction's (tokens), 128 bytes =
+// 64 columns each; the next 64 columns are `block_bytes` further on.
+KERN_DEVICE uint64_t tile_desc_mn(uint32_t smem_addr, uint32_t block_bytes) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
+  d |= (uint64_t)((block_bytes >> 4) & 0x3FFF) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+// kind::f16 with f32 sums: 16-bit operands, f16 or bf16
+template <bool F16>
+KERN_DEVICE constexpr uint32_t tile_idesc(int m, int n, bool b_mn) {
+  return (1u << 4) | ((F16 ? 0u : 1u) << 7) | ((F16 ? 0u : 1u) << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// D[tmem] (+)= A[tmem] * B[smem]; one thread
+KERN_DEVICE void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+KERN_DEVICE void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+KERN_DEVICE void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <bool F16>
+KERN_DEVICE uint32_t max_pair(uint32_t a, uint32_t b) {
+  if constexpr (F16) {
+    const __half2 v = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+template <bool F16>
+KERN_DEVICE float larger_half(uint32_t a) {
+  if constexpr (F16) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
+    return fmaxf(f.x, f.y);
+  } else {
+    const float2 f = unpack_bf16x2(a);
+    return fmaxf(f.x, f.y);
+  }
+}
+KERN_DEVICE uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// 2^x as f16, 0 below its range
+KERN_DEVICE uint32_t pow2_f16(int x) { return x >= -14 ? (uint32_t)(x + 15) << 10 : (x >= -24 ? 1u << (x + 24) : 0u); }
+
+// D, cache format, tree or causal
+template <int D, bool E4M3, bool TREE>
+KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const int seqs) {
+  using Cfg = TileCfg<D>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_s = smem;                                        // two tiles, D / 64 column blocks of [128 rows][128 bytes] each
+  uint8_t* k_s = q_s + Cfg::kQBytes;                          // [2 stages]
+  uint8_t* v_s = k_s + 2 * Cfg::kHalf;
+  float* f_s = reinterpret_cast<float*>(v_s + 2 * Cfg::kHalf);// [256] what turns a row's products into base-2 scores
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(f_s + 2 * kQ);
+  uint64_t* v_full = k_full + 2;
+  uint64_t* k_empty = v_full + 2;
+  uint64_t* v_empty = k_empty + 2;
+  uint64_t* k_came = v_empty + 2;                             // (bf16) TMA done
+  uint64_t* v_came = k_came + 2;
+  uint64_t* s_full = v_came + 2;                              // per tile of rows: scores in TMEM,
+  uint64_t* p_full = s_full + 2;                              // weights in TMEM,
+  uint64_t* o_done = p_full + 2;                              // P V done
+  float2* e_s = reinterpret_cast<float2*>(o_done + 2);        // [4] a key tile's (2^E of K, E of V)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(e_s + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* found = reinterpret_cast<int*>(tmem_slot + 2);         // [2] sequence and block of this CTA
+  volatile int* bad_s = found + 2;                            // a value that is not finite in a tile whose rows see different tokens
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = a.hq / a.hk, kvh = blockIdx.x, toks = 2 * kQ / G;
+  pdl_wait();
+  if (warp == 0) {
+    // block y of the call: blocks are counted through the sequences
+    int base = 0, sq = -1, bk = 0;
+    for (int s0 = 0; s0 < seqs && sq < 0; s0 += 32) {
+      const int s = s0 + lane;
+      int rows = 0;
+      if (s < seqs) rows = a.cu_q ? a.cu_q[s + 1] - a.cu_q[s] : a.rows_per_seq;
+      int n = rows > 0 ? (rows + toks - 1) / toks : 0;
+      const int own = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, n, d);
+        if (lane >= d) n += up;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, (int)blockIdx.y < base + n);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        sq = s0 + l;
+        const int upto = __shfl_sync(0xffffffffu, n, l), mine = __shfl_sync(0xffffffffu, own, l);
+        bk = (int)blockIdx.y - (base + upto - mine);
+        if (!TREE) bk = mine - 1 - bk;                        // causal: the longest walks first
+      }
+      base += __shfl_sync(0xffffffffu, n, 31);
+    }
+    if (lane == 0) {
+      found[0] = sq;
+      found[1] = bk;
+    }
+  }
+  if (threadIdx.x == 32) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&k_full[s], 128); mbar_init(&v_full[s], 128);
+      mbar_init(&k_empty[s], 1); mbar_init(&v_empty[s], 1);
+      mbar_init(&k_came[s], 1); mbar_init(&v_came[s], 1);
+      mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 128); mbar_init(&o_done[s], 1);
+    }
+    *abort_flag = 0;
+    *bad_s = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(kv_map);
+  }
+  __syncthreads();
+  const int seq = found[0], blk = found[1];
+  if (seq < 0) return;                                        // past the last block: uniform, before any allocation
+  const int L = max(a.seq_lens[seq], 0);
+  const int row0 = a.cu_q ? a.cu_q[seq] : seq * a.rows_per_seq;
+  const int R = a.cu_q ? a.cu_q[seq + 1] - row0 : a.rows_per_seq;
+  const int tok_lo = blk * toks, tok_n = min(toks, R - tok_lo), valid = tok_n * G, past = L - R;
+  const int end = TREE ? L : max(0, past + tok_lo + tok_n);
+  const int shares = rows_shares(end, gridDim.z), share_len = rows_share_len(end, shares);
+  if ((int)blockIdx.z >= shares) return;
+  const int from = min(end, (int)blockIdx.z * share_len), to = min(end, from + share_len);
+  const int ntiles = (to - from + kT - 1) / kT;
+  const bool twice = valid <= kQ;                             // both tiles are the same rows, on alternate key tiles
+  const int clear = min(to, TREE ? past : past + tok_lo + 1); // the first token that some row may not see
+
+  if (warp == 12) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  // ---- Q -> shared memory, K-major with the 128-byte swizzle: D / 8 lanes to a row ----
+  {
+    constexpr int kLanes = D / 8;
+    const int c = threadIdx.x % kLanes;
+#pragma unroll 2
+    for (int r = threadIdx.x / kLanes; r < 2 * kQ; r += kTileThreads / kLanes) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      const int rr = twice ? r & (kQ - 1) : r;
+      if (rr < valid) v = *reinterpret_cast<const uint4*>(a.q + (size_t)(row0 + tok_lo + rr / G) * a.q_stride + (size_t)(kvh * G + rr % G) * D + c * 8);
+      float f = a.scale_log2;
+      if constexpr (E4M3) {
+        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 u = unpack_bf16x2(w[i]);
+          top = fmaxf(top, fmaxf(fabsf(u.x), fabsf(u.y)));
+        }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int x = min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100), 100);
+        const float inv = pow2i(-x);
+        f *= pow2i(x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 u = unpack_bf16x2(w[i]);
+          w[i] = pack_f16x2(u.x * inv, u.y * inv);
+        }
+        v = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      *reinterpret_cast<uint4*>(q_s + (r >> 7) * (kQ * D * 2) + (c >> 3) * (kQ * 128) + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+      if (c == 0) f_s[r] = f;
+    }
+  }
+  fence_proxy_async();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  bool ok = true;
+
+  if (warp >= 8 && warp < 12) {
+    // ---------------- keys and values ----------------
+    const int tid = threadIdx.x - 256, w4 = warp - 8;
+    const int* pages = a.block_table + (size_t)seq * a.max_pages;
+    const int bits = a.page_size < 64 ? 31 - __clz(a.page_size) : 6, per = a.page_size < 64 ? 1 : a.page_size >> 6;
+    // page and row in it of a token (runs of 2^bits tokens lie in one page)
+    auto place = [&](int tok, int& page, int& off) {
+      const int u = tok >> bits, pi = per == 1 ? u : u / per;
+      off = ((u - pi * per) << bits) + (tok & ((1 << bits) - 1));
+      page = pi < a.max_pages ? pages[pi] : -1;
+      if (page < 0 || page >= a.pool_pages) {
+        set_error(a.err, ERR_BOUNDS);
+        page = 0;
+      }
+    };
+    // the order of the halves: K(0), then K(t + 1) before V(t)
+    const int items = 2 * ntiles;
+    auto item = [&](int i, int& which, int& t) {
+      which = i == items - 1 ? 1 : (i == 0 ? 0 : !(i & 1));
+      t = i == items - 1 ? ntiles - 1 : (i == 0 ? 0 : (which ? i / 2 - 1 : (i + 1) / 2));
+    };
+    auto half_free = [&](int which, int t) -> bool {
+      if (mbar_wait_ns(which ? &v_empty[t & 1] : &k_empty[t & 1], ((t >> 1) & 1) ^ 1, abort_flag)) return true;
+      set_error(a.err, ERR_WAIT_EMPTY);
+      *abort_flag = 1;
+      return false;
+    };
+    if constexpr (E4M3) {
+      constexpr int kLanes = D / 16, kRowsWarp = 32 / kLanes, kLoads = kT / (4 * kRowsWarp);     // lanes to a row of codes
+      const int c = lane % kLanes, sub = lane / kLanes;
+      const size_t codes = (size_t)2 * a.hk * a.page_size * D, page_bytes = codes + 2 * a.hk * a.page_size;
+      // the scale bytes of a tile's tokens 4 lane .. 4 lane + 3; those of tokens behind the end are 0
+      auto scale_word = [&](int which, int tok0) -> uint32_t {
+        const int tok = tok0 + 4 * lane;
+        if (tok >= to) return 0;
+        int page, off;
+        place(tok, page, off);
+        const uint8_t* src = a.pool + (size_t)page * page_bytes + codes + (size_t)(which * a.hk + kvh) * a.page_size + off;
+        uint32_t w = KERN_CHECK(src, 4, SITE_KV_ROW) ? *reinterpret_cast<const uint32_t*>(src) : 0;
+        if (to - tok < 4) w &= (1u << (8 * (to - tok))) - 1;
+        return w;
+      };
+      auto top_byte = [&](uint32_t w) -> int {
+        const uint32_t m = __vmaxu4(w, w >> 16);
+        return (int)__reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u));
+      };
+      struct Codes {
+        uint4 v[kLoads];
+        uint32_t scale, vscale;
+      };
+      auto fetch = [&](int i, Codes& x) {
+        int which, t;
+        item(i, which, t);
+        const int tok0 = from + t * kT;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          const int tok = tok0 + j * 4 * kRowsWarp + w4 * kRowsWarp + sub;
+          x.v[j] = make_uint4(0, 0, 0, 0);
+          if (tok < to) {
+            int page, off;
+            place(tok, page, off);
+            const uint8_t* src = a.pool + (size_t)page * page_bytes + ((size_t)(which * a.hk + kvh) * a.page_size + off) * D + c * 16;
+            if (KERN_CHECK(src, 16, SITE_KV_ROW)) x.v[j] = *reinterpret_cast<const uint4*>(src);
+          }
+        }
+        x.scale = scale_word(which, tok0);
+        x.vscale = which ? 0 : scale_word(1, tok0);
+      };
+      auto put = [&](int i, const Codes& x) -> bool {
+        int which, t;
+        item(i, which, t);
+        if (!half_free(which, t)) return false;
+        const int tok0 = from + t * kT, top = top_byte(x.scale);
+        const bool edge = tok0 + kT > clear;
+        uint8_t* dst = (which ? v_s : k_s) + (t & 1) * Cfg::kHalf;
+        bool nan = false;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          const int r = j * 4 * kRowsWarp + w4 * kRowsWarp + sub;
+          const uint32_t word = __shfl_sync(0xffffffffu, x.scale, r >> 2);
+          const uint32_t f = pow2_f16((int)((word >> (8 * (r & 3))) & 255u) - top + 6) * 0x10001u;
+          uint32_t w[4] = {x.v[j].x, x.v[j].y, x.v[j].z, x.v[j].w}, o[8];
+          if (which && edge) {
+            // values that are not finite stay out of the product: rows that see them get them at the end
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t m = __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              nan |= m != 0;
+              w[k] &= ~m;
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            codes_f16x4(w[k], o[2 * k], o[2 * k + 1]);
+            o[2 * k] = mul_f16x2(o[2 * k], f);
+            o[2 * k + 1] = mul_f16x2(o[2 * k + 1], f);
+          }
+          // 16 values: two pieces of the row; lanes of the second half of the row store theirs the other way round, since their
+          // column block lies on the same banks
+          const int p0 = 2 * c, flip = (c >> 2) & 1;
+          uint8_t* row = dst + (p0 >> 3) * (kT * 128) + r * 128;
+          const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+          *reinterpret_cast<uint4*>(row + ((((p0 + flip) & 7) ^ (r & 7)) << 4)) = flip ? hi : lo;
+          *reinterpret_cast<uint4*>(row + ((((p0 + 1 - flip) & 7) ^ (r & 7)) << 4)) = flip ? lo : hi;
+        }
+        if (nan) *bad_s = 1;
+        if (!which) {
+          const int vtop = top_byte(x.vscale);
+          if (tid == 0) e_s[t & 3] = make_float2(pow2i(top - 127 - 6), (float)(vtop - 127 - 6));
+        }
+        fence_proxy_async();
+        mbar_arrive(which ? &v_full[t & 1] : &k_full[t & 1]);
+        return true;
+      };
+      Codes x, y;
+      if (items > 0) fetch(0, x);
+      for (int i = 0; i < items && ok; i += 2) {              // (items is even)
+        fetch(i + 1, y);
+        ok = put(i, x);
+        if (!ok) break;
+        if (i + 2 < items) fetch(i + 2, x);
+        ok = put(i + 1, y);
+      }
+    } else {
+      const int box = a.page_size < 64 ? a.page_size : 64;
+      auto bring = [&](int i) -> bool {                       // warp 8: a half by TMA, boxes up to the share's end
+        int which, t;
+        item(i, which, t);
+        if (!half_free(which, t)) return false;
+        const int tok0 = from + t * kT, boxes = (min(kT, to - tok0) + box - 1) / box;
+        uint64_t* bar = which ? &v_came[t & 1] : &k_came[t & 1];
+        uint8_t* dst = (which ? v_s : k_s) + (t & 1) * Cfg::kHalf;
+        if (lane == 0) mbar_expect_tx(bar, boxes * box * D * 2);
+        __syncwarp();
+        if (lane < boxes) {
+          int page, off;
+          place(tok0 + lane * box, page, off);
+#pragma unroll
+          for (int cb = 0; cb < D / 64; ++cb)
+            tma_load_3d(dst + cb * (kT * 128) + lane * box * 128, kv_map, cb * 64, (which * a.hk + kvh) * a.page_size + off, page, bar);
+        }
+        return true;
+      };
+      const int ahead = min(items, 3);                        // K(0), K(1), V(0) fill what is free at the start
+      if (w4 == 0)
+        for (int i = 0; i < ahead && ok; ++i) ok = bring(i);
+      for (int i = 0; i < items && ok; ++i) {
+        int which, t;
+        item(i, which, t);
+        if (!mbar_wait_ns(which ? &v_came[t & 1] : &k_came[t & 1], (t >> 1) & 1, abort_flag)) {
+          set_error(a.err, ERR_WAIT_FULL);
+          *abort_flag = 1;
+          ok = false;
+          break;
+        }
+        const int tok0 = from + t * kT;
+        if (which && tok0 + kT > clear) {
+          uint8_t* dst = v_s + (t & 1) * Cfg::kHalf;
+          bool bad = false;
+          for (int x = tid; x < kT * (D / 8); x += 128) {
+            const int r = x / (D / 8), p = x % (D / 8);
+            uint4* at = reinterpret_cast<uint4*>(dst + (p >> 3) * (kT * 128) + r * 128 + (((p & 7) ^ (r & 7)) << 4));
+            if (tok0 + r >= to) {
+              *at = make_uint4(0, 0, 0, 0);
+            } else {
+              uint4 v = *at;
+              const uint32_t m0 = not_finite<false>(v.x), m1 = not_finite<false>(v.y), m2 = not_finite<false>(v.z), m3 = not_finite<false>(v.w);
+              if (m0 | m1 | m2 | m3) {
+                bad = true;
+                *at = make_uint4(v.x & ~m0, v.y & ~m1, v.z & ~m2, v.w & ~m3);
+              }
+            }
+          }
+          if (bad) *bad_s = 1;
+          fence_proxy_async();
+        }
+        mbar_arrive(which ? &v_full[t & 1] : &k_full[t & 1]);
+        if (w4 == 0 && i + ahead < items) ok = bring(i + ahead);
+      }
+    }
+  } else if (warp == 12) {
+    // ---------------- products ----------------
+    if (lane == 0) {
+      constexpr uint32_t idesc_qk = tile_idesc<E4M3>(kQ, kT, false), idesc_pv = tile_idesc<E4M3>(kQ, D, true);
+      const int steps = twice ? ntiles : 2 * ntiles;
+      auto qk = [&](int u) -> bool {
+        const int side = u & 1, t = twice ? u : u >> 1;
+        if (!mbar_wait_ns(&k_full[t & 1], (t >> 1) & 1, abort_flag)) return false;
+        tc_fence_after();
+        const uint32_t sq = smem_u32(q_s) + side * (kQ * D * 2), sk = smem_u32(k_s) + (t & 1) * Cfg::kHalf;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          umma_bf16(tmem + side * 128, umma_desc_sw128(sq + (k >> 2) * (kQ * 128) + (k & 3) * 32), umma_desc_sw128(sk + (k >> 2) * (kT * 128) + (k & 3) * 32),
+                    idesc_qk, k != 0);
+        tc_commit(&s_full[side]);
+        if (twice || side) tc_commit(&k_empty[t & 1]);
+        return true;
+      };
+      auto pv = [&](int u) -> bool {
+        const int side = u & 1, t = twice ? u : u >> 1, n = u >> 1;
+        if (!mbar_wait_ns(&v_full[t & 1], (t >> 1) & 1, abort_flag)) return false;
+        if (!mbar_wait_ns(&p_full[side], n & 1, abort_flag)) return false;
+        tc_fence_after();
+        const uint32_t sv = smem_u32(v_s) + (t & 1) * Cfg::kHalf;
+#pragma unroll
+        for (int k = 0; k < kT / 16; ++k)
+          umma_ts(tmem + 256 + side * D, tmem + side * 128 + k * 8, tile_desc_mn(sv + k * 16 * 128, kT * 128), idesc_pv, (n | k) != 0);
+        tc_commit(&o_done[side]);
+        if (twice || side) tc_commit(&v_empty[t & 1]);
+        return true;
+      };
+      if (steps > 0) ok = qk(0);
+      if (ok && steps > 1) ok = qk(1);
+      for (int u = 0; u < steps && ok; ++u) {
+        ok = pv(u);
+        if (ok && u + 2 < steps) ok = qk(u + 2);              // (overwrites the scores whose weights P V has just been given)
+      }
+      if (!ok) {
+        set_error(a.err, ERR_WAIT_FULL);
+        *abort_flag = 1;
+      }
+    }
+    __syncwarp();
+  } else if (warp < 8) {
+    // ---------------- softmax: a thread to a row ----------------
+    const int side = warp >> 2, row = (warp & 3) * 32 + lane;
+    const int r = twice ? row : side * kQ + row;              // of the block's rows
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_t = tmem + lanes + side * 128, o_t = tmem + lanes + 256 + side * D;
+    const int tk = tok_lo + (r < valid ? r / G : 0), pos = past + tk;
+    const long long* mask = TREE ? a.masks + (size_t)(row0 + tk) * a.words : nullptr;
+    const int steps = twice ? (ntiles + 1 - side) / 2 : ntiles;
+    const float f = f_s[side * kQ + row];
+    float ref = kUnset, l = 0.f;
+    // which of tokens j .. j + 31 the row sees
+    auto seen32 = [&](int j) -> uint32_t {
+      uint32_t b;
+      auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
+      if constexpr (TREE) {
+        b = below(past - j);
+        const int n0 = j - past;                              // the node of bit 0 (negative: the context's last tokens before it)
+        for (int w = max(n0 >> 6, 0); w <= (n0 + 31) >> 6 && w < a.words && n0 + 31 >= 0; ++w) {
+          const unsigned long long m = (unsigned long long)mask[w];
+          const int sh = n0 - w * 64;
+          b |= sh >= 0 ? (uint32_t)(m >> sh) : (uint32_t)((m & 0xffffffffull) << -sh);
+        }
+      } else {
+        b = below(pos + 1 - j);
+      }
+      return b & below(to - j);
+    };
+    for (int n = 0; n < steps && ok; ++n) {
+      const int t = twice ? 2 * n + side : n;
+      const int tok0 = from + t * kT;
+      if (!mbar_wait_ns(&s_full[side], n & 1, abort_flag)) {
+        set_error(a.err, ERR_WAIT_TMEM_FULL);
+        *abort_flag = 1;
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const bool edge = tok0 + kT > clear;                    // uniform
+      float scale = f, ev = 0.f;
+      if constexpr (E4M3) {
+        const float2 e = e_s[t & 3];
+        scale *= e.x;
+        ev = e.y;
+      }
+      uint32_t pk[64];
+      float sum[2];
+      auto weigh = [&](float shift) -> float {
+        sum[0] = sum[1] = 0.f;
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[32];
+          tmem_ld_32x32(s_t + c * 32, x);
+          tmem_ld_wait();
+          if (edge) {
+            const uint32_t b = seen32(tok0 + c * 32);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(b >> i & 1)) x[i] = 0xff800000u;          // -inf
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float u = exp2f(fmaf(__uint_as_float(x[2 * i]), scale, -shift)), v = exp2f(fmaf(__uint_as_float(x[2 * i + 1]), scale, -shift));
+            sum[0] += u;
+            sum[1] += v;
+            pk[c * 16 + i] = pack_pair<E4M3>(u, v);
+            top = max_pair<E4M3>(top, pk[c * 16 + i]);
+          }
+        }
+        return larger_half<E4M3>(top);
+      };
+      if (__any_sync(0xffffffffu, weigh(ref - ev) > kOutgrown)) {
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[32];
+          tmem_ld_32x32(s_t + c * 32, x);
+          tmem_ld_wait();
+          const uint32_t b = edge ? seen32(tok0 + c * 32) : 0xffffffffu;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (b >> i & 1) mx = fmaxf(mx, __uint_as_float(x[i]));
+        }
+        const float to_ref = fmaxf(ref, ceilf(mx * scale + ev) - 7.f), corr = exp2f(ref - to_ref);
+        ref = to_ref;
+        l *= corr;
+        if (n > 0) {
+          if (!mbar_wait_ns(&o_done[side], (n - 1) & 1, abort_flag)) {
+            set_error(a.err, ERR_WAIT_TMEM_EMPTY);
+            *abort_flag = 1;
+            ok = false;
+          }
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t x[32];
+            tmem_ld_32x32(o_t + c * 32, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * corr);
+            tmem_st32(o_t + c * 32, x);
+          }
+          tmem_st_done();
+        }
+        weigh(ref - ev);
+      }
+      l += E4M3 ? (sum[0] + sum[1]) * exp2f(-ev) : sum[0] + sum[1];
+      tmem_st32(s_t, pk);
+      tmem_st32(s_t + 32, pk + 32);
+      tmem_st_done();
+      tc_fence_before();
+      mbar_arrive(&p_full[side]);
+    }
+    if (ok && steps > 0 && !mbar_wait_ns(&o_done[side], (steps - 1) & 1, abort_flag)) {
+      set_error(a.err, ERR_WAIT_TMEM_FULL);
+      *abort_flag = 1;
+      ok = false;
+    }
+    tc_fence_after();
+    // ---------------- the rows' end ----------------
+    float* other = reinterpret_cast<float*>(k_s);             // (twice) the second side's rows: [128][D + 3]
+    if (twice) {
+      asm volatile("bar.sync 1, 256;" ::: "memory");          // both sides' products are done: the ring is free
+      if (side == 1) {
+        float* mine = other + row * (D + 3);
+        mine[D] = ref;
+        mine[D + 1] = l;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t x[32];
+          tmem_ld_32x32(o_t + c * 32, x);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mine[c * 32 + i] = steps > 0 ? __uint_as_float(x[i]) : 0.f;
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    if (!(twice && side)) {
+      float own = 1.f, his = 0.f, m = ref;
+      if (twice) {
+        const float* x = other + row * (D + 3);
+        m = fmaxf(ref, x[D]);
+        own = l == 0.f ? 0.f : exp2f(ref - m);
+        his = x[D + 1] == 0.f ? 0.f : exp2f(x[D] - m);
+        l = (l == 0.f ? 0.f : l * own) + (x[D + 1] == 0.f ? 0.f : x[D + 1] * his);
+      }
+      const bool whole = shares == 1, store = r < valid && ok;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int head = kvh * G + (r < valid ? r % G : 0);
+      const size_t at = ((size_t)(row0 + tk) * a.hq + head) * gridDim.z + blockIdx.z;
+      const bool bad = *bad_s != 0;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t x[32];
+        float y[32];
+        tmem_ld_32x32(o_t + c * 32, x);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) y[i] = own != 0.f && steps > 0 ? __uint_as_float(x[i]) * own : 0.f;
+        if (twice && his != 0.f) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) y[i] += other[row * (D + 3) + c * 32 + i] * his;
+        }
+        if (bad && store) {
+          // infinities and NaN that this row sees in the tiles that were looked through, from the cache itself
+#pragma unroll 1
+          for (int j = from + max(clear - from, 0) / kT * kT; j < to; ++j) {
+            if (!(seen32(j) & 1u)) continue;
+            const int pi = j / a.page_size, off = j - pi * a.page_size;
+            int page = pi < a.max_pages ? a.block_table[(size_t)seq * a.max_pages + pi] : 0;
+            if (page < 0 || page >= a.pool_pages) page = 0;
+            const size_t v_row = (size_t)(a.hk + kvh) * a.page_size + off;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if constexpr (E4M3) {
+                const uint8_t code = a.pool[(size_t)page * (2 * a.hk * a.page_size * (size_t)(D + 1)) + v_row * D + c * 32 + i];
+                if ((code & 0x7f) == 0x7f) y[i] = __uint_as_float(0x7fffffffu);
+              } else {
+                const uint16_t w = reinterpret_cast<const uint16_t*>(a.pool)[(size_t)page * (2 * a.hk * a.page_size * (size_t)D) + v_row * D + c * 32 + i];
+                if ((w & 0x7f80u) == 0x7f80u) y[i] += __uint_as_float((uint32_t)w << 16);
+              }
+            }
+          }
+        }
+        if (!store) continue;
+        if (whole) {
+          __nv_bfloat16* dst = a.out + (size_t)(row0 + tk) * a.out_stride + (size_t)head * D + c * 32;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(dst + i * 8) =
+                make_uint4(pack_bf16x2(y[8 * i] * inv, y[8 * i + 1] * inv), pack_bf16x2(y[8 * i + 2] * inv, y[8 * i + 3] * inv),
+                           pack_bf16x2(y[8 * i + 4] * inv, y[8 * i + 5] * inv), pack_bf16x2(y[8 * i + 6] * inv, y[8 * i + 7] * inv));
+        } else {
+          float4* dst = reinterpret_cast<float4*>(a.ws_o + at * D + c * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dst[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+        }
+      }
+      if (!whole && store) {
+        a.ws_ml[at * 2] = m;
+        a.ws_ml[at * 2 + 1] = l;
+      }
+    }
+  }
+
+  // ---------------- teardown ----------------
+  pdl_launch_dependents();
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0) {
+    const uint64_t t0 = globaltimer_ns();       // let copies and products in flight end before the memory goes away
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+  }
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace kern
+
+using namespace kern;
+
+#define KERN_TILE_ENTRY(D, KIND, E4M3, FORM, TREE)                                                                                \
+  extern "C" __global__ void __launch_bounds__(kTileThreads, 1) kern_attn_tile_##KIND##_##FORM##_d##D(                            \
+      const __grid_constant__ CUtensorMap kv_map, const __nv_bfloat16* q, __nv_bfloat16* out, float* ws_o, float* ws_ml,          \
+      const uint8_t* pool, const int* block_table, const int* seq_lens, const int* cu_q, const long long* masks, int words,       \
+      int rows_per_seq, int hq, int hk, int q_stride, int out_stride, int max_pages, int page_size, int seqs, int pool_pages,     \
+      float scale_log2, int* err) {                                                                                               \
+    tile_body<D, E4M3, TREE>(&kv_map, RowsArgs{q, out, ws_o, ws_ml, pool, block_table, seq_lens, cu_q, masks, err, words,         \
+                                               rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, 1, pool_pages,   \
+                                               scale_log2},                                                                       \
+                             seqs);                                                                                               \
+  }
+#define KERN_TILE(D)                            \
+  KERN_TILE_ENTRY(D, e4m3, true, causal, false) \
+  KERN_TILE_ENTRY(D, e4m3, true, tree, true)    \
+  KERN_TILE_ENTRY(D, bf16, false, tree, true)
+KERN_TILE(64)
+KERN_TILE(128)

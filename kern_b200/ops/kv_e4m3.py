@@ -196,6 +196,19 @@ def rows_shares(ctas: int, max_len: int, resident: int) -> tuple[int, int]:
     return want // cluster * cluster, cluster
 
 
+# query rows of a sequence and kv head above which the tensor-core kernel runs (head_dim 64 and 128)
+TILE_ROWS = 32
+
+
+def tile_smem(d: int) -> int:
+    """Dynamic shared memory of the many-row kernel: two tiles of Q, two stages of K and of V as 16-bit values, barriers."""
+    return 1024 + 2 * 128 * d * 2 + 4 * 128 * d * 2 + 1024 + 512
+
+
+def tile_shares(ctas: int, max_len: int, sms: int) -> int:
+    return max(1, min(-(-3 * sms // ctas), -(-max_len // 512), 64)) if ctas < 3 * sms else 1
+
+
 def pool_map(k: Kernels, pool: torch.Tensor, e4m3: bool, pages: int, hk: int, d: int, page_size: int) -> bytes:
     """3-D descriptor over a pool of either format: (value, row of a page's k | v x head x token, page)."""
     es = 1 if e4m3 else 2
@@ -211,12 +224,20 @@ def attention_rows(q, pool, pages, block_table, seq_lens, masks, cu_q, hq, hk, d
     e4m3 = pool.dtype == torch.uint8
     k = Kernels.get(gpu)
     g = hq // hk
-    # query rows of a CTA: the fewest eights that hold a sequence's, up to what registers hold
-    nt = 1 if g * max_rows <= 8 else 2 if g * max_rows <= 16 or d == 256 else 4
-    toks = 8 * nt // g
-    nblk = -(-max_rows // toks)
-    smem, per_sm = rows_form(d, e4m3, nt)
-    shares, cluster = rows_shares(hk * nblk * seqs, max_len, k.sm_count * per_sm)
+    tiled = g * max_rows > TILE_ROWS and d <= 128
+    if tiled:
+        entry, toks, cluster, threads, smem = "attn_tile", 256 // g, 1, 512, tile_smem(d)
+        nblk = min(n // toks + seqs, seqs * -(-max_rows // toks))          # blocks of all sequences, at most
+        shares = tile_shares(hk * nblk, max_len, k.sm_count)
+        gx, gy, last, name = hk, nblk, seqs, ""
+    else:
+        # query rows of a CTA: the fewest eights that hold a sequence's, up to what registers hold
+        nt = 1 if g * max_rows <= 8 else 2 if g * max_rows <= 16 or d == 256 else 4
+        toks, threads = 8 * nt // g, 160
+        nblk = -(-max_rows // toks)
+        smem, per_sm = rows_form(d, e4m3, nt)
+        shares, cluster = rows_shares(hk * nblk * seqs, max_len, k.sm_count * per_sm)
+        entry, gx, gy, last, name = "attn_rows", hk * nblk, seqs, cluster, f"_n{nt}"
     ws_o = ws_ml = 0
     if shares > cluster:
         parts = n * hq * (shares // cluster)
@@ -227,11 +248,10 @@ def attention_rows(q, pool, pages, block_table, seq_lens, masks, cu_q, hq, hk, d
     out_at, lens_at, cu_at = out.data_ptr(), seq_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr()
     image = _ROWS.pack(pool_map(k, pool, e4m3, pages, hk, d, page_size), q.data_ptr(), out_at, ws_o, ws_ml, pool.data_ptr(),
                        block_table.data_ptr(), lens_at, cu_at, 0 if masks is None else masks.data_ptr(),
-                       0 if masks is None else masks.shape[1], rows_per_seq, hq, hk, q_step, out_step, width, page_size, cluster, pages,
+                       0 if masks is None else masks.shape[1], rows_per_seq, hq, hk, q_step, out_step, width, page_size, last, pages,
                        scale * LOG2E, k.err_ptr)
     with on_device(q):
-        k.launch_image("attn_rows", f"kern_attn_rows_{'e4m3' if e4m3 else 'bf16'}_{form}_d{d}_n{nt}", hk * nblk, seqs, shares, 160, image, smem,
-                       False, cluster)
+        k.launch_image(entry, f"kern_{entry}_{'e4m3' if e4m3 else 'bf16'}_{form}_d{d}{name}", gx, gy, shares, threads, image, smem, False, cluster)
         if shares > cluster:
             image = _MERGE.pack(ws_o, ws_ml, out_at, lens_at, cu_at, rows_per_seq, hq, toks, shares, cluster, out_step)
             k.launch_image("attn_rows", f"kern_attn_rows_merge_{form}_d{d}", -(-max_rows * hq // 8), seqs, 1, 256, image, 0, True)
