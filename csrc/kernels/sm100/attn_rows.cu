@@ -221,7 +221,7 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
           off -= a.page_size;
         }
       };
-      if (!mbar_wait_ns(&empty_bar[stage], phase ^ 1, abort_flag)) {
+      if (!bar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) {
         set_error(a.err, ERR_WAIT_EMPTY);
         *abort_flag = 1;
         break;
@@ -349,7 +349,7 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
     int stage = 0;
     uint32_t phase = 0;
     for (int t = 0; t < ntiles; ++t) {
-      if (!mbar_wait_ns(&full_bar[stage], phase, abort_flag)) {
+      if (!bar_wait(&full_bar[stage], phase, abort_flag)) {
         set_error(a.err, ERR_WAIT_FULL);
         *abort_flag = 1;
         break;

@@ -25,6 +25,16 @@ struct RowsArgs {
   float scale_log2;
 };
 
+// A wait bounded by the SM's own clock (some 2 s), which is read in a few cycles.
+KERN_DEVICE bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (uint32_t i = 0;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 0x3f) == 0x3f && (*abort_flag != 0 || clock64() - t0 > 4000000000ll)) return false;
+  }
+}
+
 // four e4m3 codes -> two pairs of f16, exact
 KERN_DEVICE void codes_f16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"

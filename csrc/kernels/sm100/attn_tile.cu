@@ -4,10 +4,11 @@
 // One CTA = (256 query rows: the G heads of 256 / G tokens, one kv head, a share of the context), 16 warps:
 //
 //   warps 0..3, 4..7   softmax of one 128-row tile each, a thread to a row: scores out of TMEM, weights back into TMEM over them
-//   warps 8..11        bring key and value tiles of 128 tokens into shared memory, two stages of each. 8-bit codes come by plain
-//                      loads one tile ahead, become f16 and are stored in the swizzle that the tensor cores read; bf16 tiles come
-//                      by TMA, and only tiles in which rows see different tokens are looked through
+//   warps 8..11        key and value tiles of 128 tokens in shared memory, two stages of each. 8-bit codes become f16 there, in the
+//                      swizzle that the tensor cores read; bf16 tiles are brought by warp 8 as they are, by TMA, and only looked
+//                      through where rows see different tokens
 //   warp 12            issues the products:  S = Q K^T  and  O += P V  (P from TMEM), for the two tiles in turn
+//   warp 13            (8-bit) brings codes by TMA and scale bytes, two halves ahead
 //
 // The two tiles take turns on the tensor cores: while one's products run, the other's exponentials do. At most 128 rows (a small
 // tree): both tiles are the same rows, on alternate key tiles, and are added up at the end, so the turns remain. TMEM: S and O of
@@ -28,12 +29,13 @@ namespace kern {
 constexpr int kQ = 128, kT = 128;    // query rows of a tile, tokens of a tile
 constexpr int kTileThreads = 512;
 
-template <int D>
+template <int D, bool E4M3>
 struct TileCfg {
   static constexpr int kQBytes = 2 * kQ * D * 2;
   static constexpr int kHalf = kT * D * 2;                  // a tile of K or of V
   static constexpr int kRing = 4 * kHalf;                   // two stages of each
-  static constexpr int kSmem = 1024 + kQBytes + kRing + 2 * kQ * 4 + 512;
+  static constexpr int kCodes = E4M3 ? kT * D : 0;          // a half as codes, as it comes; two of them
+  static constexpr int kSmem = 1024 + kQBytes + kRing + 2 * kCodes + 2 * kQ * 4 + (E4M3 ? 512 : 0) + 512;
 };
 
 // Shared-memory descriptor of an MN-major operand tile with the 128-byte swizzle: rows are the contraction's (tokens), 128 bytes =
@@ -73,25 +75,68 @@ KERN_DEVICE void tmem_st32(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 KERN_DEVICE void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-template <bool F16>
-KERN_DEVICE uint32_t max_pair(uint32_t a, uint32_t b) {
-  if constexpr (F16) {
-    const __half2 v = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
+// 64 columns of this thread's TMEM lane
+KERN_DEVICE void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
 }
-template <bool F16>
-KERN_DEVICE float larger_half(uint32_t a) {
-  if constexpr (F16) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
-    return fmaxf(f.x, f.y);
-  } else {
-    const float2 f = unpack_bf16x2(a);
-    return fmaxf(f.x, f.y);
-  }
+KERN_DEVICE void tmem_st64(uint32_t taddr, const uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x64.b32 [%0], {"
+      "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, "
+      "%33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, "
+      "%49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, %64};"
+      ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+      "r"(r[32]), "r"(r[33]), "r"(r[34]), "r"(r[35]), "r"(r[36]), "r"(r[37]), "r"(r[38]), "r"(r[39]),
+      "r"(r[40]), "r"(r[41]), "r"(r[42]), "r"(r[43]), "r"(r[44]), "r"(r[45]), "r"(r[46]), "r"(r[47]),
+      "r"(r[48]), "r"(r[49]), "r"(r[50]), "r"(r[51]), "r"(r[52]), "r"(r[53]), "r"(r[54]), "r"(r[55]),
+      "r"(r[56]), "r"(r[57]), "r"(r[58]), "r"(r[59]), "r"(r[60]), "r"(r[61]), "r"(r[62]), "r"(r[63])
+      : "memory");
+}
+// two f32 in one register pair: one instruction for both
+KERN_DEVICE uint64_t pair64(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+KERN_DEVICE float2 split64(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+KERN_DEVICE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+KERN_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+KERN_DEVICE float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 KERN_DEVICE uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -104,19 +149,21 @@ KERN_DEVICE uint32_t pow2_f16(int x) { return x >= -14 ? (uint32_t)(x + 15) << 1
 // D, cache format, tree or causal
 template <int D, bool E4M3, bool TREE>
 KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const int seqs) {
-  using Cfg = TileCfg<D>;
+  using Cfg = TileCfg<D, E4M3>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = smem;                                        // two tiles, D / 64 column blocks of [128 rows][128 bytes] each
   uint8_t* k_s = q_s + Cfg::kQBytes;                          // [2 stages]
   uint8_t* v_s = k_s + 2 * Cfg::kHalf;
-  float* f_s = reinterpret_cast<float*>(v_s + 2 * Cfg::kHalf);// [256] what turns a row's products into base-2 scores
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(f_s + 2 * kQ);
+  uint8_t* c_s = v_s + 2 * Cfg::kHalf;                        // (8-bit) codes of two halves,
+  float* f_s = reinterpret_cast<float*>(c_s + 2 * Cfg::kCodes);// [256] what turns a row's products into base-2 scores
+  uint8_t* b_s = reinterpret_cast<uint8_t*>(f_s + 2 * kQ);    // and their scale bytes: [2][K or V's own, V's beside K's][128]
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(b_s + (E4M3 ? 512 : 0));
   uint64_t* v_full = k_full + 2;
   uint64_t* k_empty = v_full + 2;
   uint64_t* v_empty = k_empty + 2;
-  uint64_t* k_came = v_empty + 2;                             // (bf16) TMA done
-  uint64_t* v_came = k_came + 2;
+  uint64_t* k_came = v_empty + 2;                             // TMA done: bf16, K's halves; 8-bit, codes of either
+  uint64_t* v_came = k_came + 2;                              // bf16, V's halves; 8-bit, the codes have been read
   uint64_t* s_full = v_came + 2;                              // per tile of rows: scores in TMEM,
   uint64_t* p_full = s_full + 2;                              // weights in TMEM,
   uint64_t* o_done = p_full + 2;                              // P V done
@@ -162,7 +209,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     for (int s = 0; s < 2; ++s) {
       mbar_init(&k_full[s], 128); mbar_init(&v_full[s], 128);
       mbar_init(&k_empty[s], 1); mbar_init(&v_empty[s], 1);
-      mbar_init(&k_came[s], 1); mbar_init(&v_came[s], 1);
+      mbar_init(&k_came[s], E4M3 ? 33 : 1); mbar_init(&v_came[s], E4M3 ? 4 : 1);
       mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 128); mbar_init(&o_done[s], 1);
     }
     *abort_flag = 0;
@@ -230,29 +277,30 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
 
+  const int* pages = a.block_table + (size_t)seq * a.max_pages;
+  // page and row in it of a token (runs of 64 tokens, or of a smaller page's, lie in one page)
+  auto place = [&](int tok, int& page, int& off) {
+    const int bits = a.page_size < 64 ? 31 - __clz(a.page_size) : 6, per = a.page_size < 64 ? 1 : a.page_size >> 6;
+    const int u = tok >> bits, pi = per == 1 ? u : u / per;
+    off = ((u - pi * per) << bits) + (tok & ((1 << bits) - 1));
+    page = pi < a.max_pages ? pages[pi] : -1;
+    if (page < 0 || page >= a.pool_pages) {
+      set_error(a.err, ERR_BOUNDS);
+      page = 0;
+    }
+  };
+  // the order of the halves: K(0), then K(t + 1) before V(t)
+  const int items = 2 * ntiles;
+  auto item = [&](int i, int& which, int& t) {
+    which = i == items - 1 ? 1 : (i == 0 ? 0 : !(i & 1));
+    t = i == items - 1 ? ntiles - 1 : (i == 0 ? 0 : (which ? i / 2 - 1 : (i + 1) / 2));
+  };
+
   if (warp >= 8 && warp < 12) {
     // ---------------- keys and values ----------------
     const int tid = threadIdx.x - 256, w4 = warp - 8;
-    const int* pages = a.block_table + (size_t)seq * a.max_pages;
-    const int bits = a.page_size < 64 ? 31 - __clz(a.page_size) : 6, per = a.page_size < 64 ? 1 : a.page_size >> 6;
-    // page and row in it of a token (runs of 2^bits tokens lie in one page)
-    auto place = [&](int tok, int& page, int& off) {
-      const int u = tok >> bits, pi = per == 1 ? u : u / per;
-      off = ((u - pi * per) << bits) + (tok & ((1 << bits) - 1));
-      page = pi < a.max_pages ? pages[pi] : -1;
-      if (page < 0 || page >= a.pool_pages) {
-        set_error(a.err, ERR_BOUNDS);
-        page = 0;
-      }
-    };
-    // the order of the halves: K(0), then K(t + 1) before V(t)
-    const int items = 2 * ntiles;
-    auto item = [&](int i, int& which, int& t) {
-      which = i == items - 1 ? 1 : (i == 0 ? 0 : !(i & 1));
-      t = i == items - 1 ? ntiles - 1 : (i == 0 ? 0 : (which ? i / 2 - 1 : (i + 1) / 2));
-    };
     auto half_free = [&](int which, int t) -> bool {
-      if (mbar_wait_ns(which ? &v_empty[t & 1] : &k_empty[t & 1], ((t >> 1) & 1) ^ 1, abort_flag)) return true;
+      if (bar_wait(which ? &v_empty[t & 1] : &k_empty[t & 1], ((t >> 1) & 1) ^ 1, abort_flag)) return true;
       set_error(a.err, ERR_WAIT_EMPTY);
       *abort_flag = 1;
       return false;
@@ -260,98 +308,76 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     if constexpr (E4M3) {
       constexpr int kLanes = D / 16, kRowsWarp = 32 / kLanes, kLoads = kT / (4 * kRowsWarp);     // lanes to a row of codes
       const int c = lane % kLanes, sub = lane / kLanes;
-      const size_t codes = (size_t)2 * a.hk * a.page_size * D, page_bytes = codes + 2 * a.hk * a.page_size;
-      // the scale bytes of a tile's tokens 4 lane .. 4 lane + 3; those of tokens behind the end are 0
-      auto scale_word = [&](int which, int tok0) -> uint32_t {
-        const int tok = tok0 + 4 * lane;
-        if (tok >= to) return 0;
-        int page, off;
-        place(tok, page, off);
-        const uint8_t* src = a.pool + (size_t)page * page_bytes + codes + (size_t)(which * a.hk + kvh) * a.page_size + off;
-        uint32_t w = KERN_CHECK(src, 4, SITE_KV_ROW) ? *reinterpret_cast<const uint32_t*>(src) : 0;
-        if (to - tok < 4) w &= (1u << (8 * (to - tok))) - 1;
-        return w;
-      };
-      auto top_byte = [&](uint32_t w) -> int {
+      auto top_byte = [&](uint32_t at, int here) -> int {     // the largest of a tile's scale bytes; those behind the end do not count
+        uint32_t w;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at + 4 * lane));
+        const int n = here - 4 * lane;
+        if (n < 4) w = n <= 0 ? 0u : w & ((1u << (8 * n)) - 1);
         const uint32_t m = __vmaxu4(w, w >> 16);
         return (int)__reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u));
       };
-      struct Codes {
-        uint4 v[kLoads];
-        uint32_t scale, vscale;
-      };
-      auto fetch = [&](int i, Codes& x) {
+      for (int i = 0; i < items && ok; ++i) {
         int which, t;
         item(i, which, t);
-        const int tok0 = from + t * kT;
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-          const int tok = tok0 + j * 4 * kRowsWarp + w4 * kRowsWarp + sub;
-          x.v[j] = make_uint4(0, 0, 0, 0);
-          if (tok < to) {
-            int page, off;
-            place(tok, page, off);
-            const uint8_t* src = a.pool + (size_t)page * page_bytes + ((size_t)(which * a.hk + kvh) * a.page_size + off) * D + c * 16;
-            if (KERN_CHECK(src, 16, SITE_KV_ROW)) x.v[j] = *reinterpret_cast<const uint4*>(src);
-          }
+        const int slot = i & 1, tok0 = from + t * kT;
+        if (!bar_wait(&k_came[slot], (i >> 1) & 1, abort_flag)) {
+          set_error(a.err, ERR_WAIT_FULL);
+          *abort_flag = 1;
+          ok = false;
+          break;
         }
-        x.scale = scale_word(which, tok0);
-        x.vscale = which ? 0 : scale_word(1, tok0);
-      };
-      auto put = [&](int i, const Codes& x) -> bool {
-        int which, t;
-        item(i, which, t);
-        if (!half_free(which, t)) return false;
-        const int tok0 = from + t * kT, top = top_byte(x.scale);
+        const uint32_t src = smem_u32(c_s) + slot * Cfg::kCodes, by = smem_u32(b_s) + slot * 256;
+        const int here = to - tok0, top = top_byte(by, here), vtop = which ? 0 : top_byte(by + 128, here);
+        if (!half_free(which, t)) {
+          ok = false;
+          break;
+        }
         const bool edge = tok0 + kT > clear;
         uint8_t* dst = (which ? v_s : k_s) + (t & 1) * Cfg::kHalf;
         bool nan = false;
-#pragma unroll
+        // a lane: 8 codes of the row's first half and 8 of its second (one piece of 16-bit values each; D = 64: two neighbours)
+        constexpr int kApart = D == 64 ? 1 : 8;
+        const int p0 = D == 64 ? 2 * c : c;
+#pragma unroll 2
         for (int j = 0; j < kLoads; ++j) {
-          const int r = j * 4 * kRowsWarp + w4 * kRowsWarp + sub;
-          const uint32_t word = __shfl_sync(0xffffffffu, x.scale, r >> 2);
-          const uint32_t f = pow2_f16((int)((word >> (8 * (r & 3))) & 255u) - top + 6) * 0x10001u;
-          uint32_t w[4] = {x.v[j].x, x.v[j].y, x.v[j].z, x.v[j].w}, o[8];
-          if (which && edge) {
-            // values that are not finite stay out of the product: rows that see them get them at the end
+          const int r = (j * 4 + w4) * kRowsWarp + sub;
+          uint32_t w[4], b;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t m = __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-              nan |= m != 0;
-              w[k] &= ~m;
+          for (int h = 0; h < 2; ++h) {
+            const int p = p0 + h * kApart;                    // eight codes: half of a 16-byte piece of the code row
+            const uint32_t at = src + (D == 64 ? r * 64 + (((p >> 1) ^ ((r >> 1) & 3)) << 4) : r * 128 + (((p >> 1) ^ (r & 7)) << 4)) + (p & 1) * 8;
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[2 * h]), "=r"(w[2 * h + 1]) : "r"(at));
+          }
+          asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b) : "r"(by + r));
+          const uint32_t f = pow2_f16(min((int)b - top, 0) + 6) * 0x10001u;
+          if (edge) {
+            if (tok0 + r >= to) w[0] = w[1] = w[2] = w[3] = 0;            // (not brought: anything may lie there)
+            if (which) {
+              // values that are not finite stay out of the product: rows that see them get them at the end
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t m = __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                nan |= m != 0;
+                w[k] &= ~m;
+              }
             }
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            codes_f16x4(w[k], o[2 * k], o[2 * k + 1]);
-            o[2 * k] = mul_f16x2(o[2 * k], f);
-            o[2 * k + 1] = mul_f16x2(o[2 * k + 1], f);
+          for (int h = 0; h < 2; ++h) {
+            uint32_t o[4];
+            codes_f16x4(w[2 * h], o[0], o[1]);
+            codes_f16x4(w[2 * h + 1], o[2], o[3]);
+            const int p = p0 + h * kApart;
+            *reinterpret_cast<uint4*>(dst + (p >> 3) * (kT * 128) + r * 128 + (((p & 7) ^ (r & 7)) << 4)) =
+                make_uint4(mul_f16x2(o[0], f), mul_f16x2(o[1], f), mul_f16x2(o[2], f), mul_f16x2(o[3], f));
           }
-          // 16 values: two pieces of the row; lanes of the second half of the row store theirs the other way round, since their
-          // column block lies on the same banks
-          const int p0 = 2 * c, flip = (c >> 2) & 1;
-          uint8_t* row = dst + (p0 >> 3) * (kT * 128) + r * 128;
-          const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
-          *reinterpret_cast<uint4*>(row + ((((p0 + flip) & 7) ^ (r & 7)) << 4)) = flip ? hi : lo;
-          *reinterpret_cast<uint4*>(row + ((((p0 + 1 - flip) & 7) ^ (r & 7)) << 4)) = flip ? lo : hi;
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_came[slot]);            // (the codes have been read)
         if (nan) *bad_s = 1;
-        if (!which) {
-          const int vtop = top_byte(x.vscale);
-          if (tid == 0) e_s[t & 3] = make_float2(pow2i(top - 127 - 6), (float)(vtop - 127 - 6));
-        }
+        if (!which && tid == 0) e_s[t & 3] = make_float2(pow2i(top - 127 - 6), (float)(vtop - 127 - 6));
         fence_proxy_async();
         mbar_arrive(which ? &v_full[t & 1] : &k_full[t & 1]);
-        return true;
-      };
-      Codes x, y;
-      if (items > 0) fetch(0, x);
-      for (int i = 0; i < items && ok; i += 2) {              // (items is even)
-        fetch(i + 1, y);
-        ok = put(i, x);
-        if (!ok) break;
-        if (i + 2 < items) fetch(i + 2, x);
-        ok = put(i + 1, y);
       }
     } else {
       const int box = a.page_size < 64 ? a.page_size : 64;
@@ -379,7 +405,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       for (int i = 0; i < items && ok; ++i) {
         int which, t;
         item(i, which, t);
-        if (!mbar_wait_ns(which ? &v_came[t & 1] : &k_came[t & 1], (t >> 1) & 1, abort_flag)) {
+        if (!bar_wait(which ? &v_came[t & 1] : &k_came[t & 1], (t >> 1) & 1, abort_flag)) {
           set_error(a.err, ERR_WAIT_FULL);
           *abort_flag = 1;
           ok = false;
@@ -410,6 +436,39 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         if (w4 == 0 && i + ahead < items) ok = bring(i + ahead);
       }
     }
+  } else if (E4M3 && warp == 13) {
+    // ---------------- (8-bit) codes and scale bytes, two halves ahead ----------------
+    const size_t codes = (size_t)2 * a.hk * a.page_size * D, page_bytes = codes + 2 * a.hk * a.page_size;
+    const int box = a.page_size < 64 ? a.page_size : 64;
+    for (int i = 0; i < items && ok; ++i) {
+      int which, t;
+      item(i, which, t);
+      const int slot = i & 1, tok0 = from + t * kT, here = min(kT, to - tok0), boxes = (here + box - 1) / box;
+      int page = 0, off = 0;                                  // of the eight tokens from 8 lane on
+      if (lane < kT / 8 && 8 * lane < here) place(tok0 + 8 * lane, page, off);
+      if (!bar_wait(&v_came[slot], ((i >> 1) & 1) ^ 1, abort_flag)) {
+        set_error(a.err, ERR_WAIT_EMPTY);
+        *abort_flag = 1;
+        ok = false;
+        break;
+      }
+      if (lane == 0) mbar_expect_tx(&k_came[slot], boxes * box * D);
+      __syncwarp();
+      const int b_page = __shfl_sync(0xffffffffu, page, (lane * box >> 3) & 31), b_off = __shfl_sync(0xffffffffu, off, (lane * box >> 3) & 31);
+      if (lane < boxes)
+        tma_load_3d(c_s + slot * Cfg::kCodes + lane * box * D, kv_map, 0, (which * a.hk + kvh) * a.page_size + b_off, b_page, &k_came[slot]);
+      const int s_page = __shfl_sync(0xffffffffu, page, lane >> 1), s_off = __shfl_sync(0xffffffffu, off, lane >> 1) + (lane & 1) * 4;
+      uint8_t* by = b_s + slot * 256;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (k && which) break;
+        const int kind = k ? 1 : which;
+        const uint8_t* src = a.pool + (size_t)s_page * page_bytes + codes + (size_t)(kind * a.hk + kvh) * a.page_size + s_off;
+        if (4 * lane < here && KERN_CHECK(src, 4, SITE_KV_ROW))
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(by + k * 128 + 4 * lane)), "l"(src) : "memory");
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&k_came[slot])) : "memory");
+    }
   } else if (warp == 12) {
     // ---------------- products ----------------
     if (lane == 0) {
@@ -417,7 +476,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       const int steps = twice ? ntiles : 2 * ntiles;
       auto qk = [&](int u) -> bool {
         const int side = u & 1, t = twice ? u : u >> 1;
-        if (!mbar_wait_ns(&k_full[t & 1], (t >> 1) & 1, abort_flag)) return false;
+        if (!bar_wait(&k_full[t & 1], (t >> 1) & 1, abort_flag)) return false;
         tc_fence_after();
         const uint32_t sq = smem_u32(q_s) + side * (kQ * D * 2), sk = smem_u32(k_s) + (t & 1) * Cfg::kHalf;
 #pragma unroll
@@ -430,8 +489,8 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       };
       auto pv = [&](int u) -> bool {
         const int side = u & 1, t = twice ? u : u >> 1, n = u >> 1;
-        if (!mbar_wait_ns(&v_full[t & 1], (t >> 1) & 1, abort_flag)) return false;
-        if (!mbar_wait_ns(&p_full[side], n & 1, abort_flag)) return false;
+        if (!bar_wait(&v_full[t & 1], (t >> 1) & 1, abort_flag)) return false;
+        if (!bar_wait(&p_full[side], n & 1, abort_flag)) return false;
         tc_fence_after();
         const uint32_t sv = smem_u32(v_s) + (t & 1) * Cfg::kHalf;
 #pragma unroll
@@ -484,7 +543,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     for (int n = 0; n < steps && ok; ++n) {
       const int t = twice ? 2 * n + side : n;
       const int tok0 = from + t * kT;
-      if (!mbar_wait_ns(&s_full[side], n & 1, abort_flag)) {
+      if (!bar_wait(&s_full[side], n & 1, abort_flag)) {
         set_error(a.err, ERR_WAIT_TMEM_FULL);
         *abort_flag = 1;
         ok = false;
@@ -498,76 +557,76 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         scale *= e.x;
         ev = e.y;
       }
-      uint32_t pk[64];
-      float sum[2];
-      auto weigh = [&](float shift) -> float {
-        sum[0] = sum[1] = 0.f;
-        uint32_t top = 0;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t x[32];
-          tmem_ld_32x32(s_t + c * 32, x);
-          tmem_ld_wait();
-          if (edge) {
-            const uint32_t b = seen32(tok0 + c * 32);
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(b >> i & 1)) x[i] = 0xff800000u;          // -inf
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float u = exp2f(fmaf(__uint_as_float(x[2 * i]), scale, -shift)), v = exp2f(fmaf(__uint_as_float(x[2 * i + 1]), scale, -shift));
-            sum[0] += u;
-            sum[1] += v;
-            pk[c * 16 + i] = pack_pair<E4M3>(u, v);
-            top = max_pair<E4M3>(top, pk[c * 16 + i]);
-          }
-        }
-        return larger_half<E4M3>(top);
-      };
-      if (__any_sync(0xffffffffu, weigh(ref - ev) > kOutgrown)) {
-        float mx = -INFINITY;
+      // ---- the largest score; in a tile whose rows see different tokens the others become -inf where they lie ----
+      float mx = -INFINITY;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t x[32];
-          tmem_ld_32x32(s_t + c * 32, x);
-          tmem_ld_wait();
-          const uint32_t b = edge ? seen32(tok0 + c * 32) : 0xffffffffu;
+      for (int c = 0; c < kT; c += 64) {
+        uint32_t x[64];
+        tmem_ld64(s_t + c, x);
+        tmem_ld_wait();
+        if (edge) {
+          const uint32_t b0 = seen32(tok0 + c), b1 = seen32(tok0 + c + 32);
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (b >> i & 1) mx = fmaxf(mx, __uint_as_float(x[i]));
+          for (int i = 0; i < 32; ++i) {
+            if (!(b0 >> i & 1)) x[i] = 0xff800000u;
+            if (!(b1 >> i & 1)) x[32 + i] = 0xff800000u;
+          }
+          tmem_st64(s_t + c, x);
         }
-        const float to_ref = fmaxf(ref, ceilf(mx * scale + ev) - 7.f), corr = exp2f(ref - to_ref);
+        float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+        mx = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
+      }
+      if (edge) tmem_st_done();
+      mx = fmaf(mx, scale, ev);
+      if (__any_sync(0xffffffffu, mx > ref + 15.f)) {
+        const float to_ref = mx > ref + 15.f ? ceilf(mx) - 7.f : ref, corr = exp2f(ref - to_ref);
         ref = to_ref;
         l *= corr;
         if (n > 0) {
-          if (!mbar_wait_ns(&o_done[side], (n - 1) & 1, abort_flag)) {
+          if (!bar_wait(&o_done[side], (n - 1) & 1, abort_flag)) {
             set_error(a.err, ERR_WAIT_TMEM_EMPTY);
             *abort_flag = 1;
             ok = false;
           }
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
+          for (int c = 0; c < D; c += 32) {
             uint32_t x[32];
-            tmem_ld_32x32(o_t + c * 32, x);
+            tmem_ld_32x32(o_t + c, x);
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * corr);
-            tmem_st32(o_t + c * 32, x);
+            tmem_st32(o_t + c, x);
           }
           tmem_st_done();
         }
-        weigh(ref - ev);
       }
-      l += E4M3 ? (sum[0] + sum[1]) * exp2f(-ev) : sum[0] + sum[1];
-      tmem_st32(s_t, pk);
-      tmem_st32(s_t + 32, pk + 32);
+      // ---- weights, over the scores that have been read; their sum ----
+      const uint64_t scale2 = pair64(scale, scale), shift2 = pair64(ev - ref, ev - ref);
+      uint64_t sum2[2] = {0, 0};
+#pragma unroll 1
+      for (int c = 0; c < kT; c += 64) {
+        uint32_t x[64];
+        tmem_ld64(s_t + c, x);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float2 y = split64(fma2(pair64(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, shift2));
+          const float u = exp2f(y.x), v = exp2f(y.y);
+          sum2[i & 1] = add2(sum2[i & 1], pair64(u, v));
+          x[i] = pack_pair<E4M3>(u, v);
+        }
+        tmem_st32(s_t + (c >> 1), x);
+      }
+      const float2 sum = split64(add2(sum2[0], sum2[1]));
+      l += E4M3 ? (sum.x + sum.y) * exp2f(-ev) : sum.x + sum.y;
       tmem_st_done();
       tc_fence_before();
       mbar_arrive(&p_full[side]);
     }
-    if (ok && steps > 0 && !mbar_wait_ns(&o_done[side], (steps - 1) & 1, abort_flag)) {
+    if (ok && steps > 0 && !bar_wait(&o_done[side], (steps - 1) & 1, abort_flag)) {
       set_error(a.err, ERR_WAIT_TMEM_FULL);
       *abort_flag = 1;
       ok = false;

@@ -200,9 +200,9 @@ def rows_shares(ctas: int, max_len: int, resident: int) -> tuple[int, int]:
 TILE_ROWS = 32
 
 
-def tile_smem(d: int) -> int:
-    """Dynamic shared memory of the many-row kernel: two tiles of Q, two stages of K and of V as 16-bit values, barriers."""
-    return 1024 + 2 * 128 * d * 2 + 4 * 128 * d * 2 + 1024 + 512
+def tile_smem(d: int, e4m3: bool) -> int:
+    """Dynamic shared memory of the many-row kernel: two tiles of Q, two stages of K and of V as 16-bit values, codes, barriers."""
+    return 1024 + 2 * 128 * d * 2 + 4 * 128 * d * 2 + 1024 + 512 + (2 * 128 * d + 512 if e4m3 else 0)
 
 
 def tile_shares(ctas: int, max_len: int, sms: int) -> int:
@@ -226,7 +226,7 @@ def attention_rows(q, pool, pages, block_table, seq_lens, masks, cu_q, hq, hk, d
     g = hq // hk
     tiled = g * max_rows > TILE_ROWS and d <= 128
     if tiled:
-        entry, toks, cluster, threads, smem = "attn_tile", 256 // g, 1, 512, tile_smem(d)
+        entry, toks, cluster, threads, smem = "attn_tile", 256 // g, 1, 512, tile_smem(d, e4m3)
         nblk = min(n // toks + seqs, seqs * -(-max_rows // toks))          # blocks of all sequences, at most
         shares = tile_shares(hk * nblk, max_len, k.sm_count)
         gx, gy, last, name = hk, nblk, seqs, ""
@@ -288,6 +288,8 @@ def attention_args(q, pool, block_table, seq_lens, cu_q, masks, hq, d, page_size
         max_len = width * page_size
     elif max_len < 0:
         raise ValueError(f"max_len {max_len}")
+    if scale is not None and not scale > 0:
+        raise ValueError(f"scale {scale}: above zero")
     gpu = same_device(q, pool, block_table, seq_lens, cu_q, masks, out)
     return out, (gpu, n, q_step, out_step, seqs, width, rows_per_seq, max_rows, max_len, d ** -0.5 if scale is None else float(scale))
 
