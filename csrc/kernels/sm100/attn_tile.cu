@@ -4,11 +4,12 @@
 // One CTA = (256 query rows: the G heads of 256 / G tokens, one kv head, a share of the context), 16 warps:
 //
 //   warps 0..3, 4..7   softmax of one 128-row tile each, a thread to a row: scores out of TMEM, weights back into TMEM over them
-//   warps 8..11        key and value tiles of 128 tokens in shared memory, two stages of each. 8-bit codes become f16 there, in the
-//                      swizzle that the tensor cores read; bf16 tiles are brought by warp 8 as they are, by TMA, and only looked
-//                      through where rows see different tokens
+//   warps 8..11        halves (a tile of 128 keys, or of values) for the products to read: 8-bit codes become f16 there, in the
+//                      swizzle that the tensor cores read; bf16 halves lie as they came, and are only looked through where rows
+//                      see different tokens
 //   warp 12            issues the products:  S = Q K^T  and  O += P V  (P from TMEM), for the two tiles in turn
-//   warp 13            (8-bit) brings codes by TMA and scale bytes, two halves ahead
+//   warp 13            copies by TMA: bf16 halves into a ring of five; codes, with their scale bytes, into four slots (two were
+//                      bound by the copies' latency), beside a ring of three halves
 //
 // The two tiles take turns on the tensor cores: while one's products run, the other's exponentials do. At most 128 rows (a small
 // tree): both tiles are the same rows, on alternate key tiles, and are added up at the end, so the turns remain. TMEM: S and O of
@@ -32,10 +33,15 @@ constexpr int kTileThreads = 512;
 template <int D, bool E4M3>
 struct TileCfg {
   static constexpr int kQBytes = 2 * kQ * D * 2;
-  static constexpr int kHalf = kT * D * 2;                  // a tile of K or of V
-  static constexpr int kRing = 4 * kHalf;                   // two stages of each
-  static constexpr int kCodes = E4M3 ? kT * D : 0;          // a half as codes, as it comes; two of them
-  static constexpr int kSmem = 1024 + kQBytes + kRing + 2 * kCodes + 2 * kQ * 4 + (E4M3 ? 512 : 0) + 512;
+  static constexpr int kHalf = kT * D * 2;                  // a half: a tile of K or of V, as 16-bit values
+  static constexpr int kRing = E4M3 ? 3 : 5;                // halves that the products read
+  static constexpr int kCodes = E4M3 ? kT * D : 0;          // a half as codes, as it comes
+  static constexpr int kSlots = E4M3 ? 4 : 0;               // of which there are so many under way
+  static constexpr int kScales = kSlots * 2 * kT;           // with their scale bytes, and V's beside K's
+  // room to bring the tiles to a 1024-byte boundary (all of the SM's 227 KB are in use: the base, aligned in practice, is checked)
+  static constexpr int kSlack = 768;
+  static constexpr int kSmem = kSlack + kQBytes + kRing * kHalf + kSlots * kCodes + kScales + 2 * kQ * 4 + (E4M3 ? 256 : 512);
+  static_assert(kSmem <= 232448, "more shared memory than a CTA has");
 };
 
 // Shared-memory descriptor of an MN-major operand tile with the 128-byte swizzle: rows are the contraction's (tokens), 128 bytes =
@@ -150,24 +156,27 @@ KERN_DEVICE uint32_t pow2_f16(int x) { return x >= -14 ? (uint32_t)(x + 15) << 1
 template <int D, bool E4M3, bool TREE>
 KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const int seqs) {
   using Cfg = TileCfg<D, E4M3>;
+  constexpr int kRing = Cfg::kRing, kSlots = Cfg::kSlots, kCame = E4M3 ? kSlots : kRing;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  if ((int)(smem - smem_raw) > Cfg::kSlack) {                 // uniform, before any barrier or allocation
+    if (threadIdx.x == 0) set_error(a.err, ERR_BOUNDS);
+    return;
+  }
   uint8_t* q_s = smem;                                        // two tiles, D / 64 column blocks of [128 rows][128 bytes] each
-  uint8_t* k_s = q_s + Cfg::kQBytes;                          // [2 stages]
-  uint8_t* v_s = k_s + 2 * Cfg::kHalf;
-  uint8_t* c_s = v_s + 2 * Cfg::kHalf;                        // (8-bit) codes of two halves,
-  float* f_s = reinterpret_cast<float*>(c_s + 2 * Cfg::kCodes);// [256] what turns a row's products into base-2 scores
-  uint8_t* b_s = reinterpret_cast<uint8_t*>(f_s + 2 * kQ);    // and their scale bytes: [2][K or V's own, V's beside K's][128]
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(b_s + (E4M3 ? 512 : 0));
-  uint64_t* v_full = k_full + 2;
-  uint64_t* k_empty = v_full + 2;
-  uint64_t* v_empty = k_empty + 2;
-  uint64_t* k_came = v_empty + 2;                             // TMA done: bf16, K's halves; 8-bit, codes of either
-  uint64_t* v_came = k_came + 2;                              // bf16, V's halves; 8-bit, the codes have been read
-  uint64_t* s_full = v_came + 2;                              // per tile of rows: scores in TMEM,
+  uint8_t* h_s = q_s + Cfg::kQBytes;                          // halves
+  uint8_t* c_s = h_s + kRing * Cfg::kHalf;                    // (8-bit) codes,
+  uint8_t* b_s = c_s + kSlots * Cfg::kCodes;                  // scale bytes [slot][the half's own, V's beside K's][128]
+  float* f_s = reinterpret_cast<float*>(b_s + Cfg::kScales);  // [256] what turns a row's products into base-2 scores
+  uint64_t* full = reinterpret_cast<uint64_t*>(f_s + 2 * kQ); // [ring] a half can be read by the products,
+  uint64_t* empty = full + kRing;                             // [ring] has been read;
+  uint64_t* came = empty + kRing;                             // [ring; 8-bit: slots] the copy has landed;
+  uint64_t* taken = came + kCame;                             // [slots] the codes have been read
+  uint64_t* s_full = taken + kCame;                              // per tile of rows: scores in TMEM,
   uint64_t* p_full = s_full + 2;                              // weights in TMEM,
   uint64_t* o_done = p_full + 2;                              // P V done
-  float2* e_s = reinterpret_cast<float2*>(o_done + 2);        // [4] a key tile's (2^E of K, E of V)
+  uint64_t* q_full = o_done + 2;                              // Q in shared memory
+  float2* e_s = reinterpret_cast<float2*>(q_full + 2);        // [4] a key tile's (2^E of K, E of V)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(e_s + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* found = reinterpret_cast<int*>(tmem_slot + 2);         // [2] sequence and block of this CTA
@@ -206,12 +215,20 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     }
   }
   if (threadIdx.x == 32) {
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&k_full[s], 128); mbar_init(&v_full[s], 128);
-      mbar_init(&k_empty[s], 1); mbar_init(&v_empty[s], 1);
-      mbar_init(&k_came[s], E4M3 ? 33 : 1); mbar_init(&v_came[s], E4M3 ? 4 : 1);
-      mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 128); mbar_init(&o_done[s], 1);
+    for (int s = 0; s < kRing; ++s) {
+      mbar_init(&full[s], 4);
+      mbar_init(&empty[s], 1);
     }
+    for (int s = 0; s < kCame; ++s) {
+      mbar_init(&came[s], E4M3 ? 33 : 1);
+      mbar_init(&taken[s], 4);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 128);
+      mbar_init(&o_done[s], 1);
+    }
+    mbar_init(q_full, 256);
     *abort_flag = 0;
     *bad_s = 0;
     mbar_fence_init();
@@ -236,41 +253,6 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  // ---- Q -> shared memory, K-major with the 128-byte swizzle: D / 8 lanes to a row ----
-  {
-    constexpr int kLanes = D / 8;
-    const int c = threadIdx.x % kLanes;
-#pragma unroll 2
-    for (int r = threadIdx.x / kLanes; r < 2 * kQ; r += kTileThreads / kLanes) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      const int rr = twice ? r & (kQ - 1) : r;
-      if (rr < valid) v = *reinterpret_cast<const uint4*>(a.q + (size_t)(row0 + tok_lo + rr / G) * a.q_stride + (size_t)(kvh * G + rr % G) * D + c * 8);
-      float f = a.scale_log2;
-      if constexpr (E4M3) {
-        uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 u = unpack_bf16x2(w[i]);
-          top = fmaxf(top, fmaxf(fabsf(u.x), fabsf(u.y)));
-        }
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int x = min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100), 100);
-        const float inv = pow2i(-x);
-        f *= pow2i(x);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 u = unpack_bf16x2(w[i]);
-          w[i] = pack_f16x2(u.x * inv, u.y * inv);
-        }
-        v = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      *reinterpret_cast<uint4*>(q_s + (r >> 7) * (kQ * D * 2) + (c >> 3) * (kQ * 128) + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
-      if (c == 0) f_s[r] = f;
-    }
-  }
-  fence_proxy_async();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -295,16 +277,12 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     which = i == items - 1 ? 1 : (i == 0 ? 0 : !(i & 1));
     t = i == items - 1 ? ntiles - 1 : (i == 0 ? 0 : (which ? i / 2 - 1 : (i + 1) / 2));
   };
+  auto k_item = [&](int t) { return t == 0 ? 0 : 2 * t - 1; };
+  auto v_item = [&](int t) { return t == ntiles - 1 ? items - 1 : 2 * t + 2; };
 
   if (warp >= 8 && warp < 12) {
     // ---------------- keys and values ----------------
     const int tid = threadIdx.x - 256, w4 = warp - 8;
-    auto half_free = [&](int which, int t) -> bool {
-      if (bar_wait(which ? &v_empty[t & 1] : &k_empty[t & 1], ((t >> 1) & 1) ^ 1, abort_flag)) return true;
-      set_error(a.err, ERR_WAIT_EMPTY);
-      *abort_flag = 1;
-      return false;
-    };
     if constexpr (E4M3) {
       constexpr int kLanes = D / 16, kRowsWarp = 32 / kLanes, kLoads = kT / (4 * kRowsWarp);     // lanes to a row of codes
       const int c = lane % kLanes, sub = lane / kLanes;
@@ -319,21 +297,23 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       for (int i = 0; i < items && ok; ++i) {
         int which, t;
         item(i, which, t);
-        const int slot = i & 1, tok0 = from + t * kT;
-        if (!bar_wait(&k_came[slot], (i >> 1) & 1, abort_flag)) {
+        const int slot = i % kSlots, half = i % kRing, tok0 = from + t * kT;
+        if (!bar_wait(&came[slot], (i / kSlots) & 1, abort_flag)) {
           set_error(a.err, ERR_WAIT_FULL);
           *abort_flag = 1;
           ok = false;
           break;
         }
-        const uint32_t src = smem_u32(c_s) + slot * Cfg::kCodes, by = smem_u32(b_s) + slot * 256;
-        const int here = to - tok0, top = top_byte(by, here), vtop = which ? 0 : top_byte(by + 128, here);
-        if (!half_free(which, t)) {
+        const uint32_t src = smem_u32(c_s) + slot * Cfg::kCodes, by = smem_u32(b_s) + slot * 2 * kT;
+        const int here = to - tok0, top = top_byte(by, here), vtop = which ? 0 : top_byte(by + kT, here);
+        if (!bar_wait(&empty[half], ((i / kRing) & 1) ^ 1, abort_flag)) {
+          set_error(a.err, ERR_WAIT_EMPTY);
+          *abort_flag = 1;
           ok = false;
           break;
         }
         const bool edge = tok0 + kT > clear;
-        uint8_t* dst = (which ? v_s : k_s) + (t & 1) * Cfg::kHalf;
+        uint8_t* dst = h_s + half * Cfg::kHalf;
         bool nan = false;
         // a lane: 8 codes of the row's first half and 8 of its second (one piece of 16-bit values each; D = 64: two neighbours)
         constexpr int kApart = D == 64 ? 1 : 8;
@@ -372,56 +352,37 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
                 make_uint4(mul_f16x2(o[0], f), mul_f16x2(o[1], f), mul_f16x2(o[2], f), mul_f16x2(o[3], f));
           }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_came[slot]);            // (the codes have been read)
         if (nan) *bad_s = 1;
         if (!which && tid == 0) e_s[t & 3] = make_float2(pow2i(top - 127 - 6), (float)(vtop - 127 - 6));
         fence_proxy_async();
-        mbar_arrive(which ? &v_full[t & 1] : &k_full[t & 1]);
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&full[half]);
+          mbar_arrive(&taken[slot]);                          // (the codes have been read)
+        }
       }
     } else {
-      const int box = a.page_size < 64 ? a.page_size : 64;
-      auto bring = [&](int i) -> bool {                       // warp 8: a half by TMA, boxes up to the share's end
-        int which, t;
-        item(i, which, t);
-        if (!half_free(which, t)) return false;
-        const int tok0 = from + t * kT, boxes = (min(kT, to - tok0) + box - 1) / box;
-        uint64_t* bar = which ? &v_came[t & 1] : &k_came[t & 1];
-        uint8_t* dst = (which ? v_s : k_s) + (t & 1) * Cfg::kHalf;
-        if (lane == 0) mbar_expect_tx(bar, boxes * box * D * 2);
-        __syncwarp();
-        if (lane < boxes) {
-          int page, off;
-          place(tok0 + lane * box, page, off);
-#pragma unroll
-          for (int cb = 0; cb < D / 64; ++cb)
-            tma_load_3d(dst + cb * (kT * 128) + lane * box * 128, kv_map, cb * 64, (which * a.hk + kvh) * a.page_size + off, page, bar);
-        }
-        return true;
-      };
-      const int ahead = min(items, 3);                        // K(0), K(1), V(0) fill what is free at the start
-      if (w4 == 0)
-        for (int i = 0; i < ahead && ok; ++i) ok = bring(i);
       for (int i = 0; i < items && ok; ++i) {
         int which, t;
         item(i, which, t);
-        if (!bar_wait(which ? &v_came[t & 1] : &k_came[t & 1], (t >> 1) & 1, abort_flag)) {
+        const int half = i % kRing, tok0 = from + t * kT;
+        if (!bar_wait(&came[half], (i / kRing) & 1, abort_flag)) {
           set_error(a.err, ERR_WAIT_FULL);
           *abort_flag = 1;
           ok = false;
           break;
         }
-        const int tok0 = from + t * kT;
         if (which && tok0 + kT > clear) {
-          uint8_t* dst = v_s + (t & 1) * Cfg::kHalf;
+          // values that are not finite stay out of the product: rows that see them get them at the end
+          uint8_t* dst = h_s + half * Cfg::kHalf;
           bool bad = false;
           for (int x = tid; x < kT * (D / 8); x += 128) {
             const int r = x / (D / 8), p = x % (D / 8);
             uint4* at = reinterpret_cast<uint4*>(dst + (p >> 3) * (kT * 128) + r * 128 + (((p & 7) ^ (r & 7)) << 4));
             if (tok0 + r >= to) {
-              *at = make_uint4(0, 0, 0, 0);
+              *at = make_uint4(0, 0, 0, 0);                   // (not brought: anything may lie there)
             } else {
-              uint4 v = *at;
+              const uint4 v = *at;
               const uint32_t m0 = not_finite<false>(v.x), m1 = not_finite<false>(v.y), m2 = not_finite<false>(v.z), m3 = not_finite<false>(v.w);
               if (m0 | m1 | m2 | m3) {
                 bad = true;
@@ -432,42 +393,47 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
           if (bad) *bad_s = 1;
           fence_proxy_async();
         }
-        mbar_arrive(which ? &v_full[t & 1] : &k_full[t & 1]);
-        if (w4 == 0 && i + ahead < items) ok = bring(i + ahead);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[half]);
       }
     }
-  } else if (E4M3 && warp == 13) {
-    // ---------------- (8-bit) codes and scale bytes, two halves ahead ----------------
+  } else if (warp == 13) {
+    // ---------------- copies: bf16 halves into the ring, 8-bit codes and scale bytes into their slots ----------------
     const size_t codes = (size_t)2 * a.hk * a.page_size * D, page_bytes = codes + 2 * a.hk * a.page_size;
     const int box = a.page_size < 64 ? a.page_size : 64;
     for (int i = 0; i < items && ok; ++i) {
       int which, t;
       item(i, which, t);
-      const int slot = i & 1, tok0 = from + t * kT, here = min(kT, to - tok0), boxes = (here + box - 1) / box;
+      const int slot = i % kCame, tok0 = from + t * kT, here = min(kT, to - tok0), boxes = (here + box - 1) / box;
       int page = 0, off = 0;                                  // of the eight tokens from 8 lane on
       if (lane < kT / 8 && 8 * lane < here) place(tok0 + 8 * lane, page, off);
-      if (!bar_wait(&v_came[slot], ((i >> 1) & 1) ^ 1, abort_flag)) {
+      if (!bar_wait(E4M3 ? &taken[slot] : &empty[slot], ((i / kCame) & 1) ^ 1, abort_flag)) {
         set_error(a.err, ERR_WAIT_EMPTY);
         *abort_flag = 1;
         ok = false;
         break;
       }
-      if (lane == 0) mbar_expect_tx(&k_came[slot], boxes * box * D);
+      // boxes behind the share's end are not brought
+      if (lane == 0) mbar_expect_tx(&came[slot], boxes * box * D * (E4M3 ? 1 : 2));
       __syncwarp();
       const int b_page = __shfl_sync(0xffffffffu, page, (lane * box >> 3) & 31), b_off = __shfl_sync(0xffffffffu, off, (lane * box >> 3) & 31);
-      if (lane < boxes)
-        tma_load_3d(c_s + slot * Cfg::kCodes + lane * box * D, kv_map, 0, (which * a.hk + kvh) * a.page_size + b_off, b_page, &k_came[slot]);
-      const int s_page = __shfl_sync(0xffffffffu, page, lane >> 1), s_off = __shfl_sync(0xffffffffu, off, lane >> 1) + (lane & 1) * 4;
-      uint8_t* by = b_s + slot * 256;
+      const int b_row = (which * a.hk + kvh) * a.page_size + b_off;
+      if constexpr (E4M3) {
+        if (lane < boxes) tma_load_3d(c_s + slot * Cfg::kCodes + lane * box * D, kv_map, 0, b_row, b_page, &came[slot]);
+        const int s_page = __shfl_sync(0xffffffffu, page, lane >> 1), s_off = __shfl_sync(0xffffffffu, off, lane >> 1) + (lane & 1) * 4;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (k && which) break;
-        const int kind = k ? 1 : which;
-        const uint8_t* src = a.pool + (size_t)s_page * page_bytes + codes + (size_t)(kind * a.hk + kvh) * a.page_size + s_off;
-        if (4 * lane < here && KERN_CHECK(src, 4, SITE_KV_ROW))
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(by + k * 128 + 4 * lane)), "l"(src) : "memory");
+        for (int k = 0; k < 2; ++k) {
+          if (k && which) break;
+          const uint8_t* src = a.pool + (size_t)s_page * page_bytes + codes + (size_t)((k ? 1 : which) * a.hk + kvh) * a.page_size + s_off;
+          if (4 * lane < here && KERN_CHECK(src, 4, SITE_KV_ROW))
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(b_s + slot * 2 * kT + k * kT + 4 * lane)), "l"(src) : "memory");
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&came[slot])) : "memory");
+      } else if (lane < boxes) {
+#pragma unroll
+        for (int cb = 0; cb < D / 64; ++cb)
+          tma_load_3d(h_s + slot * Cfg::kHalf + cb * (kT * 128) + lane * box * 128, kv_map, cb * 64, b_row, b_page, &came[slot]);
       }
-      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&k_came[slot])) : "memory");
     }
   } else if (warp == 12) {
     // ---------------- products ----------------
@@ -476,31 +442,33 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       const int steps = twice ? ntiles : 2 * ntiles;
       auto qk = [&](int u) -> bool {
         const int side = u & 1, t = twice ? u : u >> 1;
-        if (!bar_wait(&k_full[t & 1], (t >> 1) & 1, abort_flag)) return false;
+        const int i = k_item(t), half = i % kRing;
+        if (!bar_wait(&full[half], (i / kRing) & 1, abort_flag)) return false;
         tc_fence_after();
-        const uint32_t sq = smem_u32(q_s) + side * (kQ * D * 2), sk = smem_u32(k_s) + (t & 1) * Cfg::kHalf;
+        const uint32_t sq = smem_u32(q_s) + side * (kQ * D * 2), sk = smem_u32(h_s) + half * Cfg::kHalf;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
           umma_bf16(tmem + side * 128, umma_desc_sw128(sq + (k >> 2) * (kQ * 128) + (k & 3) * 32), umma_desc_sw128(sk + (k >> 2) * (kT * 128) + (k & 3) * 32),
                     idesc_qk, k != 0);
         tc_commit(&s_full[side]);
-        if (twice || side) tc_commit(&k_empty[t & 1]);
+        if (twice || side) tc_commit(&empty[half]);
         return true;
       };
       auto pv = [&](int u) -> bool {
         const int side = u & 1, t = twice ? u : u >> 1, n = u >> 1;
-        if (!bar_wait(&v_full[t & 1], (t >> 1) & 1, abort_flag)) return false;
+        const int i = v_item(t), half = i % kRing;
+        if (!bar_wait(&full[half], (i / kRing) & 1, abort_flag)) return false;
         if (!bar_wait(&p_full[side], n & 1, abort_flag)) return false;
         tc_fence_after();
-        const uint32_t sv = smem_u32(v_s) + (t & 1) * Cfg::kHalf;
+        const uint32_t sv = smem_u32(h_s) + half * Cfg::kHalf;
 #pragma unroll
         for (int k = 0; k < kT / 16; ++k)
           umma_ts(tmem + 256 + side * D, tmem + side * 128 + k * 8, tile_desc_mn(sv + k * 16 * 128, kT * 128), idesc_pv, (n | k) != 0);
         tc_commit(&o_done[side]);
-        if (twice || side) tc_commit(&v_empty[t & 1]);
+        if (twice || side) tc_commit(&empty[half]);
         return true;
       };
-      if (steps > 0) ok = qk(0);
+      if (steps > 0) ok = bar_wait(q_full, 0, abort_flag) && qk(0);
       if (ok && steps > 1) ok = qk(1);
       for (int u = 0; u < steps && ok; ++u) {
         ok = pv(u);
@@ -513,6 +481,43 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     }
     __syncwarp();
   } else if (warp < 8) {
+    // ---------------- Q -> shared memory, K-major with the 128-byte swizzle: D / 8 lanes to a row ----------------
+    {
+      constexpr int kLanes = D / 8;
+      const int c = threadIdx.x % kLanes;
+#pragma unroll 4
+      for (int r = threadIdx.x / kLanes; r < 2 * kQ; r += 256 / kLanes) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        const int rr = twice ? r & (kQ - 1) : r;
+        if (rr < valid) v = *reinterpret_cast<const uint4*>(a.q + (size_t)(row0 + tok_lo + rr / G) * a.q_stride + (size_t)(kvh * G + rr % G) * D + c * 8);
+        float f = a.scale_log2;
+        if constexpr (E4M3) {
+          uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          float top = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 u = unpack_bf16x2(w[i]);
+            top = fmaxf(top, fmaxf(fabsf(u.x), fabsf(u.y)));
+          }
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const int x = min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100), 100);
+          const float inv = pow2i(-x);
+          f *= pow2i(x);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 u = unpack_bf16x2(w[i]);
+            w[i] = pack_f16x2(u.x * inv, u.y * inv);
+          }
+          v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        *reinterpret_cast<uint4*>(q_s + (r >> 7) * (kQ * D * 2) + (c >> 3) * (kQ * 128) + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+        if (c == 0) f_s[r] = f;
+      }
+      fence_proxy_async();
+      mbar_arrive(q_full);
+      asm volatile("bar.sync 1, 256;" ::: "memory");          // f_s
+    }
     // ---------------- softmax: a thread to a row ----------------
     const int side = warp >> 2, row = (warp & 3) * 32 + lane;
     const int r = twice ? row : side * kQ + row;              // of the block's rows
@@ -633,7 +638,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     }
     tc_fence_after();
     // ---------------- the rows' end ----------------
-    float* other = reinterpret_cast<float*>(k_s);             // (twice) the second side's rows: [128][D + 3]
+    float* other = reinterpret_cast<float*>(h_s);             // (twice) the second side's rows: [128][D + 3]
     if (twice) {
       asm volatile("bar.sync 1, 256;" ::: "memory");          // both sides' products are done: the ring is free
       if (side == 1) {
