@@ -44,30 +44,39 @@ struct TileCfg {
   static_assert(kSmem <= 232448, "more shared memory than a CTA has");
 };
 
-// Shared-memory descriptor of an MN-major operand tile with the 128-byte swizzle: rows are the contraction's (tokens), 128 bytes =
-// 64 columns each; the next 64 columns are `block_bytes` further on.
-KERN_DEVICE uint64_t tile_desc_mn(uint32_t smem_addr, uint32_t block_bytes) {
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
-  d |= (uint64_t)((block_bytes >> 4) & 0x3FFF) << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
-}
+// Shared-memory descriptors (128-byte swizzle, groups of 8 rows 1024 bytes apart) have the same upper word for K-major operands and
+// for MN-major ones (rows are the contraction's, 64 columns to a row, the next 64 `block_bytes` further on); a step along the
+// contraction adds to the address in the lower one. The products' warp then issues an instruction with two additions.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+KERN_DEVICE uint32_t desc_low(uint32_t smem_addr, uint32_t block_bytes) { return ((smem_addr & 0x3FFFF) >> 4) | ((block_bytes >> 4) << 16); }
 // kind::f16 with f32 sums: 16-bit operands, f16 or bf16
 template <bool F16>
 KERN_DEVICE constexpr uint32_t tile_idesc(int m, int n, bool b_mn) {
   return (1u << 4) | ((F16 ? 0u : 1u) << 7) | ((F16 ? 0u : 1u) << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// D[tmem] (+)= A[tmem] * B[smem]; one thread
-KERN_DEVICE void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[smem] B[smem], and with A in TMEM; one thread
+KERN_DEVICE void umma_ss(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
       : "memory");
+}
+KERN_DEVICE void umma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
+      : "memory");
+}
+KERN_DEVICE bool elect_lane() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 KERN_DEVICE void tmem_st32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
@@ -182,7 +191,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   int* found = reinterpret_cast<int*>(tmem_slot + 2);         // [2] sequence and block of this CTA
   volatile int* bad_s = found + 2;                            // a value that is not finite in a tile whose rows see different tokens
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (uniform registers for what follows from it)
   const int G = a.hq / a.hk, kvh = blockIdx.x, toks = 2 * kQ / G;
   pdl_wait();
   if (warp == 0) {
@@ -436,48 +445,52 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       }
     }
   } else if (warp == 12) {
-    // ---------------- products ----------------
-    if (lane == 0) {
-      constexpr uint32_t idesc_qk = tile_idesc<E4M3>(kQ, kT, false), idesc_pv = tile_idesc<E4M3>(kQ, D, true);
-      const int steps = twice ? ntiles : 2 * ntiles;
-      auto qk = [&](int u) -> bool {
-        const int side = u & 1, t = twice ? u : u >> 1;
-        const int i = k_item(t), half = i % kRing;
-        if (!bar_wait(&full[half], (i / kRing) & 1, abort_flag)) return false;
-        tc_fence_after();
-        const uint32_t sq = smem_u32(q_s) + side * (kQ * D * 2), sk = smem_u32(h_s) + half * Cfg::kHalf;
+    // ---------------- products: the whole warp walks and waits, one lane issues ----------------
+    constexpr uint32_t idesc_qk = tile_idesc<E4M3>(kQ, kT, false), idesc_pv = tile_idesc<E4M3>(kQ, D, true);
+    const int steps = twice ? ntiles : 2 * ntiles;
+    const uint32_t q_low = desc_low(smem_u32(q_s), 0), h_low = desc_low(smem_u32(h_s), 0), v_low = desc_low(smem_u32(h_s), kT * 128);
+    const bool leader = elect_lane();
+    auto qk = [&](int u) -> bool {
+      const int side = u & 1, t = twice ? u : u >> 1;
+      const int i = k_item(t), half = i % kRing;
+      if (!bar_wait(&full[half], (i / kRing) & 1, abort_flag)) return false;
+      tc_fence_after();
+      const uint32_t sq = q_low + side * (kQ * D * 2 >> 4), sk = h_low + half * (Cfg::kHalf >> 4), s_t = tmem + side * 128;
+      if (leader) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          umma_bf16(tmem + side * 128, umma_desc_sw128(sq + (k >> 2) * (kQ * 128) + (k & 3) * 32), umma_desc_sw128(sk + (k >> 2) * (kT * 128) + (k & 3) * 32),
-                    idesc_qk, k != 0);
+          umma_ss(s_t, sq + ((k >> 2) * (kQ * 128) + (k & 3) * 32 >> 4), sk + ((k >> 2) * (kT * 128) + (k & 3) * 32 >> 4), idesc_qk, k != 0);
         tc_commit(&s_full[side]);
         if (twice || side) tc_commit(&empty[half]);
-        return true;
-      };
-      auto pv = [&](int u) -> bool {
-        const int side = u & 1, t = twice ? u : u >> 1, n = u >> 1;
-        const int i = v_item(t), half = i % kRing;
-        if (!bar_wait(&full[half], (i / kRing) & 1, abort_flag)) return false;
-        if (!bar_wait(&p_full[side], n & 1, abort_flag)) return false;
-        tc_fence_after();
-        const uint32_t sv = smem_u32(h_s) + half * Cfg::kHalf;
+      }
+      __syncwarp();
+      return true;
+    };
+    auto pv = [&](int u) -> bool {
+      const int side = u & 1, t = twice ? u : u >> 1, n = u >> 1;
+      const int i = v_item(t), half = i % kRing;
+      if (!bar_wait(&full[half], (i / kRing) & 1, abort_flag)) return false;
+      if (!bar_wait(&p_full[side], n & 1, abort_flag)) return false;
+      tc_fence_after();
+      const uint32_t sv = v_low + half * (Cfg::kHalf >> 4), o_t = tmem + 256 + side * D, p_t = tmem + side * 128;
+      if (leader) {
 #pragma unroll
-        for (int k = 0; k < kT / 16; ++k)
-          umma_ts(tmem + 256 + side * D, tmem + side * 128 + k * 8, tile_desc_mn(sv + k * 16 * 128, kT * 128), idesc_pv, (n | k) != 0);
+        for (int k = 0; k < kT / 16; ++k) umma_ts(o_t, p_t + k * 8, sv + (k * 16 * 128 >> 4), idesc_pv, (n | k) != 0);
         tc_commit(&o_done[side]);
         if (twice || side) tc_commit(&empty[half]);
-        return true;
-      };
-      if (steps > 0) ok = bar_wait(q_full, 0, abort_flag) && qk(0);
-      if (ok && steps > 1) ok = qk(1);
-      for (int u = 0; u < steps && ok; ++u) {
-        ok = pv(u);
-        if (ok && u + 2 < steps) ok = qk(u + 2);              // (overwrites the scores whose weights P V has just been given)
       }
-      if (!ok) {
-        set_error(a.err, ERR_WAIT_FULL);
-        *abort_flag = 1;
-      }
+      __syncwarp();
+      return true;
+    };
+    if (steps > 0) ok = bar_wait(q_full, 0, abort_flag) && qk(0);
+    if (ok && steps > 1) ok = qk(1);
+    for (int u = 0; u < steps && ok; ++u) {
+      ok = pv(u);
+      if (ok && u + 2 < steps) ok = qk(u + 2);                // (overwrites the scores whose weights P V has just been given)
+    }
+    if (!ok) {
+      set_error(a.err, ERR_WAIT_FULL);
+      *abort_flag = 1;
     }
     __syncwarp();
   } else if (warp < 8) {
