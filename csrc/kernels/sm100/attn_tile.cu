@@ -183,7 +183,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   uint64_t* taken = came + kCame;                             // [slots] the codes have been read
   uint64_t* s_full = taken + kCame;                              // per tile of rows: scores in TMEM,
   uint64_t* p_full = s_full + 2;                              // weights in TMEM,
-  uint64_t* o_done = p_full + 2;                              // P V done
+  uint64_t* o_done = p_full + 2;                              // the last P V done
   uint64_t* q_full = o_done + 2;                              // Q in shared memory
   float2* e_s = reinterpret_cast<float2*>(q_full + 2);        // [4] a key tile's (2^E of K, E of V)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(e_s + 4);
@@ -234,7 +234,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 128);
+      mbar_init(&p_full[s], 4);
       mbar_init(&o_done[s], 1);
     }
     mbar_init(q_full, 256);
@@ -268,18 +268,6 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
 
-  const int* pages = a.block_table + (size_t)seq * a.max_pages;
-  // page and row in it of a token (runs of 64 tokens, or of a smaller page's, lie in one page)
-  auto place = [&](int tok, int& page, int& off) {
-    const int bits = a.page_size < 64 ? 31 - __clz(a.page_size) : 6, per = a.page_size < 64 ? 1 : a.page_size >> 6;
-    const int u = tok >> bits, pi = per == 1 ? u : u / per;
-    off = ((u - pi * per) << bits) + (tok & ((1 << bits) - 1));
-    page = pi < a.max_pages ? pages[pi] : -1;
-    if (page < 0 || page >= a.pool_pages) {
-      set_error(a.err, ERR_BOUNDS);
-      page = 0;
-    }
-  };
   // the order of the halves: K(0), then K(t + 1) before V(t)
   const int items = 2 * ntiles;
   auto item = [&](int i, int& which, int& t) {
@@ -314,51 +302,58 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
           break;
         }
         const uint32_t src = smem_u32(c_s) + slot * Cfg::kCodes, by = smem_u32(b_s) + slot * 2 * kT;
+        // a lane: 8 codes of the row's first half and 8 of its second (one piece of 16-bit values each; D = 64: two neighbours)
+        constexpr int kApart = D == 64 ? 1 : 8;
+        const int p0 = D == 64 ? 2 * c : c, r0 = w4 * kRowsWarp + sub;
+        uint32_t w[kLoads][4], f[kLoads];
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          const int r = r0 + j * 4 * kRowsWarp;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int p = p0 + h * kApart;                    // eight codes: half of a 16-byte piece of the code row
+            const uint32_t at = src + (D == 64 ? r * 64 + (((p >> 1) ^ ((r >> 1) & 3)) << 4) : r * 128 + (((p >> 1) ^ (r & 7)) << 4)) + (p & 1) * 8;
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2 * h]), "=r"(w[j][2 * h + 1]) : "r"(at));
+          }
+          asm volatile("ld.shared.u8 %0, [%1];" : "=r"(f[j]) : "r"(by + r));
+        }
         const int here = to - tok0, top = top_byte(by, here), vtop = which ? 0 : top_byte(by + kT, here);
+        const bool edge = tok0 + kT > clear;
+        bool nan = false;
+        if (edge) {
+#pragma unroll
+          for (int j = 0; j < kLoads; ++j) {
+            if (r0 + j * 4 * kRowsWarp >= here) w[j][0] = w[j][1] = w[j][2] = w[j][3] = 0;      // (not brought: anything may lie there)
+            if (which) {
+              // values that are not finite stay out of the product: rows that see them get them at the end
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t m = __vcmpeq4(w[j][k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                nan |= m != 0;
+                w[j][k] &= ~m;
+              }
+            }
+          }
+        }
         if (!bar_wait(&empty[half], ((i / kRing) & 1) ^ 1, abort_flag)) {
           set_error(a.err, ERR_WAIT_EMPTY);
           *abort_flag = 1;
           ok = false;
           break;
         }
-        const bool edge = tok0 + kT > clear;
         uint8_t* dst = h_s + half * Cfg::kHalf;
-        bool nan = false;
-        // a lane: 8 codes of the row's first half and 8 of its second (one piece of 16-bit values each; D = 64: two neighbours)
-        constexpr int kApart = D == 64 ? 1 : 8;
-        const int p0 = D == 64 ? 2 * c : c;
-#pragma unroll 2
+#pragma unroll
         for (int j = 0; j < kLoads; ++j) {
-          const int r = (j * 4 + w4) * kRowsWarp + sub;
-          uint32_t w[4], b;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int p = p0 + h * kApart;                    // eight codes: half of a 16-byte piece of the code row
-            const uint32_t at = src + (D == 64 ? r * 64 + (((p >> 1) ^ ((r >> 1) & 3)) << 4) : r * 128 + (((p >> 1) ^ (r & 7)) << 4)) + (p & 1) * 8;
-            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[2 * h]), "=r"(w[2 * h + 1]) : "r"(at));
-          }
-          asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b) : "r"(by + r));
-          const uint32_t f = pow2_f16(min((int)b - top, 0) + 6) * 0x10001u;
-          if (edge) {
-            if (tok0 + r >= to) w[0] = w[1] = w[2] = w[3] = 0;            // (not brought: anything may lie there)
-            if (which) {
-              // values that are not finite stay out of the product: rows that see them get them at the end
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t m = __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                nan |= m != 0;
-                w[k] &= ~m;
-              }
-            }
-          }
+          const int r = r0 + j * 4 * kRowsWarp;
+          const uint32_t fj = pow2_f16(min((int)f[j] - top, 0) + 6) * 0x10001u;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t o[4];
-            codes_f16x4(w[2 * h], o[0], o[1]);
-            codes_f16x4(w[2 * h + 1], o[2], o[3]);
+            codes_f16x4(w[j][2 * h], o[0], o[1]);
+            codes_f16x4(w[j][2 * h + 1], o[2], o[3]);
             const int p = p0 + h * kApart;
             *reinterpret_cast<uint4*>(dst + (p >> 3) * (kT * 128) + r * 128 + (((p & 7) ^ (r & 7)) << 4)) =
-                make_uint4(mul_f16x2(o[0], f), mul_f16x2(o[1], f), mul_f16x2(o[2], f), mul_f16x2(o[3], f));
+                make_uint4(mul_f16x2(o[0], fj), mul_f16x2(o[1], fj), mul_f16x2(o[2], fj), mul_f16x2(o[3], fj));
           }
         }
         if (nan) *bad_s = 1;
@@ -410,12 +405,28 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     // ---------------- copies: bf16 halves into the ring, 8-bit codes and scale bytes into their slots ----------------
     const size_t codes = (size_t)2 * a.hk * a.page_size * D, page_bytes = codes + 2 * a.hk * a.page_size;
     const int box = a.page_size < 64 ? a.page_size : 64;
+    const int* pages = a.block_table + (size_t)seq * a.max_pages;
+    // runs of 64 tokens (or of a smaller page's) lie in one page; the table is read 32 pages at a time, a lane each
+    const int bits = a.page_size < 64 ? 31 - __clz(a.page_size) : 6, per = a.page_size < 64 ? 1 : a.page_size >> 6;
+    auto page_of = [&](int tok) { return per == 1 ? tok >> bits : (tok >> bits) / per; };
+    int first = -64, id = 0;
     for (int i = 0; i < items && ok; ++i) {
       int which, t;
       item(i, which, t);
       const int slot = i % kCame, tok0 = from + t * kT, here = min(kT, to - tok0), boxes = (here + box - 1) / box;
-      int page = 0, off = 0;                                  // of the eight tokens from 8 lane on
-      if (lane < kT / 8 && 8 * lane < here) place(tok0 + 8 * lane, page, off);
+      if (page_of(tok0) < first || page_of(tok0 + here - 1) >= first + 32) {
+        // (the values of the tile before are still to come: a tile has 16 pages at most)
+        first = page_of(max(tok0 - kT, from));
+        const int pi = first + lane;
+        id = pi < a.max_pages ? pages[pi] : -1;
+        if (id < 0 || id >= a.pool_pages) {
+          if (pi * a.page_size < to) set_error(a.err, ERR_BOUNDS);
+          id = 0;
+        }
+      }
+      // page, and row in it, of the eight tokens from 8 lane on
+      const int tok = tok0 + 8 * (lane & 15), pi = page_of(tok), off = tok - pi * a.page_size;
+      const int page = __shfl_sync(0xffffffffu, id, (pi - first) & 31);
       if (!bar_wait(E4M3 ? &taken[slot] : &empty[slot], ((i / kCame) & 1) ^ 1, abort_flag)) {
         set_error(a.err, ERR_WAIT_EMPTY);
         *abort_flag = 1;
@@ -476,8 +487,8 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       if (leader) {
 #pragma unroll
         for (int k = 0; k < kT / 16; ++k) umma_ts(o_t, p_t + k * 8, sv + (k * 16 * 128 >> 4), idesc_pv, (n | k) != 0);
-        tc_commit(&o_done[side]);
         if (twice || side) tc_commit(&empty[half]);
+        if (u + 2 >= steps) tc_commit(&o_done[side]);
       }
       __syncwarp();
       return true;
@@ -603,12 +614,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         ref = to_ref;
         l *= corr;
         if (n > 0) {
-          if (!bar_wait(&o_done[side], (n - 1) & 1, abort_flag)) {
-            set_error(a.err, ERR_WAIT_TMEM_EMPTY);
-            *abort_flag = 1;
-            ok = false;
-          }
-          tc_fence_after();
+          // (these scores' products were issued behind the last P V: O is quiet)
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
             uint32_t x[32];
@@ -642,9 +648,10 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       l += E4M3 ? (sum.x + sum.y) * exp2f(-ev) : sum.x + sum.y;
       tmem_st_done();
       tc_fence_before();
-      mbar_arrive(&p_full[side]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[side]);
     }
-    if (ok && steps > 0 && !bar_wait(&o_done[side], (steps - 1) & 1, abort_flag)) {
+    if (ok && steps > 0 && !bar_wait(&o_done[side], 0, abort_flag)) {
       set_error(a.err, ERR_WAIT_TMEM_FULL);
       *abort_flag = 1;
       ok = false;
