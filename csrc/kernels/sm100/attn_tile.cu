@@ -8,8 +8,8 @@
 //                      swizzle that the tensor cores read; bf16 halves lie as they came, and are only looked through where rows
 //                      see different tokens
 //   warp 12            issues the products:  S = Q K^T  and  O += P V  (P from TMEM), for the two tiles in turn
-//   warp 13            copies by TMA: bf16 halves into a ring of five; codes, with their scale bytes, into four slots (two were
-//                      bound by the copies' latency), beside a ring of three halves
+//   warp 13            copies by TMA: bf16 halves into a ring of five; codes, with their scale bytes, into two slots, beside a
+//                      ring of four halves (three would make every V wait for the products of the K before it)
 //
 // The two tiles take turns on the tensor cores: while one's products run, the other's exponentials do. At most 128 rows (a small
 // tree): both tiles are the same rows, on alternate key tiles, and are added up at the end, so the turns remain. TMEM: S and O of
@@ -34,13 +34,13 @@ template <int D, bool E4M3>
 struct TileCfg {
   static constexpr int kQBytes = 2 * kQ * D * 2;
   static constexpr int kHalf = kT * D * 2;                  // a half: a tile of K or of V, as 16-bit values
-  static constexpr int kRing = E4M3 ? 3 : 5;                // halves that the products read
+  static constexpr int kRing = E4M3 ? 4 : 5;                // halves that the products read
   static constexpr int kCodes = E4M3 ? kT * D : 0;          // a half as codes, as it comes
-  static constexpr int kSlots = E4M3 ? 4 : 0;               // of which there are so many under way
+  static constexpr int kSlots = E4M3 ? 2 : 0;               // of which there are so many under way
   static constexpr int kScales = kSlots * 2 * kT;           // with their scale bytes, and V's beside K's
   // room to bring the tiles to a 1024-byte boundary (all of the SM's 227 KB are in use: the base, aligned in practice, is checked)
   static constexpr int kSlack = 768;
-  static constexpr int kSmem = kSlack + kQBytes + kRing * kHalf + kSlots * kCodes + kScales + 2 * kQ * 4 + (E4M3 ? 256 : 512);
+  static constexpr int kSmem = kSlack + kQBytes + kRing * kHalf + kSlots * kCodes + kScales + 2 * kQ * 4 + 512;
   static_assert(kSmem <= 232448, "more shared memory than a CTA has");
 };
 
@@ -225,12 +225,12 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   }
   if (threadIdx.x == 32) {
     for (int s = 0; s < kRing; ++s) {
-      mbar_init(&full[s], 4);
+      mbar_init(&full[s], E4M3 ? 2 : 4);
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < kCame; ++s) {
       mbar_init(&came[s], E4M3 ? 33 : 1);
-      mbar_init(&taken[s], 4);
+      mbar_init(&taken[s], 2);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
@@ -281,17 +281,22 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     // ---------------- keys and values ----------------
     const int tid = threadIdx.x - 256, w4 = warp - 8;
     if constexpr (E4M3) {
-      constexpr int kLanes = D / 16, kRowsWarp = 32 / kLanes, kLoads = kT / (4 * kRowsWarp);     // lanes to a row of codes
+      // two warps to a half, so that two halves are under way; a lane's codes of the whole half are read at once, which frees the
+      // slot for the next copy before the conversion begins
+      constexpr int kLanes = D / 16, kRowsWarp = 32 / kLanes, kLoads = kT / (2 * kRowsWarp);     // lanes to a row of codes
       const int c = lane % kLanes, sub = lane / kLanes;
-      auto top_byte = [&](uint32_t at, int here) -> int {     // the largest of a tile's scale bytes; those behind the end do not count
+      // a lane's four of a tile's scale bytes (those behind the end are 0), and the largest of all
+      auto scale_word = [&](uint32_t at, int here) -> uint32_t {
         uint32_t w;
         asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at + 4 * lane));
         const int n = here - 4 * lane;
-        if (n < 4) w = n <= 0 ? 0u : w & ((1u << (8 * n)) - 1);
+        return n >= 4 ? w : n <= 0 ? 0u : w & ((1u << (8 * n)) - 1);
+      };
+      auto top_byte = [&](uint32_t w) -> int {
         const uint32_t m = __vmaxu4(w, w >> 16);
         return (int)__reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u));
       };
-      for (int i = 0; i < items && ok; ++i) {
+      for (int i = w4 >> 1; i < items && ok; i += 2) {
         int which, t;
         item(i, which, t);
         const int slot = i % kSlots, half = i % kRing, tok0 = from + t * kT;
@@ -304,26 +309,27 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         const uint32_t src = smem_u32(c_s) + slot * Cfg::kCodes, by = smem_u32(b_s) + slot * 2 * kT;
         // a lane: 8 codes of the row's first half and 8 of its second (one piece of 16-bit values each; D = 64: two neighbours)
         constexpr int kApart = D == 64 ? 1 : 8;
-        const int p0 = D == 64 ? 2 * c : c, r0 = w4 * kRowsWarp + sub;
-        uint32_t w[kLoads][4], f[kLoads];
+        const int p0 = D == 64 ? 2 * c : c, here = to - tok0, r0 = (w4 & 1) * kRowsWarp + sub;
+        const bool edge = tok0 + kT > clear;
+        uint32_t w[kLoads][4];
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
-          const int r = r0 + j * 4 * kRowsWarp;
+          const int r = r0 + j * 2 * kRowsWarp;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int p = p0 + h * kApart;                    // eight codes: half of a 16-byte piece of the code row
             const uint32_t at = src + (D == 64 ? r * 64 + (((p >> 1) ^ ((r >> 1) & 3)) << 4) : r * 128 + (((p >> 1) ^ (r & 7)) << 4)) + (p & 1) * 8;
             asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2 * h]), "=r"(w[j][2 * h + 1]) : "r"(at));
           }
-          asm volatile("ld.shared.u8 %0, [%1];" : "=r"(f[j]) : "r"(by + r));
         }
-        const int here = to - tok0, top = top_byte(by, here), vtop = which ? 0 : top_byte(by + kT, here);
-        const bool edge = tok0 + kT > clear;
+        const uint32_t word = scale_word(by, here);
+        const int top = top_byte(word), vtop = which ? 0 : top_byte(scale_word(by + kT, here));
+        if (lane == 0) mbar_arrive(&taken[slot]);             // (the warp's codes are in registers: the reduction above waited for them)
         bool nan = false;
         if (edge) {
 #pragma unroll
           for (int j = 0; j < kLoads; ++j) {
-            if (r0 + j * 4 * kRowsWarp >= here) w[j][0] = w[j][1] = w[j][2] = w[j][3] = 0;      // (not brought: anything may lie there)
+            if (r0 + j * 2 * kRowsWarp >= here) w[j][0] = w[j][1] = w[j][2] = w[j][3] = 0;      // (not brought: anything may lie there)
             if (which) {
               // values that are not finite stay out of the product: rows that see them get them at the end
 #pragma unroll
@@ -344,8 +350,9 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         uint8_t* dst = h_s + half * Cfg::kHalf;
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
-          const int r = r0 + j * 4 * kRowsWarp;
-          const uint32_t fj = pow2_f16(min((int)f[j] - top, 0) + 6) * 0x10001u;
+          const int r = r0 + j * 2 * kRowsWarp;
+          const uint32_t b = __shfl_sync(0xffffffffu, word, r >> 2) >> (8 * (r & 3)) & 255u;
+          const uint32_t fj = pow2_f16(min((int)b - top, 0) + 6) * 0x10001u;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t o[4];
@@ -357,13 +364,10 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
           }
         }
         if (nan) *bad_s = 1;
-        if (!which && tid == 0) e_s[t & 3] = make_float2(pow2i(top - 127 - 6), (float)(vtop - 127 - 6));
+        if (!which && (w4 & 1) == 0 && lane == 0) e_s[t & 3] = make_float2(pow2i(top - 127 - 6), (float)(vtop - 127 - 6));
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&full[half]);
-          mbar_arrive(&taken[slot]);                          // (the codes have been read)
-        }
+        if (lane == 0) mbar_arrive(&full[half]);
       }
     } else {
       for (int i = 0; i < items && ok; ++i) {

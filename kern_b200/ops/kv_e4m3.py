@@ -201,9 +201,9 @@ TILE_ROWS = 32
 
 
 def tile_smem(d: int, e4m3: bool) -> int:
-    """Dynamic shared memory of the many-row kernel: two tiles of Q, a ring of K and V halves as 16-bit values (three, or five where
-    they are copied as they are), four halves of codes with their scale bytes, barriers."""
-    return 768 + 2 * 128 * d * 2 + (3 if e4m3 else 5) * 128 * d * 2 + (4 * (128 * d + 256) if e4m3 else 0) + 1024 + (256 if e4m3 else 512)
+    """Dynamic shared memory of the many-row kernel: two tiles of Q, a ring of K and V halves as 16-bit values (four, or five where
+    they are copied as they are), two halves of codes with their scale bytes, barriers."""
+    return 768 + 2 * 128 * d * 2 + (4 if e4m3 else 5) * 128 * d * 2 + (2 * (128 * d + 256) if e4m3 else 0) + 1024 + 512
 
 
 def tile_shares(ctas: int, max_len: int, sms: int) -> int:
