@@ -24,6 +24,7 @@
 // the tile's largest row, and to 2^-25 of one step beyond); 2^E of the keys is then part of the scores' scale, E of the values part
 // of the weights' exponent, w_ij = 2^(s_ij + E_t - R_i): no work per score.
 #include "attn_rows.cuh"
+#include "f32x2.cuh"
 
 namespace kern {
 
@@ -126,27 +127,6 @@ KERN_DEVICE void tmem_st64(uint32_t taddr, const uint32_t (&r)[64]) {
       "r"(r[48]), "r"(r[49]), "r"(r[50]), "r"(r[51]), "r"(r[52]), "r"(r[53]), "r"(r[54]), "r"(r[55]),
       "r"(r[56]), "r"(r[57]), "r"(r[58]), "r"(r[59]), "r"(r[60]), "r"(r[61]), "r"(r[62]), "r"(r[63])
       : "memory");
-}
-// two f32 in one register pair: one instruction for both
-KERN_DEVICE uint64_t pair64(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-KERN_DEVICE float2 split64(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-KERN_DEVICE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-KERN_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
 }
 KERN_DEVICE float max3(float a, float b, float c) {
   float r;

@@ -20,7 +20,7 @@ LOG2E = 1.4426950408889634
 HEAD_DIMS = (64, 128, 256)
 
 # the kernels' parameter blocks, in their order (native alignment)
-_APPEND = struct.Struct("9Q5if2iq3iQ")
+_APPEND = struct.Struct("9Q4ifiq3iQ")
 _READ = struct.Struct("3Q3iqQ")
 _ROWS = struct.Struct("128s9Q10ifQ")
 _MERGE = struct.Struct("5Q6i")
@@ -148,11 +148,11 @@ def rope_kv_append_e4m3(qkv: torch.Tensor, pool: torch.Tensor, positions: torch.
     if t:
         k = Kernels.get(gpu)
         image = _APPEND.pack(qkv.data_ptr(), q_out.data_ptr(), pool.data_ptr(), positions.data_ptr(), slots.data_ptr(), cos.data_ptr(),
-                             sin.data_ptr(), 0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), t, hq, hk,
-                             rot, page_size, eps, bool(norm_plus_one), pairs == "interleaved", pages * page_size, max_pos, qkv_step, out_step,
-                             k.err_ptr)
+                             sin.data_ptr(), 0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), hq, hk,
+                             rot, page_size, eps, bool(norm_plus_one), pages * page_size, max_pos, qkv_step, out_step, k.err_ptr)
+        norm = "" if q_norm is None and k_norm is None else "_norm"
         with on_device(qkv):
-            k.launch_image("kv_e4m3", f"kern_rope_kv_append_e4m3_d{d}", t, 1, 1, 256, image)
+            k.launch_image("kv_e4m3", f"kern_rope_kv_append_e4m3_{pairs}{norm}_d{d}", t, 1, 1, 128, image)
     return q_out[:t, : hq * d]
 
 
@@ -172,7 +172,7 @@ def read_rows_e4m3(pool: torch.Tensor, slots: torch.Tensor, hk: int, d: int, pag
         k = Kernels.get(gpu)
         image = _READ.pack(pool.data_ptr(), slots.data_ptr(), out.data_ptr(), t, hk, page_size, pages * page_size, k.err_ptr)
         with on_device(pool):
-            k.launch_image("kv_e4m3", f"kern_kv_read_e4m3_d{d}", -(-t * 2 * hk * (d // 8) // 256), 1, 1, 256, image)
+            k.launch_image("kv_e4m3", f"kern_kv_read_e4m3_d{d}", t, 1, 1, 128, image)
     return out
 
 

@@ -165,6 +165,41 @@ def test_append_of_values_at_the_edges(cuda):
     assert torch.equal(back[~nan], K8.dequantise_reference(codes, scales)[~nan])
 
 
+@pytest.mark.parametrize("pairs", ["half", "interleaved"])
+@pytest.mark.parametrize("norm", [False, True])
+def test_codes_are_those_of_the_exact_values(cuda, pairs, norm):
+    """Over many rows no code differs from that of the key in 64 bits: values next to a border are decided there."""
+    hq, hk, d, page, t = 8, 8, 128, 64, 4096
+    g = torch.Generator().manual_seed(11)
+    qkv = torch.randn(t, (hq + 2 * hk) * d, generator=g).bfloat16()
+    qkv[5, hq * d:(hq + 1) * d] = 0.5                       # with a cosine of 1: ties, and a power of two's border
+    qkv[6, hq * d + 3] = float("inf")
+    positions = torch.randint(0, 2000, (t,), generator=g)
+    positions[5] = 0
+    ang = torch.arange(2000, dtype=torch.float64)[:, None] * 1e4 ** (-torch.arange(0, d // 4, dtype=torch.float64) * 4 / d)
+    cos, sin = ang.cos().float(), ang.sin().float()         # half of the head turns
+    kn = (1 + 0.2 * torch.randn(d, generator=g)).bfloat16() if norm else None
+    pool = K8.new_pool(t // page, hk, page, d, cuda)
+    slots = torch.arange(t, device=cuda)
+    K8.rope_kv_append_e4m3(qkv.cuda(), pool, positions.cuda(), slots, cos.cuda(), sin.cuda(), hq, hk, d, page, rot=d // 2, pairs=pairs,
+                           k_norm=None if kn is None else kn.cuda(), eps=1e-6)
+    k = qkv[:, hq * d:(hq + hk) * d].double().view(t, hk, d)
+    if norm:
+        k = k / torch.sqrt(k.pow(2).mean(-1, keepdim=True) + 1e-6) * kn.double()
+    k = rotated64(k, cos[positions][:, None].double(), sin[positions][:, None].double(), d // 2, pairs)
+    k = torch.where(torch.isfinite(k), k, float("nan"))
+    top = k.nan_to_num(0.0).abs().amax(-1)
+    e = torch.where(top > 0, torch.ceil(torch.log2(top / 448)), -40.0).clamp(-40, 119)
+    u = (k * torch.exp2(-e)[..., None]).abs()
+    ulp = torch.exp2(torch.floor(torch.log2(u.clamp(min=2.0 ** -6))) - 3)
+    want = torch.sign(k) * torch.round(u / ulp) * ulp       # to nearest, ties to even
+    codes, scales = K8.views(pool, hk, page, d)
+    got = codes[:, 0].permute(0, 2, 1, 3).reshape(t, hk, d).float().double().cpu()
+    assert torch.equal(scales[:, 0].permute(0, 2, 1).reshape(t, hk).cpu().double() - 127, e)
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), fin) and torch.equal(got[fin], want[fin])
+
+
 LAYOUTS = [(32, 8, 128, 64), (4, 2, 64, 16), (24, 4, 256, 64), (16, 1, 128, 8), (5, 5, 64, 128), (12, 4, 128, 32)]
 
 
