@@ -66,7 +66,9 @@ void bind_device(py::module_& m) {
   m.def("cupti_dropped", [] { return CuptiTrace::get().dropped(); });
 
   py::class_<PyModule>(m, "Module");
-  py::class_<PyFunction>(m, "Function").def_readonly("name", &PyFunction::name);
+  py::class_<PyFunction>(m, "Function").def_readonly("name", &PyFunction::name).def_property_readonly("handle", [](const PyFunction& f) {
+    return reinterpret_cast<uint64_t>(f.f);
+  });
   py::class_<PyGraph, std::shared_ptr<PyGraph>>(m, "Graph").def_readonly("nodes", &PyGraph::nodes);
 
   py::class_<Device, std::shared_ptr<Device>>(m, "Device")
@@ -117,26 +119,6 @@ void bind_device(py::module_& m) {
           py::arg("function"), py::arg("grid"), py::arg("block"), py::arg("shared_mem"),
           py::arg("stream"), py::arg("params"),
           py::arg("cluster") = std::array<unsigned, 3>{1, 1, 1}, py::arg("pdl") = false)
-      .def(
-          "launch_image",
-          [](Device& d, const PyFunction& f, unsigned gx, unsigned gy, unsigned gz, unsigned threads, unsigned shared_mem, uint64_t stream,
-             py::bytes image, bool pdl, unsigned cluster_z) {
-            LaunchDims dims;
-            dims.grid[0] = gx; dims.grid[1] = gy; dims.grid[2] = gz;
-            dims.block[0] = threads; dims.block[1] = dims.block[2] = 1;
-            dims.cluster[0] = dims.cluster[1] = 1; dims.cluster[2] = cluster_z;
-            dims.shared_mem = shared_mem;
-            dims.pdl = pdl;
-            char* data = nullptr;
-            Py_ssize_t size = 0;
-            if (PyBytes_AsStringAndSize(image.ptr(), &data, &size) != 0) throw py::error_already_set();
-            alignas(64) uint8_t block[4096];              // a kernel's parameters: 4 KB at most here
-            if ((size_t)size > sizeof(block)) throw std::runtime_error("a parameter block of more than 4096 bytes");
-            std::memcpy(block, data, size);
-            d.launch(f.f, dims, reinterpret_cast<CUstream>(stream), nullptr, block, size);
-          },
-          py::arg("function"), py::arg("gx"), py::arg("gy"), py::arg("gz"), py::arg("threads"), py::arg("shared_mem"), py::arg("stream"),
-          py::arg("image"), py::arg("pdl") = false, py::arg("cluster_z") = 1)
       .def(
           "encode_tensor_map",
           [](Device& d, uint64_t base, int dtype, std::vector<uint64_t> dims,

@@ -104,7 +104,7 @@ KERN_DEVICE void append_body(const AppendArgs& a) {
   if (pos64 < 0 || pos64 >= a.max_pos || slot64 >= a.kv_slots) {
     if (threadIdx.x == 0) set_error(a.err, ERR_BOUNDS);
     if (pos64 < 0 || pos64 >= a.max_pos) pos = 0;
-    if (slot64 >= a.kv_slots) slot = -1;
+    slot = -1;
   }
   if (slot64 < 0) slot = -1;
   const int half = a.rot >> 1;

@@ -162,6 +162,26 @@ def build_native(force: bool = False) -> Path:
     return out
 
 
+def ops_host_path() -> Path:
+    return PKG / ("_ops_host" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_ops_host(force: bool = False) -> Path:
+    """Compile the host side of the short operators (``csrc/bindings/torch``) into ``kern_b200/_ops_host*.so``, against the
+    PyTorch of this environment."""
+    out, src = ops_host_path(), CSRC / "bindings" / "torch" / "ops_host.cpp"
+    if not force and not _newer([src, *(CSRC / "runtime").glob("*.hpp")], out):
+        return out
+    import torch
+    from torch.utils import cpp_extension
+
+    inc = [a for p in (*cpp_extension.include_paths(), sysconfig.get_paths()["include"], "/usr/local/cuda/include", str(CSRC)) for a in ("-isystem" if p != str(CSRC) else "-I", p)]
+    libs = [a for p in cpp_extension.library_paths() for a in ("-L", p)]
+    _run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          "-DTORCH_EXTENSION_NAME=_ops_host", *inc, "-o", str(out), str(src), *libs, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-ldl"])
+    return out
+
+
 def build_cli(force: bool = False) -> Path:
     """The native `kern` binary (verify / cut / print): the manifest library and a main, nothing else."""
     out = PKG / "bin" / "kern"
@@ -220,6 +240,7 @@ def build_all(force: bool = False, verbose: bool = False) -> None:
             if checked() or "--checked" in sys.argv:
                 build_kernels(force, verbose, checked_build=True)
             build_native(force)
+            build_ops_host(force)
             build_cli(force)
             build_runner(force)
             build_capture(force)
@@ -253,7 +274,7 @@ def ensure_built() -> None:
     """Build whatever is missing or stale. Cheap when everything is current."""
     try:
         if on_demand():
-            _locked(build_native)
+            _locked(lambda: (build_native(), build_ops_host()))
             return
         build_all(False)
     except FileNotFoundError as e:  # no compiler on this machine: use what is in the tree

@@ -12,7 +12,7 @@ from pathlib import Path
 
 import torch
 
-from .. import _native
+from .. import _native, _ops_host
 
 KDIR = Path(__file__).resolve().parent.parent / "kernels"
 
@@ -61,7 +61,7 @@ class Kernels:
         self._modules: dict[str, object] = {}
         self._functions: dict[tuple[str, str], object] = {}
         self._tmaps: dict[tuple, bytes] = {}
-        self.launches = 0  # count of kernel launches issued through this object
+        self._launches = 0
         self._err = None
 
     @classmethod
@@ -82,6 +82,11 @@ class Kernels:
             return k
 
     @property
+    def launches(self) -> int:
+        """Kernel launches issued through this object and through the host side of the short operators."""
+        return self._launches + _ops_host.launches(self.gpu)
+
+    @property
     def sm_count(self) -> int:
         return self.dev.sm_count
 
@@ -89,15 +94,7 @@ class Kernels:
         """A device int32 that kernels set when a bounded wait ran out or a checked index failed."""
         if self._err is None:
             self._err = torch.zeros(1, dtype=torch.int32, device=f"cuda:{self.gpu}")
-            self._err_ptr = self._err.data_ptr()
         return self._err
-
-    @property
-    def err_ptr(self) -> int:
-        """The error word's address."""
-        if self._err is None:
-            self.err_word()
-        return self._err_ptr
 
     def check_error(self) -> None:
         code = int(self.err_word().item())
@@ -126,17 +123,7 @@ class Kernels:
         g = tuple(grid) + (1,) * (3 - len(grid))
         b = tuple(block) + (1,) * (3 - len(block))
         self.dev.launch(f, list(g), list(b), shared_mem, stream, params, list(cluster), pdl)
-        self.launches += 1
-
-    def launch_image(self, module: str, entry: str, gx: int, gy: int, gz: int, threads: int, image: bytes, shared_mem: int = 0,
-                     pdl: bool = False, cluster_z: int = 1) -> None:
-        """`launch` for calls whose issue is a good part of their time: the parameters as one block, packed by the caller at
-        their natural alignment (a tensor map first), on the device's current stream."""
-        f = self._functions.get((module, entry))
-        if f is None:
-            f = self.function(module, entry)
-        self.dev.launch_image(f, gx, gy, gz, threads, shared_mem, torch._C._cuda_getCurrentRawStream(self.gpu), image, pdl, cluster_z)
-        self.launches += 1
+        self._launches += 1
 
     def tensor_map_2d(self, t: torch.Tensor, box_rows: int, box_cols: int, swizzle: int = 128,
                       rows: int | None = None) -> bytes:
@@ -154,3 +141,12 @@ class Kernels:
                 self._tmaps.clear()
             self._tmaps[key] = tm
         return tm
+
+
+def _provide(gpu: int) -> None:
+    """What the host side of the short operators (`_ops_host`) needs of a GPU, at its first call there."""
+    k = Kernels.get(gpu)
+    _ops_host.provide(gpu, k.sm_count, k.err_word().data_ptr(), lambda module, entry: k.function(module, entry).handle)
+
+
+_ops_host.on_missing(_provide)
