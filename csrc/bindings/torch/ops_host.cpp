@@ -239,22 +239,25 @@ RowsForm rows_form(int64_t d, bool e4m3, int64_t nt) {
   return {(unsigned)(1024 + stages * (stage + (e4m3 ? 2 * tile : 0)) + (d == 256 && nt > 1 ? nt * d * 16 : 0) + 256), per_sm};
 }
 // Shares that a row's context is cut into, and CTAs of a cluster: as many as fill the SMs once, two where the rows alone fill them up
-// to four times (a share's end then leaves less of the last wave idle), none of under 128 tokens. Up to 8 shares are one cluster,
-// more are clusters of 8 and a joining launch.
+// to four times (a share's end then leaves less of the last wave idle), none of under 128 tokens. Up to 8 shares are one cluster;
+// more are on their own, and joined by a second launch.
+int64_t g_shares = 0, g_cluster = 0;
 std::pair<int64_t, int64_t> rows_shares(int64_t ctas, int64_t max_len, int64_t resident) {
+  if (g_shares) return {g_shares, g_cluster};
   const int64_t most = std::max<int64_t>(1, (max_len + 127) / 128);
   const int64_t want = std::min<int64_t>({most, ctas < resident ? resident / ctas : ctas < 4 * resident ? 2 : 1, 256});
+  if (want > 8) return {want, 1};
   const int64_t cluster = want >= 8 ? 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
-  return {want / cluster * cluster, cluster};
+  return {cluster, cluster};
 }
 // The many-row kernel: two tiles of Q, a ring of K and V halves as 16-bit values (four, or five where they are copied as they are),
 // two halves of codes with their scale bytes, barriers.
 unsigned tile_shared(int64_t d, bool e4m3) {
-  return (unsigned)(768 + 2 * 128 * d * 2 + (e4m3 ? 4 : 5) * 128 * d * 2 + (e4m3 ? 2 * (128 * d + 256) : 0) + 1024 + 512);
+  return (unsigned)(2 * 128 * d * 2 + (e4m3 ? 4 : 5) * 128 * d * 2 + (e4m3 ? 2 * (128 * d + 256) : 0) + 4 * 128 * 4 + 512);
 }
 int64_t tile_shares(int64_t ctas, int64_t max_len, int64_t sms) {
-  if (ctas >= sms) return 1;
-  return std::max<int64_t>(1, std::min<int64_t>({(3 * sms + ctas - 1) / ctas, (max_len + 511) / 512, 64}));
+  if (g_shares) return g_shares;
+  return std::max<int64_t>(1, std::min<int64_t>({sms / ctas, (max_len + 255) / 256, 64}));
 }
 int64_t g_tile_rows = 32;       // query rows of a sequence and kv head above which the many-row kernel runs (head_dim 64 and 128)
 
@@ -311,50 +314,62 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
   if (!seqs || max_rows == 0) return out;
   Host& h = host_of(gpu);
   const int64_t g = hq / hk;
-  std::string entry = g * max_rows > g_tile_rows && d <= 128 ? "attn_tile" : "attn_rows", name = "kern_" + entry;
-  name += std::string(e4m3 ? "_e4m3" : "_bf16") + (masks ? "_tree_d" : "_causal_d") + n(d);
-  int64_t toks, cluster = 1, shares, gx, gy, last;
-  unsigned threads, shared;
-  if (entry == "attn_tile") {
-    toks = 256 / g;
-    gy = std::min(rows / toks + seqs, seqs * ((max_rows + toks - 1) / toks));              // blocks of all sequences, at most
-    shares = tile_shares(hk * gy, max_len, h.sms);
-    gx = hk;
-    last = seqs;
-    threads = 512;
-    shared = tile_shared(d, e4m3);
-  } else {
-    // query rows of a CTA: the fewest eights that hold a sequence's, up to what registers hold
-    const int64_t nt = g * max_rows <= 8 ? 1 : g * max_rows <= 16 || d == 256 ? 2 : 4;
-    toks = 8 * nt / g;
-    const int64_t blocks = (max_rows + toks - 1) / toks;
-    const RowsForm form = rows_form(d, e4m3, nt);
-    std::tie(shares, cluster) = rows_shares(hk * blocks * seqs, max_len, (int64_t)h.sms * form.per_sm);
-    gx = hk * blocks;
-    gy = seqs;
-    last = cluster;
-    threads = 160;
-    shared = form.shared;
-    name += "_n" + n(nt);
-  }
-  if (gy > 65535) refuse("more blocks of rows than a launch has: split the call");
-  Tensor ws;
-  uint64_t ws_o = 0, ws_ml = 0;
-  const int64_t groups = shares / cluster;
-  if (groups > 1) {
-    ws = at::empty({rows * hq * groups * (d + 2)}, typed(q, at::kFloat));
-    ws_o = reinterpret_cast<uint64_t>(ws.data_ptr());
-    ws_ml = ws_o + 4 * (uint64_t)(rows * hq * groups * d);
-  }
   const auto map = pool_map(h, pool, e4m3, pages, hk, d, page);
-  Block b;
-  b.bytes(map.data(), map.size()).at(q).at(out).put(ws_o).put(ws_ml).at(pool).at(table).at(lens).at(cu_q).at(masks);
-  b.ints(masks ? masks->size(1) : 0, rows_per_seq, hq, hk, q_step, out_step, width, page, last, pages).put((float)(scale * kLog2e)).put(h.err);
-  launch(h, entry.c_str(), name, gx, gy, shares, threads, b, shared, false, (unsigned)cluster);
-  if (groups > 1) {
-    Block m;
-    m.put(ws_o).put(ws_ml).at(out).at(lens).at(cu_q).ints(rows_per_seq, hq, toks, shares, cluster, out_step);
-    launch(h, "attn_rows", std::string("kern_attn_rows_merge_") + (masks ? "tree_d" : "causal_d") + n(d), (max_rows * hq + 7) / 8, seqs, 1, 256, m, 0, true);
+  const std::string form = std::string(e4m3 ? "_e4m3" : "_bf16") + (masks ? "_tree_d" : "_causal_d") + n(d);
+  // one kernel over the sequences of lo .. hi rows
+  auto run = [&](bool tiled, int64_t lo, int64_t hi) {
+    const int64_t most = std::min(max_rows, hi);
+    int64_t toks, cluster = 1, shares, gx, gy;
+    unsigned shared;
+    std::string name;
+    if (tiled) {
+      toks = 256 / g;
+      gy = std::min(rows / toks + seqs, seqs * ((most + toks - 1) / toks));                // blocks of all sequences, at most
+      shares = tile_shares(hk * gy, max_len, h.sms);
+      gx = hk;
+      shared = tile_shared(d, e4m3);
+      name = "kern_attn_tile" + form;
+    } else {
+      // query rows of a CTA: the fewest eights that hold a sequence's, up to what registers hold
+      const int64_t nt = g * most <= 8 ? 1 : g * most <= 16 || d == 256 ? 2 : 4;
+      toks = 8 * nt / g;
+      const int64_t blocks = (most + toks - 1) / toks;
+      const RowsForm f = rows_form(d, e4m3, nt);
+      std::tie(shares, cluster) = rows_shares(hk * blocks * seqs, max_len, (int64_t)h.sms * f.per_sm);
+      gx = hk * blocks;
+      gy = seqs;
+      shared = f.shared;
+      name = "kern_attn_rows" + form + "_n" + n(nt);
+    }
+    if (gy > 65535) refuse("more blocks of rows than a launch has: split the call");
+    Tensor ws;
+    uint64_t ws_o = 0, ws_ml = 0;
+    const int64_t groups = shares / cluster;
+    if (groups > 1) {
+      ws = at::empty({rows * hq * groups * (d + 2)}, typed(q, at::kFloat));
+      ws_o = reinterpret_cast<uint64_t>(ws.data_ptr());
+      ws_ml = ws_o + 4 * (uint64_t)(rows * hq * groups * d);
+    }
+    Block b;
+    b.bytes(map.data(), map.size()).at(q).at(out).put(ws_o).put(ws_ml).at(pool).at(table).at(lens).at(cu_q).at(masks);
+    b.ints(masks ? masks->size(1) : 0, rows_per_seq, hq, hk, q_step, out_step, width, page, tiled ? seqs : cluster, pages, lo, hi);
+    b.put((float)(scale * kLog2e)).put(h.err);
+    launch(h, tiled ? "attn_tile" : "attn_rows", name, gx, gy, shares, tiled ? 704 : 160, b, shared, false, (unsigned)cluster);
+    if (groups > 1) {
+      Block m;
+      m.put(ws_o).put(ws_ml).at(out).at(lens).at(cu_q).ints(rows_per_seq, hq, toks, shares, cluster, out_step, lo, hi);
+      launch(h, "attn_rows", std::string("kern_attn_rows_merge_") + (masks ? "tree_d" : "causal_d") + n(d), most * hq, seqs, 1, 128, m, 0, true);
+    }
+  };
+  const int64_t all = INT32_MAX, few = std::max<int64_t>(1, 8 / g);
+  if (g * max_rows <= g_tile_rows || d > 128) {
+    run(false, 1, all);
+  } else if (!cu_q || seqs == 1 || rows + few >= seqs * max_rows) {
+    run(true, 1, all);                                       // (rows alike)
+  } else {
+    // sequences of single tokens among prompt chunks keep the few-row kernel, which cuts their contexts into shares
+    run(true, few + 1, all);
+    run(false, 1, few);
   }
   return out;
 }
@@ -441,6 +456,7 @@ PYBIND11_MODULE(_ops_host, m) {
     if (rows) g_tile_rows = *rows;
     return was;
   }, py::arg("rows") = py::none());
+  m.def("tune", [](int64_t s, int64_t c) { g_shares = s; g_cluster = c; });
   m.def("append", &append);
   m.def("read_rows", &read_rows);
   m.def("attend", &attend);

@@ -163,7 +163,7 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
   const int R = a.cu_q ? a.cu_q[seq + 1] - row0 : a.rows_per_seq;
   const int toks = kRows / G;
   const int tok_lo = blk * toks;
-  if (tok_lo >= R) return;                                   // uniform over the cluster
+  if (tok_lo >= R || R < a.row_lo || R > a.row_hi) return;   // uniform over the cluster
   const int valid = min(toks, R - tok_lo) * G;
   const int past = L - R;                                    // what the sequence had before this call's rows
   // causal: the last row of the block decides how far the walk goes
@@ -698,31 +698,35 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
   }
 }
 
-// Joins the groups of shares of every row that was cut further than a cluster reaches: a warp per (row, head), D / 32 columns a
-// lane. grid (ceil(max_rows * hq / 8), seqs).
+// Joins the groups of shares of every row that was cut further than a cluster reaches. A block per (row, head): its four warps take
+// every fourth group, D / 32 columns a lane, and are added up in shared memory. grid (max_rows * hq, seqs). What it takes is the
+// latency of two dependent loads; what does not come from the launch before it is read ahead of it.
+constexpr int kMergeThreads = 128;
 template <int D, bool TREE>
 KERN_DEVICE void rows_merge(const float* ws_o, const float* ws_ml, __nv_bfloat16* out, const int* seq_lens, const int* cu_q, int rows_per_seq,
-                            int hq, int toks, int splits, int cluster, int out_stride) {
-  pdl_wait();
-  const int lane = threadIdx.x & 31, seq = blockIdx.y;
-  const int at = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+                            int hq, int toks, int splits, int cluster, int out_stride, int row_lo, int row_hi) {
+  constexpr int N = D / 32;
+  __shared__ float y_s[4][D], l_s[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.y;
   const int row0 = cu_q ? cu_q[seq] : seq * rows_per_seq, R = cu_q ? cu_q[seq + 1] - row0 : rows_per_seq;
-  const int tok = at / hq, head = at % hq;
-  if (tok >= R) return;
+  const int tok = blockIdx.x / hq, head = blockIdx.x % hq;
+  if (tok >= R || R < row_lo || R > row_hi) return;
   const int L = max(seq_lens[seq], 0), lo = tok / toks * toks;
   const int end = TREE ? L : max(0, L - R + lo + min(toks, R - lo));
   const int shares = rows_shares(end, splits);
   if (shares <= cluster) return;                              // written by its one cluster
   const int groups = splits / cluster, live = (shares + cluster - 1) / cluster;
   const size_t base = ((size_t)(row0 + tok) * hq + head) * groups;
+  pdl_wait();
+  // every warp: the largest reference of all groups
   float m = kUnset;
-  for (int s = 0; s < live; ++s) m = fmaxf(m, ws_ml[(base + s) * 2]);
-  constexpr int N = D / 32;
+  for (int s = lane; s < live; s += 32) m = fmaxf(m, ws_ml[(base + s) * 2]);
+  m = warp_max(m);
   float y[N], l = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) y[i] = 0.f;
 #pragma unroll 8
-  for (int s = 0; s < live; ++s) {
+  for (int s = warp; s < live; s += 4) {
     const float ms = ws_ml[(base + s) * 2], ls = ws_ml[(base + s) * 2 + 1];
     const float f = ls == 0.f ? 0.f : exp2f(ms - m);
     l += f * ls;
@@ -730,10 +734,16 @@ KERN_DEVICE void rows_merge(const float* ws_o, const float* ws_ml, __nv_bfloat16
 #pragma unroll
     for (int i = 0; i < N; ++i) y[i] += f * src[i];
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  __nv_bfloat16* dst = out + (size_t)(row0 + tok) * out_stride + (size_t)head * D + lane * N;
 #pragma unroll
-  for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(y[i] * inv, y[i + 1] * inv);
+  for (int i = 0; i < N; ++i) y_s[warp][lane * N + i] = y[i];
+  if (lane == 0) l_s[warp] = l;
+  __syncthreads();
+  l = l_s[0] + l_s[1] + l_s[2] + l_s[3];
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __nv_bfloat16* dst = out + (size_t)(row0 + tok) * out_stride + (size_t)head * D;
+  for (int c = threadIdx.x * 2; c < D; c += 2 * kMergeThreads)
+    *reinterpret_cast<uint32_t*>(dst + c) = pack_bf16x2((y_s[0][c] + y_s[1][c] + y_s[2][c] + y_s[3][c]) * inv,
+                                                        (y_s[0][c + 1] + y_s[1][c + 1] + y_s[2][c + 1] + y_s[3][c + 1]) * inv);
 }
 
 }  // namespace kern
@@ -746,16 +756,16 @@ using namespace kern;
           const __grid_constant__ CUtensorMap kv_map, const __nv_bfloat16* q, __nv_bfloat16* out, float* ws_o, float* ws_ml,      \
           const uint8_t* pool, const int* block_table, const int* seq_lens, const int* cu_q, const long long* masks, int words,   \
           int rows_per_seq, int hq, int hk, int q_stride, int out_stride, int max_pages, int page_size, int cluster,              \
-          int pool_pages, float scale_log2, int* err) {                                                                           \
+          int pool_pages, int row_lo, int row_hi, float scale_log2, int* err) {                                                                           \
     rows_body<D, E4M3, TREE, NT>(&kv_map, RowsArgs{q, out, ws_o, ws_ml, pool, block_table, seq_lens, cu_q, masks, err, words,     \
                                                    rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, cluster,     \
-                                                   pool_pages, scale_log2});                                                      \
+                                                   pool_pages, row_lo, row_hi, scale_log2});                                                      \
   }
 #define KERN_ROWS_MERGE(D, FORM, TREE)                                                                                            \
-  extern "C" __global__ void __launch_bounds__(256) kern_attn_rows_merge_##FORM##_d##D(                                           \
+  extern "C" __global__ void __launch_bounds__(kMergeThreads) kern_attn_rows_merge_##FORM##_d##D(                                           \
       const float* ws_o, const float* ws_ml, __nv_bfloat16* out, const int* seq_lens, const int* cu_q, int rows_per_seq, int hq,  \
-      int toks, int splits, int cluster, int out_stride) {                                                                        \
-    rows_merge<D, TREE>(ws_o, ws_ml, out, seq_lens, cu_q, rows_per_seq, hq, toks, splits, cluster, out_stride);                   \
+      int toks, int splits, int cluster, int out_stride, int row_lo, int row_hi) {                                                \
+    rows_merge<D, TREE>(ws_o, ws_ml, out, seq_lens, cu_q, rows_per_seq, hq, toks, splits, cluster, out_stride, row_lo, row_hi);   \
   }
 #define KERN_ROWS_FORMS(D, NT)                      \
   KERN_ROWS_ENTRY(D, e4m3, true, causal, false, NT) \

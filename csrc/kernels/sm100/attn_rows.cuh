@@ -22,6 +22,7 @@ struct RowsArgs {
   const long long* masks;    // (tree) [row][words]
   int* err;
   int words, rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, cluster, pool_pages;
+  int row_lo, row_hi;        // sequences of other row counts are another launch's
   float scale_log2;
 };
 

@@ -1,14 +1,15 @@
 // Attention of many query rows over a paged cache, bf16 or e4m3, on the 5th-generation tensor cores: prompt chunks (causal) and
 // trees of drafted tokens. The formulas, formats and what a row sees are those of attn_rows.cu, which has the few rows.
 //
-// One CTA = (256 query rows: the G heads of 256 / G tokens, one kv head, a share of the context), 16 warps:
+// One CTA = (256 query rows: the G heads of 256 / G tokens, one kv head, a share of the context), 22 warps:
 //
-//   warps 0..3, 4..7   softmax of one 128-row tile each, a thread to a row: scores out of TMEM, weights back into TMEM over them
-//   warps 8..11        halves (a tile of 128 keys, or of values) for the products to read: 8-bit codes become f16 there, in the
+//   warps 0..15        softmax of two 128-row tiles, two threads to a row, 64 of a tile's scores each: scores out of TMEM, weights
+//                      back into TMEM over them
+//   warps 16..19       halves (a tile of 128 keys, or of values) for the products to read: 8-bit codes become f16 there, in the
 //                      swizzle that the tensor cores read; bf16 halves lie as they came, and are only looked through where rows
 //                      see different tokens
-//   warp 12            issues the products:  S = Q K^T  and  O += P V  (P from TMEM), for the two tiles in turn
-//   warp 13            copies by TMA: bf16 halves into a ring of five; codes, with their scale bytes, into two slots, beside a
+//   warp 20            issues the products:  S = Q K^T  and  O += P V  (P from TMEM), for the two tiles in turn
+//   warp 21            copies by TMA: bf16 halves into a ring of five; codes, with their scale bytes, into two slots, beside a
 //                      ring of four halves (three would make every V wait for the products of the K before it)
 //
 // The two tiles take turns on the tensor cores: while one's products run, the other's exponentials do. At most 128 rows (a small
@@ -29,7 +30,7 @@
 namespace kern {
 
 constexpr int kQ = 128, kT = 128;    // query rows of a tile, tokens of a tile
-constexpr int kTileThreads = 512;
+constexpr int kTileThreads = 704;
 
 template <int D, bool E4M3>
 struct TileCfg {
@@ -39,9 +40,8 @@ struct TileCfg {
   static constexpr int kCodes = E4M3 ? kT * D : 0;          // a half as codes, as it comes
   static constexpr int kSlots = E4M3 ? 2 : 0;               // of which there are so many under way
   static constexpr int kScales = kSlots * 2 * kT;           // with their scale bytes, and V's beside K's
-  // room to bring the tiles to a 1024-byte boundary (all of the SM's 227 KB are in use: the base, aligned in practice, is checked)
-  static constexpr int kSlack = 768;
-  static constexpr int kSmem = kSlack + kQBytes + kRing * kHalf + kSlots * kCodes + kScales + 2 * kQ * 4 + 512;
+  // (all of the SM's 227 KB are in use: that the base lies on a 1024-byte boundary, as it does in practice, is checked)
+  static constexpr int kSmem = kQBytes + kRing * kHalf + kSlots * kCodes + kScales + 4 * kQ * 4 + 512;
   static_assert(kSmem <= 232448, "more shared memory than a CTA has");
 };
 
@@ -91,41 +91,11 @@ KERN_DEVICE void tmem_st32(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 KERN_DEVICE void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// 64 columns of this thread's TMEM lane
-KERN_DEVICE void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+KERN_DEVICE void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
-      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-      : "r"(taddr)
-      : "memory");
-}
-KERN_DEVICE void tmem_st64(uint32_t taddr, const uint32_t (&r)[64]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x64.b32 [%0], {"
-      "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, "
-      "%33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, "
-      "%49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, %64};"
-      ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
-      "r"(r[32]), "r"(r[33]), "r"(r[34]), "r"(r[35]), "r"(r[36]), "r"(r[37]), "r"(r[38]), "r"(r[39]),
-      "r"(r[40]), "r"(r[41]), "r"(r[42]), "r"(r[43]), "r"(r[44]), "r"(r[45]), "r"(r[46]), "r"(r[47]),
-      "r"(r[48]), "r"(r[49]), "r"(r[50]), "r"(r[51]), "r"(r[52]), "r"(r[53]), "r"(r[54]), "r"(r[55]),
-      "r"(r[56]), "r"(r[57]), "r"(r[58]), "r"(r[59]), "r"(r[60]), "r"(r[61]), "r"(r[62]), "r"(r[63])
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 KERN_DEVICE float max3(float a, float b, float c) {
@@ -147,8 +117,8 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   using Cfg = TileCfg<D, E4M3>;
   constexpr int kRing = Cfg::kRing, kSlots = Cfg::kSlots, kCame = E4M3 ? kSlots : kRing;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  if ((int)(smem - smem_raw) > Cfg::kSlack) {                 // uniform, before any barrier or allocation
+  uint8_t* smem = smem_raw;
+  if (smem_u32(smem) & 1023) {                                // uniform, before any barrier or allocation
     if (threadIdx.x == 0) set_error(a.err, ERR_BOUNDS);
     return;
   }
@@ -156,8 +126,9 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   uint8_t* h_s = q_s + Cfg::kQBytes;                          // halves
   uint8_t* c_s = h_s + kRing * Cfg::kHalf;                    // (8-bit) codes,
   uint8_t* b_s = c_s + kSlots * Cfg::kCodes;                  // scale bytes [slot][the half's own, V's beside K's][128]
-  float* f_s = reinterpret_cast<float*>(b_s + Cfg::kScales);  // [256] what turns a row's products into base-2 scores
-  uint64_t* full = reinterpret_cast<uint64_t*>(f_s + 2 * kQ); // [ring] a half can be read by the products,
+  // [2 sides][2 halves of the columns][128]: at first what turns a side's rows' products into base-2 scores, then maxima and sums
+  float* x_s = reinterpret_cast<float*>(b_s + Cfg::kScales);
+  uint64_t* full = reinterpret_cast<uint64_t*>(x_s + 4 * kQ); // [ring] a half can be read by the products,
   uint64_t* empty = full + kRing;                             // [ring] has been read;
   uint64_t* came = empty + kRing;                             // [ring; 8-bit: slots] the copy has landed;
   uint64_t* taken = came + kCame;                             // [slots] the codes have been read
@@ -181,7 +152,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       const int s = s0 + lane;
       int rows = 0;
       if (s < seqs) rows = a.cu_q ? a.cu_q[s + 1] - a.cu_q[s] : a.rows_per_seq;
-      int n = rows > 0 ? (rows + toks - 1) / toks : 0;
+      int n = rows > 0 && rows >= a.row_lo && rows <= a.row_hi ? (rows + toks - 1) / toks : 0;
       const int own = n;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -214,10 +185,10 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);
+      mbar_init(&p_full[s], 8);
       mbar_init(&o_done[s], 1);
     }
-    mbar_init(q_full, 256);
+    mbar_init(q_full, 512);
     *abort_flag = 0;
     *bad_s = 0;
     mbar_fence_init();
@@ -238,7 +209,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   const bool twice = valid <= kQ;                             // both tiles are the same rows, on alternate key tiles
   const int clear = min(to, TREE ? past : past + tok_lo + 1); // the first token that some row may not see
 
-  if (warp == 12) {
+  if (warp == 20) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -257,13 +228,12 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   auto k_item = [&](int t) { return t == 0 ? 0 : 2 * t - 1; };
   auto v_item = [&](int t) { return t == ntiles - 1 ? items - 1 : 2 * t + 2; };
 
-  if (warp >= 8 && warp < 12) {
+  if (warp >= 16 && warp < 20) {
     // ---------------- keys and values ----------------
-    const int tid = threadIdx.x - 256, w4 = warp - 8;
+    const int tid = threadIdx.x - 512, w4 = warp - 16;
     if constexpr (E4M3) {
-      // two warps to a half, so that two halves are under way; a lane's codes of the whole half are read at once, which frees the
-      // slot for the next copy before the conversion begins
-      constexpr int kLanes = D / 16, kRowsWarp = 32 / kLanes, kLoads = kT / (2 * kRowsWarp);     // lanes to a row of codes
+      // two warps to a half, so that two halves are under way; in batches of 8 rows a lane
+      constexpr int kLanes = D / 16, kRowsWarp = 32 / kLanes, kLoads = 8, kBatch = kLoads * 2 * kRowsWarp;                       // lanes to a row of codes
       const int c = lane % kLanes, sub = lane / kLanes;
       // a lane's four of a tile's scale bytes (those behind the end are 0), and the largest of all
       auto scale_word = [&](uint32_t at, int here) -> uint32_t {
@@ -289,60 +259,66 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         const uint32_t src = smem_u32(c_s) + slot * Cfg::kCodes, by = smem_u32(b_s) + slot * 2 * kT;
         // a lane: 8 codes of the row's first half and 8 of its second (one piece of 16-bit values each; D = 64: two neighbours)
         constexpr int kApart = D == 64 ? 1 : 8;
-        const int p0 = D == 64 ? 2 * c : c, here = to - tok0, r0 = (w4 & 1) * kRowsWarp + sub;
+        const int p0 = D == 64 ? 2 * c : c, here = to - tok0;
         const bool edge = tok0 + kT > clear;
-        uint32_t w[kLoads][4];
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-          const int r = r0 + j * 2 * kRowsWarp;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int p = p0 + h * kApart;                    // eight codes: half of a 16-byte piece of the code row
-            const uint32_t at = src + (D == 64 ? r * 64 + (((p >> 1) ^ ((r >> 1) & 3)) << 4) : r * 128 + (((p >> 1) ^ (r & 7)) << 4)) + (p & 1) * 8;
-            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2 * h]), "=r"(w[j][2 * h + 1]) : "r"(at));
-          }
-        }
         const uint32_t word = scale_word(by, here);
         const int top = top_byte(word), vtop = which ? 0 : top_byte(scale_word(by + kT, here));
-        if (lane == 0) mbar_arrive(&taken[slot]);             // (the warp's codes are in registers: the reduction above waited for them)
-        bool nan = false;
-        if (edge) {
+        uint8_t* dst = h_s + half * Cfg::kHalf;
+        bool nan = false, free = false;
+#pragma unroll 1
+        for (int r0 = (w4 & 1) * kRowsWarp + sub; r0 < kT; r0 += kBatch) {
+          uint32_t w[kLoads][4];
 #pragma unroll
           for (int j = 0; j < kLoads; ++j) {
-            if (r0 + j * 2 * kRowsWarp >= here) w[j][0] = w[j][1] = w[j][2] = w[j][3] = 0;      // (not brought: anything may lie there)
-            if (which) {
-              // values that are not finite stay out of the product: rows that see them get them at the end
+            const int r = r0 + j * 2 * kRowsWarp;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t m = __vcmpeq4(w[j][k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                nan |= m != 0;
-                w[j][k] &= ~m;
+            for (int h = 0; h < 2; ++h) {
+              const int p = p0 + h * kApart;                  // eight codes: half of a 16-byte piece of the code row
+              const uint32_t at = src + (D == 64 ? r * 64 + (((p >> 1) ^ ((r >> 1) & 3)) << 4) : r * 128 + (((p >> 1) ^ (r & 7)) << 4)) + (p & 1) * 8;
+              asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2 * h]), "=r"(w[j][2 * h + 1]) : "r"(at));
+            }
+          }
+          if (edge) {
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+              if (r0 + j * 2 * kRowsWarp >= here) w[j][0] = w[j][1] = w[j][2] = w[j][3] = 0;    // (not brought: anything may lie there)
+              if (which) {
+                // values that are not finite stay out of the product: rows that see them get them at the end
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const uint32_t m = __vcmpeq4(w[j][k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                  nan |= m != 0;
+                  w[j][k] &= ~m;
+                }
               }
             }
           }
-        }
-        if (!bar_wait(&empty[half], ((i / kRing) & 1) ^ 1, abort_flag)) {
-          set_error(a.err, ERR_WAIT_EMPTY);
-          *abort_flag = 1;
-          ok = false;
-          break;
-        }
-        uint8_t* dst = h_s + half * Cfg::kHalf;
+          if (!free && !bar_wait(&empty[half], ((i / kRing) & 1) ^ 1, abort_flag)) {
+            set_error(a.err, ERR_WAIT_EMPTY);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          free = true;
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-          const int r = r0 + j * 2 * kRowsWarp;
-          const uint32_t b = __shfl_sync(0xffffffffu, word, r >> 2) >> (8 * (r & 3)) & 255u;
-          const uint32_t fj = pow2_f16(min((int)b - top, 0) + 6) * 0x10001u;
+          for (int j = 0; j < kLoads; ++j) {
+            const int r = r0 + j * 2 * kRowsWarp;
+            const uint32_t b = __shfl_sync(0xffffffffu, word, r >> 2) >> (8 * (r & 3)) & 255u;
+            const uint32_t fj = pow2_f16(min((int)b - top, 0) + 6) * 0x10001u;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t o[4];
-            codes_f16x4(w[j][2 * h], o[0], o[1]);
-            codes_f16x4(w[j][2 * h + 1], o[2], o[3]);
-            const int p = p0 + h * kApart;
-            *reinterpret_cast<uint4*>(dst + (p >> 3) * (kT * 128) + r * 128 + (((p & 7) ^ (r & 7)) << 4)) =
-                make_uint4(mul_f16x2(o[0], fj), mul_f16x2(o[1], fj), mul_f16x2(o[2], fj), mul_f16x2(o[3], fj));
+            for (int h = 0; h < 2; ++h) {
+              uint32_t o[4];
+              codes_f16x4(w[j][2 * h], o[0], o[1]);
+              codes_f16x4(w[j][2 * h + 1], o[2], o[3]);
+              const int p = p0 + h * kApart;
+              *reinterpret_cast<uint4*>(dst + (p >> 3) * (kT * 128) + r * 128 + (((p & 7) ^ (r & 7)) << 4)) =
+                  make_uint4(mul_f16x2(o[0], fj), mul_f16x2(o[1], fj), mul_f16x2(o[2], fj), mul_f16x2(o[3], fj));
+            }
           }
         }
+        if (!ok) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&taken[slot]);             // (the codes have been read)
         if (nan) *bad_s = 1;
         if (!which && (w4 & 1) == 0 && lane == 0) e_s[t & 3] = make_float2(pow2i(top - 127 - 6), (float)(vtop - 127 - 6));
         fence_proxy_async();
@@ -385,7 +361,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         if (lane == 0) mbar_arrive(&full[half]);
       }
     }
-  } else if (warp == 13) {
+  } else if (warp == 21) {
     // ---------------- copies: bf16 halves into the ring, 8-bit codes and scale bytes into their slots ----------------
     const size_t codes = (size_t)2 * a.hk * a.page_size * D, page_bytes = codes + 2 * a.hk * a.page_size;
     const int box = a.page_size < 64 ? a.page_size : 64;
@@ -439,7 +415,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
           tma_load_3d(h_s + slot * Cfg::kHalf + cb * (kT * 128) + lane * box * 128, kv_map, cb * 64, b_row, b_page, &came[slot]);
       }
     }
-  } else if (warp == 12) {
+  } else if (warp == 20) {
     // ---------------- products: the whole warp walks and waits, one lane issues ----------------
     constexpr uint32_t idesc_qk = tile_idesc<E4M3>(kQ, kT, false), idesc_pv = tile_idesc<E4M3>(kQ, D, true);
     const int steps = twice ? ntiles : 2 * ntiles;
@@ -470,7 +446,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       const uint32_t sv = v_low + half * (Cfg::kHalf >> 4), o_t = tmem + 256 + side * D, p_t = tmem + side * 128;
       if (leader) {
 #pragma unroll
-        for (int k = 0; k < kT / 16; ++k) umma_ts(o_t, p_t + k * 8, sv + (k * 16 * 128 >> 4), idesc_pv, (n | k) != 0);
+        for (int k = 0; k < kT / 16; ++k) umma_ts(o_t, p_t + (k < 4 ? k : k + 4) * 8, sv + (k * 16 * 128 >> 4), idesc_pv, (n | k) != 0);
         if (twice || side) tc_commit(&empty[half]);
         if (u + 2 >= steps) tc_commit(&o_done[side]);
       }
@@ -488,13 +464,13 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       *abort_flag = 1;
     }
     __syncwarp();
-  } else if (warp < 8) {
+  } else {
     // ---------------- Q -> shared memory, K-major with the 128-byte swizzle: D / 8 lanes to a row ----------------
     {
       constexpr int kLanes = D / 8;
       const int c = threadIdx.x % kLanes;
 #pragma unroll 4
-      for (int r = threadIdx.x / kLanes; r < 2 * kQ; r += 256 / kLanes) {
+      for (int r = threadIdx.x / kLanes; r < 2 * kQ; r += 512 / kLanes) {
         uint4 v = make_uint4(0, 0, 0, 0);
         const int rr = twice ? r & (kQ - 1) : r;
         if (rr < valid) v = *reinterpret_cast<const uint4*>(a.q + (size_t)(row0 + tok_lo + rr / G) * a.q_stride + (size_t)(kvh * G + rr % G) * D + c * 8);
@@ -520,22 +496,33 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
           v = make_uint4(w[0], w[1], w[2], w[3]);
         }
         *reinterpret_cast<uint4*>(q_s + (r >> 7) * (kQ * D * 2) + (c >> 3) * (kQ * 128) + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
-        if (c == 0) f_s[r] = f;
+        if (c == 0) x_s[(r >> 7) * 2 * kQ + (r & 127)] = f;
       }
       fence_proxy_async();
       mbar_arrive(q_full);
-      asm volatile("bar.sync 1, 256;" ::: "memory");          // f_s
+      asm volatile("bar.sync 3, 512;" ::: "memory");          // x_s
     }
-    // ---------------- softmax: a thread to a row ----------------
-    const int side = warp >> 2, row = (warp & 3) * 32 + lane;
+    // ---------------- softmax: two threads to a row, half of a tile's scores each ----------------
+    const int side = (warp >> 2) & 1, part = warp >> 3, row = (warp & 3) * 32 + lane;
     const int r = twice ? row : side * kQ + row;              // of the block's rows
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_t = tmem + lanes + side * 128, o_t = tmem + lanes + 256 + side * D;
+    const uint32_t s_t = tmem + lanes + side * 128 + part * 64, o_t = tmem + lanes + 256 + side * D + part * (D / 2);
     const int tk = tok_lo + (r < valid ? r / G : 0), pos = past + tk;
     const long long* mask = TREE ? a.masks + (size_t)(row0 + tk) * a.words : nullptr;
     const int steps = twice ? (ntiles + 1 - side) / 2 : ntiles;
-    const float f = f_s[side * kQ + row];
-    float ref = kUnset, l = 0.f;
+    const float f = x_s[side * 2 * kQ + row];                 // (read before the side's threads meet, written after)
+    float* const own_x = x_s + (side * 2 + part) * kQ + row;  // what the row's two threads tell each other
+    float* const his_x = x_s + (side * 2 + 1 - part) * kQ + row;
+    auto meet = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(1 + side) : "memory"); };
+    auto any_of = [&](bool mine) -> bool {                    // over the side's 256 threads
+      uint32_t any;
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                   : "=r"(any)
+                   : "r"(1 + side), "r"((uint32_t)mine)
+                   : "memory");
+      return any != 0;
+    };
+    float ref = kUnset, l = 0.f;                              // l: of this thread's columns
     // which of tokens j .. j + 31 the row sees
     auto seen32 = [&](int j) -> uint32_t {
       uint32_t b;
@@ -553,14 +540,14 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       }
       return b & below(to - j);
     };
-    for (int n = 0; n < steps && ok; ++n) {
+    // (a wait that has run out does not leave the walk: the side's threads meet in every step)
+    for (int n = 0; n < steps; ++n) {
       const int t = twice ? 2 * n + side : n;
       const int tok0 = from + t * kT;
-      if (!bar_wait(&s_full[side], n & 1, abort_flag)) {
+      if (ok && !bar_wait(&s_full[side], n & 1, abort_flag)) {
         set_error(a.err, ERR_WAIT_TMEM_FULL);
         *abort_flag = 1;
         ok = false;
-        break;
       }
       tc_fence_after();
       const bool edge = tok0 + kT > clear;                    // uniform
@@ -573,34 +560,36 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       // ---- the largest score; in a tile whose rows see different tokens the others become -inf where they lie ----
       float mx = -INFINITY;
 #pragma unroll 1
-      for (int c = 0; c < kT; c += 64) {
-        uint32_t x[64];
-        tmem_ld64(s_t + c, x);
+      for (int c = 0; c < 64; c += 32) {
+        uint32_t x[32];
+        tmem_ld_32x32(s_t + c, x);
         tmem_ld_wait();
         if (edge) {
-          const uint32_t b0 = seen32(tok0 + c), b1 = seen32(tok0 + c + 32);
+          const uint32_t b = seen32(tok0 + part * 64 + c);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (!(b0 >> i & 1)) x[i] = 0xff800000u;
-            if (!(b1 >> i & 1)) x[32 + i] = 0xff800000u;
-          }
-          tmem_st64(s_t + c, x);
+          for (int i = 0; i < 32; ++i)
+            if (!(b >> i & 1)) x[i] = 0xff800000u;
+          tmem_st32(s_t + c, x);
         }
-        float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
+        float m2[2] = {mx, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 64; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-        mx = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
+        for (int i = 0; i < 32; i += 2) m2[(i >> 1) & 1] = max3(m2[(i >> 1) & 1], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+        mx = fmaxf(m2[0], m2[1]);
       }
       if (edge) tmem_st_done();
       mx = fmaf(mx, scale, ev);
-      if (__any_sync(0xffffffffu, mx > ref + 15.f)) {
+      if (any_of(mx > ref + 15.f)) {
+        // a row's two threads move its reference together, and each passes over half of O
+        *own_x = mx;
+        meet();
+        mx = fmaxf(mx, *his_x);
         const float to_ref = mx > ref + 15.f ? ceilf(mx) - 7.f : ref, corr = exp2f(ref - to_ref);
         ref = to_ref;
         l *= corr;
         if (n > 0) {
           // (these scores' products were issued behind the last P V: O is quiet)
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
+          for (int c = 0; c < D / 2; c += 32) {
             uint32_t x[32];
             tmem_ld_32x32(o_t + c, x);
             tmem_ld_wait();
@@ -610,23 +599,24 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
           }
           tmem_st_done();
         }
+        meet();                                               // (the places are free again)
       }
-      // ---- weights, over the scores that have been read; their sum ----
+      // ---- weights, over scores of this thread's own that have been read; their sum ----
       const uint64_t scale2 = pair64(scale, scale), shift2 = pair64(ev - ref, ev - ref);
       uint64_t sum2[2] = {0, 0};
 #pragma unroll 1
-      for (int c = 0; c < kT; c += 64) {
-        uint32_t x[64];
-        tmem_ld64(s_t + c, x);
+      for (int c = 0; c < 64; c += 32) {
+        uint32_t x[32], pk[16];
+        tmem_ld_32x32(s_t + c, x);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
+        for (int i = 0; i < 16; ++i) {
           const float2 y = split64(fma2(pair64(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, shift2));
           const float u = exp2f(y.x), v = exp2f(y.y);
           sum2[i & 1] = add2(sum2[i & 1], pair64(u, v));
-          x[i] = pack_pair<E4M3>(u, v);
+          pk[i] = pack_pair<E4M3>(u, v);
         }
-        tmem_st32(s_t + (c >> 1), x);
+        tmem_st16(s_t + (c >> 1), pk);
       }
       const float2 sum = split64(add2(sum2[0], sum2[1]));
       l += E4M3 ? (sum.x + sum.y) * exp2f(-ev) : sum.x + sum.y;
@@ -641,33 +631,37 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       ok = false;
     }
     tc_fence_after();
-    // ---------------- the rows' end ----------------
-    float* other = reinterpret_cast<float*>(h_s);             // (twice) the second side's rows: [128][D + 3]
+    // ---------------- the rows' end: half of the columns to each of a row's threads ----------------
+    *own_x = l;
+    meet();
+    l += *his_x;
+    constexpr int kHalfD = D / 2, kPad = kHalfD + 3;
+    float* other = reinterpret_cast<float*>(h_s) + part * (kQ * kPad);    // (twice) the second side's rows: columns, reference, sum
     if (twice) {
-      asm volatile("bar.sync 1, 256;" ::: "memory");          // both sides' products are done: the ring is free
+      asm volatile("bar.sync 3, 512;" ::: "memory");          // both sides' products are done: the ring is free
       if (side == 1) {
-        float* mine = other + row * (D + 3);
-        mine[D] = ref;
-        mine[D + 1] = l;
+        float* mine = other + row * kPad;
+        mine[kHalfD] = ref;
+        mine[kHalfD + 1] = l;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = 0; c < kHalfD; c += 32) {
           uint32_t x[32];
-          tmem_ld_32x32(o_t + c * 32, x);
+          tmem_ld_32x32(o_t + c, x);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) mine[c * 32 + i] = steps > 0 ? __uint_as_float(x[i]) : 0.f;
+          for (int i = 0; i < 32; ++i) mine[c + i] = steps > 0 ? __uint_as_float(x[i]) : 0.f;
         }
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 3, 512;" ::: "memory");
     }
     if (!(twice && side)) {
       float own = 1.f, his = 0.f, m = ref;
       if (twice) {
-        const float* x = other + row * (D + 3);
-        m = fmaxf(ref, x[D]);
+        const float* x = other + row * kPad;
+        m = fmaxf(ref, x[kHalfD]);
         own = l == 0.f ? 0.f : exp2f(ref - m);
-        his = x[D + 1] == 0.f ? 0.f : exp2f(x[D] - m);
-        l = (l == 0.f ? 0.f : l * own) + (x[D + 1] == 0.f ? 0.f : x[D + 1] * his);
+        his = x[kHalfD + 1] == 0.f ? 0.f : exp2f(x[kHalfD] - m);
+        l = (l == 0.f ? 0.f : l * own) + (x[kHalfD + 1] == 0.f ? 0.f : x[kHalfD + 1] * his);
       }
       const bool whole = shares == 1, store = r < valid && ok;
       const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -675,16 +669,16 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       const size_t at = ((size_t)(row0 + tk) * a.hq + head) * gridDim.z + blockIdx.z;
       const bool bad = *bad_s != 0;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = 0; c < kHalfD; c += 32) {
+        const int col = part * kHalfD + c;
         uint32_t x[32];
-        float y[32];
-        tmem_ld_32x32(o_t + c * 32, x);
+        tmem_ld_32x32(o_t + c, x);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) y[i] = own != 0.f && steps > 0 ? __uint_as_float(x[i]) * own : 0.f;
+        for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(own != 0.f && steps > 0 ? __uint_as_float(x[i]) * own : 0.f);
         if (twice && his != 0.f) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) y[i] += other[row * (D + 3) + c * 32 + i] * his;
+          for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) + other[row * kPad + c + i] * his);
         }
         if (bad && store) {
           // infinities and NaN that this row sees in the tiles that were looked through, from the cache itself
@@ -698,30 +692,32 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               if constexpr (E4M3) {
-                const uint8_t code = a.pool[(size_t)page * (2 * a.hk * a.page_size * (size_t)(D + 1)) + v_row * D + c * 32 + i];
-                if ((code & 0x7f) == 0x7f) y[i] = __uint_as_float(0x7fffffffu);
+                const uint8_t code = a.pool[(size_t)page * (2 * a.hk * a.page_size * (size_t)(D + 1)) + v_row * D + col + i];
+                if ((code & 0x7f) == 0x7f) x[i] = 0x7fffffffu;
               } else {
-                const uint16_t w = reinterpret_cast<const uint16_t*>(a.pool)[(size_t)page * (2 * a.hk * a.page_size * (size_t)D) + v_row * D + c * 32 + i];
-                if ((w & 0x7f80u) == 0x7f80u) y[i] += __uint_as_float((uint32_t)w << 16);
+                const uint16_t w = reinterpret_cast<const uint16_t*>(a.pool)[(size_t)page * (2 * a.hk * a.page_size * (size_t)D) + v_row * D + col + i];
+                if ((w & 0x7f80u) == 0x7f80u) x[i] = __float_as_uint(__uint_as_float(x[i]) + __uint_as_float((uint32_t)w << 16));
               }
             }
           }
         }
         if (!store) continue;
         if (whole) {
-          __nv_bfloat16* dst = a.out + (size_t)(row0 + tk) * a.out_stride + (size_t)head * D + c * 32;
+          __nv_bfloat16* dst = a.out + (size_t)(row0 + tk) * a.out_stride + (size_t)head * D + col;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<uint4*>(dst + i * 8) =
-                make_uint4(pack_bf16x2(y[8 * i] * inv, y[8 * i + 1] * inv), pack_bf16x2(y[8 * i + 2] * inv, y[8 * i + 3] * inv),
-                           pack_bf16x2(y[8 * i + 4] * inv, y[8 * i + 5] * inv), pack_bf16x2(y[8 * i + 6] * inv, y[8 * i + 7] * inv));
+          for (int i = 0; i < 4; ++i) {
+            uint32_t o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = pack_bf16x2(__uint_as_float(x[8 * i + 2 * k]) * inv, __uint_as_float(x[8 * i + 2 * k + 1]) * inv);
+            *reinterpret_cast<uint4*>(dst + i * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+          }
         } else {
-          float4* dst = reinterpret_cast<float4*>(a.ws_o + at * D + c * 32);
+          uint4* dst = reinterpret_cast<uint4*>(a.ws_o + at * D + col);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dst[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+          for (int i = 0; i < 8; ++i) dst[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
         }
       }
-      if (!whole && store) {
+      if (!whole && store && part == 0) {
         a.ws_ml[at * 2] = m;
         a.ws_ml[at * 2 + 1] = l;
       }
@@ -737,7 +733,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
   }
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 20) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -752,10 +748,10 @@ using namespace kern;
       const __grid_constant__ CUtensorMap kv_map, const __nv_bfloat16* q, __nv_bfloat16* out, float* ws_o, float* ws_ml,          \
       const uint8_t* pool, const int* block_table, const int* seq_lens, const int* cu_q, const long long* masks, int words,       \
       int rows_per_seq, int hq, int hk, int q_stride, int out_stride, int max_pages, int page_size, int seqs, int pool_pages,     \
-      float scale_log2, int* err) {                                                                                               \
+      int row_lo, int row_hi, float scale_log2, int* err) {                                                                                               \
     tile_body<D, E4M3, TREE>(&kv_map, RowsArgs{q, out, ws_o, ws_ml, pool, block_table, seq_lens, cu_q, masks, err, words,         \
                                                rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, 1, pool_pages,   \
-                                               scale_log2},                                                                       \
+                                               row_lo, row_hi, scale_log2},                                                                       \
                              seqs);                                                                                               \
   }
 #define KERN_TILE(D)                            \
