@@ -234,16 +234,14 @@ struct RowsForm {
 };
 RowsForm rows_form(int64_t d, bool e4m3, int64_t nt) {
   const int64_t row = d * (e4m3 ? 1 : 2), tile = row <= 128 ? 128 : 64, stage = 2 * tile * row;
-  const int per_sm = d == 256 || d * nt > 256 ? 1 : 2;
+  const int per_sm = d == 256 ? 1 : 2;
   const int64_t stages = stage >= 65536 ? 3 : (per_sm == 1 ? 196608 : 98304) / stage;
   return {(unsigned)(1024 + stages * (stage + (e4m3 ? 2 * tile : 0)) + (d == 256 && nt > 1 ? nt * d * 16 : 0) + 256), per_sm};
 }
 // Shares that a row's context is cut into, and CTAs of a cluster: as many as fill the SMs once, two where the rows alone fill them up
 // to four times (a share's end then leaves less of the last wave idle), none of under 128 tokens. Up to 8 shares are one cluster;
 // more are on their own, and joined by a second launch.
-int64_t g_shares = 0, g_cluster = 0;
 std::pair<int64_t, int64_t> rows_shares(int64_t ctas, int64_t max_len, int64_t resident) {
-  if (g_shares) return {g_shares, g_cluster};
   const int64_t most = std::max<int64_t>(1, (max_len + 127) / 128);
   const int64_t want = std::min<int64_t>({most, ctas < resident ? resident / ctas : ctas < 4 * resident ? 2 : 1, 256});
   if (want > 8) return {want, 1};
@@ -256,10 +254,16 @@ unsigned tile_shared(int64_t d, bool e4m3) {
   return (unsigned)(2 * 128 * d * 2 + (e4m3 ? 4 : 5) * 128 * d * 2 + (e4m3 ? 2 * (128 * d + 256) : 0) + 4 * 128 * 4 + 512);
 }
 int64_t tile_shares(int64_t ctas, int64_t max_len, int64_t sms) {
-  if (g_shares) return g_shares;
   return std::max<int64_t>(1, std::min<int64_t>({sms / ctas, (max_len + 255) / 256, 64}));
 }
-int64_t g_tile_rows = 32;       // query rows of a sequence and kv head above which the many-row kernel runs (head_dim 64 and 128)
+// Query rows of a sequence and kv head up to which the few-row kernel runs; the many-row kernel above them (head_dim 64 and 128).
+// Microseconds of the few-row kernel : of the many-row kernel, 8 kv heads, head_dim 128:
+//   8-bit cache, causal          16 rows       32 rows            bf16 cache, tree       16 rows       24 rows
+//     1 sequence  of 1000      10.0 :  13.1   14.4 :  14.0           1 of 1000           10.4 :  11.8    14.0 :  11.9
+//    16 sequences of 4000      39.0 :  74.9   74.2 :  75.1          16 of 4000           47.9 :  46.6    85.0 :  46.6
+//    64 sequences of 2000      88.8 : 159     206  : 161            64 of 2000          106.8 : 107.2   216.8 : 107.8
+// (the few-row kernel's matrix instructions take time for every eight rows, the other's are the same up to 128)
+constexpr int64_t kFewRows = 16;
 
 // 3-D descriptor over a pool of either format: (value, row of a page's k | v x head x token, page)
 std::array<uint8_t, 128> pool_map(Host& h, const Tensor& pool, bool e4m3, int64_t pages, int64_t hk, int64_t d, int64_t page) {
@@ -330,8 +334,7 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
       shared = tile_shared(d, e4m3);
       name = "kern_attn_tile" + form;
     } else {
-      // query rows of a CTA: the fewest eights that hold a sequence's, up to what registers hold
-      const int64_t nt = g * most <= 8 ? 1 : g * most <= 16 || d == 256 ? 2 : 4;
+      const int64_t nt = g * most <= 8 ? 1 : 2;              // query rows of a CTA, in eights
       toks = 8 * nt / g;
       const int64_t blocks = (most + toks - 1) / toks;
       const RowsForm f = rows_form(d, e4m3, nt);
@@ -362,7 +365,7 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
     }
   };
   const int64_t all = INT32_MAX, few = std::max<int64_t>(1, 8 / g);
-  if (g * max_rows <= g_tile_rows || d > 128) {
+  if (g * max_rows <= kFewRows || d > 128) {
     run(false, 1, all);
   } else if (!cu_q || seqs == 1 || rows + few >= seqs * max_rows) {
     run(true, 1, all);                                       // (rows alike)
@@ -451,12 +454,8 @@ PYBIND11_MODULE(_ops_host, m) {
     hosts().at(gpu) = std::move(h);
   });
   m.def("launches", [](int gpu) { return hosts().at(gpu) ? hosts()[gpu]->launches : 0; });
-  m.def("tile_rows", [](std::optional<int64_t> rows) {
-    const int64_t was = g_tile_rows;
-    if (rows) g_tile_rows = *rows;
-    return was;
-  }, py::arg("rows") = py::none());
-  m.def("tune", [](int64_t s, int64_t c) { g_shares = s; g_cluster = c; });
+  m.def("rows_form", [](int64_t d, bool e4m3, int64_t nt) { const RowsForm f = rows_form(d, e4m3, nt); return py::make_tuple(f.shared, f.per_sm); });
+  m.def("tile_shared", &tile_shared);
   m.def("append", &append);
   m.def("read_rows", &read_rows);
   m.def("attend", &attend);

@@ -4,8 +4,8 @@
 //
 //   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = 2^(scale log2(e) q_i.k_j - m_i)  over the j that row i sees; no such j: zeros
 //
-// One CTA = (8, 16 or 32 query rows: the G heads of some tokens, one kv head, a share of the context). A producer warp brings
-// tiles of tokens into a ring of shared memory by TMA; four or eight warps take 16 tokens of a tile at a time and keep (m, l, O) of
+// One CTA = (8 or 16 query rows: the G heads of some tokens, one kv head, a share of the context). A producer warp brings
+// tiles of tokens into a ring of shared memory by TMA; four warps take 16 tokens of a tile at a time and keep (m, l, O) of
 // their own. They are joined at the end, then the shares of one row: over distributed shared memory in a cluster of up to 8 CTAs, and
 // where that is not enough as partials that a second kernel joins (kern_attn_rows_merge).
 //
@@ -35,12 +35,12 @@ namespace kern {
 template <int D, bool E4M3, int NT>
 struct RowsCfg {
   static constexpr int kRowBytes = D * (E4M3 ? 1 : 2);
-    static constexpr int kTile = kRowBytes <= 128 ? 128 : 64;          // tokens: a stage of 32 KB where rows allow it
+  static constexpr int kTile = kRowBytes <= 128 ? 128 : 64;          // tokens: a stage of 32 KB where rows allow it
   static constexpr int kHalf = kTile * kRowBytes;                    // a tile of K or of V
   static constexpr int kStage = 2 * kHalf;
   static constexpr int kScaleBytes = E4M3 ? 2 * kTile : 0;
-  // 96 KB of ring, so that two CTAs share an SM; one where accumulators or 512-byte rows take the room of two
-  static constexpr int kPerSm = D == 256 || D * NT > 256 ? 1 : 2;
+  // 96 KB of ring, so that two CTAs share an SM; one where 512-byte rows and their accumulators take the room of two
+  static constexpr int kPerSm = D == 256 ? 1 : 2;
   static constexpr int kStages = kStage >= 65536 ? 3 : (kPerSm == 1 ? 196608 : 98304) / kStage;
   static constexpr int kBox = kRowBytes < 128 ? kRowBytes : 128;     // bytes of a row in one box
   // warps of products, 16 tokens of a tile at a time each (eight of them, at 96 registers, were 15 % slower: 75 us against 66 for
@@ -434,7 +434,7 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
               e[nt][k] = exp2f(s[nt][k] - m_run[nt][k & 1]);
               top = fmaxf(top, e[nt][k]);
               if constexpr (E4M3) {
-                w[nt][k] = e[nt][k] * (g_run[nt][k & 1] * vscale[k >> 1]);
+                w[nt][k] = e[nt][k] * fminf(g_run[nt][k & 1] * vscale[k >> 1], 3e38f);     // (0 stays 0 beside the largest scales)
                 top = fmaxf(top, w[nt][k]);
               } else {
                 w[nt][k] = e[nt][k];
@@ -779,5 +779,3 @@ using namespace kern;
 KERN_ROWS(64)
 KERN_ROWS(128)
 KERN_ROWS(256)
-KERN_ROWS_FORMS(64, 4)
-KERN_ROWS_FORMS(128, 4)

@@ -21,9 +21,10 @@
 // when a weight has outgrown it by 2^15 (found on the packed halves, one instruction for two), so one pass over the scores does:
 // scale and shift, exponential, sum, pack. No pass over O but then.
 //
-// 8-bit: a tile's rows are brought to one exponent, E = the largest of its scale bytes, as they become f16 (exact down to 2^-21 of
-// the tile's largest row, and to 2^-25 of one step beyond); 2^E of the keys is then part of the scores' scale, E of the values part
-// of the weights' exponent, w_ij = 2^(s_ij + E_t - R_i): no work per score.
+// 8-bit: a tile's rows are brought to one exponent, E = the largest of its scale bytes, as they become f16 (exact for scales down to
+// 2^-21 of the largest); 2^E of the keys is then part of the scores' scale, E of the values part of the weights' exponent,
+// w_ij = 2^(s_ij + E_t - R_i): no work per score. A block that meets a tile with scales further apart (rows that hold nothing but
+// zeros and values under 2^-31 aside) is computed again, a row to a warp, each key and value row with its own scale (tile_wide).
 #include "attn_rows.cuh"
 #include "f32x2.cuh"
 
@@ -111,6 +112,73 @@ KERN_DEVICE uint32_t mul_f16x2(uint32_t a, uint32_t b) {
 // 2^x as f16, 0 below its range
 KERN_DEVICE uint32_t pow2_f16(int x) { return x >= -14 ? (uint32_t)(x + 15) << 10 : (x >= -24 ? 1u << (x + 24) : 0u); }
 
+// A block's rows over the 8-bit cache, a row to a warp in turn and one token at a time, for scales that have no common exponent.
+template <int D, bool TREE>
+__device__ __noinline__ void tile_wide(const RowsArgs& a, int seq, int row0, int tok_lo, int valid, int past, int from, int to, int shares) {
+  constexpr int kCols = D / 32;                               // of a lane
+  const int G = a.hq / a.hk, kvh = blockIdx.x, lane = threadIdx.x & 31;
+  const size_t codes = (size_t)2 * a.hk * a.page_size * D, page_bytes = codes + 2 * a.hk * a.page_size;
+  for (int r = threadIdx.x >> 5; r < valid; r += 16) {
+    const int tk = tok_lo + r / G, head = kvh * G + r % G, stop = TREE ? to : min(to, past + tk + 1);
+    const long long* mask = TREE ? a.masks + (size_t)(row0 + tk) * a.words : nullptr;
+    float q[kCols], o[kCols], m = kUnset, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) {
+      q[i] = __bfloat162float(a.q[(size_t)(row0 + tk) * a.q_stride + (size_t)head * D + lane * kCols + i]) * a.scale_log2;
+      o[i] = 0.f;
+    }
+    for (int j = from; j < stop; ++j) {
+      if (TREE && j >= past) {
+        const int n = j - past;
+        if (n >> 6 >= a.words || !(mask[n >> 6] >> (n & 63) & 1)) continue;
+      }
+      const int pi = j / a.page_size, off = j - pi * a.page_size;
+      int page = pi < a.max_pages ? a.block_table[(size_t)seq * a.max_pages + pi] : 0;
+      if (page < 0 || page >= a.pool_pages) page = 0;         // (recorded by the walk before)
+      float kv[2][kCols], size[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const size_t at = (size_t)(h * a.hk + kvh) * a.page_size + off;
+        const uint8_t* src = a.pool + (size_t)page * page_bytes;
+        size[h] = pow2i((int)src[codes + at] - 127);
+#pragma unroll
+        for (int i = 0; i < kCols; i += 2) {
+          uint32_t lo, hi;
+          codes_f16x4(*reinterpret_cast<const uint16_t*>(src + at * D + lane * kCols + i), lo, hi);
+          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+          kv[h][i] = v.x;
+          kv[h][i + 1] = v.y;
+        }
+      }
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) s = fmaf(q[i], kv[0][i], s);
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+      s *= size[0];
+      const float top = fmaxf(m, s), keep = exp2f(m - top), p = exp2f(s - top);
+      m = top;
+      l = fmaf(l, keep, p);
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) o[i] = fmaf(o[i], keep, p * (kv[1][i] * size[1]));
+    }
+    if (shares == 1) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int i = 0; i < kCols; i += 2)
+        *reinterpret_cast<uint32_t*>(a.out + (size_t)(row0 + tk) * a.out_stride + (size_t)head * D + lane * kCols + i) = pack_bf16x2(o[i] * inv, o[i + 1] * inv);
+    } else {
+      const size_t at = ((size_t)(row0 + tk) * a.hq + head) * gridDim.z + blockIdx.z;
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) a.ws_o[at * D + lane * kCols + i] = o[i];
+      if (lane == 0) {
+        a.ws_ml[at * 2] = m;
+        a.ws_ml[at * 2 + 1] = l;
+      }
+    }
+  }
+}
+
 // D, cache format, tree or causal
 template <int D, bool E4M3, bool TREE>
 KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const int seqs) {
@@ -141,6 +209,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* found = reinterpret_cast<int*>(tmem_slot + 2);         // [2] sequence and block of this CTA
   volatile int* bad_s = found + 2;                            // a value that is not finite in a tile whose rows see different tokens
+  volatile int* wide_s = found + 3;                           // (8-bit) a tile's scales are further apart than f16 holds
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (uniform registers for what follows from it)
   const int G = a.hq / a.hk, kvh = blockIdx.x, toks = 2 * kQ / G;
@@ -191,6 +260,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     mbar_init(q_full, 512);
     *abort_flag = 0;
     *bad_s = 0;
+    *wide_s = 0;
     mbar_fence_init();
     tma_prefetch_desc(kv_map);
   }
@@ -263,6 +333,8 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         const bool edge = tok0 + kT > clear;
         const uint32_t word = scale_word(by, here);
         const int top = top_byte(word), vtop = which ? 0 : top_byte(scale_word(by + kT, here));
+        // (a row of zeros has the byte -40 + 127)
+        if (top > 0x57 + 21 && (__vcmpgtu4(word, 0x57575757u) & __vcmpltu4(word, (uint32_t)(top - 21) * 0x01010101u)) != 0) *wide_s = 1;
         uint8_t* dst = h_s + half * Cfg::kHalf;
         bool nan = false, free = false;
 #pragma unroll 1
@@ -637,8 +709,9 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     l += *his_x;
     constexpr int kHalfD = D / 2, kPad = kHalfD + 3;
     float* other = reinterpret_cast<float*>(h_s) + part * (kQ * kPad);    // (twice) the second side's rows: columns, reference, sum
+    if (twice) asm volatile("bar.sync 3, 512;" ::: "memory"); // both sides' products are done: the ring is free
+    const bool wide = E4M3 && *wide_s != 0;                   // (uniform: every half has been looked at)
     if (twice) {
-      asm volatile("bar.sync 3, 512;" ::: "memory");          // both sides' products are done: the ring is free
       if (side == 1) {
         float* mine = other + row * kPad;
         mine[kHalfD] = ref;
@@ -654,7 +727,12 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       }
       asm volatile("bar.sync 3, 512;" ::: "memory");
     }
-    if (!(twice && side)) {
+    if (wide) {
+      if constexpr (E4M3) {
+        const RowsArgs args = a;                              // (a copy on the stack, for this call alone)
+        if (ok) tile_wide<D, TREE>(args, seq, row0, tok_lo, valid, past, from, to, shares);
+      }
+    } else if (!(twice && side)) {
       float own = 1.f, his = 0.f, m = ref;
       if (twice) {
         const float* x = other + row * kPad;
