@@ -461,6 +461,79 @@ for _d in (16, 32, 64, 128, 256):
     CPU_KERNELS[f"kern_attn_decode_paged_d{_d}"] = _attention(False)
 
 
+# ---- the 8-bit cache (statements: ops/kv_e4m3.py) -------------------------------------------------------------------
+def _pool_e4m3(kv, hk: int, page: int, d: int):
+    """The codes [pages, 2, hk, page, d] and scale bytes [pages, 2, hk, page] of a state's bytes."""
+    size = 2 * hk * page * (d + 1)
+    rows = kv.view(torch.uint8).view(-1)
+    rows = rows[: rows.numel() // size * size].view(-1, size)
+    n = 2 * hk * page * d
+    return rows[:, :n].view(torch.float8_e4m3fn).unflatten(1, (2, hk, page, d)), rows[:, n:].unflatten(1, (2, hk, page))
+
+
+def _rope_append_e4m3(d: int, interleaved: bool):
+    def run(g, qkv, q_out, kv, positions, slots, cos, sin, qn, kn, hq, hk, rot, page, eps, plus_one, kv_slots, max_pos, row_stride, q_stride, err):
+        from .ops.kv_e4m3 import quantise_reference
+
+        t, half = g[0], rot // 2
+        rows = qkv[: t * row_stride].view(t, row_stride)[:, : (hq + 2 * hk) * d].unflatten(1, (hq + 2 * hk, d))
+        pos, sl = positions[:t].long(), slots[:t].long()
+        bad = (pos < 0) | (pos >= max_pos)
+        if bad.any():
+            err[0] = 300
+        pos = torch.where(bad, 0, pos)
+        c, s = (x.view(-1, half)[pos][:, None] for x in (cos, sin))
+        first, second = (slice(0, rot, 2), slice(1, rot, 2)) if interleaved else (slice(0, half), slice(half, rot))
+
+        def prep(x, w):
+            x = _f(x).clone()
+            if isinstance(w, torch.Tensor):
+                x = x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * (_f(w[:d]) + (1.0 if plus_one else 0.0))
+            a, b = x[..., first].clone(), x[..., second].clone()
+            x[..., first], x[..., second] = a * c - b * s, b * c + a * s
+            return x
+
+        q, k, v = prep(rows[:, :hq], qn), prep(rows[:, hq:hq + hk], kn), _f(rows[:, hq + hk:])
+        ok = (sl >= 0) & ~bad
+        codes, scales = _pool_e4m3(kv, hk, page, d)
+        new, size = quantise_reference(torch.stack([k, v], 1))
+        pg, off = sl[ok] // page, sl[ok] % page
+        codes.view(torch.uint8)[pg, :, :, off] = new.view(torch.uint8)[ok]
+        scales[pg, :, :, off] = size[ok]
+        torch.as_strided(q_out, (t, hq * d), (q_stride, 1), q_out.storage_offset()).copy_(q.reshape(t, -1).to(q_out.dtype))
+    return run
+
+
+def _attention_e4m3(g, m, q, out, ws_o, ws_ml, kv, table, seq_lens, cu_q, masks, words, rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page,
+                    last, pool_pages, row_lo, row_hi, scale_log2, err):
+    from .ops.kv_e4m3 import dequantise_reference
+
+    d, grp = m._head_dim, hq // hk
+    codes, scales = _pool_e4m3(kv, hk, page, d)
+    tb = table.view(-1, max_pages)
+    for s in range(int(m._vars_seqs)):
+        r0, r1 = (int(cu_q[s]), int(cu_q[s + 1])) if isinstance(cu_q, torch.Tensor) else (s * rows_per_seq, (s + 1) * rows_per_seq)
+        L, R = int(seq_lens[s]), r1 - r0
+        if not row_lo <= R <= row_hi or R <= 0:
+            continue
+        pages = tb[s, : -(-L // page)].long()
+        kk, vv = (dequantise_reference(codes[pages, i], scales[pages, i]).permute(0, 2, 1, 3).reshape(-1, hk, d)[:L].repeat_interleave(grp, 1) for i in (0, 1))
+        qq = _f(torch.as_strided(q, (R, hq, d), (q_stride, d, 1), q.storage_offset() + r0 * q_stride))
+        sc = torch.einsum("rhd,lhd->hrl", qq, kk) * (scale_log2 / 1.4426950408889634)
+        sc = sc.masked_fill(~(torch.arange(L)[None] <= torch.arange(L - R, L)[:, None])[None], float("-inf"))
+        o = torch.einsum("hrl,lhd->rhd", torch.softmax(sc, -1).nan_to_num(0.0), vv)
+        torch.as_strided(out, (R, hq * d), (out_stride, 1), out.storage_offset() + r0 * out_stride).copy_(o.reshape(R, hq * d).to(out.dtype))
+
+
+for _d in (16, 32, 64, 128, 256):
+    for _pairs in ("half", "interleaved"):
+        for _norm in ("", "_norm"):
+            CPU_KERNELS[f"kern_rope_kv_append_e4m3_{_pairs}{_norm}_d{_d}"] = _rope_append_e4m3(_d, _pairs == "interleaved")
+    CPU_KERNELS[f"kern_attn_tile_e4m3_causal_d{_d}"] = _attention_e4m3
+    for _n in (1, 2):
+        CPU_KERNELS[f"kern_attn_rows_e4m3_causal_d{_d}_n{_n}"] = _attention_e4m3
+
+
 def register(entry: str, fn) -> None:
     """Add the CPU statement of another kernel entry (model families register theirs on import)."""
     CPU_KERNELS[entry] = fn

@@ -603,6 +603,107 @@ def attn_decode_op(hq: int, hk: int, d: int, page_size: int, table_width: int, q
     return {"params": iface, "impl": impl}
 
 
+# ---- the 8-bit cache (ops/kv_e4m3.py has its layout): the same operations over it ------------------------------------------------
+def rope_append_e4m3_op(hq: int, hk: int, d: int, rot: int, page_size: int, max_pos: int, eps: float, qk_norm: bool,
+                        norm_plus_one: bool = False, row_stride: int | None = None, pairs: str = "half") -> dict:
+    """Interface [qkv, kv state, positions, slots, cos, sin, (q_norm, k_norm,) err], as `rope_append_op`."""
+    stride = row_stride or (hq + 2 * hk) * d
+    iface = ["inout buffer<bf16>", "inout state", "in buffer<i64>", "in buffer<i64>", "in buffer<f32>", "in buffer<f32>"]
+    norms, norm_params = [{"i64": 0}, {"i64": 0}], ["i64", "i64"]
+    if qk_norm:
+        iface += ["in buffer<bf16>", "in buffer<bf16>"]
+        norms, norm_params = [{"param": 6}, {"param": 7}], ["in buffer<bf16>", "in buffer<bf16>"]
+    iface.append("out buffer<i32>")
+    lp = ["inout buffer<bf16>", "inout buffer<bf16>", "inout state"] + iface[2:6] + norm_params + ["i32"] * 4 + ["f32", "i32", "i64"] + ["i32"] * 3 + ["out buffer<i32>"]
+    args = [{"param": 0}, {"param": 0}, {"param": 1}, {"param": 2}, {"param": 3}, {"param": 4}, {"param": 5}, *norms, {"i32": hq}, {"i32": hk},
+            {"i32": rot}, {"i32": page_size}, {"f32": eps}, {"i32": int(norm_plus_one)}, {"i64": I64_MAX}, {"i32": max_pos}, {"i32": stride},
+            {"i32": stride}, {"param": len(iface) - 1}]
+    return {"params": iface, "impl": {"launches": [{
+        "module": "kv_e4m3", "entry": f"kern_rope_kv_append_e4m3_{pairs}{'_norm' if qk_norm else ''}_d{d}", "block": [128, 1, 1],
+        "grid": ["tokens", 1, 1], "params": lp, "args": args}]}}
+
+
+def _e4m3_map(hk: int, d: int, page_size: int, state_param: int) -> dict:
+    cols = min(d, 128)
+    return {"pack": {"size": 128, "fields": [{"at": 0, "tensormap": {
+        "param": state_param, "dtype": "u8", "dims": [d, 2 * hk * page_size, 0], "strides": [d, 2 * hk * page_size * (d + 1)],
+        "box": [cols, min(page_size, 64), 1], "swizzle": cols if cols >= 32 else 0, "l2_promotion": 256}}]}}
+
+
+def _e4m3_attend(entry: str, grid: list, threads: int, smem: int, cluster: int, hq: int, hk: int, d: int, page_size: int, table_width: int,
+                 q_stride: int, last: dict, lo: int, hi: int, cu: int | None, err: int, when: dict | None) -> dict:
+    ptr = ["in buffer<bf16>", "out buffer<bf16>", "i64", "i64", "in state", "in buffer<i32>", "in buffer<i32>", "in buffer<i32>" if cu is not None else "i64", "i64"]
+    lp = ["bytes<128>"] + ptr + ["i32"] * 12 + ["f32", "out buffer<i32>"]
+    args = [_e4m3_map(hk, d, page_size, 1), {"param": 0}, {"param": 2}, {"i64": 0}, {"i64": 0}, {"param": 1}, {"param": 3}, {"param": 4},
+            {"i64": 0} if cu is None else {"param": cu}, {"i64": 0}, {"i32": 0}, {"i32": 1}, {"i32": hq}, {"i32": hk}, {"i32": q_stride},
+            {"i32": hq * d}, {"i32": table_width}, {"i32": page_size}, last, {"i32": I32_MAX}, {"i32": lo}, {"i32": hi},
+            {"f32": (d ** -0.5) * 1.4426950408889634}, {"param": err}]
+    out = {"module": "attn_rows" if "rows" in entry else "attn_tile", "entry": entry, "block": [threads, 1, 1], "grid": grid, "shared_mem": smem,
+           "params": lp, "args": args}
+    if cluster > 1:
+        out["cluster"] = [1, 1, cluster]
+    if when:
+        out["when"] = when
+    return out
+
+
+def _e4m3_few(hq: int, hk: int, d: int, page_size: int, table_width: int, q_stride: int, seqs_max: int, rows: int, hi: int, cu: int | None, err: int,
+              sms: int = SMS) -> list[dict]:
+    """Launches of the few-row kernel over sequences of up to `rows` rows: the shares of a context, one cluster, by `when` ranges of the batch."""
+    from .. import _ops_host
+
+    g = hq // hk
+    nt = 1 if g * rows <= 8 else 2
+    blocks = -(-rows // (8 * nt // g))
+    smem, per_sm = _ops_host.rows_form(d, True, nt)
+    per, out, lo = hk * blocks, [], 1
+    # as the call-by-call rule (ops_host.cpp, rows_shares): shares that fill the SMs once, two while the rows alone fill them up to four times
+    for cluster, most in ((8, sms * per_sm // 8), (4, sms * per_sm // 4), (2, 4 * sms * per_sm - 1), (1, None)):
+        top = seqs_max if most is None else min(seqs_max, most // per)
+        if top < lo:
+            continue
+        when = {"var": "seqs"}
+        if lo > 1:
+            when["min"] = lo
+        if top < seqs_max:
+            when["max"] = top
+        out.append(_e4m3_attend(f"kern_attn_rows_e4m3_causal_d{d}_n{nt}", [per, "seqs", cluster], 160, smem, cluster, hq, hk, d, page_size, table_width,
+                                q_stride, {"i32": cluster}, 1, hi, cu, err, when if len(when) > 1 else None))
+        lo = top + 1
+    return out
+
+
+def attn_decode_e4m3_op(hq: int, hk: int, d: int, page_size: int, table_width: int, q_stride: int, seqs_max: int) -> dict:
+    """Single tokens over the 8-bit cache. Interface [q(kv) buffer, kv state, out, block_table, seq_lens, err], as `attn_decode_op`."""
+    iface = ["in buffer<bf16>", "in state", "out buffer<bf16>", "in buffer<i32>", "in buffer<i32>", "out buffer<i32>"]
+    return {"params": iface, "impl": {"launches": _e4m3_few(hq, hk, d, page_size, table_width, q_stride, seqs_max, 1, I32_MAX, None, 5)}}
+
+
+def attn_prefill_e4m3_op(hq: int, hk: int, d: int, page_size: int, table_width: int, q_stride: int, seqs_max: int) -> dict:
+    """Ragged rows over the 8-bit cache: sequences of many rows on the tensor-core kernel (head_dim 64 and 128), of few on the few-row
+    kernel. Interface [q(kv) buffer, kv state, out, block_table, seq_lens, cu_seqlens, seqs, err]; no plan."""
+    from .. import _ops_host
+
+    g = hq // hk
+    iface = ["in buffer<bf16>", "in state", "out buffer<bf16>", "in buffer<i32>", "in buffer<i32>", "in buffer<i32>", "i32", "out buffer<i32>"]
+    few = max(1, 8 // g)
+    if d > 128:
+        nt = 2
+        toks = 8 * nt // g
+        many = _e4m3_attend(f"kern_attn_rows_e4m3_causal_d{d}_n{nt}", [{"mul": [{"ceil_div": ["tokens", toks]}, hk]}, "seqs", 1], 160,
+                            _ops_host.rows_form(d, True, nt)[0], 1,
+                            hq, hk, d, page_size, table_width, q_stride, {"i32": 1}, few + 1, I32_MAX, 5, 7, None)
+    else:
+        many = _e4m3_attend(f"kern_attn_tile_e4m3_causal_d{d}", [hk, {"add": [{"ceil_div": ["tokens", 256 // g]}, "seqs"]}, 1], 704,
+                            _ops_host.tile_shared(d, True), 1,
+                            hq, hk, d, page_size, table_width, q_stride, {"param": 6}, few + 1, I32_MAX, 5, 7, None)
+    return {"params": iface, "impl": {"launches": [many] + _e4m3_few(hq, hk, d, page_size, table_width, q_stride, seqs_max, few, few, 5, 7)}}
+
+
+def e4m3_modules(d: int) -> list[str]:
+    return ["kv_e4m3", "attn_rows"] + (["attn_tile"] if d <= 128 else [])
+
+
 def last_row_op(row_bytes: int) -> dict:
     """Interface [src, dst, cu_seqlens]: the last row of every sequence of a ragged batch."""
     return {"params": ["in buffer<bf16>", "out buffer<bf16>", "in buffer<i32>"], "impl": {"launches": [{

@@ -38,6 +38,7 @@ class DenseConfig:
     max_context: int = 8192       # longest sequence (positions); sizes the page-table row and rope tables
     sampling: bool = False        # sampling fills + sampler instead of greedy argmax
     tp: int = 1                   # tensor-parallel width (see tp.py for the fused variant)
+    kv: str = "bf16"              # the cache: "bf16", or "e4m3" (8-bit codes with a scale per row, ops/kv_e4m3.py)
 
     @property
     def table_width(self) -> int:
@@ -57,7 +58,7 @@ class DenseConfig:
 
     @property
     def kv_bytes_per_token(self) -> int:
-        return 2 * self.kv_dim * 2
+        return 2 * self.kv_heads * (self.head_dim + 1) if self.kv == "e4m3" else 2 * self.kv_dim * 2
 
     def param_count(self) -> int:
         per = self.hidden * self.qkv_dim + self.q_dim * self.hidden + 3 * self.hidden * self.intermediate + 2 * self.hidden
@@ -117,6 +118,11 @@ def build_manifest(cfg: DenseConfig, hosted: bool = False) -> dict:
     T, S, W = cfg.max_tokens, cfg.max_seqs, cfg.table_width
     inter = cfg.intermediate
     assert inter % 16 == 0 and h % 8 == 0
+    if cfg.kv not in ("bf16", "e4m3"):
+        raise ValueError(f"kv {cfg.kv!r}: bf16 or e4m3")
+    q8 = cfg.kv == "e4m3"
+    if q8 and hosted:
+        raise ValueError("a host engine's cache is bf16: no kv=\"e4m3\"")
     bufs, ops, states = {}, {}, {}
     bufs["token_ids"] = {"dtype": "i64", "shape": ["tokens"], "kind": "input", "fill": "token",
                          "domain": {"min": 0, "max": cfg.vocab - 1}}
@@ -134,10 +140,11 @@ def build_manifest(cfg: DenseConfig, hosted: bool = False) -> dict:
     bufs["last"] = {"dtype": "bf16", "shape": ["seqs", h], "kind": "workspace"}
     bufs["last_n"] = {"dtype": "bf16", "shape": ["seqs", h], "kind": "workspace"}
     bufs["logits"] = {"dtype": "bf16", "shape": ["seqs", cfg.vocab], "kind": "workspace"}
-    bufs["work"] = {"dtype": "i32", "shape": [2 * (-(-T // max(1, 64 // (hq // hk))) + S)], "kind": "workspace"}
-    bufs["work_count"] = {"dtype": "i32", "shape": [1], "kind": "workspace"}
-    bufs["work_d"] = {"dtype": "i32", "shape": [2 * S], "kind": "workspace"}
-    bufs["work_d_count"] = {"dtype": "i32", "shape": [1], "kind": "workspace"}
+    if not q8:
+        bufs["work"] = {"dtype": "i32", "shape": [2 * (-(-T // max(1, 64 // (hq // hk))) + S)], "kind": "workspace"}
+        bufs["work_count"] = {"dtype": "i32", "shape": [1], "kind": "workspace"}
+        bufs["work_d"] = {"dtype": "i32", "shape": [2 * S], "kind": "workspace"}
+        bufs["work_d_count"] = {"dtype": "i32", "shape": [1], "kind": "workspace"}
     bufs["rope_cos"] = {"dtype": "f32", "shape": [cfg.max_context, d // 2], "kind": "carry"}
     bufs["rope_sin"] = {"dtype": "f32", "shape": [cfg.max_context, d // 2], "kind": "carry"}
     if cfg.sampling:
@@ -173,10 +180,15 @@ def build_manifest(cfg: DenseConfig, hosted: bool = False) -> dict:
     ops["gate_up"] = C.gemm_op(2 * inter, h, epilogue="swiglu", rows_max=T)
     ops["down_proj"] = C.gemm_op(h, inter, epilogue="acc", rows_max=T)
     ops["lm_head"] = C.gemm_op(cfg.vocab, h, rows_var="seqs", rows_max=S)
-    ops["rope_append"] = C.rope_append_op(hq, hk, d, d, cfg.page_size, cfg.max_context, cfg.eps, cfg.qk_norm)
-    ops["attn_plan"] = C.attn_plan_op(hq, hk, S, d)
-    ops["attn_prefill"] = C.attn_prefill_op(hq, hk, d, cfg.page_size, W, cfg.qkv_dim)
-    ops["attn_decode"] = C.attn_decode_op(hq, hk, d, cfg.page_size, W, cfg.qkv_dim, S)
+    if q8:
+        ops["rope_append"] = C.rope_append_e4m3_op(hq, hk, d, d, cfg.page_size, cfg.max_context, cfg.eps, cfg.qk_norm)
+        ops["attn_prefill"] = C.attn_prefill_e4m3_op(hq, hk, d, cfg.page_size, W, cfg.qkv_dim, S)
+        ops["attn_decode"] = C.attn_decode_e4m3_op(hq, hk, d, cfg.page_size, W, cfg.qkv_dim, S)
+    else:
+        ops["rope_append"] = C.rope_append_op(hq, hk, d, d, cfg.page_size, cfg.max_context, cfg.eps, cfg.qk_norm)
+        ops["attn_plan"] = C.attn_plan_op(hq, hk, S, d)
+        ops["attn_prefill"] = C.attn_prefill_op(hq, hk, d, cfg.page_size, W, cfg.qkv_dim)
+        ops["attn_decode"] = C.attn_decode_op(hq, hk, d, cfg.page_size, W, cfg.qkv_dim, S)
     ops["last_row"] = C.last_row_op(h * 2)
     ops["rope_table"] = C.rope_table_op(cfg.max_context, d, cfg.rope_theta)
     ops["pick"] = C.sample_op(cfg.vocab) if cfg.sampling else C.argmax_op(cfg.vocab)
@@ -195,7 +207,10 @@ def build_manifest(cfg: DenseConfig, hosted: bool = False) -> dict:
             {"op": "qkv_proj", "label": lbl + "qkv", "args": [B("xn"), B(f"w.l{i}.qkv"), B("qkv"), {"var": "tokens"}, err]},
             {"op": "rope_append", "label": lbl + "rope", "args": rope_args + [err]},
         ]
-        if prefill:
+        if prefill and q8:
+            calls.append({"op": "attn_prefill", "label": lbl + "attn",
+                          "args": [B("qkv"), kv, B("attn"), B("block_table"), B("seq_lens"), B("cu_seqlens"), {"var": "seqs"}, err]})
+        elif prefill:
             calls.append({"op": "attn_prefill", "label": lbl + "attn",
                           "args": [B("qkv"), kv, B("attn"), B("block_table"), B("seq_lens"), B("cu_seqlens"), B("work"),
                                    B("work_count"), err, B("work_d"), B("work_d_count")]})
@@ -223,10 +238,11 @@ def build_manifest(cfg: DenseConfig, hosted: bool = False) -> dict:
             pick_call(),
         ]
 
-    prefill = [{"op": "embed", "label": "embed", "args": [B("token_ids"), B("w.embed"), B("x"), err]},
-               {"op": "attn_plan", "label": "plan", "args": [B("cu_seqlens"), B("work"), B("work_count"), {"var": "seqs"},
+    prefill = [{"op": "embed", "label": "embed", "args": [B("token_ids"), B("w.embed"), B("x"), err]}]
+    if not q8:
+        prefill.append({"op": "attn_plan", "label": "plan", "args": [B("cu_seqlens"), B("work"), B("work_count"), {"var": "seqs"},
                                                               {"expr": C.attn_plan_items(hq, hk)}, B("work_d"),
-                                                              B("work_d_count")]}]
+                                                              B("work_d_count")]})
     decode = [{"op": "embed", "label": "embed", "args": [B("token_ids"), B("w.embed"), B("x"), err]}]
     for i in range(cfg.layers):
         prefill += layer(i, True)
@@ -257,7 +273,7 @@ def build_manifest(cfg: DenseConfig, hosted: bool = False) -> dict:
         programs.update({"prefill": {"batch": {"groups": S, "rows": "tokens"}, "calls": prefill},
                          "decode": {"batch": {"groups": S, "rows": 1}, "graph": True, "calls": decode}})
 
-    mods = ["norm_embed", "gemm_bf16", "attn_prep", "attn_paged"] + ([] if hosted else ["misc", "sampling"])
+    mods = ["norm_embed", "gemm_bf16", "attn_prep"] + (C.e4m3_modules(d) if q8 else ["attn_paged"]) + ([] if hosted else ["misc", "sampling"])
     return C.ensure_modules({
         "schema_version": 7,
         "model": cfg.name,
@@ -340,6 +356,10 @@ class DenseOracle:
                 q = self._norm(q, w[p + "self_attn.q_norm.weight"])
                 k = self._norm(k, w[p + "self_attn.k_norm.weight"])
             q, k = self._rope(q, pos), self._rope(k, pos)
+            if cfg.kv == "e4m3":
+                from ..ops.kv_e4m3 import dequantise_reference, quantise_reference
+
+                k, v = (dequantise_reference(*quantise_reference(x)).to(x.dtype) for x in (k, v))
             if cache[i][0] is not None:
                 k = torch.cat([cache[i][0], k], 0)
                 v = torch.cat([cache[i][1], v], 0)

@@ -15,6 +15,8 @@ from . import dense
 
 
 def build_manifest_dcp(cfg: dense.DenseConfig, world: int, splits: int = 4, group: str = "dcp") -> dict:
+    if cfg.kv != "bf16":
+        raise ValueError("context parallelism deals a bf16 cache: no kv=\"e4m3\"")
     doc = dense.build_manifest(cfg)
     hq, hk, d = cfg.heads, cfg.kv_heads, cfg.head_dim
     doc["model"] = f"{doc['model']}-dcp{world}"

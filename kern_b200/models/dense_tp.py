@@ -25,6 +25,8 @@ def build_manifest_tp(cfg: DenseConfig, fused: bool = True, lamport: bool = True
     """`fused`: the o/down projections push their partial rows to the reducing rank from the GEMM epilogue
     (GEMM + reduce-scatter in one kernel); off, they store the partial and the all-reduce kernel pushes it.
     `lamport`: decode-sized calls use the flagless one-shot all-reduce."""
+    if cfg.kv != "bf16":
+        raise ValueError("the tensor-parallel decoder keeps a bf16 cache: no kv=\"e4m3\"")
     n = cfg.tp
     assert n >= 2 and cfg.heads % n == 0 and cfg.kv_heads % n == 0 and cfg.intermediate % (16 * n) == 0
     h, d = cfg.hidden, cfg.head_dim

@@ -189,7 +189,8 @@ def build_manifest(cfg: MoeConfig) -> dict:
     """The dense decoder's manifest with every layer's MLP replaced by the routed experts."""
     doc = dense.build_manifest(cfg)
     doc["model"] = cfg.name
-    return moeify(doc, cfg, ["norm_embed", "gemm_bf16", "attn_prep", "attn_paged", "misc", "sampling", "moe"])
+    attn = C.e4m3_modules(cfg.head_dim) if cfg.kv == "e4m3" else ["attn_paged"]
+    return moeify(doc, cfg, ["norm_embed", "gemm_bf16", "attn_prep", *attn, "misc", "sampling", "moe"])
 
 
 def moeify(doc: dict, cfg, modules: list[str]) -> dict:

@@ -73,6 +73,8 @@ def draft_config(target: dense.DenseConfig, layers: int = 1, hidden: int | None 
 
 
 def build_manifest(target: dense.DenseConfig, draft: dense.DenseConfig | None = None, k: int = 4) -> dict:
+    if target.kv != "bf16":
+        raise ValueError("a speculative round reads a bf16 cache: no kv=\"e4m3\"")
     draft = draft or draft_config(target)
     assert draft.vocab == target.vocab and draft.page_size == target.page_size and draft.max_context == target.max_context
     R = k + 1
