@@ -39,7 +39,8 @@ struct TileCfg {
   static constexpr int kHalf = kT * D * 2;                  // a half: a tile of K or of V, as 16-bit values
   static constexpr int kRing = E4M3 ? 4 : 5;                // halves that the products read
   static constexpr int kCodes = E4M3 ? kT * D : 0;          // a half as codes, as it comes
-  static constexpr int kSlots = E4M3 ? 2 : 0;               // of which there are so many under way
+  static constexpr int kSlots = E4M3 ? 2 : 0;               // of which there are so many under way,
+  static constexpr int kParts = E4M3 && D == 128 ? 2 : 1;   // in parts, as many rows as are converted at a time
   static constexpr int kScales = kSlots * 2 * kT;           // with their scale bytes, and V's beside K's
   // (all of the SM's 227 KB are in use: that the base lies on a 1024-byte boundary, as it does in practice, is checked)
   static constexpr int kSmem = kQBytes + kRing * kHalf + kSlots * kCodes + kScales + 4 * kQ * 4 + 512;
@@ -183,7 +184,7 @@ __device__ __noinline__ void tile_wide(const RowsArgs& a, int seq, int row0, int
 template <int D, bool E4M3, bool TREE>
 KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const int seqs) {
   using Cfg = TileCfg<D, E4M3>;
-  constexpr int kRing = Cfg::kRing, kSlots = Cfg::kSlots, kCame = E4M3 ? kSlots : kRing;
+  constexpr int kRing = Cfg::kRing, kSlots = Cfg::kSlots, kParts = Cfg::kParts, kCame = E4M3 ? kSlots * kParts : kRing;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
   if (smem_u32(smem) & 1023) {                                // uniform, before any barrier or allocation
@@ -198,8 +199,8 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   float* x_s = reinterpret_cast<float*>(b_s + Cfg::kScales);
   uint64_t* full = reinterpret_cast<uint64_t*>(x_s + 4 * kQ); // [ring] a half can be read by the products,
   uint64_t* empty = full + kRing;                             // [ring] has been read;
-  uint64_t* came = empty + kRing;                             // [ring; 8-bit: slots] the copy has landed;
-  uint64_t* taken = came + kCame;                             // [slots] the codes have been read
+  uint64_t* came = empty + kRing;                             // [ring; 8-bit: slots' parts] the copy has landed;
+  uint64_t* taken = came + kCame;                             // [slots' parts] the codes have been read
   uint64_t* s_full = taken + kCame;                              // per tile of rows: scores in TMEM,
   uint64_t* p_full = s_full + 2;                              // weights in TMEM,
   uint64_t* o_done = p_full + 2;                              // the last P V done
@@ -249,7 +250,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < kCame; ++s) {
-      mbar_init(&came[s], E4M3 ? 33 : 1);
+      mbar_init(&came[s], E4M3 && s % kParts == 0 ? 33 : 1);  // (scale bytes come with a slot's first part)
       mbar_init(&taken[s], 2);
     }
     for (int s = 0; s < 2; ++s) {
@@ -320,7 +321,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         int which, t;
         item(i, which, t);
         const int slot = i % kSlots, half = i % kRing, tok0 = from + t * kT;
-        if (!bar_wait(&came[slot], (i / kSlots) & 1, abort_flag)) {
+        if (!bar_wait(&came[slot * kParts], (i / kSlots) & 1, abort_flag)) {
           set_error(a.err, ERR_WAIT_FULL);
           *abort_flag = 1;
           ok = false;
@@ -339,6 +340,14 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         bool nan = false, free = false;
 #pragma unroll 1
         for (int r0 = (w4 & 1) * kRowsWarp + sub; r0 < kT; r0 += kBatch) {
+          static_assert(kBatch * kParts == kT, "a part is a batch");
+          const int part = r0 / kBatch;
+          if (part > 0 && !bar_wait(&came[slot * kParts + part], (i / kSlots) & 1, abort_flag)) {
+            set_error(a.err, ERR_WAIT_FULL);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
           uint32_t w[kLoads][4];
 #pragma unroll
           for (int j = 0; j < kLoads; ++j) {
@@ -350,6 +359,8 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
               asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2 * h]), "=r"(w[j][2 * h + 1]) : "r"(at));
             }
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&taken[slot * kParts + part]);      // (the codes are in registers, the scale bytes too)
           if (edge) {
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) {
@@ -389,8 +400,6 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
           }
         }
         if (!ok) break;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&taken[slot]);             // (the codes have been read)
         if (nan) *bad_s = 1;
         if (!which && (w4 & 1) == 0 && lane == 0) e_s[t & 3] = make_float2(pow2i(top - 127 - 6), (float)(vtop - 127 - 6));
         fence_proxy_async();
@@ -445,7 +454,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     for (int i = 0; i < items && ok; ++i) {
       int which, t;
       item(i, which, t);
-      const int slot = i % kCame, tok0 = from + t * kT, here = min(kT, to - tok0), boxes = (here + box - 1) / box;
+      const int slot = E4M3 ? i % kSlots : i % kRing, tok0 = from + t * kT, here = min(kT, to - tok0), boxes = (here + box - 1) / box;
       if (page_of(tok0) < first || page_of(tok0 + here - 1) >= first + 32) {
         // (the values of the tile before are still to come: a tile has 16 pages at most)
         first = page_of(max(tok0 - kT, from));
@@ -459,32 +468,49 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       // page, and row in it, of the eight tokens from 8 lane on
       const int tok = tok0 + 8 * (lane & 15), pi = page_of(tok), off = tok - pi * a.page_size;
       const int page = __shfl_sync(0xffffffffu, id, (pi - first) & 31);
-      if (!bar_wait(E4M3 ? &taken[slot] : &empty[slot], ((i / kCame) & 1) ^ 1, abort_flag)) {
-        set_error(a.err, ERR_WAIT_EMPTY);
-        *abort_flag = 1;
-        ok = false;
-        break;
-      }
-      // boxes behind the share's end are not brought
-      if (lane == 0) mbar_expect_tx(&came[slot], boxes * box * D * (E4M3 ? 1 : 2));
-      __syncwarp();
+      const int uses = i / (E4M3 ? kSlots : kRing);
       const int b_page = __shfl_sync(0xffffffffu, page, (lane * box >> 3) & 31), b_off = __shfl_sync(0xffffffffu, off, (lane * box >> 3) & 31);
       const int b_row = (which * a.hk + kvh) * a.page_size + b_off;
+      // boxes behind the share's end are not brought
       if constexpr (E4M3) {
-        if (lane < boxes) tma_load_3d(c_s + slot * Cfg::kCodes + lane * box * D, kv_map, 0, b_row, b_page, &came[slot]);
         const int s_page = __shfl_sync(0xffffffffu, page, lane >> 1), s_off = __shfl_sync(0xffffffffu, off, lane >> 1) + (lane & 1) * 4;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if (k && which) break;
-          const uint8_t* src = a.pool + (size_t)s_page * page_bytes + codes + (size_t)((k ? 1 : which) * a.hk + kvh) * a.page_size + s_off;
-          if (4 * lane < here && KERN_CHECK(src, 4, SITE_KV_ROW))
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(b_s + slot * 2 * kT + k * kT + 4 * lane)), "l"(src) : "memory");
-        }
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&came[slot])) : "memory");
-      } else if (lane < boxes) {
+        for (int p = 0; p < kParts; ++p) {
+          if (!bar_wait(&taken[slot * kParts + p], (uses & 1) ^ 1, abort_flag)) {
+            set_error(a.err, ERR_WAIT_EMPTY);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          uint64_t* bar = &came[slot * kParts + p];
+          const int lo = p * (kT / kParts) / box, hi = min(boxes, (p + 1) * (kT / kParts) / box);
+          if (lane == 0) mbar_expect_tx(bar, max(hi - lo, 0) * box * D);
+          __syncwarp();
+          if (lane >= lo && lane < hi) tma_load_3d(c_s + slot * Cfg::kCodes + lane * box * D, kv_map, 0, b_row, b_page, bar);
+          if (p) continue;
 #pragma unroll
-        for (int cb = 0; cb < D / 64; ++cb)
-          tma_load_3d(h_s + slot * Cfg::kHalf + cb * (kT * 128) + lane * box * 128, kv_map, cb * 64, b_row, b_page, &came[slot]);
+          for (int k = 0; k < 2; ++k) {
+            if (k && which) break;
+            const uint8_t* src = a.pool + (size_t)s_page * page_bytes + codes + (size_t)((k ? 1 : which) * a.hk + kvh) * a.page_size + s_off;
+            if (4 * lane < here && KERN_CHECK(src, 4, SITE_KV_ROW))
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(b_s + slot * 2 * kT + k * kT + 4 * lane)), "l"(src) : "memory");
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+        }
+      } else {
+        if (!bar_wait(&empty[slot], (uses & 1) ^ 1, abort_flag)) {
+          set_error(a.err, ERR_WAIT_EMPTY);
+          *abort_flag = 1;
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_expect_tx(&came[slot], boxes * box * D * 2);
+        __syncwarp();
+        if (lane < boxes) {
+#pragma unroll
+          for (int cb = 0; cb < D / 64; ++cb)
+            tma_load_3d(h_s + slot * Cfg::kHalf + cb * (kT * 128) + lane * box * 128, kv_map, cb * 64, b_row, b_page, &came[slot]);
+        }
       }
     }
   } else if (warp == 20) {
@@ -539,20 +565,26 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   } else {
     // ---------------- Q -> shared memory, K-major with the 128-byte swizzle: D / 8 lanes to a row ----------------
     {
-      constexpr int kLanes = D / 8;
+      constexpr int kLanes = D / 8, kPass = 512 / kLanes, kPasses = 2 * kQ / kPass;
       const int c = threadIdx.x % kLanes;
-#pragma unroll 4
-      for (int r = threadIdx.x / kLanes; r < 2 * kQ; r += 512 / kLanes) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        const int rr = twice ? r & (kQ - 1) : r;
-        if (rr < valid) v = *reinterpret_cast<const uint4*>(a.q + (size_t)(row0 + tok_lo + rr / G) * a.q_stride + (size_t)(kvh * G + rr % G) * D + c * 8);
+      uint4 rows[kPasses];                                    // (all under way together)
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = threadIdx.x / kLanes + i * kPass, rr = twice ? r & (kQ - 1) : r;
+        rows[i] = make_uint4(0, 0, 0, 0);
+        if (rr < valid) rows[i] = *reinterpret_cast<const uint4*>(a.q + (size_t)(row0 + tok_lo + rr / G) * a.q_stride + (size_t)(kvh * G + rr % G) * D + c * 8);
+      }
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = threadIdx.x / kLanes + i * kPass;
+        uint4 v = rows[i];
         float f = a.scale_log2;
         if constexpr (E4M3) {
           uint32_t w[4] = {v.x, v.y, v.z, v.w};
           float top = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 u = unpack_bf16x2(w[i]);
+          for (int k = 0; k < 4; ++k) {
+            const float2 u = unpack_bf16x2(w[k]);
             top = fmaxf(top, fmaxf(fabsf(u.x), fabsf(u.y)));
           }
 #pragma unroll
@@ -561,9 +593,9 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
           const float inv = pow2i(-x);
           f *= pow2i(x);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 u = unpack_bf16x2(w[i]);
-            w[i] = pack_f16x2(u.x * inv, u.y * inv);
+          for (int k = 0; k < 4; ++k) {
+            const float2 u = unpack_bf16x2(w[k]);
+            w[k] = pack_f16x2(u.x * inv, u.y * inv);
           }
           v = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -594,6 +626,10 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
                    : "memory");
       return any != 0;
     };
+    // A reference starts 2^5 under its first tile's maximum and moves, when a weight has outgrown f16
+    // (2^30 for bf16 weights). So weights down to 2^-19 of the largest keep all of f16's bits, and where key rows differ in size
+    // (by e^0.5) 128 rows move some 9 times in 4096 tokens; 17 times from 2^7 under it and at 2^15.
+    constexpr float kGrown = E4M3 ? 15.9f : 30.f, kBelow = E4M3 ? 5.f : 0.f;
     float ref = kUnset, l = 0.f;                              // l: of this thread's columns
     // which of tokens j .. j + 31 the row sees
     auto seen32 = [&](int j) -> uint32_t {
@@ -650,12 +686,12 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       }
       if (edge) tmem_st_done();
       mx = fmaf(mx, scale, ev);
-      if (any_of(mx > ref + 15.f)) {
+      if (any_of(mx > ref + kGrown)) {
         // a row's two threads move its reference together, and each passes over half of O
         *own_x = mx;
         meet();
         mx = fmaxf(mx, *his_x);
-        const float to_ref = mx > ref + 15.f ? ceilf(mx) - 7.f : ref, corr = exp2f(ref - to_ref);
+        const float to_ref = mx > ref + kGrown ? ceilf(mx) - kBelow : ref, corr = exp2f(ref - to_ref);
         ref = to_ref;
         l *= corr;
         if (n > 0) {
