@@ -604,7 +604,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       }
       fence_proxy_async();
       mbar_arrive(q_full);
-      asm volatile("bar.sync 3, 512;" ::: "memory");          // x_s
+      asm volatile("bar.sync 15, 512;" ::: "memory");          // x_s
     }
     // ---------------- softmax: two threads to a row, half of a tile's scores each ----------------
     const int side = (warp >> 2) & 1, part = warp >> 3, row = (warp & 3) * 32 + lane;
@@ -617,12 +617,13 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     const float f = x_s[side * 2 * kQ + row];                 // (read before the side's threads meet, written after)
     float* const own_x = x_s + (side * 2 + part) * kQ + row;  // what the row's two threads tell each other
     float* const his_x = x_s + (side * 2 + 1 - part) * kQ + row;
-    auto meet = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(1 + side) : "memory"); };
-    auto any_of = [&](bool mine) -> bool {                    // over the side's 256 threads
+    const int pair = 1 + (warp & 7);                          // barrier of the two warps that share 32 rows
+    auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory"); };
+    auto any_of = [&](bool mine) -> bool {                    // over the two warps' threads
       uint32_t any;
-      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                    : "=r"(any)
-                   : "r"(1 + side), "r"((uint32_t)mine)
+                   : "r"(pair), "r"((uint32_t)mine)
                    : "memory");
       return any != 0;
     };
@@ -745,7 +746,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     l += *his_x;
     constexpr int kHalfD = D / 2, kPad = kHalfD + 3;
     float* other = reinterpret_cast<float*>(h_s) + part * (kQ * kPad);    // (twice) the second side's rows: columns, reference, sum
-    if (twice) asm volatile("bar.sync 3, 512;" ::: "memory"); // both sides' products are done: the ring is free
+    if (twice) asm volatile("bar.sync 15, 512;" ::: "memory"); // both sides' products are done: the ring is free
     const bool wide = E4M3 && *wide_s != 0;                   // (uniform: every half has been looked at)
     if (twice) {
       if (side == 1) {
@@ -761,7 +762,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
           for (int i = 0; i < 32; ++i) mine[c + i] = steps > 0 ? __uint_as_float(x[i]) : 0.f;
         }
       }
-      asm volatile("bar.sync 3, 512;" ::: "memory");
+      asm volatile("bar.sync 15, 512;" ::: "memory");
     }
     if (wide) {
       if constexpr (E4M3) {
