@@ -1,7 +1,7 @@
 // Attention of many query rows over a paged cache, bf16 or e4m3, on the 5th-generation tensor cores: prompt chunks (causal) and
 // trees of drafted tokens. The formulas, formats and what a row sees are those of attn_rows.cu, which has the few rows.
 //
-// One CTA = (256 query rows: the G heads of 256 / G tokens, one kv head, a share of the context), 22 warps:
+// One CTA = (256 query rows: the G heads of 256 / G tokens, one kv head, a share of the context), 22 working warps of 24:
 //
 //   warps 0..15        softmax of two 128-row tiles, two threads to a row, 64 of a tile's scores each: scores out of TMEM, weights
 //                      back into TMEM over them
@@ -31,7 +31,7 @@
 namespace kern {
 
 constexpr int kQ = 128, kT = 128;    // query rows of a tile, tokens of a tile
-constexpr int kTileThreads = 704;
+constexpr int kTileThreads = 768;    // (of 24 warps, for warpgroups; the last two only hand over their registers)
 
 template <int D, bool E4M3>
 struct TileCfg {
@@ -99,6 +99,18 @@ KERN_DEVICE void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
       "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+KERN_DEVICE void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+KERN_DEVICE void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
 }
 KERN_DEVICE float max3(float a, float b, float c) {
   float r;
@@ -299,8 +311,10 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   auto k_item = [&](int t) { return t == 0 ? 0 : 2 * t - 1; };
   auto v_item = [&](int t) { return t == ntiles - 1 ? items - 1 : 2 * t + 2; };
 
+  // Registers: 80 a thread at launch, 24 * 32 * 80 in all = 16 warps of 88, 4 of 72 and 4 of 56.
   if (warp >= 16 && warp < 20) {
     // ---------------- keys and values ----------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     const int tid = threadIdx.x - 512, w4 = warp - 16;
     if constexpr (E4M3) {
       // two warps to a half, so that two halves are under way; in batches of 8 rows a lane
@@ -442,127 +456,131 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         if (lane == 0) mbar_arrive(&full[half]);
       }
     }
-  } else if (warp == 21) {
-    // ---------------- copies: bf16 halves into the ring, 8-bit codes and scale bytes into their slots ----------------
-    const size_t codes = (size_t)2 * a.hk * a.page_size * D, page_bytes = codes + 2 * a.hk * a.page_size;
-    const int box = a.page_size < 64 ? a.page_size : 64;
-    const int* pages = a.block_table + (size_t)seq * a.max_pages;
-    // runs of 64 tokens (or of a smaller page's) lie in one page; the table is read 32 pages at a time, a lane each
-    const int bits = a.page_size < 64 ? 31 - __clz(a.page_size) : 6, per = a.page_size < 64 ? 1 : a.page_size >> 6;
-    auto page_of = [&](int tok) { return per == 1 ? tok >> bits : (tok >> bits) / per; };
-    int first = -64, id = 0;
-    for (int i = 0; i < items && ok; ++i) {
-      int which, t;
-      item(i, which, t);
-      const int slot = E4M3 ? i % kSlots : i % kRing, tok0 = from + t * kT, here = min(kT, to - tok0), boxes = (here + box - 1) / box;
-      if (page_of(tok0) < first || page_of(tok0 + here - 1) >= first + 32) {
-        // (the values of the tile before are still to come: a tile has 16 pages at most)
-        first = page_of(max(tok0 - kT, from));
-        const int pi = first + lane;
-        id = pi < a.max_pages ? pages[pi] : -1;
-        if (id < 0 || id >= a.pool_pages) {
-          if (pi * a.page_size < to) set_error(a.err, ERR_BOUNDS);
-          id = 0;
+  } else if (warp >= 20) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 21) {
+      // ---------------- copies: bf16 halves into the ring, 8-bit codes and scale bytes into their slots ----------------
+      const size_t codes = (size_t)2 * a.hk * a.page_size * D, page_bytes = codes + 2 * a.hk * a.page_size;
+      const int box = a.page_size < 64 ? a.page_size : 64;
+      const int* pages = a.block_table + (size_t)seq * a.max_pages;
+      // runs of 64 tokens (or of a smaller page's) lie in one page; the table is read 32 pages at a time, a lane each
+      const int bits = a.page_size < 64 ? 31 - __clz(a.page_size) : 6, per = a.page_size < 64 ? 1 : a.page_size >> 6;
+      auto page_of = [&](int tok) { return per == 1 ? tok >> bits : (tok >> bits) / per; };
+      int first = -64, id = 0;
+      for (int i = 0; i < items && ok; ++i) {
+        int which, t;
+        item(i, which, t);
+        const int slot = E4M3 ? i % kSlots : i % kRing, tok0 = from + t * kT, here = min(kT, to - tok0), boxes = (here + box - 1) / box;
+        if (page_of(tok0) < first || page_of(tok0 + here - 1) >= first + 32) {
+          // (the values of the tile before are still to come: a tile has 16 pages at most)
+          first = page_of(max(tok0 - kT, from));
+          const int pi = first + lane;
+          id = pi < a.max_pages ? pages[pi] : -1;
+          if (id < 0 || id >= a.pool_pages) {
+            if (pi * a.page_size < to) set_error(a.err, ERR_BOUNDS);
+            id = 0;
+          }
         }
-      }
-      // page, and row in it, of the eight tokens from 8 lane on
-      const int tok = tok0 + 8 * (lane & 15), pi = page_of(tok), off = tok - pi * a.page_size;
-      const int page = __shfl_sync(0xffffffffu, id, (pi - first) & 31);
-      const int uses = i / (E4M3 ? kSlots : kRing);
-      const int b_page = __shfl_sync(0xffffffffu, page, (lane * box >> 3) & 31), b_off = __shfl_sync(0xffffffffu, off, (lane * box >> 3) & 31);
-      const int b_row = (which * a.hk + kvh) * a.page_size + b_off;
-      // boxes behind the share's end are not brought
-      if constexpr (E4M3) {
-        const int s_page = __shfl_sync(0xffffffffu, page, lane >> 1), s_off = __shfl_sync(0xffffffffu, off, lane >> 1) + (lane & 1) * 4;
-#pragma unroll
-        for (int p = 0; p < kParts; ++p) {
-          if (!bar_wait(&taken[slot * kParts + p], (uses & 1) ^ 1, abort_flag)) {
+        // page, and row in it, of the eight tokens from 8 lane on
+        const int tok = tok0 + 8 * (lane & 15), pi = page_of(tok), off = tok - pi * a.page_size;
+        const int page = __shfl_sync(0xffffffffu, id, (pi - first) & 31);
+        const int uses = i / (E4M3 ? kSlots : kRing);
+        const int b_page = __shfl_sync(0xffffffffu, page, (lane * box >> 3) & 31), b_off = __shfl_sync(0xffffffffu, off, (lane * box >> 3) & 31);
+        const int b_row = (which * a.hk + kvh) * a.page_size + b_off;
+        // boxes behind the share's end are not brought
+        if constexpr (E4M3) {
+          const int s_page = __shfl_sync(0xffffffffu, page, lane >> 1), s_off = __shfl_sync(0xffffffffu, off, lane >> 1) + (lane & 1) * 4;
+  #pragma unroll
+          for (int p = 0; p < kParts; ++p) {
+            if (!bar_wait(&taken[slot * kParts + p], (uses & 1) ^ 1, abort_flag)) {
+              set_error(a.err, ERR_WAIT_EMPTY);
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            uint64_t* bar = &came[slot * kParts + p];
+            const int lo = p * (kT / kParts) / box, hi = min(boxes, (p + 1) * (kT / kParts) / box);
+            if (lane == 0) mbar_expect_tx(bar, max(hi - lo, 0) * box * D);
+            __syncwarp();
+            if (lane >= lo && lane < hi) tma_load_3d(c_s + slot * Cfg::kCodes + lane * box * D, kv_map, 0, b_row, b_page, bar);
+            if (p) continue;
+  #pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              if (k && which) break;
+              const uint8_t* src = a.pool + (size_t)s_page * page_bytes + codes + (size_t)((k ? 1 : which) * a.hk + kvh) * a.page_size + s_off;
+              if (4 * lane < here && KERN_CHECK(src, 4, SITE_KV_ROW))
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(b_s + slot * 2 * kT + k * kT + 4 * lane)), "l"(src) : "memory");
+            }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+          }
+        } else {
+          if (!bar_wait(&empty[slot], (uses & 1) ^ 1, abort_flag)) {
             set_error(a.err, ERR_WAIT_EMPTY);
             *abort_flag = 1;
             ok = false;
             break;
           }
-          uint64_t* bar = &came[slot * kParts + p];
-          const int lo = p * (kT / kParts) / box, hi = min(boxes, (p + 1) * (kT / kParts) / box);
-          if (lane == 0) mbar_expect_tx(bar, max(hi - lo, 0) * box * D);
+          if (lane == 0) mbar_expect_tx(&came[slot], boxes * box * D * 2);
           __syncwarp();
-          if (lane >= lo && lane < hi) tma_load_3d(c_s + slot * Cfg::kCodes + lane * box * D, kv_map, 0, b_row, b_page, bar);
-          if (p) continue;
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            if (k && which) break;
-            const uint8_t* src = a.pool + (size_t)s_page * page_bytes + codes + (size_t)((k ? 1 : which) * a.hk + kvh) * a.page_size + s_off;
-            if (4 * lane < here && KERN_CHECK(src, 4, SITE_KV_ROW))
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(b_s + slot * 2 * kT + k * kT + 4 * lane)), "l"(src) : "memory");
+          if (lane < boxes) {
+  #pragma unroll
+            for (int cb = 0; cb < D / 64; ++cb)
+              tma_load_3d(h_s + slot * Cfg::kHalf + cb * (kT * 128) + lane * box * 128, kv_map, cb * 64, b_row, b_page, &came[slot]);
           }
-          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
         }
-      } else {
-        if (!bar_wait(&empty[slot], (uses & 1) ^ 1, abort_flag)) {
-          set_error(a.err, ERR_WAIT_EMPTY);
-          *abort_flag = 1;
-          ok = false;
-          break;
+      }
+    } else if (warp == 20) {
+      // ---------------- products: the whole warp walks and waits, one lane issues ----------------
+      constexpr uint32_t idesc_qk = tile_idesc<E4M3>(kQ, kT, false), idesc_pv = tile_idesc<E4M3>(kQ, D, true);
+      const int steps = twice ? ntiles : 2 * ntiles;
+      const uint32_t q_low = desc_low(smem_u32(q_s), 0), h_low = desc_low(smem_u32(h_s), 0), v_low = desc_low(smem_u32(h_s), kT * 128);
+      const bool leader = elect_lane();
+      auto qk = [&](int u) -> bool {
+        const int side = u & 1, t = twice ? u : u >> 1;
+        const int i = k_item(t), half = i % kRing;
+        if (!bar_wait(&full[half], (i / kRing) & 1, abort_flag)) return false;
+        tc_fence_after();
+        const uint32_t sq = q_low + side * (kQ * D * 2 >> 4), sk = h_low + half * (Cfg::kHalf >> 4), s_t = tmem + side * 128;
+        if (leader) {
+  #pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_ss(s_t, sq + ((k >> 2) * (kQ * 128) + (k & 3) * 32 >> 4), sk + ((k >> 2) * (kT * 128) + (k & 3) * 32 >> 4), idesc_qk, k != 0);
+          tc_commit(&s_full[side]);
+          if (twice || side) tc_commit(&empty[half]);
         }
-        if (lane == 0) mbar_expect_tx(&came[slot], boxes * box * D * 2);
         __syncwarp();
-        if (lane < boxes) {
-#pragma unroll
-          for (int cb = 0; cb < D / 64; ++cb)
-            tma_load_3d(h_s + slot * Cfg::kHalf + cb * (kT * 128) + lane * box * 128, kv_map, cb * 64, b_row, b_page, &came[slot]);
+        return true;
+      };
+      auto pv = [&](int u) -> bool {
+        const int side = u & 1, t = twice ? u : u >> 1, n = u >> 1;
+        const int i = v_item(t), half = i % kRing;
+        if (!bar_wait(&full[half], (i / kRing) & 1, abort_flag)) return false;
+        if (!bar_wait(&p_full[side], n & 1, abort_flag)) return false;
+        tc_fence_after();
+        const uint32_t sv = v_low + half * (Cfg::kHalf >> 4), o_t = tmem + 256 + side * D, p_t = tmem + side * 128;
+        if (leader) {
+  #pragma unroll
+          for (int k = 0; k < kT / 16; ++k) umma_ts(o_t, p_t + (k < 4 ? k : k + 4) * 8, sv + (k * 16 * 128 >> 4), idesc_pv, (n | k) != 0);
+          if (twice || side) tc_commit(&empty[half]);
+          if (u + 2 >= steps) tc_commit(&o_done[side]);
         }
+        __syncwarp();
+        return true;
+      };
+      if (steps > 0) ok = bar_wait(q_full, 0, abort_flag) && qk(0);
+      if (ok && steps > 1) ok = qk(1);
+      for (int u = 0; u < steps && ok; ++u) {
+        ok = pv(u);
+        if (ok && u + 2 < steps) ok = qk(u + 2);                // (overwrites the scores whose weights P V has just been given)
       }
-    }
-  } else if (warp == 20) {
-    // ---------------- products: the whole warp walks and waits, one lane issues ----------------
-    constexpr uint32_t idesc_qk = tile_idesc<E4M3>(kQ, kT, false), idesc_pv = tile_idesc<E4M3>(kQ, D, true);
-    const int steps = twice ? ntiles : 2 * ntiles;
-    const uint32_t q_low = desc_low(smem_u32(q_s), 0), h_low = desc_low(smem_u32(h_s), 0), v_low = desc_low(smem_u32(h_s), kT * 128);
-    const bool leader = elect_lane();
-    auto qk = [&](int u) -> bool {
-      const int side = u & 1, t = twice ? u : u >> 1;
-      const int i = k_item(t), half = i % kRing;
-      if (!bar_wait(&full[half], (i / kRing) & 1, abort_flag)) return false;
-      tc_fence_after();
-      const uint32_t sq = q_low + side * (kQ * D * 2 >> 4), sk = h_low + half * (Cfg::kHalf >> 4), s_t = tmem + side * 128;
-      if (leader) {
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          umma_ss(s_t, sq + ((k >> 2) * (kQ * 128) + (k & 3) * 32 >> 4), sk + ((k >> 2) * (kT * 128) + (k & 3) * 32 >> 4), idesc_qk, k != 0);
-        tc_commit(&s_full[side]);
-        if (twice || side) tc_commit(&empty[half]);
+      if (!ok) {
+        set_error(a.err, ERR_WAIT_FULL);
+        *abort_flag = 1;
       }
       __syncwarp();
-      return true;
-    };
-    auto pv = [&](int u) -> bool {
-      const int side = u & 1, t = twice ? u : u >> 1, n = u >> 1;
-      const int i = v_item(t), half = i % kRing;
-      if (!bar_wait(&full[half], (i / kRing) & 1, abort_flag)) return false;
-      if (!bar_wait(&p_full[side], n & 1, abort_flag)) return false;
-      tc_fence_after();
-      const uint32_t sv = v_low + half * (Cfg::kHalf >> 4), o_t = tmem + 256 + side * D, p_t = tmem + side * 128;
-      if (leader) {
-#pragma unroll
-        for (int k = 0; k < kT / 16; ++k) umma_ts(o_t, p_t + (k < 4 ? k : k + 4) * 8, sv + (k * 16 * 128 >> 4), idesc_pv, (n | k) != 0);
-        if (twice || side) tc_commit(&empty[half]);
-        if (u + 2 >= steps) tc_commit(&o_done[side]);
-      }
-      __syncwarp();
-      return true;
-    };
-    if (steps > 0) ok = bar_wait(q_full, 0, abort_flag) && qk(0);
-    if (ok && steps > 1) ok = qk(1);
-    for (int u = 0; u < steps && ok; ++u) {
-      ok = pv(u);
-      if (ok && u + 2 < steps) ok = qk(u + 2);                // (overwrites the scores whose weights P V has just been given)
     }
-    if (!ok) {
-      set_error(a.err, ERR_WAIT_FULL);
-      *abort_flag = 1;
-    }
-    __syncwarp();
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
     // ---------------- Q -> shared memory, K-major with the 128-byte swizzle: D / 8 lanes to a row ----------------
     {
       constexpr int kLanes = D / 8, kPass = 512 / kLanes, kPasses = 2 * kQ / kPass;
@@ -666,26 +684,33 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         scale *= e.x;
         ev = e.y;
       }
-      // ---- the largest score; in a tile whose rows see different tokens the others become -inf where they lie ----
-      float mx = -INFINITY;
+      if (edge) {
+        // the scores that a row does not see become -inf where they lie
 #pragma unroll 1
-      for (int c = 0; c < 64; c += 32) {
-        uint32_t x[32];
-        tmem_ld_32x32(s_t + c, x);
-        tmem_ld_wait();
-        if (edge) {
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t x[32];
+          tmem_ld_32x32(s_t + c, x);
+          tmem_ld_wait();
           const uint32_t b = seen32(tok0 + part * 64 + c);
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             if (!(b >> i & 1)) x[i] = 0xff800000u;
           tmem_st32(s_t + c, x);
         }
-        float m2[2] = {mx, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) m2[(i >> 1) & 1] = max3(m2[(i >> 1) & 1], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-        mx = fmaxf(m2[0], m2[1]);
+        tmem_st_done();
       }
-      if (edge) tmem_st_done();
+      // ---- the largest score (16 columns on their way while 16 are looked at) ----
+      uint32_t x[2][16];
+      float m2[2] = {-INFINITY, -INFINITY};
+      tmem_ld16(s_t, x[0]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld_wait();
+        if (c < 3) tmem_ld16(s_t + (c + 1) * 16, x[(c + 1) & 1]);
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) m2[(i >> 1) & 1] = max3(m2[(i >> 1) & 1], __uint_as_float(x[c & 1][i]), __uint_as_float(x[c & 1][i + 1]));
+      }
+      float mx = fmaxf(m2[0], m2[1]);
       mx = fmaf(mx, scale, ev);
       if (any_of(mx > ref + kGrown)) {
         // a row's two threads move its reference together, and each passes over half of O
@@ -698,13 +723,13 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         if (n > 0) {
           // (these scores' products were issued behind the last P V: O is quiet)
 #pragma unroll 1
-          for (int c = 0; c < D / 2; c += 32) {
-            uint32_t x[32];
-            tmem_ld_32x32(o_t + c, x);
+          for (int c = 0; c < D / 2; c += 16) {
+            uint32_t y[16];
+            tmem_ld16(o_t + c, y);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * corr);
-            tmem_st32(o_t + c, x);
+            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * corr);
+            tmem_st16(o_t + c, y);
           }
           tmem_st_done();
         }
@@ -713,19 +738,20 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       // ---- weights, over scores of this thread's own that have been read; their sum ----
       const uint64_t scale2 = pair64(scale, scale), shift2 = pair64(ev - ref, ev - ref);
       uint64_t sum2[2] = {0, 0};
-#pragma unroll 1
-      for (int c = 0; c < 64; c += 32) {
-        uint32_t x[32], pk[16];
-        tmem_ld_32x32(s_t + c, x);
-        tmem_ld_wait();
+      tmem_ld16(s_t, x[0]);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 y = split64(fma2(pair64(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, shift2));
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pk[8];
+        tmem_ld_wait();
+        if (c < 3) tmem_ld16(s_t + (c + 1) * 16, x[(c + 1) & 1]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 y = split64(fma2(pair64(__uint_as_float(x[c & 1][2 * i]), __uint_as_float(x[c & 1][2 * i + 1])), scale2, shift2));
           const float u = exp2f(y.x), v = exp2f(y.y);
           sum2[i & 1] = add2(sum2[i & 1], pair64(u, v));
           pk[i] = pack_pair<E4M3>(u, v);
         }
-        tmem_st16(s_t + (c >> 1), pk);
+        tmem_st8(s_t + c * 8, pk);
       }
       const float2 sum = split64(add2(sum2[0], sum2[1]));
       l += E4M3 ? (sum.x + sum.y) * exp2f(-ev) : sum.x + sum.y;

@@ -694,7 +694,7 @@ def attn_prefill_e4m3_op(hq: int, hk: int, d: int, page_size: int, table_width: 
                             _ops_host.rows_form(d, True, nt)[0], 1,
                             hq, hk, d, page_size, table_width, q_stride, {"i32": 1}, few + 1, I32_MAX, 5, 7, None)
     else:
-        many = _e4m3_attend(f"kern_attn_tile_e4m3_causal_d{d}", [hk, {"add": [{"ceil_div": ["tokens", 256 // g]}, "seqs"]}, 1], 704,
+        many = _e4m3_attend(f"kern_attn_tile_e4m3_causal_d{d}", [hk, {"add": [{"ceil_div": ["tokens", 256 // g]}, "seqs"]}, 1], 768,
                             _ops_host.tile_shared(d, True), 1,
                             hq, hk, d, page_size, table_width, q_stride, {"param": 6}, few + 1, I32_MAX, 5, 7, None)
     return {"params": iface, "impl": {"launches": [many] + _e4m3_few(hq, hk, d, page_size, table_width, q_stride, seqs_max, few, few, 5, 7)}}
