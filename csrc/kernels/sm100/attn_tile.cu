@@ -214,7 +214,8 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   uint64_t* came = empty + kRing;                             // [ring; 8-bit: slots' parts] the copy has landed;
   uint64_t* taken = came + kCame;                             // [slots' parts] the codes have been read
   uint64_t* s_full = taken + kCame;                              // per tile of rows: scores in TMEM,
-  uint64_t* p_full = s_full + 2;                              // weights in TMEM,
+  uint64_t* p_half = s_full + 2;                              // the first half of each thread's weights in TMEM,
+  uint64_t* p_full = p_half + 2;                              // the others,
   uint64_t* o_done = p_full + 2;                              // the last P V done
   uint64_t* q_full = o_done + 2;                              // Q in shared memory
   float2* e_s = reinterpret_cast<float2*>(q_full + 2);        // [4] a key tile's (2^E of K, E of V)
@@ -267,6 +268,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
+      mbar_init(&p_half[s], 8);
       mbar_init(&p_full[s], 8);
       mbar_init(&o_done[s], 1);
     }
@@ -490,7 +492,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         // boxes behind the share's end are not brought
         if constexpr (E4M3) {
           const int s_page = __shfl_sync(0xffffffffu, page, lane >> 1), s_off = __shfl_sync(0xffffffffu, off, lane >> 1) + (lane & 1) * 4;
-  #pragma unroll
+#pragma unroll
           for (int p = 0; p < kParts; ++p) {
             if (!bar_wait(&taken[slot * kParts + p], (uses & 1) ^ 1, abort_flag)) {
               set_error(a.err, ERR_WAIT_EMPTY);
@@ -504,7 +506,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
             __syncwarp();
             if (lane >= lo && lane < hi) tma_load_3d(c_s + slot * Cfg::kCodes + lane * box * D, kv_map, 0, b_row, b_page, bar);
             if (p) continue;
-  #pragma unroll
+#pragma unroll
             for (int k = 0; k < 2; ++k) {
               if (k && which) break;
               const uint8_t* src = a.pool + (size_t)s_page * page_bytes + codes + (size_t)((k ? 1 : which) * a.hk + kvh) * a.page_size + s_off;
@@ -523,7 +525,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
           if (lane == 0) mbar_expect_tx(&came[slot], boxes * box * D * 2);
           __syncwarp();
           if (lane < boxes) {
-  #pragma unroll
+#pragma unroll
             for (int cb = 0; cb < D / 64; ++cb)
               tma_load_3d(h_s + slot * Cfg::kHalf + cb * (kT * 128) + lane * box * 128, kv_map, cb * 64, b_row, b_page, &came[slot]);
           }
@@ -542,7 +544,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         tc_fence_after();
         const uint32_t sq = q_low + side * (kQ * D * 2 >> 4), sk = h_low + half * (Cfg::kHalf >> 4), s_t = tmem + side * 128;
         if (leader) {
-  #pragma unroll
+#pragma unroll
           for (int k = 0; k < D / 16; ++k)
             umma_ss(s_t, sq + ((k >> 2) * (kQ * 128) + (k & 3) * 32 >> 4), sk + ((k >> 2) * (kT * 128) + (k & 3) * 32 >> 4), idesc_qk, k != 0);
           tc_commit(&s_full[side]);
@@ -555,12 +557,25 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         const int side = u & 1, t = twice ? u : u >> 1, n = u >> 1;
         const int i = v_item(t), half = i % kRing;
         if (!bar_wait(&full[half], (i / kRing) & 1, abort_flag)) return false;
-        if (!bar_wait(&p_full[side], n & 1, abort_flag)) return false;
+        if (!bar_wait(&p_half[side], n & 1, abort_flag)) return false;
         tc_fence_after();
         const uint32_t sv = v_low + half * (Cfg::kHalf >> 4), o_t = tmem + 256 + side * D, p_t = tmem + side * 128;
         if (leader) {
-  #pragma unroll
-          for (int k = 0; k < kT / 16; ++k) umma_ts(o_t, p_t + (k < 4 ? k : k + 4) * 8, sv + (k * 16 * 128 >> 4), idesc_pv, (n | k) != 0);
+#pragma unroll
+          for (int i = 0; i < kT / 32; ++i) {
+            const int k = i < kT / 64 ? i : i + kT / 64;      // (a thread's first 32 columns are two steps, of each half of the tile)
+            umma_ts(o_t, p_t + (k < 4 ? k : k + 4) * 8, sv + (k * 16 * 128 >> 4), idesc_pv, (n | k) != 0);
+          }
+        }
+        __syncwarp();
+        if (!bar_wait(&p_full[side], n & 1, abort_flag)) return false;
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int i = 0; i < kT / 32; ++i) {
+            const int k = (i < kT / 64 ? i : i + kT / 64) + 2;
+            umma_ts(o_t, p_t + (k < 4 ? k : k + 4) * 8, sv + (k * 16 * 128 >> 4), idesc_pv, 1);
+          }
           if (twice || side) tc_commit(&empty[half]);
           if (u + 2 >= steps) tc_commit(&o_done[side]);
         }
@@ -752,6 +767,12 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
           pk[i] = pack_pair<E4M3>(u, v);
         }
         tmem_st8(s_t + c * 8, pk);
+        if (c == 1) {
+          tmem_st_done();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_half[side]);
+        }
       }
       const float2 sum = split64(add2(sum2[0], sum2[1]));
       l += E4M3 ? (sum.x + sum.y) * exp2f(-ev) : sum.x + sum.y;
