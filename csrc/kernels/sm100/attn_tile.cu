@@ -39,8 +39,7 @@ struct TileCfg {
   static constexpr int kHalf = kT * D * 2;                  // a half: a tile of K or of V, as 16-bit values
   static constexpr int kRing = E4M3 ? 4 : 5;                // halves that the products read
   static constexpr int kCodes = E4M3 ? kT * D : 0;          // a half as codes, as it comes
-  static constexpr int kSlots = E4M3 ? 2 : 0;               // of which there are so many under way,
-  static constexpr int kParts = E4M3 && D == 128 ? 2 : 1;   // in parts, as many rows as are converted at a time
+  static constexpr int kSlots = E4M3 ? 2 : 0;               // of which there are so many under way
   static constexpr int kScales = kSlots * 2 * kT;           // with their scale bytes, and V's beside K's
   // (all of the SM's 227 KB are in use: that the base lies on a 1024-byte boundary, as it does in practice, is checked)
   static constexpr int kSmem = kQBytes + kRing * kHalf + kSlots * kCodes + kScales + 4 * kQ * 4 + 512;
@@ -196,7 +195,7 @@ __device__ __noinline__ void tile_wide(const RowsArgs& a, int seq, int row0, int
 template <int D, bool E4M3, bool TREE>
 KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const int seqs) {
   using Cfg = TileCfg<D, E4M3>;
-  constexpr int kRing = Cfg::kRing, kSlots = Cfg::kSlots, kParts = Cfg::kParts, kCame = E4M3 ? kSlots * kParts : kRing;
+  constexpr int kRing = Cfg::kRing, kSlots = Cfg::kSlots, kCame = E4M3 ? kSlots : kRing;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
   if (smem_u32(smem) & 1023) {                                // uniform, before any barrier or allocation
@@ -211,8 +210,8 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   float* x_s = reinterpret_cast<float*>(b_s + Cfg::kScales);
   uint64_t* full = reinterpret_cast<uint64_t*>(x_s + 4 * kQ); // [ring] a half can be read by the products,
   uint64_t* empty = full + kRing;                             // [ring] has been read;
-  uint64_t* came = empty + kRing;                             // [ring; 8-bit: slots' parts] the copy has landed;
-  uint64_t* taken = came + kCame;                             // [slots' parts] the codes have been read
+  uint64_t* came = empty + kRing;                             // [ring; 8-bit: slots] the copy has landed;
+  uint64_t* taken = came + kCame;                             // [slots] the codes have been read
   uint64_t* s_full = taken + kCame;                              // per tile of rows: scores in TMEM,
   uint64_t* p_half = s_full + 2;                              // the first half of each thread's weights in TMEM,
   uint64_t* p_full = p_half + 2;                              // the others,
@@ -259,12 +258,12 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   }
   if (threadIdx.x == 32) {
     for (int s = 0; s < kRing; ++s) {
-      mbar_init(&full[s], E4M3 ? 2 : 4);
+      mbar_init(&full[s], 4);
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < kCame; ++s) {
-      mbar_init(&came[s], E4M3 && s % kParts == 0 ? 33 : 1);  // (scale bytes come with a slot's first part)
-      mbar_init(&taken[s], 2);
+      mbar_init(&came[s], E4M3 ? 33 : 1);
+      mbar_init(&taken[s], 4);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
@@ -319,8 +318,8 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     const int tid = threadIdx.x - 512, w4 = warp - 16;
     if constexpr (E4M3) {
-      // two warps to a half, so that two halves are under way; in batches of 8 rows a lane
-      constexpr int kLanes = D / 16, kRowsWarp = 32 / kLanes, kLoads = 8, kBatch = kLoads * 2 * kRowsWarp;                       // lanes to a row of codes
+      // all of a half's codes are in registers before the half that they go to is free, so its turn is short
+      constexpr int kLanes = D / 16, kRowsWarp = 32 / kLanes, kLoads = kT / (4 * kRowsWarp);     // lanes to a row of codes; rows of a lane
       const int c = lane % kLanes, sub = lane / kLanes;
       // a lane's four of a tile's scale bytes (those behind the end are 0), and the largest of all
       auto scale_word = [&](uint32_t at, int here) -> uint32_t {
@@ -333,11 +332,11 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         const uint32_t m = __vmaxu4(w, w >> 16);
         return (int)__reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u));
       };
-      for (int i = w4 >> 1; i < items && ok; i += 2) {
+      for (int i = 0; i < items && ok; ++i) {
         int which, t;
         item(i, which, t);
         const int slot = i % kSlots, half = i % kRing, tok0 = from + t * kT;
-        if (!bar_wait(&came[slot * kParts], (i / kSlots) & 1, abort_flag)) {
+        if (!bar_wait(&came[slot], (i / kSlots) & 1, abort_flag)) {
           set_error(a.err, ERR_WAIT_FULL);
           *abort_flag = 1;
           ok = false;
@@ -353,71 +352,59 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         // (a row of zeros has the byte -40 + 127)
         if (top > 0x57 + 21 && (__vcmpgtu4(word, 0x57575757u) & __vcmpltu4(word, (uint32_t)(top - 21) * 0x01010101u)) != 0) *wide_s = 1;
         uint8_t* dst = h_s + half * Cfg::kHalf;
-        bool nan = false, free = false;
-#pragma unroll 1
-        for (int r0 = (w4 & 1) * kRowsWarp + sub; r0 < kT; r0 += kBatch) {
-          static_assert(kBatch * kParts == kT, "a part is a batch");
-          const int part = r0 / kBatch;
-          if (part > 0 && !bar_wait(&came[slot * kParts + part], (i / kSlots) & 1, abort_flag)) {
-            set_error(a.err, ERR_WAIT_FULL);
-            *abort_flag = 1;
-            ok = false;
-            break;
+        bool nan = false;
+        const int r0 = w4 * kRowsWarp + sub;
+        uint32_t w[kLoads][4];
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          const int r = r0 + j * 4 * kRowsWarp;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int p = p0 + h * kApart;                    // eight codes: half of a 16-byte piece of the code row
+            const uint32_t at = src + (D == 64 ? r * 64 + (((p >> 1) ^ ((r >> 1) & 3)) << 4) : r * 128 + (((p >> 1) ^ (r & 7)) << 4)) + (p & 1) * 8;
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2 * h]), "=r"(w[j][2 * h + 1]) : "r"(at));
           }
-          uint32_t w[kLoads][4];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&taken[slot]);             // (the codes are in registers, the scale bytes too)
+        if (edge) {
 #pragma unroll
           for (int j = 0; j < kLoads; ++j) {
-            const int r = r0 + j * 2 * kRowsWarp;
+            if (r0 + j * 4 * kRowsWarp >= here) w[j][0] = w[j][1] = w[j][2] = w[j][3] = 0;      // (not brought: anything may lie there)
+            if (which) {
+              // values that are not finite stay out of the product: rows that see them get them at the end
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int p = p0 + h * kApart;                  // eight codes: half of a 16-byte piece of the code row
-              const uint32_t at = src + (D == 64 ? r * 64 + (((p >> 1) ^ ((r >> 1) & 3)) << 4) : r * 128 + (((p >> 1) ^ (r & 7)) << 4)) + (p & 1) * 8;
-              asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2 * h]), "=r"(w[j][2 * h + 1]) : "r"(at));
-            }
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&taken[slot * kParts + part]);      // (the codes are in registers, the scale bytes too)
-          if (edge) {
-#pragma unroll
-            for (int j = 0; j < kLoads; ++j) {
-              if (r0 + j * 2 * kRowsWarp >= here) w[j][0] = w[j][1] = w[j][2] = w[j][3] = 0;    // (not brought: anything may lie there)
-              if (which) {
-                // values that are not finite stay out of the product: rows that see them get them at the end
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const uint32_t m = __vcmpeq4(w[j][k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                  nan |= m != 0;
-                  w[j][k] &= ~m;
-                }
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t m = __vcmpeq4(w[j][k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                nan |= m != 0;
+                w[j][k] &= ~m;
               }
             }
           }
-          if (!free && !bar_wait(&empty[half], ((i / kRing) & 1) ^ 1, abort_flag)) {
-            set_error(a.err, ERR_WAIT_EMPTY);
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
-          free = true;
+        }
+        if (!bar_wait(&empty[half], ((i / kRing) & 1) ^ 1, abort_flag)) {
+          set_error(a.err, ERR_WAIT_EMPTY);
+          *abort_flag = 1;
+          ok = false;
+          break;
+        }
 #pragma unroll
-          for (int j = 0; j < kLoads; ++j) {
-            const int r = r0 + j * 2 * kRowsWarp;
-            const uint32_t b = __shfl_sync(0xffffffffu, word, r >> 2) >> (8 * (r & 3)) & 255u;
-            const uint32_t fj = pow2_f16(min((int)b - top, 0) + 6) * 0x10001u;
+        for (int j = 0; j < kLoads; ++j) {
+          const int r = r0 + j * 4 * kRowsWarp;
+          const uint32_t b = __shfl_sync(0xffffffffu, word, r >> 2) >> (8 * (r & 3)) & 255u;
+          const uint32_t fj = pow2_f16(min((int)b - top, 0) + 6) * 0x10001u;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t o[4];
-              codes_f16x4(w[j][2 * h], o[0], o[1]);
-              codes_f16x4(w[j][2 * h + 1], o[2], o[3]);
-              const int p = p0 + h * kApart;
-              *reinterpret_cast<uint4*>(dst + (p >> 3) * (kT * 128) + r * 128 + (((p & 7) ^ (r & 7)) << 4)) =
-                  make_uint4(mul_f16x2(o[0], fj), mul_f16x2(o[1], fj), mul_f16x2(o[2], fj), mul_f16x2(o[3], fj));
-            }
+          for (int h = 0; h < 2; ++h) {
+            uint32_t o[4];
+            codes_f16x4(w[j][2 * h], o[0], o[1]);
+            codes_f16x4(w[j][2 * h + 1], o[2], o[3]);
+            const int p = p0 + h * kApart;
+            *reinterpret_cast<uint4*>(dst + (p >> 3) * (kT * 128) + r * 128 + (((p & 7) ^ (r & 7)) << 4)) =
+                make_uint4(mul_f16x2(o[0], fj), mul_f16x2(o[1], fj), mul_f16x2(o[2], fj), mul_f16x2(o[3], fj));
           }
         }
-        if (!ok) break;
         if (nan) *bad_s = 1;
-        if (!which && (w4 & 1) == 0 && lane == 0) e_s[t & 3] = make_float2(pow2i(top - 127 - 6), (float)(vtop - 127 - 6));
+        if (!which && w4 == 0 && lane == 0) e_s[t & 3] = make_float2(pow2i(top - 127 - 6), (float)(vtop - 127 - 6));
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[half]);
@@ -492,29 +479,23 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         // boxes behind the share's end are not brought
         if constexpr (E4M3) {
           const int s_page = __shfl_sync(0xffffffffu, page, lane >> 1), s_off = __shfl_sync(0xffffffffu, off, lane >> 1) + (lane & 1) * 4;
-#pragma unroll
-          for (int p = 0; p < kParts; ++p) {
-            if (!bar_wait(&taken[slot * kParts + p], (uses & 1) ^ 1, abort_flag)) {
-              set_error(a.err, ERR_WAIT_EMPTY);
-              *abort_flag = 1;
-              ok = false;
-              break;
-            }
-            uint64_t* bar = &came[slot * kParts + p];
-            const int lo = p * (kT / kParts) / box, hi = min(boxes, (p + 1) * (kT / kParts) / box);
-            if (lane == 0) mbar_expect_tx(bar, max(hi - lo, 0) * box * D);
-            __syncwarp();
-            if (lane >= lo && lane < hi) tma_load_3d(c_s + slot * Cfg::kCodes + lane * box * D, kv_map, 0, b_row, b_page, bar);
-            if (p) continue;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              if (k && which) break;
-              const uint8_t* src = a.pool + (size_t)s_page * page_bytes + codes + (size_t)((k ? 1 : which) * a.hk + kvh) * a.page_size + s_off;
-              if (4 * lane < here && KERN_CHECK(src, 4, SITE_KV_ROW))
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(b_s + slot * 2 * kT + k * kT + 4 * lane)), "l"(src) : "memory");
-            }
-            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+          if (!bar_wait(&taken[slot], (uses & 1) ^ 1, abort_flag)) {
+            set_error(a.err, ERR_WAIT_EMPTY);
+            *abort_flag = 1;
+            ok = false;
+            break;
           }
+          if (lane == 0) mbar_expect_tx(&came[slot], boxes * box * D);
+          __syncwarp();
+          if (lane < boxes) tma_load_3d(c_s + slot * Cfg::kCodes + lane * box * D, kv_map, 0, b_row, b_page, &came[slot]);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (k && which) break;
+            const uint8_t* src = a.pool + (size_t)s_page * page_bytes + codes + (size_t)((k ? 1 : which) * a.hk + kvh) * a.page_size + s_off;
+            if (4 * lane < here && KERN_CHECK(src, 4, SITE_KV_ROW))
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(b_s + slot * 2 * kT + k * kT + 4 * lane)), "l"(src) : "memory");
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&came[slot])) : "memory");
         } else {
           if (!bar_wait(&empty[slot], (uses & 1) ^ 1, abort_flag)) {
             set_error(a.err, ERR_WAIT_EMPTY);
