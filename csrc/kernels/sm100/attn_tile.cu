@@ -22,7 +22,7 @@
 // scale and shift, exponential, sum, pack. No pass over O but then.
 //
 // 8-bit: a tile's rows are brought to one exponent, E = the largest of its scale bytes, as they become f16 (exact for scales down to
-// 2^-21 of the largest); 2^E of the keys is then part of the scores' scale, E of the values part of the weights' exponent,
+// 2^-20 of the largest); 2^E of the keys is then part of the scores' scale, E of the values part of the weights' exponent,
 // w_ij = 2^(s_ij + E_t - R_i): no work per score. A block that meets a tile with scales further apart (rows that hold nothing but
 // zeros and values under 2^-31 aside) is computed again, a row to a warp, each key and value row with its own scale (tile_wide).
 #include "attn_rows.cuh"
@@ -121,8 +121,6 @@ KERN_DEVICE uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// 2^x as f16, 0 below its range
-KERN_DEVICE uint32_t pow2_f16(int x) { return x >= -14 ? (uint32_t)(x + 15) << 10 : (x >= -24 ? 1u << (x + 24) : 0u); }
 
 // A block's rows over the 8-bit cache, a row to a warp in turn and one token at a time, for scales that have no common exponent.
 template <int D, bool TREE>
@@ -350,27 +348,27 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         const uint32_t word = scale_word(by, here);
         const int top = top_byte(word), vtop = which ? 0 : top_byte(scale_word(by + kT, here));
         // (a row of zeros has the byte -40 + 127)
-        if (top > 0x57 + 21 && (__vcmpgtu4(word, 0x57575757u) & __vcmpltu4(word, (uint32_t)(top - 21) * 0x01010101u)) != 0) *wide_s = 1;
+        if (top > 0x57 + 20 && (__vcmpgtu4(word, 0x57575757u) & __vcmpltu4(word, (uint32_t)(top - 20) * 0x01010101u)) != 0) *wide_s = 1;
         uint8_t* dst = h_s + half * Cfg::kHalf;
         bool nan = false;
+        // rows r0 + j * kStep: all in the same place of the swizzle and of their words of scale bytes
+        constexpr int kStep = 4 * kRowsWarp;
         const int r0 = w4 * kRowsWarp + sub;
         uint32_t w[kLoads][4];
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-          const int r = r0 + j * 4 * kRowsWarp;
+        for (int h = 0; h < 2; ++h) {
+          const int p = p0 + h * kApart;                      // eight codes: half of a 16-byte piece of the code row
+          const uint32_t at = src + r0 * D + (((p >> 1) ^ (D == 64 ? (r0 >> 1) & 3 : r0 & 7)) << 4) + (p & 1) * 8;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int p = p0 + h * kApart;                    // eight codes: half of a 16-byte piece of the code row
-            const uint32_t at = src + (D == 64 ? r * 64 + (((p >> 1) ^ ((r >> 1) & 3)) << 4) : r * 128 + (((p >> 1) ^ (r & 7)) << 4)) + (p & 1) * 8;
-            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2 * h]), "=r"(w[j][2 * h + 1]) : "r"(at));
-          }
+          for (int j = 0; j < kLoads; ++j)
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2 * h]), "=r"(w[j][2 * h + 1]) : "r"(at + j * kStep * D));
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&taken[slot]);             // (the codes are in registers, the scale bytes too)
         if (edge) {
 #pragma unroll
           for (int j = 0; j < kLoads; ++j) {
-            if (r0 + j * 4 * kRowsWarp >= here) w[j][0] = w[j][1] = w[j][2] = w[j][3] = 0;      // (not brought: anything may lie there)
+            if (r0 + j * kStep >= here) w[j][0] = w[j][1] = w[j][2] = w[j][3] = 0;      // (not brought: anything may lie there)
             if (which) {
               // values that are not finite stay out of the product: rows that see them get them at the end
 #pragma unroll
@@ -388,18 +386,19 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
           ok = false;
           break;
         }
+        uint8_t* to0 = dst + (p0 >> 3) * (kT * 128) + r0 * 128 + (((p0 & 7) ^ (r0 & 7)) << 4);
+        uint8_t* to1 = dst + ((p0 + kApart) >> 3) * (kT * 128) + r0 * 128 + ((((p0 + kApart) & 7) ^ (r0 & 7)) << 4);
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
-          const int r = r0 + j * 4 * kRowsWarp;
-          const uint32_t b = __shfl_sync(0xffffffffu, word, r >> 2) >> (8 * (r & 3)) & 255u;
-          const uint32_t fj = pow2_f16(min((int)b - top, 0) + 6) * 0x10001u;
+          // 2^(e - E + 6) twice over, as f16: 1 to 21 in the exponent's bits (0: a row of zeros, or one computed again)
+          const uint32_t b = __shfl_sync(0xffffffffu, word, (r0 + j * kStep) >> 2) >> (8 * (r0 & 3)) & 255u;
+          const uint32_t fj = (uint32_t)max((int)b + 21 - top, 0) * 0x04000400u;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t o[4];
             codes_f16x4(w[j][2 * h], o[0], o[1]);
             codes_f16x4(w[j][2 * h + 1], o[2], o[3]);
-            const int p = p0 + h * kApart;
-            *reinterpret_cast<uint4*>(dst + (p >> 3) * (kT * 128) + r * 128 + (((p & 7) ^ (r & 7)) << 4)) =
+            *reinterpret_cast<uint4*>((h ? to1 : to0) + j * kStep * 128) =
                 make_uint4(mul_f16x2(o[0], fj), mul_f16x2(o[1], fj), mul_f16x2(o[2], fj), mul_f16x2(o[3], fj));
           }
         }
