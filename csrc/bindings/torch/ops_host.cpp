@@ -238,12 +238,18 @@ RowsForm rows_form(int64_t d, bool e4m3, int64_t nt) {
   const int64_t stages = stage >= 65536 ? 3 : (per_sm == 1 ? 196608 : 98304) / stage;
   return {(unsigned)(1024 + stages * (stage + (e4m3 ? 2 * tile : 0)) + (d == 256 && nt > 1 ? nt * d * 16 : 0) + 256), per_sm};
 }
-// Shares that a row's context is cut into, and CTAs of a cluster: as many as fill the SMs once, two where the rows alone fill them up
-// to four times (a share's end then leaves less of the last wave idle), none of under 128 tokens. Up to 8 shares are one cluster;
-// more are on their own, and joined by a second launch.
+// Shares that a row's context is cut into, and CTAs of a cluster: as many as fill the SMs once, none of under 128 tokens, and one where
+// the rows alone fill them, the longest first then. Up to 8 shares are one cluster; more are on their own, and joined by a second
+// launch. Microseconds of decode, 8 kv heads, head_dim 128, by shares (* the rule's):
+//   sequences of tokens    1      2      4      8     16     32          sequences of tokens (ragged: up to)    1       2       4
+//     1 of 1000          10.6    9.8    8.6    7.8*                       64 of 4000                            90.9*  101.6   114.6
+//     1 of 30000          192    100   54.1   31.5   20.1   19.0*         64 of up to 4000                      48.3*   60.2    81.5
+//     4 of 4000          30.1   18.8   12.9   13.1*  15.5                 48 of up to 4000                      41.0*   54.9    66.0
+//    16 of 4000          32.7   29.5*  34.8   47.1   45.0                 48 of 4000                            86.8*   79.0    89.7
+//     2 of 100000         631    324    166    116   71.7*  77.4          128 of up to 8000                    167.9*  183.5   225.3
 std::pair<int64_t, int64_t> rows_shares(int64_t ctas, int64_t max_len, int64_t resident) {
   const int64_t most = std::max<int64_t>(1, (max_len + 127) / 128);
-  const int64_t want = std::min<int64_t>({most, ctas < resident ? resident / ctas : ctas < 4 * resident ? 2 : 1, 256});
+  const int64_t want = std::min<int64_t>({most, std::max<int64_t>(1, resident / ctas), 256});
   if (want > 8) return {want, 1};
   const int64_t cluster = want >= 8 ? 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
   return {cluster, cluster};
@@ -253,6 +259,13 @@ std::pair<int64_t, int64_t> rows_shares(int64_t ctas, int64_t max_len, int64_t r
 unsigned tile_shared(int64_t d, bool e4m3) {
   return (unsigned)(2 * 128 * d * 2 + (e4m3 ? 4 : 5) * 128 * d * 2 + (e4m3 ? 2 * (128 * d + 256) : 0) + 4 * 128 * 4 + 512);
 }
+// Shares of the many-row kernel: as many as fill the SMs once. Microseconds, 64 rows of 4 heads each, by shares (* the rule's):
+//   sequences of tokens    1      2      4      8     16     32
+//     1 of 8000           134   78.6   48.3   33.9   28.3*  43.8
+//     4 of 4000          76.2   56.9   42.2*  56.5   86.0
+//     9 of 4000          77.4   69.2*  82.7    112
+//    16 of 4000          79.1*   127    154
+// (a CTA takes the SM's whole memory, so a second wave begins with copies that nothing hides)
 int64_t tile_shares(int64_t ctas, int64_t max_len, int64_t sms) {
   return std::max<int64_t>(1, std::min<int64_t>({sms / ctas, (max_len + 255) / 256, 64}));
 }
@@ -339,6 +352,7 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
       const int64_t blocks = (most + toks - 1) / toks;
       const RowsForm f = rows_form(d, e4m3, nt);
       std::tie(shares, cluster) = rows_shares(hk * blocks * seqs, max_len, (int64_t)h.sms * f.per_sm);
+      if (shares == 1 && hi < INT32_MAX && max_len > 128) shares = cluster = 2;    // (sequences of more rows leave at once: fewer CTAs work)
       gx = hk * blocks;
       gy = seqs;
       shared = f.shared;
@@ -367,8 +381,8 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
   const int64_t all = INT32_MAX, few = std::max<int64_t>(1, 8 / g);
   if (g * max_rows <= kFewRows || d > 128) {
     run(false, 1, all);
-  } else if (!cu_q || seqs == 1 || rows + few >= seqs * max_rows) {
-    run(true, 1, all);                                       // (rows alike)
+  } else if (masks || !cu_q || seqs == 1 || rows + few >= seqs * max_rows) {
+    run(true, 1, all);                                       // (rows alike; trees of a node or two among the others end before those)
   } else {
     // sequences of single tokens among prompt chunks keep the few-row kernel, which cuts their contexts into shares
     run(true, few + 1, all);

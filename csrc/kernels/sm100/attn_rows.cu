@@ -144,7 +144,8 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.hq / a.hk;
-  const int seq = blockIdx.y, blk = blockIdx.x / a.hk, kvh = blockIdx.x % a.hk;
+  const int blk = blockIdx.x / a.hk, kvh = blockIdx.x % a.hk;
+  int seq = blockIdx.y;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -155,8 +156,17 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
     mbar_fence_init();
     tma_prefetch_desc(kv_map);
   }
-  __syncthreads();
   pdl_wait();
+  if (gridDim.z == 1 && gridDim.y <= kThreads && gridDim.x * gridDim.y > sm_count() * Cfg::kPerSm) {
+    // more blocks than run at once: block y takes the sequence of rank y by length, so that the last to start are the shortest
+    volatile int* found = abort_flag + 1;
+    if (by_length(a.seq_lens, gridDim.y, reinterpret_cast<int*>(stages)) == seq) *found = threadIdx.x;
+    fence_proxy_async();                                      // (copies come to the same place)
+    __syncthreads();
+    seq = *found;
+  } else {
+    __syncthreads();
+  }
 
   const int L = max(a.seq_lens[seq], 0);
   const int row0 = a.cu_q ? a.cu_q[seq] : seq * a.rows_per_seq;

@@ -68,4 +68,23 @@ KERN_DEVICE float pow2i(int e) { return __uint_as_float((uint32_t)(min(max(e, -1
 KERN_DEVICE int rows_shares(int end, int splits) { return min(splits, max(1, (end + 127) / 128)); }
 KERN_DEVICE int rows_share_len(int end, int shares) { return ((end + 127) / 128 + shares - 1) / shares * 128; }
 
+KERN_DEVICE unsigned sm_count() {
+  unsigned n;
+  asm("mov.u32 %0, %%nsmid;" : "=r"(n));
+  return n;
+}
+// Of n <= 256 sequences (and a thread to each): the rank of this thread's by length, the longest first; -1 in further threads. Every
+// thread of the block calls; keys: 256 places in shared memory.
+KERN_DEVICE int by_length(const int* seq_lens, int n, int* keys) {
+  const int t = threadIdx.x, own = t < n ? min(max(seq_lens[t], 0), 0x7fffff) << 8 | (255 - t) : -1;
+  if (t < 256) keys[t] = own;
+  __syncthreads();
+  int before = 0;
+  for (int i = 0; i < n; i += 4) {
+    const int4 k = *reinterpret_cast<const int4*>(keys + i);
+    before += (k.x > own) + (k.y > own) + (k.z > own) + (k.w > own);
+  }
+  return t < n ? before : -1;
+}
+
 }  // namespace kern

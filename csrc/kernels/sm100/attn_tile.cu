@@ -225,11 +225,19 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (uniform registers for what follows from it)
   const int G = a.hq / a.hk, kvh = blockIdx.x, toks = 2 * kQ / G;
   pdl_wait();
+  // more blocks than run at once: the sequences are taken by length, so that the last blocks to start are the shortest
+  const bool ranked = seqs > 1 && seqs <= 256 && gridDim.z == 1 && gridDim.x * gridDim.y > sm_count();
+  int* order = reinterpret_cast<int*>(q_s) + 256;
+  if (ranked) {
+    const int rank = by_length(a.seq_lens, seqs, reinterpret_cast<int*>(q_s));
+    if (rank >= 0) order[rank] = threadIdx.x;
+    __syncthreads();
+  }
   if (warp == 0) {
     // block y of the call: blocks are counted through the sequences
     int base = 0, sq = -1, bk = 0;
     for (int s0 = 0; s0 < seqs && sq < 0; s0 += 32) {
-      const int s = s0 + lane;
+      const int s = ranked && s0 + lane < seqs ? order[s0 + lane] : s0 + lane;
       int rows = 0;
       if (s < seqs) rows = a.cu_q ? a.cu_q[s + 1] - a.cu_q[s] : a.rows_per_seq;
       int n = rows > 0 && rows >= a.row_lo && rows <= a.row_hi ? (rows + toks - 1) / toks : 0;
@@ -242,7 +250,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       const unsigned hit = __ballot_sync(0xffffffffu, (int)blockIdx.y < base + n);
       if (hit) {
         const int l = __ffs(hit) - 1;
-        sq = s0 + l;
+        sq = __shfl_sync(0xffffffffu, s, l);
         const int upto = __shfl_sync(0xffffffffu, n, l), mine = __shfl_sync(0xffffffffu, own, l);
         bk = (int)blockIdx.y - (base + upto - mine);
         if (!TREE) bk = mine - 1 - bk;                        // causal: the longest walks first

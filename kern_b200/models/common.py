@@ -657,8 +657,8 @@ def _e4m3_few(hq: int, hk: int, d: int, page_size: int, table_width: int, q_stri
     blocks = -(-rows // (8 * nt // g))
     smem, per_sm = _ops_host.rows_form(d, True, nt)
     per, out, lo = hk * blocks, [], 1
-    # as the call-by-call rule (ops_host.cpp, rows_shares): shares that fill the SMs once, two while the rows alone fill them up to four times
-    for cluster, most in ((8, sms * per_sm // 8), (4, sms * per_sm // 4), (2, 4 * sms * per_sm - 1), (1, None)):
+    # as the call-by-call rule (ops_host.cpp, rows_shares): shares that fill the SMs once; two at least where sequences of more rows leave at once
+    for cluster, most in ((8, sms * per_sm // 8), (4, sms * per_sm // 4), (2, sms * per_sm // 2 if hi == I32_MAX else None), (1, None)):
         top = seqs_max if most is None else min(seqs_max, most // per)
         if top < lo:
             continue
@@ -670,6 +670,8 @@ def _e4m3_few(hq: int, hk: int, d: int, page_size: int, table_width: int, q_stri
         out.append(_e4m3_attend(f"kern_attn_rows_e4m3_causal_d{d}_n{nt}", [per, "seqs", cluster], 160, smem, cluster, hq, hk, d, page_size, table_width,
                                 q_stride, {"i32": cluster}, 1, hi, cu, err, when if len(when) > 1 else None))
         lo = top + 1
+        if most is None:
+            break
     return out
 
 
