@@ -86,8 +86,10 @@ constexpr int kAppendThreads = 128;
 
 // One block per token: its rows (q heads, then k and v heads) are dealt to groups of D / 8 lanes, a pass of all groups at a time, the
 // next pass's loads ahead; the cosines and sines that a lane needs are the same for every head and stay in registers. What bounds it
-// is the number of instructions, not the bytes: the form of the pairs and the norms are fixed when it is compiled, pairs of values
-// go through two-wide products, and k rows alone pay for exact codes.
+// is how many loads are under way and the number of instructions, not the bytes: 8 blocks to an SM at 64 registers (8192 tokens of
+// 32 + 8 heads of 128, written and read back: 53 us; 6 blocks at 80 registers 58, 9 at 56 55; 256 threads to a token 71). The form of
+// the pairs and the norms are fixed when it is compiled, pairs of values go through two-wide products, and k rows alone pay for
+// exact codes.
 template <int D, bool INTER, bool NORM>
 KERN_DEVICE void append_body(const AppendArgs& a) {
   constexpr int kLanes = D / 8, kGroups = kAppendThreads / kLanes;
@@ -345,7 +347,7 @@ KERN_DEVICE void read_body(const uint8_t* pool, const long long* slots, __nv_bfl
 }  // namespace kern
 
 #define KERN_APPEND_ENTRY(D, PAIRS, INTER, NAME, NORM)                                                                            \
-  extern "C" __global__ void __launch_bounds__(kAppendThreads, 6) kern_rope_kv_append_e4m3_##PAIRS##NAME##_d##D(                  \
+  extern "C" __global__ void __launch_bounds__(kAppendThreads, 8) kern_rope_kv_append_e4m3_##PAIRS##NAME##_d##D(                  \
       const __nv_bfloat16* qkv, __nv_bfloat16* q_out, uint8_t* pool, const long long* positions, const long long* slots,          \
       const float* cos_tab, const float* sin_tab, const __nv_bfloat16* q_norm, const __nv_bfloat16* k_norm, int hq, int hk,       \
       int rot, int page_size, float eps, int norm_plus_one, long long kv_slots, int max_pos, int row_stride, int q_stride,        \
