@@ -333,6 +333,7 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
   const int64_t g = hq / hk;
   const auto map = pool_map(h, pool, e4m3, pages, hk, d, page);
   const std::string form = std::string(e4m3 ? "_e4m3" : "_bf16") + (masks ? "_tree_d" : "_causal_d") + n(d);
+  const int64_t all = INT32_MAX, few = std::max<int64_t>(1, 8 / g);
   // one kernel over the sequences of lo .. hi rows
   auto run = [&](bool tiled, int64_t lo, int64_t hi) {
     const int64_t most = std::min(max_rows, hi);
@@ -352,7 +353,8 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
       const int64_t blocks = (most + toks - 1) / toks;
       const RowsForm f = rows_form(d, e4m3, nt);
       std::tie(shares, cluster) = rows_shares(hk * blocks * seqs, max_len, (int64_t)h.sms * f.per_sm);
-      if (shares == 1 && hi < INT32_MAX && max_len > 128) shares = cluster = 2;    // (sequences of more rows leave at once: fewer CTAs work)
+      // among sequences of more rows, whose CTAs leave at once: two shares at least, and no second launch for what may be none
+      if (hi < all && max_len > 128) shares = cluster = std::min<int64_t>(std::max<int64_t>(shares, 2), 8);
       gx = hk * blocks;
       gy = seqs;
       shared = f.shared;
@@ -371,14 +373,13 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
     b.bytes(map.data(), map.size()).at(q).at(out).put(ws_o).put(ws_ml).at(pool).at(table).at(lens).at(cu_q).at(masks);
     b.ints(masks ? masks->size(1) : 0, rows_per_seq, hq, hk, q_step, out_step, width, page, tiled ? seqs : cluster, pages, lo, hi);
     b.put((float)(scale * kLog2e)).put(h.err);
-    launch(h, tiled ? "attn_tile" : "attn_rows", name, gx, gy, shares, tiled ? 768 : 160, b, shared, false, (unsigned)cluster);
+    launch(h, tiled ? "attn_tile" : "attn_rows", name, gx, gy, shares, tiled ? 768 : 160, b, shared, !tiled && hi < all, (unsigned)cluster);
     if (groups > 1) {
       Block m;
       m.put(ws_o).put(ws_ml).at(out).at(lens).at(cu_q).ints(rows_per_seq, hq, toks, shares, cluster, out_step, lo, hi);
       launch(h, "attn_rows", std::string("kern_attn_rows_merge_") + (masks ? "tree_d" : "causal_d") + n(d), most * hq, seqs, 1, 128, m, 0, true);
     }
   };
-  const int64_t all = INT32_MAX, few = std::max<int64_t>(1, 8 / g);
   if (g * max_rows <= kFewRows || d > 128) {
     run(false, 1, all);
   } else if (masks || !cu_q || seqs == 1 || rows + few >= seqs * max_rows) {
