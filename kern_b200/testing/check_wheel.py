@@ -104,6 +104,8 @@ def check(wheel: str | Path) -> list[str]:
         native = [n for n in names if n.startswith("kern_b200/_native") and n.endswith(".so")]
         if not native:
             errs.append("the native module kern_b200/_native*.so is missing")
+        if not any(n.startswith("kern_b200/_ops_host") and n.endswith(".so") for n in names):
+            errs.append("the native module kern_b200/_ops_host*.so is missing")
         for n in ("kern_b200/bin/kern", "kern_b200/bin/kern-run", "kern_b200/libattn_decode_noalloc.so", "kern_b200/libkern_capture.so"):
             if n not in names:
                 errs.append(f"{n} is missing")
