@@ -371,12 +371,12 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
     }
     Block b;
     b.bytes(map.data(), map.size()).at(q).at(out).put(ws_o).put(ws_ml).at(pool).at(table).at(lens).at(cu_q).at(masks);
-    b.ints(masks ? masks->size(1) : 0, rows_per_seq, hq, hk, q_step, out_step, width, page, tiled ? seqs : cluster, pages, lo, hi);
+    b.ints(masks ? masks->size(1) : 0, rows_per_seq, hq, hk, q_step, out_step, width, page, tiled ? seqs : cluster, pages, lo, hi, rows);
     b.put((float)(scale * kLog2e)).put(h.err);
     launch(h, tiled ? "attn_tile" : "attn_rows", name, gx, gy, shares, tiled ? 768 : 160, b, shared, !tiled && hi < all, (unsigned)cluster);
     if (groups > 1) {
       Block m;
-      m.put(ws_o).put(ws_ml).at(out).at(lens).at(cu_q).ints(rows_per_seq, hq, toks, shares, cluster, out_step, lo, hi);
+      m.put(ws_o).put(ws_ml).at(out).at(lens).at(cu_q).ints(rows_per_seq, hq, toks, shares, cluster, out_step, lo, hi, rows);
       launch(h, "attn_rows", std::string("kern_attn_rows_merge_") + (masks ? "tree_d" : "causal_d") + n(d), most * hq, seqs, 1, 128, m, 0, true);
     }
   };

@@ -178,6 +178,10 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
   const int toks = kRows / G;
   const int tok_lo = blk * toks;
   if (tok_lo >= R || R < a.row_lo || R > a.row_hi) return;   // uniform over the cluster
+  if (!rows_lie(row0, R, a.rows)) {
+    if (threadIdx.x == 0) set_error(a.err, ERR_BOUNDS);
+    return;
+  }
   const int valid = min(toks, R - tok_lo) * G;
   const int past = L - R;                                    // what the sequence had before this call's rows
   // causal: the last row of the block decides how far the walk goes
@@ -718,20 +722,20 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
 constexpr int kMergeThreads = 128;
 template <int D, bool TREE>
 KERN_DEVICE void rows_merge(const float* ws_o, const float* ws_ml, __nv_bfloat16* out, const int* seq_lens, const int* cu_q, int rows_per_seq,
-                            int hq, int toks, int splits, int cluster, int out_stride, int row_lo, int row_hi) {
+                            int hq, int toks, int splits, int cluster, int out_stride, int row_lo, int row_hi, int rows) {
   constexpr int N = D / 32;
   __shared__ float y_s[4][D], l_s[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.y;
   const int row0 = cu_q ? cu_q[seq] : seq * rows_per_seq, R = cu_q ? cu_q[seq + 1] - row0 : rows_per_seq;
   const int tok = blockIdx.x / hq, head = blockIdx.x % hq;
-  if (tok >= R || R < row_lo || R > row_hi) return;
   const int L = max(seq_lens[seq], 0), lo = tok / toks * toks;
   const int end = TREE ? L : max(0, L - R + lo + min(toks, R - lo));
   const int shares = rows_shares(end, splits);
-  if (shares <= cluster) return;                              // written by its one cluster
   const int groups = splits / cluster, live = (shares + cluster - 1) / cluster;
   const size_t base = ((size_t)(row0 + tok) * hq + head) * groups;
-  pdl_wait();
+  pdl_wait();                                                 // (in every block: what follows this launch follows the one before it too)
+  if (tok >= R || R < row_lo || R > row_hi || !rows_lie(row0, R, rows)) return;
+  if (shares <= cluster) return;                              // written by its one cluster
   // every warp: the largest reference of all groups
   float m = kUnset;
   for (int s = lane; s < live; s += 32) m = fmaxf(m, ws_ml[(base + s) * 2]);
@@ -770,16 +774,16 @@ using namespace kern;
           const __grid_constant__ CUtensorMap kv_map, const __nv_bfloat16* q, __nv_bfloat16* out, float* ws_o, float* ws_ml,      \
           const uint8_t* pool, const int* block_table, const int* seq_lens, const int* cu_q, const long long* masks, int words,   \
           int rows_per_seq, int hq, int hk, int q_stride, int out_stride, int max_pages, int page_size, int cluster,              \
-          int pool_pages, int row_lo, int row_hi, float scale_log2, int* err) {                                                                           \
+          int pool_pages, int row_lo, int row_hi, int rows, float scale_log2, int* err) {                                                                           \
     rows_body<D, E4M3, TREE, NT>(&kv_map, RowsArgs{q, out, ws_o, ws_ml, pool, block_table, seq_lens, cu_q, masks, err, words,     \
                                                    rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, cluster,     \
-                                                   pool_pages, row_lo, row_hi, scale_log2});                                                      \
+                                                   pool_pages, row_lo, row_hi, rows, scale_log2});                                                      \
   }
 #define KERN_ROWS_MERGE(D, FORM, TREE)                                                                                            \
   extern "C" __global__ void __launch_bounds__(kMergeThreads) kern_attn_rows_merge_##FORM##_d##D(                                           \
       const float* ws_o, const float* ws_ml, __nv_bfloat16* out, const int* seq_lens, const int* cu_q, int rows_per_seq, int hq,  \
-      int toks, int splits, int cluster, int out_stride, int row_lo, int row_hi) {                                                \
-    rows_merge<D, TREE>(ws_o, ws_ml, out, seq_lens, cu_q, rows_per_seq, hq, toks, splits, cluster, out_stride, row_lo, row_hi);   \
+      int toks, int splits, int cluster, int out_stride, int row_lo, int row_hi, int rows) {                                                \
+    rows_merge<D, TREE>(ws_o, ws_ml, out, seq_lens, cu_q, rows_per_seq, hq, toks, splits, cluster, out_stride, row_lo, row_hi, rows);   \
   }
 #define KERN_ROWS_FORMS(D, NT)                      \
   KERN_ROWS_ENTRY(D, e4m3, true, causal, false, NT) \

@@ -23,6 +23,7 @@ struct RowsArgs {
   int* err;
   int words, rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, cluster, pool_pages;
   int row_lo, row_hi;        // sequences of other row counts are another launch's
+  int rows;                  // of q and out: a sequence's have to lie in them
   float scale_log2;
 };
 
@@ -60,6 +61,9 @@ KERN_DEVICE uint32_t not_finite(uint32_t w) {
   if ((w & (lo << 16)) == (lo << 16)) r |= 0xffff0000u;
   return r;
 }
+
+// whether R rows from row0 on are rows of the call
+KERN_DEVICE bool rows_lie(int row0, int R, int rows) { return row0 >= 0 && R >= 0 && R <= rows - row0; }
 
 KERN_DEVICE float pow2i(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 

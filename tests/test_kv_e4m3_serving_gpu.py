@@ -246,3 +246,125 @@ def test_a_batch_that_is_padded(cuda):
             n = 130 - (cu[2] - 1 - i)
             ref, spread = attend64(q[i:i + 1].cpu().view(1, hq, d), kv[1][:, :n], torch.ones(1, n, dtype=torch.bool), d ** -0.5)
             close(out[i:i + 1].view(1, hq, d), ref, spread, WEIGHT["e4m3"])
+
+
+@pytest.mark.parametrize("hq,hk,d,page", [(12, 4, 128, 192), (16, 1, 64, 320), (10, 2, 128, 64), (3, 3, 256, 192), (24, 2, 64, 8)])
+def test_mixed_calls_of_odd_groups_and_pages(cuda, hq, hk, d, page):
+    """Single tokens, short blocks and chunks together, one longer than its context; groups of 3, 16, 5, 1 and 12, pages of 192 and 320."""
+    g = torch.Generator().manual_seed(hq)
+    rows, lens = [1, 90, 1, 7, 300, 0, 2], [900, 90, 0, 400, 260, 5, 129]
+    pool, table, kv = fill_cache("e4m3", lens, hk, d, page, g)
+    cu = [0]
+    for r in rows:
+        cu.append(cu[-1] + r)
+    q = torch.randn(cu[-1], hq * d, generator=g).bfloat16().cuda()
+    out = K8.paged_attention_e4m3(q, pool, table, i32(lens), hq, hk, d, page, cu_q=i32(cu), max_rows=300)
+    for s, l in enumerate(lens):
+        r = rows[s]
+        seen = torch.arange(l)[None] <= (l - r + torch.arange(r))[:, None]
+        ref, spread = attend64(q[cu[s]:cu[s + 1]].cpu().view(r, hq, d), kv[s], seen, d ** -0.5)
+        close(out[cu[s]:cu[s + 1]].view(r, hq, d), ref, spread, WEIGHT["e4m3"])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_the_largest_trees(cuda, kind):
+    """256 nodes, 4 words; more trees than run at once, of very different lengths."""
+    hq, hk, d, page = 16, 8, 64, 16
+    g = torch.Generator().manual_seed(4)
+    rows = [256, 3, 255, 1] + [40] * 36
+    past = [33, 2000, 0, 700] + torch.randint(0, 600, (36,), generator=g).tolist()
+    lens = [r + p for r, p in zip(rows, past)]
+    pool, table, kv = fill_cache(kind, lens, hk, d, page, g)
+    cu = [0]
+    for r in rows:
+        cu.append(cu[-1] + r)
+    bits = torch.rand(cu[-1], 256, generator=g) < 0.2
+    q = torch.randn(cu[-1], hq * d, generator=g).bfloat16().cuda()
+    out = TR.tree_attention(q, pool, table, i32(lens), bits_of(bits).cuda(), i32(cu), hq, hk, d, page, max_rows=256)
+    for s in range(0, len(rows), 3):
+        r, l = rows[s], lens[s]
+        seen = torch.ones(r, l, dtype=torch.bool)
+        seen[:, l - r:] = bits[cu[s]:cu[s + 1], :r]
+        ref, spread = attend64(q[cu[s]:cu[s + 1]].cpu().view(r, hq, d), kv[s], seen, d ** -0.5)
+        close(out[cu[s]:cu[s + 1]].view(r, hq, d), ref, spread, WEIGHT[kind])
+
+
+@pytest.mark.parametrize("seqs", [90, 200])
+def test_more_single_tokens_than_run_at_once(cuda, seqs):
+    hq, hk, d, page = 16, 8, 64, 16
+    g = torch.Generator().manual_seed(seqs)
+    lens = torch.randint(0, 400, (seqs,), generator=g).tolist()
+    pool, table, kv = fill_cache("e4m3", lens, hk, d, page, g)
+    q = torch.randn(seqs, hq * d, generator=g).bfloat16().cuda()
+    out = K8.paged_attention_e4m3(q, pool, table, i32(lens), hq, hk, d, page).view(seqs, 1, hq, d)
+    for s, l in enumerate(lens):
+        ref, spread = attend64(q[s:s + 1].cpu().view(1, hq, d), kv[s], torch.ones(1, l, dtype=torch.bool), d ** -0.5)
+        close(out[s], ref, spread, WEIGHT["e4m3"])
+
+
+def test_a_wide_table_and_short_contexts(cuda):
+    """Contexts far shorter than the table says they may be: shares that nobody has, and a joining launch with nothing to join."""
+    hq, hk, d, page = 8, 2, 128, 64
+    g = torch.Generator().manual_seed(0)
+    lens = [70, 1]
+    pool, table, kv = fill_cache("e4m3", lens, hk, d, page, g)
+    table = torch.cat([table, torch.zeros(2, 2000, dtype=torch.int32, device=cuda)], 1).contiguous()
+    for rows in (1, 60):
+        q = torch.randn(2 * rows, hq * d, generator=g).bfloat16().cuda()
+        out = K8.paged_attention_e4m3(q, pool, table, i32(lens), hq, hk, d, page, rows_per_seq=rows)
+        twice = out + 0                                    # (follows both launches)
+        assert torch.equal(twice, out)
+        for s, l in enumerate(lens):
+            seen = torch.arange(l)[None] <= (l - rows + torch.arange(rows))[:, None]
+            ref, spread = attend64(q[s * rows:(s + 1) * rows].cpu().view(rows, hq, d), kv[s], seen, d ** -0.5)
+            close(twice[s * rows:(s + 1) * rows].view(rows, hq, d), ref, spread, WEIGHT["e4m3"])
+
+
+def test_calls_of_nothing(cuda):
+    hq, hk, d, page = 8, 2, 64, 16
+    pool = K8.new_pool(2, hk, page, d, cuda)
+    none, some = torch.zeros(0, dtype=torch.int64, device=cuda), torch.zeros(0, hq * d, dtype=torch.bfloat16, device=cuda)
+    tab = torch.zeros(4, d // 2, device=cuda)
+    assert K8.rope_kv_append_e4m3(torch.zeros(0, (hq + 2 * hk) * d, dtype=torch.bfloat16, device=cuda), pool, none, none, tab, tab, hq, hk, d, page).shape == (0, hq * d)
+    assert K8.read_rows_e4m3(pool, none, hk, d, page).shape == (0, 2, hk, d)
+    table = torch.zeros(0, 1, dtype=torch.int32, device=cuda)
+    assert K8.paged_attention_e4m3(some, pool, table, i32([]), hq, hk, d, page).shape == (0, hq * d)
+    assert TR.tree_attention(some, pool, torch.zeros(1, 1, dtype=torch.int32, device=cuda), i32([3]), torch.zeros(0, 1, dtype=torch.int64, device=cuda),
+                             i32([0, 0]), hq, hk, d, page).shape == (0, hq * d)
+    for t, base in ((table, none), (torch.zeros(1, 1, dtype=torch.int32, device=cuda), none.new_zeros(1))):
+        n = t.shape[0]
+        cu = torch.zeros(n + 1, dtype=torch.int32, device=cuda)
+        pos, slots, lens, masks = TR.tree_rows(i32([]), cu, base, t, page)
+        assert pos.numel() == slots.numel() == masks.numel() == 0 and lens.tolist() == [0] * n
+        count, path, emitted = TR.tree_keep(none, i32([]), none, cu, base, t, [pool], hk, d, page)
+        assert count.tolist() == [0] * n and path.numel() == emitted.numel() == 0
+
+
+def test_rows_and_parents_that_do_not_exist(cuda):
+    hq, hk, d, page = 8, 2, 64, 16
+    g = torch.Generator().manual_seed(0)
+    pool, table, _ = fill_cache("e4m3", [40], hk, d, page, g)
+    err = Kernels.get(cuda)
+
+    def failed(f):
+        out = f()
+        with pytest.raises(RuntimeError, match="device error"):
+            err.check_error()
+        return out
+    masks = torch.ones(60, 1, dtype=torch.int64, device=cuda)
+    for rows, cu in ((2, [0, 3]), (2, [-1, 1]), (2, [2, 1]), (60, [0, 61]), (60, [-1, 59])):
+        q = torch.randn(rows, hq * d, generator=g).bfloat16().cuda()
+        out = torch.full_like(q, 3.0)
+        if cu[1] >= cu[0]:                                 # (a sequence of less than no rows has none)
+            failed(lambda: K8.paged_attention_e4m3(q, pool, table, i32([40]), hq, hk, d, page, cu_q=i32(cu), out=out))
+            failed(lambda: TR.tree_attention(q, pool, table, i32([40]), masks, i32(cu), hq, hk, d, page, out=out))
+        else:
+            K8.paged_attention_e4m3(q, pool, table, i32([40]), hq, hk, d, page, cu_q=i32(cu), out=out)
+        assert bool((out == 3).all())
+    base, ids = torch.zeros(1, dtype=torch.int64, device=cuda), torch.zeros(4, dtype=torch.int64, device=cuda)
+    failed(lambda: TR.tree_rows(i32([-1, 0, 3, 0]), i32([0, 4]), base, table, page))
+    failed(lambda: TR.tree_rows(i32([-1, 0, -7, 0]), i32([0, 4]), base, table, page))
+    failed(lambda: TR.tree_rows(i32([-1, 0, 0, 0]), i32([0, 5]), base, table, page))
+    before = pool.clone()
+    failed(lambda: TR.tree_keep(ids, i32([-1, 0, 0, 0]), ids, i32([-2, 2]), base, table, [pool], hk, d, page))
+    assert torch.equal(pool, before)
