@@ -254,9 +254,13 @@ std::pair<int64_t, int64_t> rows_shares(int64_t ctas, int64_t max_len, int64_t r
   const int64_t cluster = want >= 8 ? 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
   return {cluster, cluster};
 }
-// The many-row kernel: two tiles of Q, a ring of K and V halves as 16-bit values (four, or five where they are copied as they are),
+// The many-row kernels: two tiles of Q (head_dim 256: one, and halves of 64 tokens), a ring of K and V halves as 16-bit values (four, or five where they are copied as they are),
 // two halves of codes with their scale bytes, barriers.
+int64_t tile_rows(int64_t d) { return d == 256 ? 128 : 256; }        // query rows of a CTA
+int64_t tile_threads(int64_t d) { return d == 256 ? 576 : 768; }
+const char* tile_module(int64_t d) { return d == 256 ? "attn_tile256" : "attn_tile"; }
 unsigned tile_shared(int64_t d, bool e4m3) {
+  if (d == 256) return (unsigned)(128 * d * 2 + (e4m3 ? 4 : 5) * 64 * d * 2 + (e4m3 ? 2 * (64 * d + 128) : 0) + 2 * 128 * 4 + 512);
   return (unsigned)(2 * 128 * d * 2 + (e4m3 ? 4 : 5) * 128 * d * 2 + (e4m3 ? 2 * (128 * d + 256) : 0) + 4 * 128 * 4 + 512);
 }
 // Shares of the many-row kernel: as many as fill the SMs once. Microseconds, 64 rows of 4 heads each, by shares (* the rule's):
@@ -269,7 +273,7 @@ unsigned tile_shared(int64_t d, bool e4m3) {
 int64_t tile_shares(int64_t ctas, int64_t max_len, int64_t sms) {
   return std::max<int64_t>(1, std::min<int64_t>({sms / ctas, (max_len + 255) / 256, 64}));
 }
-// Query rows of a sequence and kv head up to which the few-row kernel runs; the many-row kernel above them (head_dim 64 and 128).
+// Query rows of a sequence and kv head up to which the few-row kernel runs; the many-row kernel above them.
 // Microseconds of the few-row kernel : of the many-row kernel, 8 kv heads, head_dim 128:
 //   8-bit cache, causal          16 rows       32 rows            bf16 cache, tree       16 rows       24 rows
 //     1 sequence  of 1000      10.0 :  13.1   14.4 :  14.0           1 of 1000           10.4 :  11.8    14.0 :  11.9
@@ -341,7 +345,7 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
     unsigned shared;
     std::string name;
     if (tiled) {
-      toks = 256 / g;
+      toks = tile_rows(d) / g;
       gy = std::min(rows / toks + seqs, seqs * ((most + toks - 1) / toks));                // blocks of all sequences, at most
       shares = tile_shares(hk * gy, max_len, h.sms);
       gx = hk;
@@ -373,14 +377,14 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
     b.bytes(map.data(), map.size()).at(q).at(out).put(ws_o).put(ws_ml).at(pool).at(table).at(lens).at(cu_q).at(masks);
     b.ints(masks ? masks->size(1) : 0, rows_per_seq, hq, hk, q_step, out_step, width, page, tiled ? seqs : cluster, pages, lo, hi, rows);
     b.put((float)(scale * kLog2e)).put(h.err);
-    launch(h, tiled ? "attn_tile" : "attn_rows", name, gx, gy, shares, tiled ? 768 : 160, b, shared, !tiled && hi < all, (unsigned)cluster);
+    launch(h, tiled ? tile_module(d) : "attn_rows", name, gx, gy, shares, tiled ? (unsigned)tile_threads(d) : 160, b, shared, !tiled && hi < all, (unsigned)cluster);
     if (groups > 1) {
       Block m;
       m.put(ws_o).put(ws_ml).at(out).at(lens).at(cu_q).ints(rows_per_seq, hq, toks, shares, cluster, out_step, lo, hi, rows);
       launch(h, "attn_rows", std::string("kern_attn_rows_merge_") + (masks ? "tree_d" : "causal_d") + n(d), most * hq, seqs, 1, 128, m, 0, true);
     }
   };
-  if (g * max_rows <= kFewRows || d > 128) {
+  if (g * max_rows <= kFewRows) {
     run(false, 1, all);
   } else if (masks || !cu_q || seqs == 1 || rows + few >= seqs * max_rows) {
     run(true, 1, all);                                       // (rows alike; trees of a node or two among the others end before those)
@@ -470,7 +474,7 @@ PYBIND11_MODULE(_ops_host, m) {
   });
   m.def("launches", [](int gpu) { return hosts().at(gpu) ? hosts()[gpu]->launches : 0; });
   m.def("rows_form", [](int64_t d, bool e4m3, int64_t nt) { const RowsForm f = rows_form(d, e4m3, nt); return py::make_tuple(f.shared, f.per_sm); });
-  m.def("tile_shared", &tile_shared);
+  m.def("tile_form", [](int64_t d, bool e4m3) { return py::make_tuple(tile_module(d), tile_rows(d), tile_threads(d), tile_shared(d, e4m3)); });
   m.def("append", &append);
   m.def("read_rows", &read_rows);
   m.def("attend", &attend);

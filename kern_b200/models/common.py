@@ -682,28 +682,22 @@ def attn_decode_e4m3_op(hq: int, hk: int, d: int, page_size: int, table_width: i
 
 
 def attn_prefill_e4m3_op(hq: int, hk: int, d: int, page_size: int, table_width: int, q_stride: int, seqs_max: int) -> dict:
-    """Ragged rows over the 8-bit cache: sequences of many rows on the tensor-core kernel (head_dim 64 and 128), of few on the few-row
+    """Ragged rows over the 8-bit cache: sequences of many rows on the tensor-core kernel, of few on the few-row
     kernel. Interface [q(kv) buffer, kv state, out, block_table, seq_lens, cu_seqlens, seqs, err]; no plan."""
     from .. import _ops_host
 
     g = hq // hk
     iface = ["in buffer<bf16>", "in state", "out buffer<bf16>", "in buffer<i32>", "in buffer<i32>", "in buffer<i32>", "i32", "out buffer<i32>"]
     few = max(1, 8 // g)
-    if d > 128:
-        nt = 2
-        toks = 8 * nt // g
-        many = _e4m3_attend(f"kern_attn_rows_e4m3_causal_d{d}_n{nt}", [{"mul": [{"ceil_div": ["tokens", toks]}, hk]}, "seqs", 1], 160,
-                            _ops_host.rows_form(d, True, nt)[0], 1,
-                            hq, hk, d, page_size, table_width, q_stride, {"i32": 1}, few + 1, I32_MAX, 5, 7, None)
-    else:
-        many = _e4m3_attend(f"kern_attn_tile_e4m3_causal_d{d}", [hk, {"add": [{"ceil_div": ["tokens", 256 // g]}, "seqs"]}, 1], 768,
-                            _ops_host.tile_shared(d, True), 1,
-                            hq, hk, d, page_size, table_width, q_stride, {"param": 6}, few + 1, I32_MAX, 5, 7, None)
+    module, rows, threads, smem = _ops_host.tile_form(d, True)
+    many = _e4m3_attend(f"kern_attn_tile_e4m3_causal_d{d}", [hk, {"add": [{"ceil_div": ["tokens", rows // g]}, "seqs"]}, 1], threads, smem, 1,
+                        hq, hk, d, page_size, table_width, q_stride, {"param": 6}, few + 1, I32_MAX, 5, 7, None)
+    many["module"] = module
     return {"params": iface, "impl": {"launches": [many] + _e4m3_few(hq, hk, d, page_size, table_width, q_stride, seqs_max, few, few, 5, 7)}}
 
 
 def e4m3_modules(d: int) -> list[str]:
-    return ["kv_e4m3", "attn_rows"] + (["attn_tile"] if d <= 128 else [])
+    return ["kv_e4m3", "attn_rows", "attn_tile256" if d == 256 else "attn_tile"]
 
 
 def last_row_op(row_bytes: int) -> dict:

@@ -264,9 +264,10 @@ def test_tree_attention(cuda, kind, hq, hk, d, page, rows, past):
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 @pytest.mark.parametrize("nodes", [6, 90])
-def test_what_a_row_does_not_see_does_not_reach_it(cuda, kind, nodes):
+@pytest.mark.parametrize("d", [128, 64, 256])
+def test_what_a_row_does_not_see_does_not_reach_it(cuda, kind, nodes, d):
     """Infinities and NaN behind the sequence's end, and in nodes that some rows see and others do not."""
-    hq, hk, d, page, past = 8, 2, 128, 64, 100
+    hq, hk, page, past = 8, 2, 64, 100
     l = past + nodes
     g = torch.Generator().manual_seed(9)
     pool, table, kv = fill_cache(kind, [l], hk, d, page, g)

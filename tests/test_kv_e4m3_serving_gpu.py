@@ -33,9 +33,10 @@ def bits_of(seen):
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 @pytest.mark.parametrize("nodes", [3, 20, 40, 90])
-def test_huge_rows_that_are_not_seen(cuda, kind, nodes):
+@pytest.mark.parametrize("d", [128, 64, 256])
+def test_huge_rows_that_are_not_seen(cuda, kind, nodes, d):
     """Every third node has keys and values near the largest bf16: rows that do not see them are as if they were not there."""
-    hq, hk, d, page, past = 8, 2, 128, 64, 70
+    hq, hk, page, past = 8, 2, 64, 70
     l = past + nodes
     g = torch.Generator().manual_seed(nodes)
     pool, table, kv = fill_cache(kind, [l], hk, d, page, g)
@@ -58,9 +59,10 @@ def test_huge_rows_that_are_not_seen(cuda, kind, nodes):
 
 @pytest.mark.parametrize("rows", [2, 100, 300])
 @pytest.mark.parametrize("shared", [1, 4000])
-def test_huge_values_behind_a_causal_row(cuda, rows, shared):
+@pytest.mark.parametrize("d", [128, 64, 256])
+def test_huge_values_behind_a_causal_row(cuda, rows, shared, d):
     """The block's last token has huge values: only its own row may show it. With and without shares of the context."""
-    hq, hk, d, page = 8, 2, 128, 64
+    hq, hk, page = 8, 2, 64
     l = shared + rows
     g = torch.Generator().manual_seed(rows)
     pool, table, kv = fill_cache("e4m3", [l], hk, d, page, g)
