@@ -3,8 +3,8 @@
 // places, and Q K^T of the next 64 keys runs while a tile's softmax does.
 //
 //   warps 0..7      softmax, two threads to a row, 32 of a tile's 64 scores each, held in registers from the maximum to the weights
-//   warps 8..15     two teams of four, a half (64 keys, or values) each in turn: 8-bit codes become f16, as in attn_tile.cu; bf16
-//                   halves are looked through where rows see different tokens
+//   warps 8..15     two teams of four, a half (64 keys, or values) each in turn: 8-bit codes become f16, as in attn_tile.cu; one team
+//                   looks through bf16 halves where rows see different tokens
 //   warp 16         issues the products in the order Q K^T(t + 2) behind P V(t); O is quiet for a reference to move once the P V before
 //                   has ended, which a barrier of its own tells
 //   warp 17         copies by TMA: codes into two slots, a team's each, beside a ring of four halves; bf16 halves into a ring of five
@@ -125,9 +125,11 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
   auto v_item = [&](int t) { return t == ntiles - 1 ? items - 1 : 2 * t + 2; };
 
   if (warp >= 8 && warp < 16) {
-    // ---------------- keys and values: item i is team i & 1's ----------------
+    // ---------------- keys and values: item i is team i & 1's, so a place of the ring is always the same team's, which has seen every
+    // turn of its barriers (8-bit; of five places each would change hands: bf16 halves, which take next to no work, have one team) ------
     const int team = (warp >> 2) & 1, w4 = warp & 3;
-    for (int i = team; i < items && ok; i += 2) {
+    static_assert(!E4M3 || kRing % 2 == 0, "a place belongs to one team");
+    for (int i = E4M3 || !team ? team : items; i < items && ok; i += E4M3 ? 2 : 1) {
       int which, t;
       item(i, which, t);
       const int half = i % kRing, tok0 = from + t * kKeys, here = to - tok0;

@@ -291,6 +291,28 @@ def test_the_largest_trees(cuda, kind):
         close(out[cu[s]:cu[s + 1]].view(r, hq, d), ref, spread, WEIGHT[kind])
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hq,hk,d,seqs,least,most", [(24, 4, 256, 16, 3900, 4000), (24, 4, 256, 60, 1, 900), (8, 4, 128, 16, 2000, 2100), (8, 8, 64, 30, 10, 1500)])
+def test_trees_on_long_contexts(cuda, kind, hq, hk, d, seqs, least, most):
+    """Many key tiles a block, in one share and in several, every place of the rings used many times."""
+    page, nodes = 64, 20
+    g = torch.Generator().manual_seed(seqs)
+    lens = (torch.randint(least, most, (seqs,), generator=g) + nodes).tolist()
+    pool, table, kv = fill_cache(kind, lens, hk, d, page, g)
+    cu = [nodes * s for s in range(seqs + 1)]
+    bits = torch.rand(cu[-1], nodes, generator=g) < 0.4
+    q = torch.randn(cu[-1], hq * d, generator=g).bfloat16().cuda()
+    out = TR.tree_attention(q, pool, table, i32(lens), bits_of(bits).cuda(), i32(cu), hq, hk, d, page, max_rows=nodes)
+    for _ in range(20):
+        assert torch.equal(out, TR.tree_attention(q, pool, table, i32(lens), bits_of(bits).cuda(), i32(cu), hq, hk, d, page, max_rows=nodes))
+    for s in range(0, seqs, 5):
+        l = lens[s]
+        seen = torch.ones(nodes, l, dtype=torch.bool)
+        seen[:, l - nodes:] = bits[cu[s]:cu[s + 1]]
+        ref, spread = attend64(q[cu[s]:cu[s + 1]].cpu().view(nodes, hq, d), kv[s], seen, d ** -0.5)
+        close(out[cu[s]:cu[s + 1]].view(nodes, hq, d), ref, spread, WEIGHT[kind])
+
+
 @pytest.mark.parametrize("seqs", [90, 200])
 def test_more_single_tokens_than_run_at_once(cuda, seqs):
     hq, hk, d, page = 16, 8, 64, 16
