@@ -279,6 +279,7 @@ int64_t tile_shares(int64_t ctas, int64_t max_len, int64_t sms) {
 //     1 sequence  of 1000      10.0 :  13.1   14.4 :  14.0           1 of 1000           10.4 :  11.8    14.0 :  11.9
 //    16 sequences of 4000      39.0 :  74.9   74.2 :  75.1          16 of 4000           47.9 :  46.6    85.0 :  46.6
 //    64 sequences of 2000      88.8 : 159     206  : 161            64 of 2000          106.8 : 107.2   216.8 : 107.8
+// and head_dim 256, 16 sequences of 4000: 12 rows 42.5 : 54.3, 18 rows 66.0 : 54.8.
 // (the few-row kernel's matrix instructions take time for every eight rows, the other's are the same up to 128)
 constexpr int64_t kFewRows = 16;
 
