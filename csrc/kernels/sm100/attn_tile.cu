@@ -25,7 +25,7 @@
 // between the two warps that share the row; no pass over O but then). Registers are dealt by role, as a spill costs an L2 access
 // where shared memory has taken the L1's place.
 //
-// Measured (8 kv heads, 32 heads of 128): 4 prompts of up to 2048 rows on 8-bit contexts of up to 6000 387 us, 0.60 of the measured
+// Measured (8 kv heads, 32 heads of 128): 4 prompts of up to 2048 rows on 8-bit contexts of up to 6000 384 us, 0.60 of the measured
 // tensor peak; 18 trees of 128 nodes over 4000 tokens 1100 TFLOP/s (bf16) and 970 (8-bit); 64 trees of up to 32 nodes over bf16
 // contexts of up to 8192 210 us, 0.88 of the measured bandwidth.
 //
@@ -201,10 +201,8 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
           const uint32_t at = src + r0 * D + (((p >> 1) ^ (D == 64 ? (r0 >> 1) & 3 : r0 & 7)) << 4) + (p & 1) * 8;
 #pragma unroll
           for (int j = 0; j < kLoads; ++j)
-            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2 * h]), "=r"(w[j][2 * h + 1]) : "r"(at + j * kStep * D));
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2 * h]), "=r"(w[j][2 * h + 1]) : "r"(at + j * kStep * D) : "memory");
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&taken[slot]);             // (the codes are in registers, the scale bytes too)
         if (edge) {
 #pragma unroll
           for (int j = 0; j < kLoads; ++j) {
@@ -246,7 +244,11 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         if (!which && w4 == 0 && lane == 0) e_s[t & 3] = make_float2(pow2i(top - 127 - 6), (float)(vtop - 127 - 6));
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[half]);
+        if (lane == 0) {
+          mbar_arrive(&full[half]);
+          // (not before the codes have been used: behind the loads alone, what the next copy brought was read now and then; and no slower)
+          mbar_arrive(&taken[slot]);
+        }
       }
     } else {
       for (int i = 0; i < items && ok; ++i) {
@@ -420,12 +422,15 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
     {
       constexpr int kLanes = D / 8, kPass = 512 / kLanes, kPasses = 2 * kQ / kPass;
       const int c = threadIdx.x % kLanes;
+      const float per_g = 1.f / (float)G;
+      const __nv_bfloat16* q_at = a.q + (size_t)(row0 + tok_lo) * a.q_stride + (size_t)kvh * G * D + c * 8;
       uint4 rows[kPasses];                                    // (all under way together)
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
         const int r = threadIdx.x / kLanes + i * kPass, rr = twice ? r & (kQ - 1) : r;
+        const int tok = (int)((rr + 0.5f) * per_g), head = rr - tok * G;      // (rr / G, exact: rr < 256)
         rows[i] = make_uint4(0, 0, 0, 0);
-        if (rr < valid) rows[i] = *reinterpret_cast<const uint4*>(a.q + (size_t)(row0 + tok_lo + rr / G) * a.q_stride + (size_t)(kvh * G + rr % G) * D + c * 8);
+        if (rr < valid) rows[i] = *reinterpret_cast<const uint4*>(q_at + (size_t)tok * a.q_stride + head * D);
       }
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {

@@ -13,7 +13,7 @@
 //
 // Bound: 2 * 128 * 64 * 256 multiply-adds a tile take 1024 clocks, its exponentials 512; 32 KB of f16 values a half go through shared
 // memory for 128 query rows where attn_tile.cu has 256, so the conversions weigh twice as much. Measured: 4 prompts of 1024 rows on 4000
-// tokens, 8-bit, 24 heads over 4, 434 us, 810 TFLOP/s (16 query rows at a time in the few-row kernel: 3100 us).
+// tokens, 8-bit, 24 heads over 4, 424 us, 830 TFLOP/s (16 query rows at a time in the few-row kernel: 3100 us).
 #include "attn_umma.cuh"
 
 namespace kern {
@@ -29,6 +29,18 @@ struct Tile256Cfg {
   static constexpr int kSmem = kQBytes + kRing * kHalf + kSlots * kCodes + kScales + 2 * kQRows * 4 + 512;
   static_assert(kSmem <= 232448, "more shared memory than a CTA has");
 };
+
+// An arrival that says that a warp's loads from shared memory are done, before anything has used them. The address takes in every lane's
+// values (`zero` is 0, which the compiler does not know): behind the loads alone the arrival came before some of them now and then,
+// and they read what the next copy brought.
+template <int N>
+KERN_DEVICE void arrive_loaded(uint64_t* bar, const uint32_t (&w)[N][4], uint32_t zero) {
+  uint32_t all = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) all |= w[i][0] | w[i][1] | w[i][2] | w[i][3];
+  const uint32_t off = __reduce_or_sync(0xffffffffu, all & zero);
+  if ((threadIdx.x & 31) == 0) mbar_arrive(reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(bar) + off));
+}
 
 // cache format, tree or causal
 template <bool E4M3, bool TREE>
@@ -128,6 +140,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
     // ---------------- keys and values: item i is team i & 1's, so a place of the ring is always the same team's, which has seen every
     // turn of its barriers (8-bit; of five places each would change hands: bf16 halves, which take next to no work, have one team) ------
     const int team = (warp >> 2) & 1, w4 = warp & 3;
+    const uint32_t zero = (uint32_t)(a.rows >> 31);
     static_assert(!E4M3 || kRing % 2 == 0, "a place belongs to one team");
     for (int i = E4M3 || !team ? team : items; i < items && ok; i += E4M3 ? 2 : 1) {
       int which, t;
@@ -170,9 +183,8 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
         for (int j = 0; j < kLoads; ++j)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2 * h]), "=r"(w[j][2 * h + 1]) : "r"(at + h * kBlock + j * 8 * 128));
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&taken[slot]);             // (the codes are in registers, the scale bytes too)
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2 * h]), "=r"(w[j][2 * h + 1]) : "r"(at + h * kBlock + j * 8 * 128) : "memory");
+        arrive_loaded(&taken[slot], w, zero);                 // (once the codes have been used: 473 us, not 424, for the prompts above)
         if (edge) {
 #pragma unroll
           for (int j = 0; j < kLoads; ++j) {
@@ -346,14 +358,17 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
     __syncwarp();
   } else if (warp < 8) {
     // ---------------- Q -> shared memory, K-major with the 128-byte swizzle: a warp to a row ----------------
+    const float per_g = 1.f / (float)G;
+    const __nv_bfloat16* q_at = a.q + (size_t)(row0 + tok_lo) * a.q_stride + (size_t)kvh * G * D + lane * 8;
 #pragma unroll 1
     for (int r1 = warp; r1 < kQRows; r1 += 64) {
       uint4 rows[8];                                          // (all under way together)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = r1 + i * 8;
+        const int tok = (int)((r + 0.5f) * per_g), head = r - tok * G;        // (r / G, exact: r < 128)
         rows[i] = make_uint4(0, 0, 0, 0);
-        if (r < valid) rows[i] = *reinterpret_cast<const uint4*>(a.q + (size_t)(row0 + tok_lo + r / G) * a.q_stride + (size_t)(kvh * G + r % G) * D + lane * 8);
+        if (r < valid) rows[i] = *reinterpret_cast<const uint4*>(q_at + (size_t)tok * a.q_stride + head * D);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
