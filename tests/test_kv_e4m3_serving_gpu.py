@@ -400,3 +400,29 @@ def test_rows_and_parents_that_do_not_exist(cuda):
     before = pool.clone()
     failed(lambda: TR.tree_keep(ids, i32([-1, 0, 0, 0]), ids, i32([-2, 2]), base, table, [pool], hk, d, page))
     assert torch.equal(pool, before)
+
+
+@pytest.mark.parametrize("hq,hk,d", [(32, 8, 128), (16, 8, 64), (24, 4, 256)])
+@pytest.mark.parametrize("rows,seqs,most", [(1, 60, 900), (1, 2, 20000), (3, 20, 3000), (40, 20, 1500), (300, 2, 2500)])
+def test_a_call_gives_the_same_bits_each_time(cuda, hq, hk, d, rows, seqs, most):
+    """Causal calls of every kernel and way of sharing, from idle with cold caches and one behind the other."""
+    page = 64
+    g = torch.Generator().manual_seed(rows)
+    lens = torch.randint(rows, most, (seqs,), generator=g).tolist()
+    pool, table, kv = fill_cache("e4m3", lens, hk, d, page, g)
+    q = torch.randn(seqs * rows, hq * d, generator=g).bfloat16().cuda()
+    args = (table, i32(lens), hq, hk, d, page)
+    out = K8.paged_attention_e4m3(q, pool, *args, rows_per_seq=rows)
+    cold = torch.empty(200 << 20, dtype=torch.uint8, device=cuda)
+    wrong = torch.zeros((), dtype=torch.int64, device=cuda)
+    for i in range(60):
+        if i % 3 == 0:
+            cold.fill_(i)
+        if i % 3 < 2:
+            torch.cuda.synchronize()
+        wrong += (K8.paged_attention_e4m3(q, pool, *args, rows_per_seq=rows) != out).any()
+    assert int(wrong) == 0
+    s = seqs - 1
+    seen = torch.arange(lens[s])[None] <= (lens[s] - rows + torch.arange(rows))[:, None]
+    ref, spread = attend64(q[s * rows:].cpu().view(rows, hq, d), kv[s], seen, d ** -0.5)
+    close(out[s * rows:].view(rows, hq, d), ref, spread, WEIGHT["e4m3"])
