@@ -487,8 +487,8 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
       for (int i = 0; i < 16; ++i) {
         const float2 y = split64(fma2(pair64(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, shift2));
         const float u = exp2f(y.x), v = exp2f(y.y);
-        sum2[i & 1] = add2(sum2[i & 1], pair64(u, v));
         pk[i] = pack_pair<E4M3>(u, v);
+        sum2[i & 1] = add2(sum2[i & 1], E4M3 ? pair64(u, v) : pair64(__uint_as_float(pk[i] << 16), __uint_as_float(pk[i] & 0xffff0000u)));
       }
       tmem_st16(s_t, pk);
       const float2 sum = split64(add2(sum2[0], sum2[1]));
