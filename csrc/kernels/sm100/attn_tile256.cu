@@ -31,11 +31,11 @@ struct Tile256Cfg {
 };
 
 // An arrival that says that a warp's loads from shared memory are done, before anything has used them. The address takes in every lane's
-// values (`zero` is 0, which the compiler does not know): behind the loads alone the arrival came before some of them now and then,
-// and they read what the next copy brought.
+// values (`zero` is 0, which the compiler does not know; `others`: what else was loaded from the slot): behind the loads alone the arrival
+// came before some of them now and then, and they read what the next copy brought.
 template <int N>
-KERN_DEVICE void arrive_loaded(uint64_t* bar, const uint32_t (&w)[N][4], uint32_t zero) {
-  uint32_t all = 0;
+KERN_DEVICE void arrive_loaded(uint64_t* bar, const uint32_t (&w)[N][4], uint32_t others, uint32_t zero) {
+  uint32_t all = others;
 #pragma unroll
   for (int i = 0; i < N; ++i) all |= w[i][0] | w[i][1] | w[i][2] | w[i][3];
   const uint32_t off = __reduce_or_sync(0xffffffffu, all & zero);
@@ -169,8 +169,8 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
           const uint32_t m = __vmaxu4(w, w >> 16);
           return (int)__reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u));
         };
-        const uint32_t word = scale_word(by);
-        const int top = top_byte(word), vtop = which ? 0 : top_byte(scale_word(by + kKeys));
+        const uint32_t word = scale_word(by), v_word = which ? 0u : scale_word(by + kKeys);
+        const int top = top_byte(word), vtop = top_byte(v_word);
         // (a row of zeros has the byte -40 + 127)
         if (top > 0x57 + 20 && (__vcmpgtu4(word, 0x57575757u) & __vcmpltu4(word, (uint32_t)(top - 20) * 0x01010101u)) != 0) *wide_s = 1;
         // a lane: 8 codes of the row's first 128 and 8 of its second (a piece of 16-bit values each), in rows r0 + 8 j: all in the
@@ -184,7 +184,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
 #pragma unroll
           for (int h = 0; h < 2; ++h)
             asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2 * h]), "=r"(w[j][2 * h + 1]) : "r"(at + h * kBlock + j * 8 * 128) : "memory");
-        arrive_loaded(&taken[slot], w, zero);                 // (once the codes have been used: 473 us, not 424, for the prompts above)
+        arrive_loaded(&taken[slot], w, word | v_word, zero);                 // (once the codes have been used: 473 us, not 424, for the prompts above)
         if (edge) {
 #pragma unroll
           for (int j = 0; j < kLoads; ++j) {

@@ -1,0 +1,88 @@
+"""Attention over the 8-bit cache, and its append, where scales, rows and arguments are at their ends (sm_100a)."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from kern_b200.ops import kv_e4m3 as K8
+from kern_b200.ops import tree as TR
+from kern_b200.ops.launcher import Kernels
+from test_kv_e4m3_gpu import WEIGHT, attend64, close
+
+
+@pytest.fixture(autouse=True)
+def _no_device_error(cuda):
+    yield
+    Kernels.get(cuda).check_error()
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def cache_of(k, v, page):
+    """A pool with the rows k and v [L, hk, d] of one sequence on scattered pages; (pool, table, 64-bit rows [2, L, hk, d])."""
+    l, hk, d = k.shape
+    need = -(-l // page)
+    kv = torch.zeros(need * page, 2, hk, d)
+    kv[:l] = torch.stack([k, v], 1)
+    codes, scales = K8.quantise_reference(kv.bfloat16())
+    exact = torch.ldexp(codes.double(), (scales.int() - 127)[..., None])
+    table = torch.randperm(need + 2, generator=torch.Generator().manual_seed(l))[:need].int()
+    pool = K8.new_pool(need + 2, hk, page, d, "cuda")
+    c, s = K8.views(pool, hk, page, d)
+    at = table.long().cuda()
+    c.view(torch.uint8)[at] = codes.view(torch.uint8).view(need, page, 2, hk, d).permute(0, 2, 3, 1, 4).cuda()
+    s[at] = scales.view(need, page, 2, hk).permute(0, 2, 3, 1).cuda()
+    return pool, table.cuda()[None], exact[:l].permute(1, 0, 2, 3)
+
+
+def causal(rows, l):
+    return torch.arange(l)[None] <= (l - rows + torch.arange(rows))[:, None]
+
+
+def bits_of(seen):
+    """[rows, nodes] bool -> i64 [rows, words]"""
+    rows, nodes = seen.shape
+    words = -(-nodes // 64)
+    wide = torch.zeros(rows, words * 64, dtype=torch.bool)
+    wide[:, :nodes] = seen
+    weights = torch.tensor([1 << i if i < 63 else -(1 << 63) for i in range(64)])
+    return (wide.view(rows, words, 64).long() * weights).sum(-1).cuda()
+
+
+def both_ways(q, pool, table, l, hq, hk, d, page, **k):
+    """The rows as causal ones and as a tree that is a chain: (causal, tree), [rows, hq, d]."""
+    rows = q.shape[0]
+    a = K8.paged_attention_e4m3(q, pool, table, i32([l]), hq, hk, d, page, rows_per_seq=rows, **k)
+    out = [a.view(rows, hq, d)]
+    if rows <= TR.MAX_NODES:
+        chain = bits_of(torch.ones(rows, rows).tril().bool())
+        out.append(TR.tree_attention(q, pool, table, i32([l]), chain, i32([0, rows]), hq, hk, d, page, **k).view(rows, hq, d))
+    return out
+
+
+@pytest.mark.parametrize("d", [256, 128, 64])
+def test_value_tiles_of_other_sizes(cuda, d):
+    """Every 64 tokens' values have another size: a value tile's exponent taken from a neighbour's scale bytes shows at once. From idle with
+    cold caches, and one behind the other."""
+    hq, hk, page, l, rows = 24, 4, 64, 4000, 40
+    g = torch.Generator().manual_seed(d)
+    k, v = torch.randn(2, l, hk, d, generator=g)
+    v *= torch.exp2(torch.randint(-8, 9, (-(-l // 64),), generator=g).float()).repeat_interleave(64)[:l, None, None]
+    pool, table, kv = cache_of(k, v, page)
+    q = torch.randn(rows, hq * d, generator=g).bfloat16().cuda()
+    first = both_ways(q, pool, table, l, hq, hk, d, page)
+    ref, spread = attend64(q.cpu().view(rows, hq, d), kv, causal(rows, l), d ** -0.5)
+    for out in first:
+        close(out, ref, spread, WEIGHT["e4m3"])
+    cold = torch.empty(200 << 20, dtype=torch.uint8, device=cuda)
+    wrong = torch.zeros((), dtype=torch.int64, device=cuda)
+    for i in range(100):
+        if i % 3 == 0:
+            cold.fill_(i)
+        if i % 3 < 2:
+            torch.cuda.synchronize()
+        for x, y in zip(first, both_ways(q, pool, table, l, hq, hk, d, page)):
+            wrong += (x != y).any()
+    assert int(wrong) == 0
