@@ -73,7 +73,8 @@ def quantise_reference(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     x = torch.where(torch.isfinite(x.float()), x.float(), float("nan"))
     m, e = torch.frexp(x.nan_to_num(0.0).abs().amax(-1))
     e = torch.where(m > 0, torch.clamp(e - 9 + (m > 0.875).int(), -40, 119), -40)
-    return torch.ldexp(x, -e[..., None]).to(torch.float8_e4m3fn), (e + 127).to(torch.uint8)
+    # (values past 448 * 2^119 end there)
+    return torch.ldexp(x, -e[..., None]).clamp(-448.0, 448.0).to(torch.float8_e4m3fn), (e + 127).to(torch.uint8)
 
 
 def dequantise_reference(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:

@@ -1,0 +1,15 @@
+"""The 8-bit cache without a GPU: values, arguments and builds at their ends."""
+import pytest
+import torch
+
+from kern_b200.ops import kv_e4m3 as K8
+
+
+def test_the_largest_bf16_values_keep_their_sign_and_size():
+    """The format ends at 448 * 2^119: what is past it, and finite, becomes that."""
+    top = float(torch.finfo(torch.bfloat16).max)
+    x = torch.tensor([[top, -top, 2.9e38, 1.0] * 16])
+    codes, scales = K8.quantise_reference(x)
+    back = K8.dequantise_reference(codes, scales)[0]
+    end = 448 * 2.0 ** 119
+    assert scales.tolist() == [246] and back[:4].tolist() == [end, -end, end, 0.0]
