@@ -243,8 +243,9 @@ KERN_DEVICE void append_body(const AppendArgs& a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 u = split64(y[i]), q = split64(v[i]);
-        off[2 * i] = (fabsf(u.x) + fabsf(q.x)) * unit;
-        off[2 * i + 1] = (fabsf(u.y) + fabsf(q.y)) * unit;
+        // (values are as they are, and an infinite neighbour is none of theirs: no product with a unit of 0)
+        off[2 * i] = unit > 0.f ? (fabsf(u.x) + fabsf(q.x)) * unit : 0.f;
+        off[2 * i + 1] = unit > 0.f ? (fabsf(u.y) + fabsf(q.y)) * unit : 0.f;
         const float2 f = is_k && turns ? split64(fma2(y[i], cs[i], mul2(v[i], sn[i]))) : u;
         x[2 * i] = f.x;
         x[2 * i + 1] = f.y;

@@ -86,3 +86,36 @@ def test_value_tiles_of_other_sizes(cuda, d):
         for x, y in zip(first, both_ways(q, pool, table, l, hq, hk, d, page)):
             wrong += (x != y).any()
     assert int(wrong) == 0
+
+
+def _partners(d, rot, pairs):
+    """(places of a pair) that turn together"""
+    return (3, 3 + rot // 2) if pairs == "half" else (6, 7)
+
+
+@pytest.mark.parametrize("pairs", ["half", "interleaved"])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("hq,hk,d", [(4, 2, 64), (2, 1, 128), (3, 3, 64), (5, 5, 128), (2, 1, 256)])
+def test_values_whose_neighbours_are_infinite_or_huge(cuda, hq, hk, d, pairs, norm):
+    """Values do not turn: what stands at a rotation partner's place reaches no code but its own, whatever rows share a warp."""
+    page, rot = 16, d
+    a, b = _partners(d, rot, pairs)
+    top = float(torch.finfo(torch.bfloat16).max)
+    ends = [(float("inf"), 1.5), (1.5, float("-inf")), (float("nan"), -2.0), (top, top), (-top, 0.75 * top), (3e38, 1.0), (1.0, 2.0)]
+    t = len(ends)
+    g = torch.Generator().manual_seed(d)
+    x = torch.randn(t, hq + 2 * hk, d, generator=g)
+    for i, (u, w) in enumerate(ends):
+        x[i, hq + hk:, a], x[i, hq + hk:, b] = u, w
+    qkv = x.view(t, -1).bfloat16()
+    ang = torch.rand(t, rot // 2, generator=g) * 6
+    kn = (1 + 0.2 * torch.randn(d, generator=g)).bfloat16().cuda() if norm else None
+    pool = K8.new_pool(1, hk, page, d, cuda)
+    slots = torch.arange(t, device=cuda)
+    K8.rope_kv_append_e4m3(qkv.cuda(), pool, slots, slots, ang.cos().cuda(), ang.sin().cuda(), hq, hk, d, page, rot=rot, pairs=pairs, k_norm=kn)
+    want_c, want_s = K8.quantise_reference(qkv.view(t, -1, d)[:, hq + hk:])
+    codes, scales = K8.views(pool, hk, page, d)
+    got = codes[0, 1, :, :t].permute(1, 0, 2).float().cpu()
+    nan = torch.isnan(want_c.float())
+    assert torch.equal(torch.isnan(got), nan) and int(nan.sum()) == 3 * hk
+    assert torch.equal(got[~nan], want_c.float()[~nan]) and torch.equal(scales[0, 1, :, :t].t().cpu(), want_s)
