@@ -436,7 +436,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
       float scale = f, ev = 0.f;
       if constexpr (E4M3) {
         const float2 e = e_s[t & 3];
-        scale *= e.x;
+        scale = row_scale(f, e.x);
         ev = e.y;
       }
       uint32_t x[32];

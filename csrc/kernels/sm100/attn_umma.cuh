@@ -82,6 +82,11 @@ KERN_DEVICE uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   return r;
 }
 
+// (8-bit) What turns a row's products with a key tile into base-2 scores: the row's factor times the tile's. Kept a normal number:
+// a score that is not seen is -inf and stays it (zero queries on zero keys would make the factor 2^-149, which flushes to 0, and
+// -inf * 0 NaN), and a product of 0 stays 0.
+KERN_DEVICE float row_scale(float row, float tile) { return fminf(fmaxf(row * tile, 1.17549435e-38f), 3.402823466e38f); }
+
 // Block y of the call: (sequence, block of its rows) to found[0] and [1]; sequence -1 past the last. Blocks are counted through the
 // sequences; where more are launched than run at once these are taken by length, so that the last blocks to start are the shortest.
 // Every thread of the block calls (at least 256), warp 0 writes; scratch: 512 places in shared memory.

@@ -119,3 +119,21 @@ def test_values_whose_neighbours_are_infinite_or_huge(cuda, hq, hk, d, pairs, no
     nan = torch.isnan(want_c.float())
     assert torch.equal(torch.isnan(got), nan) and int(nan.sum()) == 3 * hk
     assert torch.equal(got[~nan], want_c.float()[~nan]) and torch.equal(scales[0, 1, :, :t].t().cpu(), want_s)
+
+
+@pytest.mark.parametrize("rows", [1, 4, 100, 300])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("size", [0.0, 2.0 ** -30])
+@pytest.mark.parametrize("query", [0.0, 1e-3, 1.0])
+def test_caches_of_zeros_or_next_to_nothing(cuda, rows, d, size, query):
+    """Keys and values of zeros give zeros; tiny ones, or queries of zeros, the mean of the values."""
+    hq, hk, page, l = 8, 2, 64, 450
+    g = torch.Generator().manual_seed(d)
+    pool, table, kv = cache_of(*(torch.randn(2, l, hk, d, generator=g) * size), page)
+    q = (torch.randn(rows, hq * d, generator=g) * query).bfloat16().cuda()
+    ref, spread = attend64(q.cpu().view(rows, hq, d), kv, causal(rows, l), d ** -0.5)
+    for out in both_ways(q, pool, table, l, hq, hk, d, page):
+        if size:
+            close(out, ref, spread, WEIGHT["e4m3"])
+        else:
+            assert bool((out == 0).all())
