@@ -469,7 +469,8 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
             for (int x = 0; x < 2; ++x) {
               float mx = fmaxf(s[nt][x], s[nt][2 + x]), rx = mx;
               if constexpr (E4M3)
-                rx = fmaxf(s[nt][x] + (float)((int)(__float_as_uint(vscale[0]) >> 23) - 127), s[nt][2 + x] + (float)((int)(__float_as_uint(vscale[1]) >> 23) - 127));
+                rx = fmaxf(s[nt][x] + (float)(max((int)(__float_as_uint(vscale[0]) >> 23), kLeastScale) - 127),
+                           s[nt][2 + x] + (float)(max((int)(__float_as_uint(vscale[1]) >> 23), kLeastScale) - 127));
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1) {
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));

@@ -159,7 +159,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       // all of a half's codes are in registers before the half that they go to is free, so its turn is short
       constexpr int kLanes = D / 16, kRowsWarp = 32 / kLanes, kLoads = kT / (4 * kRowsWarp);     // lanes to a row of codes; rows of a lane
       const int c = lane % kLanes, sub = lane / kLanes;
-      // a lane's four of a tile's scale bytes (those behind the end are 0), and the largest of all
+      // a lane's four of a tile's scale bytes (those behind the end are 0), and the largest of all (kLeastScale at least)
       auto scale_word = [&](uint32_t at, int here) -> uint32_t {
         uint32_t w;
         asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at + 4 * lane));
@@ -168,7 +168,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       };
       auto top_byte = [&](uint32_t w) -> int {
         const uint32_t m = __vmaxu4(w, w >> 16);
-        return (int)__reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u));
+        return max((int)__reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u)), kLeastScale);
       };
       for (int i = 0; i < items && ok; ++i) {
         int which, t;

@@ -158,7 +158,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
           break;
         }
         const uint32_t src = smem_u32(c_s) + slot * Cfg::kCodes, by = smem_u32(b_s) + slot * 2 * kKeys;
-        // a lane's four of the tile's scale bytes (those behind the end are 0; 16 lanes have some), and the largest of all
+        // a lane's four of the tile's scale bytes (those behind the end are 0; 16 lanes have some), and the largest of all (kLeastScale at least)
         auto scale_word = [&](uint32_t at) -> uint32_t {
           uint32_t w;
           asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at + 4 * (lane & 15)));
@@ -167,7 +167,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
         };
         auto top_byte = [&](uint32_t w) -> int {
           const uint32_t m = __vmaxu4(w, w >> 16);
-          return (int)__reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u));
+          return max((int)__reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u)), kLeastScale);
         };
         const uint32_t word = scale_word(by), v_word = which ? 0u : scale_word(by + kKeys);
         const int top = top_byte(word), vtop = top_byte(v_word);

@@ -3,7 +3,7 @@ GQA attention over it (single tokens, short causal blocks, prompt chunks), with 
 
 A row (one token, k or v, one kv head) is ``head_dim`` e4m3 codes and one scale byte ``e + 127``; it stands for ``code * 2**e``,
 which bf16 holds exactly. ``e`` is the smallest exponent that brings the row's largest finite value to 448 or less, kept within
-[-40, 119]; a value that is not finite is stored as NaN. One layer's cache is a uint8 tensor ``[pages, page_bytes(...)]``: a
+[-40, 119]; a value that is not finite is stored as NaN. A fresh pool's rows (all bytes 0) are rows of zeros. One layer's cache is a uint8 tensor ``[pages, page_bytes(...)]``: a
 page's codes ``[2, kv_heads, page_size, head_dim]`` (k then v), then its scale bytes ``[2, kv_heads, page_size]``; slot =
 page * page_size + offset, as in the bf16 cache, at 0.504 of its bytes (head_dim 128).
 """

@@ -137,3 +137,34 @@ def test_caches_of_zeros_or_next_to_nothing(cuda, rows, d, size, query):
             close(out, ref, spread, WEIGHT["e4m3"])
         else:
             assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("rows", [1, 4, 100, 300])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("query", [0.0, 1e-3, 1.0])
+def test_a_pool_that_nobody_has_written_to(cuda, rows, d, query):
+    hq, hk, page, l = 8, 2, 64, 450
+    pool, table = K8.new_pool(9, hk, page, d, cuda), torch.arange(8, dtype=torch.int32, device=cuda)[None]
+    q = (torch.randn(rows, hq * d, generator=torch.Generator().manual_seed(rows)) * query).bfloat16().cuda()
+    for out in both_ways(q, pool, table, l, hq, hk, d, page):
+        assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("rows", [1, 4, 100, 300])
+@pytest.mark.parametrize("past", [100, 4000])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("first", [False, True])
+def test_rows_that_nobody_has_written_to_beside_others(cuda, rows, past, d, first):
+    """Every other run of 128 tokens is as `new_pool` leaves it: tokens of zeros, which count in the sum of weights."""
+    hq, hk, page = 8, 2, 64
+    l = past + rows
+    g = torch.Generator().manual_seed(rows + past)
+    empty = (torch.arange(l) // 128) % 2 == int(not first)
+    k, v = torch.where(empty[:, None, None], 0.0, torch.randn(2, l, hk, d, generator=g))
+    pool, table, kv = cache_of(k, v, page)
+    at = empty.nonzero()[:, 0].cuda()
+    K8.views(pool, hk, page, d)[1][table[0].long()[at // page], :, :, at % page] = 0
+    q = torch.randn(rows, hq * d, generator=g).bfloat16().cuda()
+    ref, spread = attend64(q.cpu().view(rows, hq, d), kv, causal(rows, l), d ** -0.5)
+    for out in both_ways(q, pool, table, l, hq, hk, d, page):
+        close(out, ref, spread, WEIGHT["e4m3"])
