@@ -32,7 +32,8 @@
 // 8-bit: a tile's rows are brought to one exponent, E = the largest of its scale bytes, as they become f16 (exact for scales down to
 // 2^-20 of the largest); 2^E of the keys is then part of the scores' scale, E of the values part of the weights' exponent,
 // w_ij = 2^(s_ij + E_t - R_i): no work per score. A block that meets a tile with scales further apart (rows that hold nothing but
-// zeros and values under 2^-31 aside) is computed again, a row to a warp, each key and value row with its own scale (tile_wide).
+// zeros and values under 2^-31 aside), or value tiles whose exponents are more than 100 apart, is computed again, a row to a warp, each key and
+// value row with its own scale (tile_wide).
 #include "attn_umma.cuh"
 
 namespace kern {
@@ -170,6 +171,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         const uint32_t m = __vmaxu4(w, w >> 16);
         return max((int)__reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u)), kLeastScale);
       };
+      int v_least = 255, v_most = 0;                          // the value tiles' exponents
       for (int i = 0; i < items && ok; ++i) {
         int which, t;
         item(i, which, t);
@@ -189,6 +191,11 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         const int top = top_byte(word), vtop = which ? 0 : top_byte(scale_word(by + kT, here));
         // (a row of zeros has the byte -40 + 127)
         if (top > 0x57 + 20 && (__vcmpgtu4(word, 0x57575757u) & __vcmpltu4(word, (uint32_t)(top - 20) * 0x01010101u)) != 0) *wide_s = 1;
+        if (!which) {
+          v_least = min(v_least, vtop);
+          v_most = max(v_most, vtop);
+          if (v_most - v_least > kTilesApart) *wide_s = 1;
+        }
         uint8_t* dst = h_s + half * Cfg::kHalf;
         bool nan = false;
         // rows r0 + j * kStep: all in the same place of the swizzle and of their words of scale bytes
@@ -635,6 +642,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       }
       const bool whole = shares == 1, store = r < valid && ok;
       const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float level = E4M3 && !whole ? level_share(m, l) : 1.f;
       const int head = kvh * G + (r < valid ? r % G : 0);
       const size_t at = ((size_t)(row0 + tk) * a.hq + head) * gridDim.z + blockIdx.z;
       const bool bad = *bad_s != 0;
@@ -664,7 +672,13 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         } else {
           uint4* dst = reinterpret_cast<uint4*>(a.ws_o + at * D + col);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dst[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          for (int i = 0; i < 8; ++i) {
+            if constexpr (E4M3) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) x[4 * i + k] = __float_as_uint(__uint_as_float(x[4 * i + k]) * level);
+            }
+            dst[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          }
         }
       }
       if (!whole && store && part == 0) {

@@ -421,6 +421,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
     };
     constexpr float kGrown = E4M3 ? 15.9f : 30.f, kBelow = E4M3 ? 5.f : 0.f;      // (attn_tile.cu)
     float ref = kUnset, l = 0.f;                              // l: of this thread's columns
+    float ev_least = 255.f, ev_most = -255.f;                 // (8-bit) the value tiles' exponents
     // P V of tile t has ended (that of tile t - 2, whose place the scores of tile t took, has before those came)
     auto quiet = [&](int t) -> bool { return bar_wait(&o_quiet[t & 1], (t >> 1) & 1, abort_flag); };
     // (a wait that has run out does not leave the walk: the two warps meet in every step)
@@ -438,6 +439,8 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
         const float2 e = e_s[t & 3];
         scale = row_scale(f, e.x);
         ev = e.y;
+        ev_least = fminf(ev_least, ev);
+        ev_most = fmaxf(ev_most, ev);
       }
       uint32_t x[32];
       tmem_ld_32x32(s_t, x);
@@ -508,7 +511,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
     *own_x = l;
     meet();
     l += *his_x;
-    if (E4M3 && *wide_s != 0) {
+    if (E4M3 && (*wide_s != 0 || ev_most - ev_least > (float)kTilesApart)) {      // (uniform)
       if constexpr (E4M3) {
         const RowsArgs args = a;                              // (a copy on the stack, for this call alone)
         if (ok) tile_wide<D, TREE>(args, seq, row0, tok_lo, valid, past, from, to, shares, 8);
@@ -516,6 +519,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
     } else {
       const bool whole = shares == 1, store = row < valid && ok, bad = *bad_s != 0;
       const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float level = E4M3 && !whole ? level_share(ref, l) : 1.f;
       const int head = kvh * G + (row < valid ? row % G : 0);
       const size_t at = ((size_t)(row0 + tk) * a.hq + head) * gridDim.z + blockIdx.z;
 #pragma unroll 1
@@ -543,7 +547,13 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
         } else {
           uint4* dst = reinterpret_cast<uint4*>(a.ws_o + at * D + col);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dst[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          for (int i = 0; i < 8; ++i) {
+            if constexpr (E4M3) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) x[4 * i + k] = __float_as_uint(__uint_as_float(x[4 * i + k]) * level);
+            }
+            dst[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          }
         }
       }
       if (!whole && store && part == 0) {

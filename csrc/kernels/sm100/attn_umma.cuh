@@ -87,6 +87,22 @@ KERN_DEVICE uint32_t mul_f16x2(uint32_t a, uint32_t b) {
 // -inf * 0 NaN), and a product of 0 stays 0.
 KERN_DEVICE float row_scale(float row, float tile) { return fminf(fmaxf(row * tile, 1.17549435e-38f), 3.402823466e38f); }
 
+// (8-bit) The sum of weights is of weights that hold their value tile's exponent, and is freed of it tile by tile, so tiles' exponents
+// may lie this far apart: 2^-26 of the largest weight is then 2^-126 of the largest product, f32's end. Blocks past it are computed again.
+constexpr int kTilesApart = 100;
+
+// (8-bit) A share's partials (reference m, sum l, O) are left with l in [0.5, 1): m is then of scores alone, and comparable with other
+// shares', whose values may be of quite another size. Returns what O is to be multiplied by, a power of two.
+KERN_DEVICE float level_share(float& m, float& l) {
+  const int e = (int)(__float_as_uint(l) >> 23) & 255;
+  if (e == 0 || e == 255) return 1.f;                         // (nothing seen, or what is not finite)
+  const int shift = min(e - 126, 126);
+  const float f = pow2i(-shift);
+  m += (float)shift;
+  l *= f;
+  return f;
+}
+
 // Block y of the call: (sequence, block of its rows) to found[0] and [1]; sequence -1 past the last. Blocks are counted through the
 // sequences; where more are launched than run at once these are taken by length, so that the last blocks to start are the shortest.
 // Every thread of the block calls (at least 256), warp 0 writes; scratch: 512 places in shared memory.
@@ -174,7 +190,8 @@ KERN_DEVICE void put_back(const RowsArgs& a, const long long* mask, int seq, int
   }
 }
 
-// A block's rows over the 8-bit cache, a row to a warp in turn and one token at a time, for scales that have no common exponent.
+// A block's rows over the 8-bit cache, a row to a warp in turn and one token at a time, for scales that have no common exponent, in a tile
+// or over the tiles.
 template <int D, bool TREE>
 __device__ __noinline__ void tile_wide(const RowsArgs& a, int seq, int row0, int tok_lo, int valid, int past, int from, int to, int shares,
                                        int warps) {

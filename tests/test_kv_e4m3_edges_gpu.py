@@ -168,3 +168,24 @@ def test_rows_that_nobody_has_written_to_beside_others(cuda, rows, past, d, firs
     ref, spread = attend64(q.cpu().view(rows, hq, d), kv, causal(rows, l), d ** -0.5)
     for out in both_ways(q, pool, table, l, hq, hk, d, page):
         close(out, ref, spread, WEIGHT["e4m3"])
+
+
+@pytest.mark.parametrize("rows", [1, 4, 100, 300])
+@pytest.mark.parametrize("past", [100, 4000])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("low,high", [(None, 100), (-38, 100), (-30, 60), (-38, 118)])
+@pytest.mark.parametrize("swap", [False, True])
+def test_value_tiles_far_apart(cuda, rows, past, d, low, high, swap):
+    """Runs of 128 tokens with the smallest values (or zeros) beside runs with huge ones, in either order: every token counts in the sum
+    of weights. With one share of the context and with several."""
+    hq, hk, page = 8, 2, 64
+    l = past + rows
+    g = torch.Generator().manual_seed(rows + past)
+    k, v = torch.randn(2, l, hk, d, generator=g)
+    small = ((torch.arange(l) // 128) % 2 == int(swap))[:, None, None]
+    v = torch.where(small, v * (0.0 if low is None else 2.0 ** low), v * 2.0 ** high).clamp(-2.9e38, 2.9e38)
+    pool, table, kv = cache_of(k, v, page)
+    q = torch.randn(rows, hq * d, generator=g).bfloat16().cuda()
+    ref, spread = attend64(q.cpu().view(rows, hq, d), kv, causal(rows, l), d ** -0.5)
+    for out in both_ways(q, pool, table, l, hq, hk, d, page):
+        close(out, ref, spread, WEIGHT["e4m3"])
