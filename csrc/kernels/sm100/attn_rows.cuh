@@ -11,7 +11,7 @@ constexpr float kUnset = -1e30f;     // a reference before its first score
 constexpr float kOutgrown = 32768.f; // the weight at which references move: f16 holds twice that
 
 // the scale byte of a row of zeros, and of the smallest rows: -40 + 127. A page that nobody has written to has bytes of 0 (and codes of
-// 0): references and a tile's common exponent take these for the least, or what undoes their 2^-127 would pass f32's range
+// 0): references and a value tile's exponent take these for the least, or what undoes their 2^-127 would pass f32's range
 constexpr int kLeastScale = 87;
 
 struct RowsArgs {

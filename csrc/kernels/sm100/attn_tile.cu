@@ -160,7 +160,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       // all of a half's codes are in registers before the half that they go to is free, so its turn is short
       constexpr int kLanes = D / 16, kRowsWarp = 32 / kLanes, kLoads = kT / (4 * kRowsWarp);     // lanes to a row of codes; rows of a lane
       const int c = lane % kLanes, sub = lane / kLanes;
-      // a lane's four of a tile's scale bytes (those behind the end are 0), and the largest of all (kLeastScale at least)
+      // a lane's four of a tile's scale bytes (those behind the end are 0), and the largest of all
       auto scale_word = [&](uint32_t at, int here) -> uint32_t {
         uint32_t w;
         asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at + 4 * lane));
@@ -169,9 +169,8 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       };
       auto top_byte = [&](uint32_t w) -> int {
         const uint32_t m = __vmaxu4(w, w >> 16);
-        return max((int)__reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u)), kLeastScale);
+        return (int)__reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u));
       };
-      int v_least = 255, v_most = 0;                          // the value tiles' exponents
       for (int i = 0; i < items && ok; ++i) {
         int which, t;
         item(i, which, t);
@@ -191,11 +190,6 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         const int top = top_byte(word), vtop = which ? 0 : top_byte(scale_word(by + kT, here));
         // (a row of zeros has the byte -40 + 127)
         if (top > 0x57 + 20 && (__vcmpgtu4(word, 0x57575757u) & __vcmpltu4(word, (uint32_t)(top - 20) * 0x01010101u)) != 0) *wide_s = 1;
-        if (!which) {
-          v_least = min(v_least, vtop);
-          v_most = max(v_most, vtop);
-          if (v_most - v_least > kTilesApart) *wide_s = 1;
-        }
         uint8_t* dst = h_s + half * Cfg::kHalf;
         bool nan = false;
         // rows r0 + j * kStep: all in the same place of the swizzle and of their words of scale bytes
@@ -366,6 +360,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       const int steps = twice ? ntiles : 2 * ntiles;
       const uint32_t q_low = desc_low(smem_u32(q_s), 0), h_low = desc_low(smem_u32(h_s), 0), v_low = desc_low(smem_u32(h_s), kT * 128);
       const bool leader = elect_lane();
+      float ev_least = 255.f, ev_most = -255.f;               // (8-bit) the value tiles' exponents
       auto qk = [&](int u) -> bool {
         const int side = u & 1, t = twice ? u : u >> 1;
         const int i = k_item(t), half = i % kRing;
@@ -380,6 +375,13 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
           if (twice || side) tc_commit(&empty[half]);
         }
         __syncwarp();
+        if constexpr (E4M3) {
+          // (here, where a few instructions make nobody wait: 386 us for the prompts above, 404 in the warps that convert)
+          const float ev = fmaxf(e_s[t & 3].y, kLeastShift);
+          ev_least = fminf(ev_least, ev);
+          ev_most = fmaxf(ev_most, ev);
+          if (ev_most - ev_least > (float)kTilesApart) *wide_s = 1;
+        }
         return true;
       };
       auto pv = [&](int u) -> bool {
@@ -512,7 +514,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       if constexpr (E4M3) {
         const float2 e = e_s[t & 3];
         scale = row_scale(f, e.x);
-        ev = e.y;
+        ev = fmaxf(e.y, kLeastShift);
       }
       if (edge) {
         // the scores that a row does not see become -inf where they lie
@@ -642,7 +644,11 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
       }
       const bool whole = shares == 1, store = r < valid && ok;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const float level = E4M3 && !whole ? level_share(m, l) : 1.f;
+      if (E4M3 && !whole) {
+        const float level = level_share(m, l);
+        own *= level;
+        his *= level;
+      }
       const int head = kvh * G + (r < valid ? r % G : 0);
       const size_t at = ((size_t)(row0 + tk) * a.hq + head) * gridDim.z + blockIdx.z;
       const bool bad = *bad_s != 0;
@@ -672,13 +678,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         } else {
           uint4* dst = reinterpret_cast<uint4*>(a.ws_o + at * D + col);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if constexpr (E4M3) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) x[4 * i + k] = __float_as_uint(__uint_as_float(x[4 * i + k]) * level);
-            }
-            dst[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-          }
+          for (int i = 0; i < 8; ++i) dst[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
         }
       }
       if (!whole && store && part == 0) {

@@ -158,7 +158,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
           break;
         }
         const uint32_t src = smem_u32(c_s) + slot * Cfg::kCodes, by = smem_u32(b_s) + slot * 2 * kKeys;
-        // a lane's four of the tile's scale bytes (those behind the end are 0; 16 lanes have some), and the largest of all (kLeastScale at least)
+        // a lane's four of the tile's scale bytes (those behind the end are 0; 16 lanes have some), and the largest of all
         auto scale_word = [&](uint32_t at) -> uint32_t {
           uint32_t w;
           asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at + 4 * (lane & 15)));
@@ -167,7 +167,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
         };
         auto top_byte = [&](uint32_t w) -> int {
           const uint32_t m = __vmaxu4(w, w >> 16);
-          return max((int)__reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u)), kLeastScale);
+          return (int)__reduce_max_sync(0xffffffffu, max(m & 255u, (m >> 8) & 255u));
         };
         const uint32_t word = scale_word(by), v_word = which ? 0u : scale_word(by + kKeys);
         const int top = top_byte(word), vtop = top_byte(v_word);
@@ -314,6 +314,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
     constexpr uint32_t idesc_qk = tile_idesc<E4M3>(kQRows, kKeys, false), idesc_pv = tile_idesc<E4M3>(kQRows, D, true);
     const uint32_t q_low = desc_low(smem_u32(q_s), 0), h_low = desc_low(smem_u32(h_s), 0), v_low = desc_low(smem_u32(h_s), kBlock);
     const bool leader = elect_lane();
+    float ev_least = 255.f, ev_most = -255.f;                 // (8-bit) the value tiles' exponents
     auto qk = [&](int t) -> bool {
       const int i = k_item(t), half = i % kRing;
       if (!bar_wait(&full[half], (i / kRing) & 1, abort_flag)) return false;
@@ -327,6 +328,13 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
         tc_commit(&empty[half]);
       }
       __syncwarp();
+      if constexpr (E4M3) {
+        // (here, where a few instructions make nobody wait, as in attn_tile.cu)
+        const float ev = fmaxf(e_s[t & 3].y, kLeastShift);
+        ev_least = fminf(ev_least, ev);
+        ev_most = fmaxf(ev_most, ev);
+        if (ev_most - ev_least > (float)kTilesApart) *wide_s = 1;
+      }
       return true;
     };
     auto pv = [&](int t) -> bool {
@@ -421,7 +429,6 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
     };
     constexpr float kGrown = E4M3 ? 15.9f : 30.f, kBelow = E4M3 ? 5.f : 0.f;      // (attn_tile.cu)
     float ref = kUnset, l = 0.f;                              // l: of this thread's columns
-    float ev_least = 255.f, ev_most = -255.f;                 // (8-bit) the value tiles' exponents
     // P V of tile t has ended (that of tile t - 2, whose place the scores of tile t took, has before those came)
     auto quiet = [&](int t) -> bool { return bar_wait(&o_quiet[t & 1], (t >> 1) & 1, abort_flag); };
     // (a wait that has run out does not leave the walk: the two warps meet in every step)
@@ -438,9 +445,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
       if constexpr (E4M3) {
         const float2 e = e_s[t & 3];
         scale = row_scale(f, e.x);
-        ev = e.y;
-        ev_least = fminf(ev_least, ev);
-        ev_most = fmaxf(ev_most, ev);
+        ev = fmaxf(e.y, kLeastShift);
       }
       uint32_t x[32];
       tmem_ld_32x32(s_t, x);
@@ -511,7 +516,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
     *own_x = l;
     meet();
     l += *his_x;
-    if (E4M3 && (*wide_s != 0 || ev_most - ev_least > (float)kTilesApart)) {      // (uniform)
+    if (E4M3 && *wide_s != 0) {                               // (uniform: every half has been looked at)
       if constexpr (E4M3) {
         const RowsArgs args = a;                              // (a copy on the stack, for this call alone)
         if (ok) tile_wide<D, TREE>(args, seq, row0, tok_lo, valid, past, from, to, shares, 8);

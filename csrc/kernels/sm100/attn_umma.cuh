@@ -90,6 +90,8 @@ KERN_DEVICE float row_scale(float row, float tile) { return fminf(fmaxf(row * ti
 // (8-bit) The sum of weights is of weights that hold their value tile's exponent, and is freed of it tile by tile, so tiles' exponents
 // may lie this far apart: 2^-26 of the largest weight is then 2^-126 of the largest product, f32's end. Blocks past it are computed again.
 constexpr int kTilesApart = 100;
+// the exponent E of a value tile that holds the least scale (6 less: keys and values are multiplied by 2^6 as they become f16)
+constexpr float kLeastShift = kLeastScale - 127 - 6;
 
 // (8-bit) A share's partials (reference m, sum l, O) are left with l in [0.5, 1): m is then of scores alone, and comparable with other
 // shares', whose values may be of quite another size. Returns what O is to be multiplied by, a power of two.
