@@ -31,9 +31,9 @@
 //
 // 8-bit: a tile's rows are brought to one exponent, E = the largest of its scale bytes, as they become f16 (exact for scales down to
 // 2^-20 of the largest); 2^E of the keys is then part of the scores' scale, E of the values part of the weights' exponent,
-// w_ij = 2^(s_ij + E_t - R_i): no work per score. A block that meets a tile with scales further apart (rows that hold nothing but
-// zeros and values under 2^-31 aside), or value tiles whose exponents are more than 100 apart, is computed again, a row to a warp, each key and
-// value row with its own scale (tile_wide).
+// w_ij = 2^(s_ij + E_t - R_i): no work per score. A block that meets a tile with scales further apart (rows of zeros aside), or
+// value tiles whose exponents are more than 100 apart, is computed again, a row to a warp, each key and value row with its own
+// scale (tile_wide).
 #include "attn_umma.cuh"
 
 namespace kern {
@@ -189,7 +189,9 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         const uint32_t word = scale_word(by, here);
         const int top = top_byte(word), vtop = which ? 0 : top_byte(scale_word(by + kT, here));
         // (a row of zeros has the byte -40 + 127)
-        if (top > 0x57 + 20 && (__vcmpgtu4(word, 0x57575757u) & __vcmpltu4(word, (uint32_t)(top - 20) * 0x01010101u)) != 0) *wide_s = 1;
+        if (top > kLeastScale + 20 && (__vcmpgtu4(word, 0u) & __vcmpltu4(word, (uint32_t)(top - 20) * 0x01010101u)) != 0 &&
+            rows_lost<D, 1>(src, 0, lane, word, top))
+          *wide_s = 1;
         uint8_t* dst = h_s + half * Cfg::kHalf;
         bool nan = false;
         // rows r0 + j * kStep: all in the same place of the swizzle and of their words of scale bytes

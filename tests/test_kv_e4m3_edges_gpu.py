@@ -189,3 +189,23 @@ def test_value_tiles_far_apart(cuda, rows, past, d, low, high, swap):
     ref, spread = attend64(q.cpu().view(rows, hq, d), kv, causal(rows, l), d ** -0.5)
     for out in both_ways(q, pool, table, l, hq, hk, d, page):
         close(out, ref, spread, WEIGHT["e4m3"])
+
+
+@pytest.mark.parametrize("rows", [4, 100, 300])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("which", ["values", "keys"])
+def test_rows_under_the_smallest_scale_beside_ordinary_ones(cuda, rows, d, which):
+    """The first tokens' values (or keys) are under 2^-31 and share a tile with ordinary ones: rows that see them alone get them."""
+    hq, hk, page, l = 8, 2, 64, rows
+    g = torch.Generator().manual_seed(rows)
+    k, v = torch.randn(2, l, hk, d, generator=g)
+    (v if which == "values" else k)[:20] *= 2.0 ** -35
+    pool, table, kv = cache_of(k, v, page)
+    q = torch.randn(rows, hq * d, generator=g)
+    if which == "keys":
+        q *= 2.0 ** 36
+        q[20:] = 0
+    q = q.bfloat16().cuda()
+    ref, spread = attend64(q.cpu().view(rows, hq, d), kv, causal(rows, l), d ** -0.5)
+    for out in both_ways(q, pool, table, l, hq, hk, d, page):
+        close(out, ref, spread, WEIGHT["e4m3"])
