@@ -333,7 +333,7 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
   const int gpu = Same(q)(pool)(table)(lens)(cu_q)(masks)(out_).gpu;
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)gpu);
   const Tensor out = out_ ? *out_ : at::empty({rows, hq * d}, typed(q, at::kBFloat16));
-  if (!seqs || max_rows == 0) return out;
+  if (!seqs || !rows) return out;
   Host& h = host_of(gpu);
   const int64_t g = hq / hk;
   const auto map = pool_map(h, pool, e4m3, pages, hk, d, page);
@@ -341,7 +341,7 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
   const int64_t all = INT32_MAX, few = std::max<int64_t>(1, 8 / g);
   // one kernel over the sequences of lo .. hi rows
   auto run = [&](bool tiled, int64_t lo, int64_t hi) {
-    const int64_t most = std::min(max_rows, hi);
+    const int64_t most = std::max<int64_t>(1, std::min(max_rows, hi));       // (no rows, by the call's own word: the kernels see whether that is so)
     int64_t toks, cluster = 1, shares, gx, gy;
     unsigned shared;
     std::string name;
@@ -376,12 +376,12 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
     }
     Block b;
     b.bytes(map.data(), map.size()).at(q).at(out).put(ws_o).put(ws_ml).at(pool).at(table).at(lens).at(cu_q).at(masks);
-    b.ints(masks ? masks->size(1) : 0, rows_per_seq, hq, hk, q_step, out_step, width, page, tiled ? seqs : cluster, pages, lo, hi, rows);
+    b.ints(masks ? masks->size(1) : 0, rows_per_seq, hq, hk, q_step, out_step, width, page, tiled ? seqs : cluster, pages, lo, hi, rows, max_rows);
     b.put((float)(scale * kLog2e)).put(h.err);
     launch(h, tiled ? tile_module(d) : "attn_rows", name, gx, gy, shares, tiled ? (unsigned)tile_threads(d) : 160, b, shared, !tiled && hi < all, (unsigned)cluster);
     if (groups > 1) {
       Block m;
-      m.put(ws_o).put(ws_ml).at(out).at(lens).at(cu_q).ints(rows_per_seq, hq, toks, shares, cluster, out_step, lo, hi, rows);
+      m.put(ws_o).put(ws_ml).at(out).at(lens).at(cu_q).ints(rows_per_seq, hq, toks, shares, cluster, out_step, lo, hi, rows, max_rows);
       launch(h, "attn_rows", std::string("kern_attn_rows_merge_") + (masks ? "tree_d" : "causal_d") + n(d), most * hq, seqs, 1, 128, m, 0, true);
     }
   };

@@ -28,6 +28,7 @@ struct RowsArgs {
   int words, rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, cluster, pool_pages;
   int row_lo, row_hi;        // sequences of other row counts are another launch's
   int rows;                  // of q and out: a sequence's have to lie in them
+  int max_rows;              // the most rows of one sequence, by which blocks were counted
   float scale_log2;
 };
 
@@ -66,8 +67,8 @@ KERN_DEVICE uint32_t not_finite(uint32_t w) {
   return r;
 }
 
-// whether R rows from row0 on are rows of the call
-KERN_DEVICE bool rows_lie(int row0, int R, int rows) { return row0 >= 0 && R >= 0 && R <= rows - row0; }
+// whether R rows from row0 on are rows of the call, and no more than it has said
+KERN_DEVICE bool rows_lie(int row0, int R, int rows, int max_rows) { return row0 >= 0 && R >= 0 && R <= rows - row0 && R <= max_rows; }
 
 KERN_DEVICE float pow2i(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 

@@ -105,7 +105,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
   const int L = max(a.seq_lens[seq], 0);
   const int row0 = a.cu_q ? a.cu_q[seq] : seq * a.rows_per_seq;
   const int R = a.cu_q ? a.cu_q[seq + 1] - row0 : a.rows_per_seq;
-  if (!rows_lie(row0, R, a.rows)) {
+  if (!rows_lie(row0, R, a.rows, a.max_rows)) {
     if (threadIdx.x == 0) set_error(a.err, ERR_BOUNDS);
     return;                                                   // (uniform)
   }
@@ -594,10 +594,10 @@ using namespace kern;
       const __grid_constant__ CUtensorMap kv_map, const __nv_bfloat16* q, __nv_bfloat16* out, float* ws_o, float* ws_ml,          \
       const uint8_t* pool, const int* block_table, const int* seq_lens, const int* cu_q, const long long* masks, int words,       \
       int rows_per_seq, int hq, int hk, int q_stride, int out_stride, int max_pages, int page_size, int seqs, int pool_pages,     \
-      int row_lo, int row_hi, int rows, float scale_log2, int* err) {                                                             \
+      int row_lo, int row_hi, int rows, int max_rows, float scale_log2, int* err) {                                               \
     tile256_body<E4M3, TREE>(&kv_map, RowsArgs{q, out, ws_o, ws_ml, pool, block_table, seq_lens, cu_q, masks, err, words,         \
                                                rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, 1, pool_pages,   \
-                                               row_lo, row_hi, rows, scale_log2},                                                 \
+                                               row_lo, row_hi, rows, max_rows, scale_log2},                                       \
                              seqs);                                                                                               \
   }
 KERN_TILE256_ENTRY(e4m3, true, causal, false)

@@ -148,6 +148,10 @@ KERN_DEVICE void find_block(const RowsArgs& a, int seqs, int toks, int* scratch,
     const int s = ranked && s0 + lane < seqs ? order[s0 + lane] : s0 + lane;
     int rows = 0;
     if (s < seqs) rows = a.cu_q ? a.cu_q[s + 1] - a.cu_q[s] : a.rows_per_seq;
+    if (rows > a.max_rows) {                                  // (there may be no blocks for them)
+      set_error(a.err, ERR_BOUNDS);
+      rows = 0;
+    }
     int n = rows > 0 && rows >= a.row_lo && rows <= a.row_hi ? (rows + toks - 1) / toks : 0;
     const int own = n;
 #pragma unroll

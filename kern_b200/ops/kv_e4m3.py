@@ -63,7 +63,8 @@ def paged_attention_e4m3(q: torch.Tensor, pool: torch.Tensor, block_table: torch
     ``s * rows_per_seq`` onward, and row i of R sees tokens 0 .. seq_lens[s] - R + i. ``max_rows``: the most rows of one sequence
     (all of q's unless given), ``max_len``: the longest context, which sets how it is shared out (the table's width unless given).
     A row that sees nothing gives zeros; rows of ``out`` behind the last sequence's stay as they are. Pages
-    outside the pool, contexts longer than the table and rows outside ``q`` set the device's error word. Returns ``out[rows, hq * d]``."""
+    outside the pool, contexts longer than the table, rows outside ``q`` and sequences of more rows than ``max_rows`` (which are
+    left out) set the device's error word. Returns ``out[rows, hq * d]``."""
     return _ops_host.attend(q, pool, block_table, seq_lens, None, cu_q, hq, hk, d, page_size, out, rows_per_seq, max_rows, max_len, scale)
 
 

@@ -209,3 +209,38 @@ def test_rows_under_the_smallest_scale_beside_ordinary_ones(cuda, rows, d, which
     ref, spread = attend64(q.cpu().view(rows, hq, d), kv, causal(rows, l), d ** -0.5)
     for out in both_ways(q, pool, table, l, hq, hk, d, page):
         close(out, ref, spread, WEIGHT["e4m3"])
+
+
+def failed(f):
+    out = f()
+    with pytest.raises(RuntimeError, match="device error"):
+        Kernels.get(torch.device("cuda:0")).check_error()
+    return out
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("sizes,most", [([1, 3, 1], 1), ([2, 5], 3), ([30, 90], 60), ([1, 300, 1, 200], 250), ([300], 5), ([3, 40], 0)])
+def test_more_rows_than_max_rows(cuda, d, sizes, most):
+    """A sequence of more rows than the call says sets the error word and is left alone; the others are as ever."""
+    hq, hk, page, l = 8, 2, 64, 400
+    g = torch.Generator().manual_seed(most)
+    k, v = torch.randn(2, l, hk, d, generator=g)
+    pool, table, kv = cache_of(k, v, page)
+    n, cu = len(sizes), [0]
+    for r in sizes:
+        cu.append(cu[-1] + r)
+    table, lens = table.expand(n, -1).contiguous(), i32([l] * n)
+    q = torch.randn(cu[-1], hq * d, generator=g).bfloat16().cuda()
+    masks = torch.full((cu[-1], 1), -1, dtype=torch.int64, device=cuda)
+    calls = [lambda out: K8.paged_attention_e4m3(q, pool, table, lens, hq, hk, d, page, cu_q=i32(cu), max_rows=most, out=out),
+             lambda out: TR.tree_attention(q, pool, table, lens, masks, i32(cu), hq, hk, d, page, max_rows=most, out=out)]
+    for tree, call in enumerate(calls):
+        out = failed(lambda: call(torch.full((cu[-1], hq * d), 7.0, dtype=torch.bfloat16, device=cuda)))
+        for s, r in enumerate(sizes):
+            mine = out[cu[s]:cu[s + 1]]
+            if r > most:
+                assert bool((mine == 7).all())
+            elif not tree or r <= 64:
+                seen = torch.ones(r, l, dtype=torch.bool) if tree else causal(r, l)
+                ref, spread = attend64(q[cu[s]:cu[s + 1]].cpu().view(r, hq, d), kv, seen, d ** -0.5)
+                close(mine.view(r, hq, d), ref, spread, WEIGHT["e4m3"])
