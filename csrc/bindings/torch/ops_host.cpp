@@ -369,19 +369,20 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
     Tensor ws;
     uint64_t ws_o = 0, ws_ml = 0;
     const int64_t groups = shares / cluster;
+    const int64_t ws_step = seqs * most < rows ? most : 0, places = std::min(rows, seqs * most);
     if (groups > 1) {
-      ws = at::empty({rows * hq * groups * (d + 2)}, typed(q, at::kFloat));
+      ws = at::empty({places * hq * groups * (d + 2)}, typed(q, at::kFloat));
       ws_o = reinterpret_cast<uint64_t>(ws.data_ptr());
-      ws_ml = ws_o + 4 * (uint64_t)(rows * hq * groups * d);
+      ws_ml = ws_o + 4 * (uint64_t)(places * hq * groups * d);
     }
     Block b;
     b.bytes(map.data(), map.size()).at(q).at(out).put(ws_o).put(ws_ml).at(pool).at(table).at(lens).at(cu_q).at(masks);
-    b.ints(masks ? masks->size(1) : 0, rows_per_seq, hq, hk, q_step, out_step, width, page, tiled ? seqs : cluster, pages, lo, hi, rows, max_rows);
+    b.ints(masks ? masks->size(1) : 0, rows_per_seq, hq, hk, q_step, out_step, width, page, tiled ? seqs : cluster, pages, lo, hi, rows, max_rows, ws_step);
     b.put((float)(scale * kLog2e)).put(h.err);
     launch(h, tiled ? tile_module(d) : "attn_rows", name, gx, gy, shares, tiled ? (unsigned)tile_threads(d) : 160, b, shared, !tiled && hi < all, (unsigned)cluster);
     if (groups > 1) {
       Block m;
-      m.put(ws_o).put(ws_ml).at(out).at(lens).at(cu_q).ints(rows_per_seq, hq, toks, shares, cluster, out_step, lo, hi, rows, max_rows);
+      m.put(ws_o).put(ws_ml).at(out).at(lens).at(cu_q).ints(rows_per_seq, hq, toks, shares, cluster, out_step, lo, hi, rows, max_rows, ws_step);
       launch(h, "attn_rows", std::string("kern_attn_rows_merge_") + (masks ? "tree_d" : "causal_d") + n(d), most * hq, seqs, 1, 128, m, 0, true);
     }
   };

@@ -654,7 +654,7 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
                      pack_bf16x2(y[6] * inv, y[7] * inv));
     } else {
       const int groups = gridDim.z / a.cluster;
-      const size_t at = ((size_t)tk * a.hq + head) * groups + blockIdx.z / a.cluster;
+      const size_t at = (ws_row(a.ws_step, seq, row0, tok_lo + r / G) * a.hq + head) * groups + blockIdx.z / a.cluster;
       float4* dst = reinterpret_cast<float4*>(a.ws_o + at * D + col);
       dst[0] = make_float4(y[0], y[1], y[2], y[3]);
       dst[1] = make_float4(y[4], y[5], y[6], y[7]);
@@ -725,7 +725,7 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
 constexpr int kMergeThreads = 128;
 template <int D, bool TREE>
 KERN_DEVICE void rows_merge(const float* ws_o, const float* ws_ml, __nv_bfloat16* out, const int* seq_lens, const int* cu_q, int rows_per_seq,
-                            int hq, int toks, int splits, int cluster, int out_stride, int row_lo, int row_hi, int rows, int max_rows) {
+                            int hq, int toks, int splits, int cluster, int out_stride, int row_lo, int row_hi, int rows, int max_rows, int ws_step) {
   constexpr int N = D / 32;
   __shared__ float y_s[4][D], l_s[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.y;
@@ -735,7 +735,7 @@ KERN_DEVICE void rows_merge(const float* ws_o, const float* ws_ml, __nv_bfloat16
   const int end = TREE ? L : max(0, L - R + lo + min(toks, R - lo));
   const int shares = rows_shares(end, splits);
   const int groups = splits / cluster, live = (shares + cluster - 1) / cluster;
-  const size_t base = ((size_t)(row0 + tok) * hq + head) * groups;
+  const size_t base = (ws_row(ws_step, seq, row0, tok) * hq + head) * groups;
   pdl_wait();                                                 // (in every block: what follows this launch follows the one before it too)
   if (tok >= R || R < row_lo || R > row_hi || !rows_lie(row0, R, rows, max_rows)) return;
   if (shares <= cluster) return;                              // written by its one cluster
@@ -777,16 +777,16 @@ using namespace kern;
           const __grid_constant__ CUtensorMap kv_map, const __nv_bfloat16* q, __nv_bfloat16* out, float* ws_o, float* ws_ml,      \
           const uint8_t* pool, const int* block_table, const int* seq_lens, const int* cu_q, const long long* masks, int words,   \
           int rows_per_seq, int hq, int hk, int q_stride, int out_stride, int max_pages, int page_size, int cluster,              \
-          int pool_pages, int row_lo, int row_hi, int rows, int max_rows, float scale_log2, int* err) {                           \
+          int pool_pages, int row_lo, int row_hi, int rows, int max_rows, int ws_step, float scale_log2, int* err) {                           \
     rows_body<D, E4M3, TREE, NT>(&kv_map, RowsArgs{q, out, ws_o, ws_ml, pool, block_table, seq_lens, cu_q, masks, err, words,     \
                                                    rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, cluster,     \
-                                                   pool_pages, row_lo, row_hi, rows, max_rows, scale_log2});                      \
+                                                   pool_pages, row_lo, row_hi, rows, max_rows, ws_step, scale_log2});                      \
   }
 #define KERN_ROWS_MERGE(D, FORM, TREE)                                                                                            \
   extern "C" __global__ void __launch_bounds__(kMergeThreads) kern_attn_rows_merge_##FORM##_d##D(                                           \
       const float* ws_o, const float* ws_ml, __nv_bfloat16* out, const int* seq_lens, const int* cu_q, int rows_per_seq, int hq,  \
-      int toks, int splits, int cluster, int out_stride, int row_lo, int row_hi, int rows, int max_rows) {                        \
-    rows_merge<D, TREE>(ws_o, ws_ml, out, seq_lens, cu_q, rows_per_seq, hq, toks, splits, cluster, out_stride, row_lo, row_hi, rows, max_rows); \
+      int toks, int splits, int cluster, int out_stride, int row_lo, int row_hi, int rows, int max_rows, int ws_step) {                        \
+    rows_merge<D, TREE>(ws_o, ws_ml, out, seq_lens, cu_q, rows_per_seq, hq, toks, splits, cluster, out_stride, row_lo, row_hi, rows, max_rows, ws_step); \
   }
 #define KERN_ROWS_FORMS(D, NT)                      \
   KERN_ROWS_ENTRY(D, e4m3, true, causal, false, NT) \

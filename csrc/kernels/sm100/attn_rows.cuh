@@ -17,8 +17,8 @@ constexpr int kLeastScale = 87;
 struct RowsArgs {
   const __nv_bfloat16* q;
   __nv_bfloat16* out;
-  float* ws_o;               // partials [row][head][groups][D] (one group: none)
-  float* ws_ml;              // [row][head][groups][2]
+  float* ws_o;               // partials [place][head][groups][D] (one group: none)
+  float* ws_ml;              // [place][head][groups][2]
   const uint8_t* pool;       // (8-bit) scale bytes are read from here
   const int* block_table;
   const int* seq_lens;
@@ -29,6 +29,7 @@ struct RowsArgs {
   int row_lo, row_hi;        // sequences of other row counts are another launch's
   int rows;                  // of q and out: a sequence's have to lie in them
   int max_rows;              // the most rows of one sequence, by which blocks were counted
+  int ws_step;               // places of partials to a sequence; 0: they lie as the rows of q
   float scale_log2;
 };
 
@@ -69,6 +70,9 @@ KERN_DEVICE uint32_t not_finite(uint32_t w) {
 
 // whether R rows from row0 on are rows of the call, and no more than it has said
 KERN_DEVICE bool rows_lie(int row0, int R, int rows, int max_rows) { return row0 >= 0 && R >= 0 && R <= rows - row0 && R <= max_rows; }
+
+// where the partials of a sequence's row `tok` lie: q may have many rows that are nobody's in this call
+KERN_DEVICE size_t ws_row(int ws_step, int seq, int row0, int tok) { return ws_step ? (size_t)seq * ws_step + tok : (size_t)(row0 + tok); }
 
 KERN_DEVICE float pow2i(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 

@@ -528,7 +528,7 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const float level = E4M3 && !whole ? level_share(ref, l) : 1.f;
       const int head = kvh * G + (row < valid ? row % G : 0);
-      const size_t at = ((size_t)(row0 + tk) * a.hq + head) * gridDim.z + blockIdx.z;
+      const size_t at = (ws_row(a.ws_step, seq, row0, tk) * a.hq + head) * gridDim.z + blockIdx.z;
 #pragma unroll 1
       for (int c = 0; c < D / 2; c += 32) {
         const int col = part * (D / 2) + c;
@@ -594,10 +594,10 @@ using namespace kern;
       const __grid_constant__ CUtensorMap kv_map, const __nv_bfloat16* q, __nv_bfloat16* out, float* ws_o, float* ws_ml,          \
       const uint8_t* pool, const int* block_table, const int* seq_lens, const int* cu_q, const long long* masks, int words,       \
       int rows_per_seq, int hq, int hk, int q_stride, int out_stride, int max_pages, int page_size, int seqs, int pool_pages,     \
-      int row_lo, int row_hi, int rows, int max_rows, float scale_log2, int* err) {                                               \
+      int row_lo, int row_hi, int rows, int max_rows, int ws_step, float scale_log2, int* err) {                                               \
     tile256_body<E4M3, TREE>(&kv_map, RowsArgs{q, out, ws_o, ws_ml, pool, block_table, seq_lens, cu_q, masks, err, words,         \
                                                rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page_size, 1, pool_pages,   \
-                                               row_lo, row_hi, rows, max_rows, scale_log2},                                       \
+                                               row_lo, row_hi, rows, max_rows, ws_step, scale_log2},                                       \
                              seqs);                                                                                               \
   }
 KERN_TILE256_ENTRY(e4m3, true, causal, false)

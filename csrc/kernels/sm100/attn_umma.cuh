@@ -278,7 +278,7 @@ __device__ __noinline__ void tile_wide(const RowsArgs& a, int seq, int row0, int
       for (int i = 0; i < kCols; i += 2)
         *reinterpret_cast<uint32_t*>(a.out + (size_t)(row0 + tk) * a.out_stride + (size_t)head * D + lane * kCols + i) = pack_bf16x2(o[i] * inv, o[i + 1] * inv);
     } else {
-      const size_t at = ((size_t)(row0 + tk) * a.hq + head) * gridDim.z + blockIdx.z;
+      const size_t at = (ws_row(a.ws_step, seq, row0, tk) * a.hq + head) * gridDim.z + blockIdx.z;
 #pragma unroll
       for (int i = 0; i < kCols; ++i) a.ws_o[at * D + lane * kCols + i] = o[i];
       if (lane == 0) {

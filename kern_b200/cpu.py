@@ -505,7 +505,7 @@ def _rope_append_e4m3(d: int, interleaved: bool):
 
 
 def _attention_e4m3(g, m, q, out, ws_o, ws_ml, kv, table, seq_lens, cu_q, masks, words, rows_per_seq, hq, hk, q_stride, out_stride, max_pages, page,
-                    last, pool_pages, row_lo, row_hi, rows, max_rows, scale_log2, err):
+                    last, pool_pages, row_lo, row_hi, rows, max_rows, ws_step, scale_log2, err):
     from .ops.kv_e4m3 import dequantise_reference
 
     d, grp = m._head_dim, hq // hk

@@ -633,11 +633,11 @@ def _e4m3_map(hk: int, d: int, page_size: int, state_param: int) -> dict:
 def _e4m3_attend(entry: str, grid: list, threads: int, smem: int, cluster: int, hq: int, hk: int, d: int, page_size: int, table_width: int,
                  q_stride: int, last: dict, lo: int, hi: int, cu: int | None, err: int, when: dict | None) -> dict:
     ptr = ["in buffer<bf16>", "out buffer<bf16>", "i64", "i64", "in state", "in buffer<i32>", "in buffer<i32>", "in buffer<i32>" if cu is not None else "i64", "i64"]
-    lp = ["bytes<128>"] + ptr + ["i32"] * 14 + ["f32", "out buffer<i32>"]
+    lp = ["bytes<128>"] + ptr + ["i32"] * 15 + ["f32", "out buffer<i32>"]
     args = [_e4m3_map(hk, d, page_size, 1), {"param": 0}, {"param": 2}, {"i64": 0}, {"i64": 0}, {"param": 1}, {"param": 3}, {"param": 4},
             {"i64": 0} if cu is None else {"param": cu}, {"i64": 0}, {"i32": 0}, {"i32": 1}, {"i32": hq}, {"i32": hk}, {"i32": q_stride},
             {"i32": hq * d}, {"i32": table_width}, {"i32": page_size}, last, {"i32": I32_MAX}, {"i32": lo}, {"i32": hi}, {"i32": I32_MAX}, {"i32": I32_MAX},
-            {"f32": (d ** -0.5) * 1.4426950408889634}, {"param": err}]
+            {"i32": 0}, {"f32": (d ** -0.5) * 1.4426950408889634}, {"param": err}]
     out = {"module": "attn_rows" if "rows" in entry else "attn_tile", "entry": entry, "block": [threads, 1, 1], "grid": grid, "shared_mem": smem,
            "params": lp, "args": args}
     if cluster > 1:

@@ -244,3 +244,41 @@ def test_more_rows_than_max_rows(cuda, d, sizes, most):
                 seen = torch.ones(r, l, dtype=torch.bool) if tree else causal(r, l)
                 ref, spread = attend64(q[cu[s]:cu[s + 1]].cpu().view(r, hq, d), kv, seen, d ** -0.5)
                 close(mine.view(r, hq, d), ref, spread, WEIGHT["e4m3"])
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_the_workspace_is_of_the_rows_in_use(cuda, rows):
+    """A few rows at the end of a buffer of 8192, over a long context in many shares."""
+    hq, hk, d, page, l, all_rows = 32, 8, 128, 64, 30000, 8192
+    g = torch.Generator().manual_seed(0)
+    k, v = torch.randn(2, l, hk, d, generator=g)
+    pool, table, kv = cache_of(k, v, page)
+    q = torch.randn(all_rows, hq * d, generator=g).bfloat16().cuda()
+    out = torch.zeros_like(q)
+    cu, lens = i32([all_rows - rows, all_rows]), i32([l])
+    call = lambda: K8.paged_attention_e4m3(q, pool, table, lens, hq, hk, d, page, cu_q=cu, max_rows=rows, out=out)
+    call()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    call()
+    # 256 shares at most, of d + 2 floats for every head of the rows in use
+    assert torch.cuda.max_memory_allocated() - before <= rows * hq * 256 * (d + 2) * 4 + 4096
+    ref, spread = attend64(q[-rows:].cpu().view(rows, hq, d), kv, causal(rows, l), d ** -0.5)
+    close(out[-rows:].view(rows, hq, d), ref, spread, WEIGHT["e4m3"])
+    assert bool((out[:-rows] == 0).all())
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_partials_of_some_rows_of_a_wide_buffer(cuda, rows):
+    """Three sequences, one of no rows, whose rows are some of q's: each joins its own shares."""
+    hq, hk, d, page, l = 8, 2, 128, 64, 9000
+    g = torch.Generator().manual_seed(rows)
+    k, v = torch.randn(2, l, hk, d, generator=g)
+    pool, table, kv = cache_of(k, v, page)
+    lens, cu = [l, 50, l - 777], [5, 5 + rows, 5 + rows, 5 + 2 * rows]
+    q = torch.randn(1000, hq * d, generator=g).bfloat16().cuda()
+    out = K8.paged_attention_e4m3(q, pool, table.expand(3, -1).contiguous(), i32(lens), hq, hk, d, page, cu_q=i32(cu), max_rows=rows)
+    for s in (0, 2):
+        ref, spread = attend64(q[cu[s]:cu[s + 1]].cpu().view(rows, hq, d), kv[:, :lens[s]], causal(rows, lens[s]), d ** -0.5)
+        close(out[cu[s]:cu[s + 1]].view(rows, hq, d), ref, spread, WEIGHT["e4m3"])
