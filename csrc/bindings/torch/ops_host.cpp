@@ -326,6 +326,7 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
     if (m < rows) refuse("out has a row for each of q's");
     out_step = s;
   }
+  if (width * page > INT32_MAX - 256) refuse("a table of " + n(width) + " pages: contexts past 32 bits");
   const int64_t max_len = max_len_.value_or(width * page);
   if (max_len < 0) refuse("max_len " + n(max_len));
   const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)d);
@@ -382,7 +383,7 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
     launch(h, tiled ? tile_module(d) : "attn_rows", name, gx, gy, shares, tiled ? (unsigned)tile_threads(d) : 160, b, shared, !tiled && hi < all, (unsigned)cluster);
     if (groups > 1) {
       Block m;
-      m.put(ws_o).put(ws_ml).at(out).at(lens).at(cu_q).ints(rows_per_seq, hq, toks, shares, cluster, out_step, lo, hi, rows, max_rows, ws_step);
+      m.put(ws_o).put(ws_ml).at(out).at(lens).at(cu_q).ints(rows_per_seq, hq, toks, shares, cluster, out_step, lo, hi, rows, max_rows, ws_step, width * page);
       launch(h, "attn_rows", std::string("kern_attn_rows_merge_") + (masks ? "tree_d" : "causal_d") + n(d), most * hq, seqs, 1, 128, m, 0, true);
     }
   };

@@ -173,7 +173,7 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
     __syncthreads();
   }
 
-  const int L = max(a.seq_lens[seq], 0);
+  const int L = context_of(a, seq);
   const int row0 = a.cu_q ? a.cu_q[seq] : seq * a.rows_per_seq;
   const int R = a.cu_q ? a.cu_q[seq + 1] - row0 : a.rows_per_seq;
   const int toks = kRows / G;
@@ -725,13 +725,13 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
 constexpr int kMergeThreads = 128;
 template <int D, bool TREE>
 KERN_DEVICE void rows_merge(const float* ws_o, const float* ws_ml, __nv_bfloat16* out, const int* seq_lens, const int* cu_q, int rows_per_seq,
-                            int hq, int toks, int splits, int cluster, int out_stride, int row_lo, int row_hi, int rows, int max_rows, int ws_step) {
+                            int hq, int toks, int splits, int cluster, int out_stride, int row_lo, int row_hi, int rows, int max_rows, int ws_step, int capacity) {
   constexpr int N = D / 32;
   __shared__ float y_s[4][D], l_s[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.y;
   const int row0 = cu_q ? cu_q[seq] : seq * rows_per_seq, R = cu_q ? cu_q[seq + 1] - row0 : rows_per_seq;
   const int tok = blockIdx.x / hq, head = blockIdx.x % hq;
-  const int L = max(seq_lens[seq], 0), lo = tok / toks * toks;
+  const int L = within(seq_lens[seq], capacity), lo = tok / toks * toks;
   const int end = TREE ? L : max(0, L - R + lo + min(toks, R - lo));
   const int shares = rows_shares(end, splits);
   const int groups = splits / cluster, live = (shares + cluster - 1) / cluster;
@@ -785,8 +785,8 @@ using namespace kern;
 #define KERN_ROWS_MERGE(D, FORM, TREE)                                                                                            \
   extern "C" __global__ void __launch_bounds__(kMergeThreads) kern_attn_rows_merge_##FORM##_d##D(                                           \
       const float* ws_o, const float* ws_ml, __nv_bfloat16* out, const int* seq_lens, const int* cu_q, int rows_per_seq, int hq,  \
-      int toks, int splits, int cluster, int out_stride, int row_lo, int row_hi, int rows, int max_rows, int ws_step) {                        \
-    rows_merge<D, TREE>(ws_o, ws_ml, out, seq_lens, cu_q, rows_per_seq, hq, toks, splits, cluster, out_stride, row_lo, row_hi, rows, max_rows, ws_step); \
+      int toks, int splits, int cluster, int out_stride, int row_lo, int row_hi, int rows, int max_rows, int ws_step, int capacity) { \
+    rows_merge<D, TREE>(ws_o, ws_ml, out, seq_lens, cu_q, rows_per_seq, hq, toks, splits, cluster, out_stride, row_lo, row_hi, rows, max_rows, ws_step, capacity); \
   }
 #define KERN_ROWS_FORMS(D, NT)                      \
   KERN_ROWS_ENTRY(D, e4m3, true, causal, false, NT) \

@@ -68,6 +68,15 @@ KERN_DEVICE uint32_t not_finite(uint32_t w) {
   return r;
 }
 
+// A sequence's tokens: no more than its row of the table has pages for, or a length that is not one would be walked to its end, seconds
+// of it. (capacity: below 2^31 - 256, so that lengths can be rounded up)
+KERN_DEVICE int within(int len, int capacity) { return min(max(len, 0), capacity); }
+KERN_DEVICE int context_of(const RowsArgs& a, int seq) {
+  const int len = a.seq_lens[seq], capacity = a.max_pages * a.page_size;
+  if (len > capacity) set_error(a.err, ERR_BOUNDS);
+  return within(len, capacity);
+}
+
 // whether R rows from row0 on are rows of the call, and no more than it has said
 KERN_DEVICE bool rows_lie(int row0, int R, int rows, int max_rows) { return row0 >= 0 && R >= 0 && R <= rows - row0 && R <= max_rows; }
 

@@ -116,7 +116,7 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
   __syncthreads();
   const int seq = found[0], blk = found[1];
   if (seq < 0) return;                                        // past the last block: uniform, before any allocation
-  const int L = max(a.seq_lens[seq], 0);
+  const int L = context_of(a, seq);
   const int row0 = a.cu_q ? a.cu_q[seq] : seq * a.rows_per_seq;
   const int R = a.cu_q ? a.cu_q[seq + 1] - row0 : a.rows_per_seq;
   if (!rows_lie(row0, R, a.rows, a.max_rows)) {

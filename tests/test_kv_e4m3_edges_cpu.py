@@ -13,3 +13,12 @@ def test_the_largest_bf16_values_keep_their_sign_and_size():
     back = K8.dequantise_reference(codes, scales)[0]
     end = 448 * 2.0 ** 119
     assert scales.tolist() == [246] and back[:4].tolist() == [end, -end, end, 0.0]
+
+
+def test_a_table_whose_contexts_pass_32_bits_is_refused():
+    hq, hk, d, page = 4, 2, 64, 1 << 20
+    pool = torch.zeros(1, K8.page_bytes(hk, page, d), dtype=torch.uint8)
+    q, lens = torch.zeros(1, hq * d, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32)
+    for pages, why in ((2048, "32 bits"), (2047, "CUDA device")):
+        with pytest.raises(ValueError, match=why):
+            K8.paged_attention_e4m3(q, pool, torch.zeros(1, pages, dtype=torch.int32), lens, hq, hk, d, page)

@@ -282,3 +282,23 @@ def test_partials_of_some_rows_of_a_wide_buffer(cuda, rows):
     for s in (0, 2):
         ref, spread = attend64(q[cu[s]:cu[s + 1]].cpu().view(rows, hq, d), kv[:, :lens[s]], causal(rows, lens[s]), d ** -0.5)
         close(out[cu[s]:cu[s + 1]].view(rows, hq, d), ref, spread, WEIGHT["e4m3"])
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_lengths_past_the_table(cuda, d, rows):
+    """A length that the table has no pages for, up to the largest number there is: the error word, and no walk to its end."""
+    hq, hk, page, l = 8, 2, 64, 400
+    g = torch.Generator().manual_seed(rows)
+    k, v = torch.randn(2, l, hk, d, generator=g)
+    pool, table, kv = cache_of(k, v, page)
+    table = table.expand(2, -1).contiguous()
+    q = torch.randn(2 * rows, hq * d, generator=g).bfloat16().cuda()
+    masks, cu = torch.ones(2 * rows, 1, dtype=torch.int64, device=cuda), i32([0, rows, 2 * rows])
+    ref, spread = attend64(q[rows:].cpu().view(rows, hq, d), kv, causal(rows, l), d ** -0.5)
+    for far in (l + 49, 1 << 20, (1 << 31) - 100, (1 << 31) - 1):
+        lens = i32([far, l])
+        for max_len in (None, 9000):                      # (in one share, and in several that are joined)
+            out = failed(lambda: K8.paged_attention_e4m3(q, pool, table, lens, hq, hk, d, page, rows_per_seq=rows, max_len=max_len))
+            close(out[rows:].view(rows, hq, d), ref, spread, WEIGHT["e4m3"])
+            failed(lambda: TR.tree_attention(q, pool, table, lens, masks, cu, hq, hk, d, page, max_rows=rows, max_len=max_len))
