@@ -26,6 +26,16 @@ struct PoolTable {
   unsigned long long at[kMaxPools];
 };
 
+// The rows of a sequence, cu[s] to cu[s + 1] - 1; `lie`: whether they are rows of the call. If not, the bounds cut to the call's.
+struct Span {
+  int from, to;
+  bool lie;
+};
+KERN_DEVICE Span span_of(const int* cu, int s, int nodes) {
+  const int from = cu[s], to = cu[s + 1];
+  return {min(max(from, 0), nodes), min(max(to, 0), nodes), from >= 0 && to >= from && to <= nodes};
+}
+
 // the cache slot of a sequence's token place, or -1
 KERN_DEVICE long long place_slot(long long place, const int* pages, int max_pages, int page_size) {
   const long long pi = place / page_size;
@@ -34,8 +44,8 @@ KERN_DEVICE long long place_slot(long long place, const int* pages, int max_page
 
 }  // namespace kern
 
-// grid seqs, block 256. Nodes that no tree holds (of padding sequences, behind the last sequence, over the limit) get position 0,
-// slot -1 and no mask.
+// grid seqs, block 256. Nodes that no tree holds (of padding sequences, before the first sequence and behind the last, over the limit,
+// between bounds that are none) get position 0, slot -1 and no mask.
 extern "C" __global__ void __launch_bounds__(256)
     kern_tree_rows(const int* parents, const int* cu, const long long* base, const int* block_table, long long* positions, long long* slots,
                    int* seq_lens, long long* masks, int nodes, int words, int max_pages, int page_size, int* err) {
@@ -43,11 +53,9 @@ extern "C" __global__ void __launch_bounds__(256)
   __shared__ int jump_s[kMaxNodes], depth_s[kMaxNodes];
   pdl_wait();
   const int s = blockIdx.x, i = threadIdx.x;
-  int row0 = cu[s], all = cu[s + 1] - row0;
-  if (row0 < 0 || all < 0 || all > nodes - row0) {
-    if (i == 0) set_error(err, ERR_BOUNDS);
-    row0 = all = 0;
-  }
+  const Span mine = span_of(cu, s, nodes);
+  const int row0 = mine.from, all = mine.lie ? mine.to - mine.from : 0;
+  if (!mine.lie && i == 0) set_error(err, ERR_BOUNDS);
   const long long b = base[s];
   const int n = b < 0 ? 0 : min(min(all, kMaxNodes), words * 64);
   auto none = [&](int from, int to) {
@@ -61,8 +69,9 @@ extern "C" __global__ void __launch_bounds__(256)
     if (b >= 0 && all > n) set_error(err, ERR_BOUNDS);
     seq_lens[s] = b < 0 ? 0 : (int)(b + all);
   }
-  none(row0 + n, row0 + all);
-  if (s == (int)gridDim.x - 1) none(max(cu[s + 1], 0), nodes);
+  none(row0 + n, mine.to);
+  if (s == 0) none(0, row0);
+  if (s == (int)gridDim.x - 1) none(mine.to, nodes);
   if (n == 0) return;
   int jump = -1, depth = 0;
   unsigned long long m[4] = {0, 0, 0, 0};
@@ -115,11 +124,9 @@ extern "C" __global__ void __launch_bounds__(128)
   __shared__ int len_s;
   pdl_wait();
   const int s = blockIdx.x, t = threadIdx.x;
-  int row0 = cu[s], all = cu[s + 1] - row0;
-  if (row0 < 0 || all < 0 || all > nodes - row0) {
-    if (t == 0) set_error(err, ERR_BOUNDS);
-    row0 = all = 0;
-  }
+  const Span mine = span_of(cu, s, nodes);
+  const int row0 = mine.from, all = mine.lie ? mine.to - mine.from : 0;
+  if (!mine.lie && t == 0) set_error(err, ERR_BOUNDS);
   const int n = min(all, kMaxNodes);
   const long long b = base[s];
   if (t < 32) {
@@ -158,11 +165,15 @@ extern "C" __global__ void __launch_bounds__(128)
       path[row0 + i] = i < len ? path_s[i] : -1;
       emitted[row0 + i] = i < len ? verify[row0 + path_s[i]] : 0;
     }
-    if (s == (int)gridDim.x - 1)                  // behind the last sequence
-      for (int i = max(cu[s + 1], 0) + t; i < nodes; i += blockDim.x) {
+    auto none = [&](int from, int to) {
+      for (int i = from + t; i < to; i += blockDim.x) {
         path[i] = -1;
         emitted[i] = 0;
       }
+    };
+    none(row0 + all, mine.to);
+    if (s == 0) none(0, row0);
+    if (s == (int)gridDim.x - 1) none(mine.to, nodes);
   }
   if ((int)blockIdx.y >= layers) return;
   const int* pages = block_table + (size_t)s * max_pages;

@@ -37,7 +37,8 @@ def tree_rows(parents: torch.Tensor, cu: torch.Tensor, base: torch.Tensor, block
 
     ``parents`` (i32): a node's parent within its sequence, -1 for the anchor. A parent that is not an earlier node, a place past
     the page table, or more than ``max_rows`` (256) nodes set the error word: the node then has no parent, or slot -1 (nothing
-    written), or is left out. A sequence of base < 0 is padding: slots -1, positions 0, masks 0, context 0."""
+    written), or is left out. So do bounds in ``cu`` that are none. A sequence of base < 0 is padding: slots -1, positions 0, masks 0,
+    context 0; so are nodes before the first sequence and behind the last."""
     return _ops_host.tree_rows(parents, cu, base, block_table, page_size, max_rows)
 
 

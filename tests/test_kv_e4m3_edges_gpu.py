@@ -302,3 +302,25 @@ def test_lengths_past_the_table(cuda, d, rows):
             out = failed(lambda: K8.paged_attention_e4m3(q, pool, table, lens, hq, hk, d, page, rows_per_seq=rows, max_len=max_len))
             close(out[rows:].view(rows, hq, d), ref, spread, WEIGHT["e4m3"])
             failed(lambda: TR.tree_attention(q, pool, table, lens, masks, cu, hq, hk, d, page, max_rows=rows, max_len=max_len))
+
+
+def test_nodes_that_no_tree_holds(cuda):
+    """Rows before the first tree, and those of a tree whose bounds are wrong: no slot, no mask, no step of a walk."""
+    page = 16
+    table = torch.arange(4, dtype=torch.int32, device=cuda)[None].contiguous()
+    par = i32([-1, 0, 0, -1, 0, 1, 0])
+    ids = torch.zeros(7, dtype=torch.int64, device=cuda)
+    for cu, bad, live in (([2, 5], False, range(2, 5)), ([1, 9], True, ()), ([-3, 4], True, ()), ([4, 2], True, ())):
+        for _ in range(3):                                # (places that something else has used before)
+            junk = [torch.full((7,), 5, dtype=torch.int64, device=cuda) for _ in range(8)]
+            del junk
+            base = torch.tensor([3], device=cuda)
+            flat = i32([0, 0, -1, 0, 1, 0, 0]) if live else par
+            call = lambda: TR.tree_rows(flat, i32(cu), base, table, page)
+            pos, slots, lens, masks = failed(call) if bad else call()
+            walk = lambda: TR.tree_keep(ids, flat, ids, i32(cu), base, table, [], 2, 64, page)
+            count, path, emitted = failed(walk) if bad else walk()
+            rest = [i for i in range(7) if i not in live]
+            assert all(int(slots[i]) == -1 and int(pos[i]) == 0 and int(masks[i]) == 0 for i in rest)
+            assert all(int(path[i]) == -1 and int(emitted[i]) == 0 for i in rest)
+            assert all(int(slots[i]) == 3 + i - 2 for i in live) and int(count[0]) == (3 if live else 0)
