@@ -22,6 +22,7 @@ using namespace kern;
 namespace kern {
 
 constexpr int kMaxNodes = 256, kMaxPools = 128;
+constexpr long long kFar = 1ll << 62;                       // a place that no table holds, and that its nodes can be added to
 struct PoolTable {
   unsigned long long at[kMaxPools];
 };
@@ -56,7 +57,7 @@ extern "C" __global__ void __launch_bounds__(256)
   const Span mine = span_of(cu, s, nodes);
   const int row0 = mine.from, all = mine.lie ? mine.to - mine.from : 0;
   if (!mine.lie && i == 0) set_error(err, ERR_BOUNDS);
-  const long long b = base[s];
+  const long long b = min(base[s], kFar);
   const int n = b < 0 ? 0 : min(min(all, kMaxNodes), words * 64);
   auto none = [&](int from, int to) {
     for (int x = from + i; x < to; x += blockDim.x) {
@@ -67,7 +68,7 @@ extern "C" __global__ void __launch_bounds__(256)
   };
   if (i == 0) {
     if (b >= 0 && all > n) set_error(err, ERR_BOUNDS);
-    seq_lens[s] = b < 0 ? 0 : (int)(b + all);
+    seq_lens[s] = b < 0 ? 0 : (int)min(b + all, (long long)INT_MAX);
   }
   none(row0 + n, mine.to);
   if (s == 0) none(0, row0);
@@ -128,7 +129,7 @@ extern "C" __global__ void __launch_bounds__(128)
   const int row0 = mine.from, all = mine.lie ? mine.to - mine.from : 0;
   if (!mine.lie && t == 0) set_error(err, ERR_BOUNDS);
   const int n = min(all, kMaxNodes);
-  const long long b = base[s];
+  const long long b = min(base[s], kFar);
   if (t < 32) {
     // lane holds nodes t, t + 32, ..: the edge into each, and whether the model agrees with it
     int par[8];

@@ -324,3 +324,11 @@ def test_nodes_that_no_tree_holds(cuda):
             assert all(int(slots[i]) == -1 and int(pos[i]) == 0 and int(masks[i]) == 0 for i in rest)
             assert all(int(path[i]) == -1 and int(emitted[i]) == 0 for i in rest)
             assert all(int(slots[i]) == 3 + i - 2 for i in live) and int(count[0]) == (3 if live else 0)
+
+
+def test_places_past_32_bits(cuda):
+    """A base near the largest number: no slot, and a context that no table holds, not one of some other length."""
+    table = torch.arange(4, dtype=torch.int32, device=cuda)[None].contiguous()
+    for base in ((1 << 32) + 3, 1 << 62, (1 << 63) - 1):
+        _, slots, lens, _ = failed(lambda: TR.tree_rows(i32([-1, 0]), i32([0, 2]), torch.tensor([base], device=cuda), table, 16))
+        assert slots.tolist() == [-1, -1] and lens.tolist() == [(1 << 31) - 1]
