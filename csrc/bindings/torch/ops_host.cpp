@@ -466,6 +466,7 @@ py::tuple tree_keep(const Tensor& ids, const Tensor& parents, const Tensor& veri
 
 PYBIND11_MODULE(_ops_host, m) {
   m.doc() = "Host side of the operators over 8-bit caches and drafted trees";
+  m.attr("torch_version") = KERN_TORCH_VERSION;              // that it was built for
   m.def("on_missing", [](py::object f) { missing() = std::move(f); });
   m.def("provide", [](int gpu, int sms, uint64_t err, py::object resolve) {
     auto h = std::make_unique<Host>();

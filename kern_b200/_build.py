@@ -19,6 +19,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -166,20 +167,51 @@ def ops_host_path() -> Path:
     return PKG / ("_ops_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
-def build_ops_host(force: bool = False) -> Path:
+def _torch_here() -> tuple[str, bool]:
+    """The version of this environment's PyTorch, and whether it is built with CUDA, without importing it ("" if there is none)."""
+    import importlib.metadata
+    import importlib.util
+
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        return "", False
+    return importlib.metadata.version("torch"), (Path(spec.submodule_search_locations[0]) / "lib" / "libc10_cuda.so").exists()
+
+
+def build_ops_host(force: bool = False, needed: bool = True) -> Path | None:
     """Compile the host side of the short operators (``csrc/bindings/torch``) into ``kern_b200/_ops_host*.so``, against the
-    PyTorch of this environment."""
+    PyTorch of this environment, and again when that changes. None beside a PyTorch without CUDA, which has no use for it. Not
+    `needed` (an import of the package, most of which does without): a build that fails is a warning, once for the same sources."""
     out, src = ops_host_path(), CSRC / "bindings" / "torch" / "ops_host.cpp"
-    if not force and not _newer([src, *(CSRC / "runtime").glob("*.hpp")], out):
+    stamp = BUILD / "ops_host.torch"                    # the PyTorch that it was last built for
+    stale = _newer([src, *(CSRC / "runtime").glob("*.hpp")], stamp)
+    version, cuda = _torch_here()
+    if not cuda:
+        return None
+    last = stamp.read_text() if stamp.exists() else ""
+    if not force and not stale and (last == version and out.exists() or not needed and last == version + " failed"):
         return out
+    try:
+        _compile_ops_host(src, out)
+    except RuntimeError as e:
+        stamp.write_text(version + " failed")
+        if needed:
+            raise
+        warnings.warn(f"kern_b200: no operators over 8-bit caches and drafted trees: {e}")
+        return None
+    stamp.write_text(version)
+    return out
+
+
+def _compile_ops_host(src: Path, out: Path) -> None:
     import torch
     from torch.utils import cpp_extension
 
     inc = [a for p in (*cpp_extension.include_paths(), sysconfig.get_paths()["include"], "/usr/local/cuda/include", str(CSRC)) for a in ("-isystem" if p != str(CSRC) else "-I", p)]
     libs = [a for p in cpp_extension.library_paths() for a in ("-L", p)]
     _run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-          "-DTORCH_EXTENSION_NAME=_ops_host", *inc, "-o", str(out), str(src), *libs, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-ldl"])
-    return out
+          "-DTORCH_EXTENSION_NAME=_ops_host", f'-DKERN_TORCH_VERSION="{torch.__version__}"', *inc, "-o", str(out), str(src), *libs,
+          "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-ldl"])
 
 
 def build_cli(force: bool = False) -> Path:
@@ -231,7 +263,7 @@ def build_host_libs(force: bool = False) -> list[Path]:
     return outs
 
 
-def build_all(force: bool = False, verbose: bool = False) -> None:
+def build_all(force: bool = False, verbose: bool = False, importing: bool = False) -> None:
     BUILD.mkdir(exist_ok=True)
     with open(BUILD / ".lock", "w") as lock:
         fcntl.flock(lock, fcntl.LOCK_EX)
@@ -240,7 +272,7 @@ def build_all(force: bool = False, verbose: bool = False) -> None:
             if checked() or "--checked" in sys.argv:
                 build_kernels(force, verbose, checked_build=True)
             build_native(force)
-            build_ops_host(force)
+            build_ops_host(force, needed=not importing)
             build_cli(force)
             build_runner(force)
             build_capture(force)
@@ -274,9 +306,9 @@ def ensure_built() -> None:
     """Build whatever is missing or stale. Cheap when everything is current."""
     try:
         if on_demand():
-            _locked(lambda: (build_native(), build_ops_host()))
+            _locked(lambda: (build_native(), build_ops_host(needed=False)))
             return
-        build_all(False)
+        build_all(False, importing=True)
     except FileNotFoundError as e:  # no compiler on this machine: use what is in the tree
         if not native_path().exists():
             raise RuntimeError(f"native core is not built and no toolchain was found: {e}")

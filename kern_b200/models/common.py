@@ -650,12 +650,12 @@ def _e4m3_attend(entry: str, grid: list, threads: int, smem: int, cluster: int, 
 def _e4m3_few(hq: int, hk: int, d: int, page_size: int, table_width: int, q_stride: int, seqs_max: int, rows: int, hi: int, cu: int | None, err: int,
               sms: int = SMS) -> list[dict]:
     """Launches of the few-row kernel over sequences of up to `rows` rows: the shares of a context, one cluster, by `when` ranges of the batch."""
-    from .. import _ops_host
+    from ..ops import host
 
     g = hq // hk
     nt = 1 if g * rows <= 8 else 2
     blocks = -(-rows // (8 * nt // g))
-    smem, per_sm = _ops_host.rows_form(d, True, nt)
+    smem, per_sm = host.ops().rows_form(d, True, nt)
     per, out, lo = hk * blocks, [], 1
     # as the call-by-call rule (ops_host.cpp, rows_shares): shares that fill the SMs once; two at least where sequences of more rows leave at once
     for cluster, most in ((8, sms * per_sm // 8), (4, sms * per_sm // 4), (2, sms * per_sm // 2 if hi == I32_MAX else None), (1, None)):
@@ -684,12 +684,12 @@ def attn_decode_e4m3_op(hq: int, hk: int, d: int, page_size: int, table_width: i
 def attn_prefill_e4m3_op(hq: int, hk: int, d: int, page_size: int, table_width: int, q_stride: int, seqs_max: int) -> dict:
     """Ragged rows over the 8-bit cache: sequences of many rows on the tensor-core kernel, of few on the few-row
     kernel. Interface [q(kv) buffer, kv state, out, block_table, seq_lens, cu_seqlens, seqs, err]; no plan."""
-    from .. import _ops_host
+    from ..ops import host
 
     g = hq // hk
     iface = ["in buffer<bf16>", "in state", "out buffer<bf16>", "in buffer<i32>", "in buffer<i32>", "in buffer<i32>", "i32", "out buffer<i32>"]
     few = max(1, 8 // g)
-    module, rows, threads, smem = _ops_host.tile_form(d, True)
+    module, rows, threads, smem = host.ops().tile_form(d, True)
     many = _e4m3_attend(f"kern_attn_tile_e4m3_causal_d{d}", [hk, {"add": [{"ceil_div": ["tokens", rows // g]}, "seqs"]}, 1], threads, smem, 1,
                         hq, hk, d, page_size, table_width, q_stride, {"param": 6}, few + 1, I32_MAX, 5, 7, None)
     many["module"] = module

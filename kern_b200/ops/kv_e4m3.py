@@ -11,8 +11,7 @@ from __future__ import annotations
 
 import torch
 
-from .. import _ops_host
-from . import launcher as _launcher  # noqa: F401  (brings the kernels to `_ops_host`)
+from . import host as _host
 
 HEAD_DIMS = (64, 128, 256)
 
@@ -43,12 +42,12 @@ def rope_kv_append_e4m3(qkv: torch.Tensor, pool: torch.Tensor, positions: torch.
     of a head turn, the others pass. ``cos`` / ``sin``: f32 ``[max_pos, rot / 2]``, scaled for long contexts as the model has it
     (`attention.rope_tables`, the load programs' tables). A slot below zero (a padding row) is not written; a position or slot
     past its table sets the device's error word, and the row is not written. Two tokens may not have the same slot."""
-    return _ops_host.append(qkv, pool, positions, slots, cos, sin, hq, hk, d, page_size, rot, pairs, q_norm, k_norm, eps, norm_plus_one, tokens, q_out)
+    return _host.ops().append(qkv, pool, positions, slots, cos, sin, hq, hk, d, page_size, rot, pairs, q_norm, k_norm, eps, norm_plus_one, tokens, q_out)
 
 
 def read_rows_e4m3(pool: torch.Tensor, slots: torch.Tensor, hk: int, d: int, page_size: int, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """The rows at ``slots`` (i64) as bf16 ``[tokens, 2, hk, d]``, exact; zeros for a slot below zero."""
-    return _ops_host.read_rows(pool, slots, hk, d, page_size, out)
+    return _host.ops().read_rows(pool, slots, hk, d, page_size, out)
 
 
 # ---- attention -----------------------------------------------------------------------------------------------------------------
@@ -65,7 +64,7 @@ def paged_attention_e4m3(q: torch.Tensor, pool: torch.Tensor, block_table: torch
     A row that sees nothing gives zeros; rows of ``out`` behind the last sequence's stay as they are. Pages
     outside the pool, contexts longer than the table, rows outside ``q`` and sequences of more rows than ``max_rows`` (which are
     left out) set the device's error word. Returns ``out[rows, hq * d]``."""
-    return _ops_host.attend(q, pool, block_table, seq_lens, None, cu_q, hq, hk, d, page_size, out, rows_per_seq, max_rows, max_len, scale)
+    return _host.ops().attend(q, pool, block_table, seq_lens, None, cu_q, hq, hk, d, page_size, out, rows_per_seq, max_rows, max_len, scale)
 
 
 # ---- PyTorch references --------------------------------------------------------------------------------------------------------

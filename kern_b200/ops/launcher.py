@@ -12,7 +12,8 @@ from pathlib import Path
 
 import torch
 
-from .. import _native, _ops_host
+from .. import _native
+from . import host as _host
 
 KDIR = Path(__file__).resolve().parent.parent / "kernels"
 
@@ -84,7 +85,8 @@ class Kernels:
     @property
     def launches(self) -> int:
         """Kernel launches issued through this object and through the host side of the short operators."""
-        return self._launches + _ops_host.launches(self.gpu)
+        short = _host.loaded()
+        return self._launches + (short.launches(self.gpu) if short else 0)
 
     @property
     def sm_count(self) -> int:
@@ -141,12 +143,3 @@ class Kernels:
                 self._tmaps.clear()
             self._tmaps[key] = tm
         return tm
-
-
-def _provide(gpu: int) -> None:
-    """What the host side of the short operators (`_ops_host`) needs of a GPU, at its first call there."""
-    k = Kernels.get(gpu)
-    _ops_host.provide(gpu, k.sm_count, k.err_word().data_ptr(), lambda module, entry: k.function(module, entry).handle)
-
-
-_ops_host.on_missing(_provide)

@@ -10,8 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from .. import _ops_host
-from . import launcher as _launcher  # noqa: F401  (brings the kernels to `_ops_host`)
+from . import host as _host
 
 MAX_NODES = 256
 MAX_POOLS = 128
@@ -27,7 +26,7 @@ def tree_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tenso
     `tree_rows` gives them, or any other set. A node without a bit of its own (past the words) is seen by none; a row that sees
     nothing gives zeros; what a row does not see does not reach it, infinities and NaN included. Other arguments, and rows
     behind the last sequence's, as in `kv_e4m3.paged_attention_e4m3`."""
-    return _ops_host.attend(q, pool, block_table, seq_lens, masks, cu_q, hq, hk, d, page_size, out, 1, max_rows, max_len, scale)
+    return _host.ops().attend(q, pool, block_table, seq_lens, masks, cu_q, hq, hk, d, page_size, out, 1, max_rows, max_len, scale)
 
 
 def tree_rows(parents: torch.Tensor, cu: torch.Tensor, base: torch.Tensor, block_table: torch.Tensor, page_size: int, *,
@@ -39,7 +38,7 @@ def tree_rows(parents: torch.Tensor, cu: torch.Tensor, base: torch.Tensor, block
     the page table, or more than ``max_rows`` (256) nodes set the error word: the node then has no parent, or slot -1 (nothing
     written), or is left out. So do bounds in ``cu`` that are none. A sequence of base < 0 is padding: slots -1, positions 0, masks 0,
     context 0; so are nodes before the first sequence and behind the last."""
-    return _ops_host.tree_rows(parents, cu, base, block_table, page_size, max_rows)
+    return _host.ops().tree_rows(parents, cu, base, block_table, page_size, max_rows)
 
 
 def tree_keep(ids: torch.Tensor, parents: torch.Tensor, verify: torch.Tensor, cu: torch.Tensor, base: torch.Tensor,
@@ -52,7 +51,7 @@ def tree_keep(ids: torch.Tensor, parents: torch.Tensor, verify: torch.Tensor, cu
 
     In every pool of ``pools`` (all layers, one format, up to 128) the cache rows of path node i move from place base + path[i]
     to base + i. Places outside the table or the pool set the error word and are not touched."""
-    return _ops_host.tree_keep(ids, parents, verify, cu, base, block_table, pools, hk, d, page_size, max_rows)
+    return _host.ops().tree_keep(ids, parents, verify, cu, base, block_table, pools, hk, d, page_size, max_rows)
 
 
 # ---- PyTorch references --------------------------------------------------------------------------------------------------------

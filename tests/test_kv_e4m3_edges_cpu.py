@@ -1,7 +1,13 @@
 """The 8-bit cache without a GPU: values, arguments and builds at their ends."""
+import subprocess
+import sys
+import types
+
 import pytest
 import torch
 
+from kern_b200 import _build
+from kern_b200.ops import host
 from kern_b200.ops import kv_e4m3 as K8
 
 
@@ -22,3 +28,88 @@ def test_a_table_whose_contexts_pass_32_bits_is_refused():
     for pages, why in ((2048, "32 bits"), (2047, "CUDA device")):
         with pytest.raises(ValueError, match=why):
             K8.paged_attention_e4m3(q, pool, torch.zeros(1, pages, dtype=torch.int32), lens, hq, hk, d, page)
+
+
+# ---- what hangs on the host side's library ---------------------------------------------------------------------------------------
+def test_other_operators_do_without_the_host_library():
+    """Everything that was there before it imports and runs where it does not load; the operators that need it say so."""
+    code = """
+import sys
+import kern_b200
+sys.modules["kern_b200._ops_host"] = None
+import torch
+from kern_b200.ops import attention, basic, draft, gdn, gemm, gemm_fp8, gemm_mx, launcher, mla, moe, spec
+from kern_b200 import cpu, engine, runtime
+from kern_b200.models import dense
+assert dense.build_manifest(dense.TOY)["programs"]
+from kern_b200.ops import kv_e4m3, tree
+codes, _ = kv_e4m3.quantise_reference(torch.ones(1, 64))
+for call in (lambda: kv_e4m3.read_rows_e4m3(None, None, 2, 64, 16), lambda: tree.tree_rows(None, None, None, None, 16)):
+    try:
+        call()
+    except RuntimeError as e:
+        assert "_ops_host" in str(e) and "python -m kern_b200._build" in str(e), e
+    else:
+        raise SystemExit("no error")
+print("fine")
+"""
+    p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0 and "fine" in p.stdout, p.stderr[-2000:]
+
+
+def test_a_library_built_for_another_pytorch_is_refused(monkeypatch):
+    monkeypatch.setattr(host, "_ops", None)
+    monkeypatch.setitem(sys.modules, "kern_b200._ops_host", types.SimpleNamespace(torch_version="1.0.0", on_missing=lambda f: None))
+    with pytest.raises(RuntimeError, match="built for PyTorch 1.0.0"):
+        host.ops()
+
+
+@pytest.fixture
+def a_build(monkeypatch, tmp_path):
+    """`build_ops_host` on a tree of its own, its compiler replaced: (calls, settings)"""
+    (tmp_path / "csrc" / "bindings" / "torch").mkdir(parents=True)
+    (tmp_path / "csrc" / "bindings" / "torch" / "ops_host.cpp").write_text("")
+    (tmp_path / "build").mkdir()
+    calls, here = [], dict(version="2.0.0+cu", cuda=True, fails=False)
+
+    def compiled(src, out):
+        calls.append(here["version"])
+        if here["fails"]:
+            raise RuntimeError("no such function")
+        out.write_text(here["version"])
+    for name, value in (("PKG", tmp_path), ("CSRC", tmp_path / "csrc"), ("BUILD", tmp_path / "build"), ("_compile_ops_host", compiled),
+                        ("_torch_here", lambda: (here["version"], here["cuda"]))):
+        monkeypatch.setattr(_build, name, value)
+    return calls, here
+
+
+def test_the_library_is_built_again_for_another_pytorch(a_build):
+    calls, here = a_build
+    assert _build.build_ops_host().exists()
+    _build.build_ops_host()
+    assert calls == ["2.0.0+cu"]
+    here["version"] = "2.1.0+cu"
+    _build.build_ops_host(needed=False)
+    _build.build_ops_host()
+    assert calls == ["2.0.0+cu", "2.1.0+cu"]
+    _build.ops_host_path().unlink()
+    _build.build_ops_host()
+    assert len(calls) == 3
+
+
+def test_an_import_survives_a_library_that_cannot_be_built(a_build):
+    calls, here = a_build
+    here["fails"] = True
+    with pytest.warns(UserWarning, match="no operators over 8-bit caches"):
+        assert _build.build_ops_host(needed=False) is None
+    _build.build_ops_host(needed=False)                    # (the same sources: not tried at every import)
+    assert len(calls) == 1
+    with pytest.raises(RuntimeError, match="no such function"):
+        _build.build_ops_host()
+    here.update(fails=False, cuda=False)                   # a PyTorch without CUDA has no use for it
+    assert _build.build_ops_host() is None and len(calls) == 2
+
+
+def test_the_pytorch_that_is_here():
+    version, cuda = _build._torch_here()
+    assert version == torch.__version__ and cuda == (torch.version.cuda is not None)
