@@ -126,8 +126,9 @@ void table_of(const Tensor& t, const char* name) {
   if (t.scalar_type() != at::kInt || t.dim() != 2 || !whole(t)) refuse(std::string(name) + ": contiguous i32 [seqs, pages]");
   if (t.size(0) > 65535 || (t.size(0) > 0 && t.size(1) < 1)) refuse(std::string(name) + " [" + n(t.size(0)) + ", " + n(t.size(1)) + "]: at most 65535 sequences, a page to a row");
 }
-void heads(int64_t hq, int64_t hk, int64_t d, int64_t page) {
-  if (hk < 1 || hq < 1 || hq % hk || hq > 16 * hk) refuse(n(hq) + " query heads over " + n(hk) + " kv heads: a whole group of at most 16");
+void heads(int64_t hq, int64_t hk, int64_t d, int64_t page, bool attends) {
+  if (hk < 1 || hq < 1 || hq % hk || (attends && hq > 16 * hk))
+    refuse(n(hq) + " query heads over " + n(hk) + " kv heads: a whole group" + (attends ? " of at most 16" : ""));
   if (d != 64 && d != 128 && d != 256) refuse("head_dim " + n(d) + ": built for 64, 128, 256");
   if (page < 8 || (page <= kTile ? kTile % page : page % kTile)) refuse("page_size " + n(page) + ": 8, 16, 32, or a multiple of 64");
   if (hq > 4096 || page > (1 << 20) || 2 * hk * page * (d + 1) > INT32_MAX) refuse("heads or pages past 32 bits");
@@ -166,7 +167,7 @@ at::TensorOptions typed(const Tensor& like, at::ScalarType type) { return like.o
 Tensor append(const Tensor& qkv, const Tensor& pool, const Tensor& positions, const Tensor& slots, const Tensor& cos, const Tensor& sin, int64_t hq,
               int64_t hk, int64_t d, int64_t page, std::optional<int64_t> rot_, const std::string& pairs, const Maybe& q_norm, const Maybe& k_norm,
               double eps, bool plus_one, std::optional<int64_t> tokens, const Maybe& q_out) {
-  heads(hq, hk, d, page);
+  heads(hq, hk, d, page, false);
   const int64_t pages = pages8(pool, hk, page, d);
   auto [t, step] = rows_of(qkv, (hq + 2 * hk) * d, "qkv");
   if (tokens) {
@@ -206,7 +207,7 @@ Tensor append(const Tensor& qkv, const Tensor& pool, const Tensor& positions, co
 }
 
 Tensor read_rows(const Tensor& pool, const Tensor& slots, int64_t hk, int64_t d, int64_t page, const Maybe& out_) {
-  heads(hk, hk, d, page);
+  heads(hk, hk, d, page, false);
   const int64_t pages = pages8(pool, hk, page, d);
   if (slots.scalar_type() != at::kLong || slots.dim() != 1 || !whole(slots)) refuse("slots: i64 [tokens]");
   const int64_t t = slots.numel();
@@ -300,7 +301,7 @@ std::array<uint8_t, 128> pool_map(Host& h, const Tensor& pool, bool e4m3, int64_
 Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Tensor& lens, const Maybe& masks, const Maybe& cu_q, int64_t hq,
               int64_t hk, int64_t d, int64_t page, const Maybe& out_, int64_t rows_per_seq, std::optional<int64_t> max_rows_, std::optional<int64_t> max_len_,
               std::optional<double> scale_) {
-  heads(hq, hk, d, page);
+  heads(hq, hk, d, page, true);
   const int64_t pages = masks ? pages_any(pool, hk, page, d) : pages8(pool, hk, page, d);
   const bool e4m3 = pool.scalar_type() == at::kByte;
   const auto [rows, q_step] = rows_of(q, hq * d, "q");
@@ -430,7 +431,7 @@ py::tuple tree_rows(const Tensor& parents, const Tensor& cu, const Tensor& base,
 
 py::tuple tree_keep(const Tensor& ids, const Tensor& parents, const Tensor& verify, const Tensor& cu, const Tensor& base, const Tensor& table,
                     const std::vector<Tensor>& pools, int64_t hk, int64_t d, int64_t page, std::optional<int64_t> max_rows) {
-  heads(hk, hk, d, page);
+  heads(hk, hk, d, page, false);
   glue(parents, cu, base, table, page, max_rows);
   const int64_t nodes = parents.size(0), seqs = table.size(0);
   numbers(ids, at::kLong, nodes, "ids");

@@ -30,6 +30,17 @@ def test_a_table_whose_contexts_pass_32_bits_is_refused():
             K8.paged_attention_e4m3(q, pool, torch.zeros(1, pages, dtype=torch.int32), lens, hq, hk, d, page)
 
 
+def test_only_attention_limits_the_group():
+    """32 query heads over one kv head: written and read back as any (what is left to refuse is the device), attended by neither form."""
+    hq, hk, d, page = 32, 1, 64, 16
+    pool, i64 = K8.new_pool(2, hk, page, d, "cpu"), torch.zeros(3, dtype=torch.int64)
+    qkv, tab = torch.zeros(3, (hq + 2 * hk) * d, dtype=torch.bfloat16), torch.zeros(9, d // 2)
+    with pytest.raises(ValueError, match="CUDA device"):
+        K8.rope_kv_append_e4m3(qkv, pool, i64, i64, tab, tab, hq, hk, d, page)
+    with pytest.raises(ValueError, match="group of at most 16"):
+        K8.paged_attention_e4m3(qkv[:, : hq * d], pool, torch.zeros(3, 1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), hq, hk, d, page)
+
+
 # ---- what hangs on the host side's library ---------------------------------------------------------------------------------------
 def test_other_operators_do_without_the_host_library():
     """Everything that was there before it imports and runs where it does not load; the operators that need it say so."""

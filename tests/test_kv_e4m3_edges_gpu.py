@@ -332,3 +332,21 @@ def test_places_past_32_bits(cuda):
     for base in ((1 << 32) + 3, 1 << 62, (1 << 63) - 1):
         _, slots, lens, _ = failed(lambda: TR.tree_rows(i32([-1, 0]), i32([0, 2]), torch.tensor([base], device=cuda), table, 16))
         assert slots.tolist() == [-1, -1] and lens.tolist() == [(1 << 31) - 1]
+
+
+@pytest.mark.parametrize("hq,hk,d", [(32, 1, 128), (48, 2, 64), (40, 1, 256)])
+def test_append_of_wide_groups(cuda, hq, hk, d):
+    """More than 16 query heads to a kv head: the append has no use for the group."""
+    page, t = 16, 9
+    g = torch.Generator().manual_seed(hq)
+    qkv = torch.randn(t, (hq + 2 * hk) * d, generator=g).bfloat16()
+    ang = torch.rand(t, d // 2, generator=g) * 6
+    pool = K8.new_pool(1, hk, page, d, cuda)
+    slots = torch.arange(t, device=cuda)
+    got = K8.rope_kv_append_e4m3(qkv.cuda(), pool, slots, slots, ang.cos().cuda(), ang.sin().cuda(), hq, hk, d, page)
+    x = qkv.double().view(t, -1, d)
+    c, s = ang.cos().double()[:, None], ang.sin().double()[:, None]
+    q = torch.cat([x[:, :hq, : d // 2] * c - x[:, :hq, d // 2:] * s, x[:, :hq, d // 2:] * c + x[:, :hq, : d // 2] * s], -1).view(t, -1)
+    assert bool(((got.double().cpu() - q).abs() <= 2.0 ** -8 * q.abs() + 2.0 ** -20 * q.abs().max()).all())
+    want = K8.dequantise_reference(*K8.quantise_reference(x[:, hq + hk:].float()))
+    assert torch.equal(K8.read_rows_e4m3(pool, slots, hk, d, page)[:, 1].float().cpu(), want)
