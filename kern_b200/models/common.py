@@ -604,6 +604,16 @@ def attn_decode_op(hq: int, hk: int, d: int, page_size: int, table_width: int, q
 
 
 # ---- the 8-bit cache (ops/kv_e4m3.py has its layout): the same operations over it ------------------------------------------------
+def check_e4m3(hq: int, hk: int, d: int, page_size: int) -> None:
+    """What the kernels over the 8-bit cache (head_dim 16 and 32: their statements on the host) take of a decoder's layout."""
+    if hq % hk or hq > 16 * hk:
+        raise ValueError(f"kv=\"e4m3\": {hq} query heads over {hk} kv heads: a whole group of at most 16")
+    if d not in (16, 32, 64, 128, 256):
+        raise ValueError(f"kv=\"e4m3\": head_dim {d}: built for 64, 128, 256")
+    if page_size < 8 or (64 % page_size if page_size <= 64 else page_size % 64):
+        raise ValueError(f"kv=\"e4m3\": page_size {page_size}: 8, 16, 32, or a multiple of 64")
+
+
 def rope_append_e4m3_op(hq: int, hk: int, d: int, rot: int, page_size: int, max_pos: int, eps: float, qk_norm: bool,
                         norm_plus_one: bool = False, row_stride: int | None = None, pairs: str = "half") -> dict:
     """Interface [qkv, kv state, positions, slots, cos, sin, (q_norm, k_norm,) err], as `rope_append_op`."""

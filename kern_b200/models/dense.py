@@ -123,6 +123,8 @@ def build_manifest(cfg: DenseConfig, hosted: bool = False) -> dict:
     q8 = cfg.kv == "e4m3"
     if q8 and hosted:
         raise ValueError("a host engine's cache is bf16: no kv=\"e4m3\"")
+    if q8:
+        C.check_e4m3(hq, hk, d, cfg.page_size)
     bufs, ops, states = {}, {}, {}
     bufs["token_ids"] = {"dtype": "i64", "shape": ["tokens"], "kind": "input", "fill": "token",
                          "domain": {"min": 0, "max": cfg.vocab - 1}}

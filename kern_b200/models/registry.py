@@ -56,11 +56,18 @@ def families() -> dict:
     return out
 
 
+def _one_cache(name: str, kv: str | None) -> None:
+    if kv is not None:
+        raise ValueError(f"kv={kv!r}: `{name}` has a cache of its own; the dense and routed decoders take the option")
+
+
 def resolve(name: str, **overrides):
     """-> (config with overrides applied, builder, device loader, host weights maker). `name`: a family, or a checkpoint folder."""
+    kv = overrides.get("kv")
     if is_folder(name):
         from .common import read_safetensors
 
+        _one_cache(name, kv)
         cfg, build = from_folder(name, **overrides)
         files = sorted(str(p) for p in Path(name).glob("*.safetensors"))
         return cfg, build, lambda rt, cfg: rt.load_weights(files), \
@@ -69,6 +76,8 @@ def resolve(name: str, **overrides):
     if name not in fam:
         raise KeyError(f"unknown model `{name}`; known: {', '.join(sorted(fam))}")
     cfg, build, load, make = fam[name]
+    if not hasattr(cfg, "kv"):
+        _one_cache(name, kv)
     overrides = {k: v for k, v in overrides.items() if v is not None}
     if not dataclasses.is_dataclass(cfg):
         return cfg, build, load, make          # a family without a config object (the integer model)

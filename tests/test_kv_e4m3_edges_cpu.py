@@ -1,4 +1,5 @@
 """The 8-bit cache without a GPU: values, arguments and builds at their ends."""
+import dataclasses
 import subprocess
 import sys
 import types
@@ -7,6 +8,7 @@ import pytest
 import torch
 
 from kern_b200 import _build
+from kern_b200.models import dense, moe, registry
 from kern_b200.ops import host
 from kern_b200.ops import kv_e4m3 as K8
 
@@ -39,6 +41,34 @@ def test_only_attention_limits_the_group():
         K8.rope_kv_append_e4m3(qkv, pool, i64, i64, tab, tab, hq, hk, d, page)
     with pytest.raises(ValueError, match="group of at most 16"):
         K8.paged_attention_e4m3(qkv[:, : hq * d], pool, torch.zeros(3, 1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), hq, hk, d, page)
+
+
+@pytest.mark.parametrize("change,why", [(dict(heads=32, kv_heads=1), "group of at most 16"), (dict(page_size=48), "page_size 48"), (dict(page_size=96), "page_size 96"),
+                                        (dict(page_size=4), "page_size 4"), (dict(head_dim=96), "head_dim 96"), (dict(heads=3), "whole group")])
+def test_decoders_whose_layout_the_cache_does_not_have(change, why):
+    cfg = dataclasses.replace(dense.TINY, kv="e4m3", **change)
+    with pytest.raises(ValueError, match=why):
+        dense.build_manifest(cfg)
+    with pytest.raises(ValueError, match=why):
+        moe.build_manifest(dataclasses.replace(moe.TINY_MOE, kv="e4m3", **change))
+
+
+@pytest.mark.parametrize("page", [8, 32, 64, 192])
+def test_decoders_whose_layout_it_has(page):
+    assert dense.build_manifest(dataclasses.replace(dense.TINY, kv="e4m3", page_size=page))["states"]
+
+
+@pytest.mark.parametrize("name", ["tiny-hybrid", "tiny-latent", "tiny-gafapel", "toy-int"])
+def test_families_that_have_no_such_option(name, tmp_path):
+    known = registry.families()
+    name = next(n for n in known if n.startswith(name))
+    for kv in ("e4m3", "bf16"):
+        with pytest.raises(ValueError, match="cache of its own"):
+            registry.resolve(name, kv=kv)
+    assert registry.resolve(name, kv=None)
+    (tmp_path / "config.json").write_text("{}")
+    with pytest.raises(ValueError, match="cache of its own"):
+        registry.resolve(str(tmp_path), kv="e4m3")
 
 
 # ---- what hangs on the host side's library ---------------------------------------------------------------------------------------
