@@ -331,7 +331,8 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
   const int64_t max_len = max_len_.value_or(width * page);
   if (max_len < 0) refuse("max_len " + n(max_len));
   const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)d);
-  if (!(scale > 0)) refuse("scale: above zero");
+  const float scale_log2 = (float)(scale * kLog2e);
+  if (!(scale > 0) || !std::isnormal(scale_log2)) refuse("scale: above zero, and a number that f32 holds");
   const int gpu = Same(q)(pool)(table)(lens)(cu_q)(masks)(out_).gpu;
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)gpu);
   const Tensor out = out_ ? *out_ : at::empty({rows, hq * d}, typed(q, at::kBFloat16));
@@ -380,7 +381,7 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
     Block b;
     b.bytes(map.data(), map.size()).at(q).at(out).put(ws_o).put(ws_ml).at(pool).at(table).at(lens).at(cu_q).at(masks);
     b.ints(masks ? masks->size(1) : 0, rows_per_seq, hq, hk, q_step, out_step, width, page, tiled ? seqs : cluster, pages, lo, hi, rows, max_rows, ws_step);
-    b.put((float)(scale * kLog2e)).put(h.err);
+    b.put(scale_log2).put(h.err);
     launch(h, tiled ? tile_module(d) : "attn_rows", name, gx, gy, shares, tiled ? (unsigned)tile_threads(d) : 160, b, shared, !tiled && hi < all, (unsigned)cluster);
     if (groups > 1) {
       Block m;

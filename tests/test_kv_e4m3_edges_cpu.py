@@ -11,6 +11,7 @@ from kern_b200 import _build
 from kern_b200.models import dense, moe, registry
 from kern_b200.ops import host
 from kern_b200.ops import kv_e4m3 as K8
+from kern_b200.ops import tree as TR
 
 
 def test_the_largest_bf16_values_keep_their_sign_and_size():
@@ -30,6 +31,19 @@ def test_a_table_whose_contexts_pass_32_bits_is_refused():
     for pages, why in ((2048, "32 bits"), (2047, "CUDA device")):
         with pytest.raises(ValueError, match=why):
             K8.paged_attention_e4m3(q, pool, torch.zeros(1, pages, dtype=torch.int32), lens, hq, hk, d, page)
+
+
+@pytest.mark.parametrize("scale,why", [(1e-39, "f32 holds"), (1e-300, "f32 holds"), (3e38, "f32 holds"), (float("inf"), "f32 holds"), (-1.0, "f32 holds"),
+                                       (1e-37, "CUDA device"), (2e38, "CUDA device")])
+def test_scales_that_f32_does_not_hold(scale, why):
+    """A scale of 0 in f32 would make NaN of scores that are not seen."""
+    hq, hk, d, page = 4, 2, 64, 16
+    pool, q = K8.new_pool(2, hk, page, d, "cpu"), torch.zeros(3, hq * d, dtype=torch.bfloat16)
+    table, lens, cu = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.tensor([0, 3], dtype=torch.int32)
+    with pytest.raises(ValueError, match=why):
+        K8.paged_attention_e4m3(q, pool, table, lens, hq, hk, d, page, rows_per_seq=3, scale=scale)
+    with pytest.raises(ValueError, match=why):
+        TR.tree_attention(q, pool, table, lens, torch.zeros(3, 1, dtype=torch.int64), cu, hq, hk, d, page, scale=scale)
 
 
 def test_only_attention_limits_the_group():
