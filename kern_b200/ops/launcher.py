@@ -85,8 +85,15 @@ class Kernels:
     @property
     def launches(self) -> int:
         """Kernel launches issued through this object and through the host side of the short operators."""
+        return self._launches + self._short_launches()
+
+    @launches.setter
+    def launches(self, count: int) -> None:
+        self._launches = count - self._short_launches()
+
+    def _short_launches(self) -> int:
         short = _host.loaded()
-        return self._launches + (short.launches(self.gpu) if short else 0)
+        return short.launches(self.gpu) if short else 0
 
     @property
     def sm_count(self) -> int:

@@ -9,7 +9,7 @@ import torch
 
 from kern_b200 import _build
 from kern_b200.models import dense, moe, registry
-from kern_b200.ops import host
+from kern_b200.ops import host, launcher
 from kern_b200.ops import kv_e4m3 as K8
 from kern_b200.ops import tree as TR
 
@@ -168,3 +168,14 @@ def test_an_import_survives_a_library_that_cannot_be_built(a_build):
 def test_the_pytorch_that_is_here():
     version, cuda = _build._torch_here()
     assert version == torch.__version__ and cuda == (torch.version.cuda is not None)
+
+
+def test_the_count_of_launches_can_be_set(monkeypatch):
+    """As it could before part of it was counted elsewhere."""
+    k = object.__new__(launcher.Kernels)
+    k.gpu, k._launches = 0, 5
+    monkeypatch.setattr(host, "_ops", types.SimpleNamespace(launches=lambda gpu: 7))
+    assert k.launches == 12
+    k.launches = 0
+    k._launches += 2
+    assert k.launches == 2
