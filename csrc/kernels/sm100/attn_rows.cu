@@ -440,7 +440,8 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            s[nt][k] = (s[nt][k] + s2[nt][k]) * (f_col[nt][k & 1] * kscale[k >> 1]);
+            // (one factor after the other: together they may pass f32's range where a product is 0)
+            s[nt][k] = (s[nt][k] + s2[nt][k]) * f_col[nt][k & 1] * kscale[k >> 1];
             if (edge && !(see >> (nt * 4 + k) & 1)) s[nt][k] = -INFINITY;
           }
         float e[NT][4], w[NT][4];

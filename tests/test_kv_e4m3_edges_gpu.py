@@ -350,3 +350,18 @@ def test_append_of_wide_groups(cuda, hq, hk, d):
     assert bool(((got.double().cpu() - q).abs() <= 2.0 ** -8 * q.abs() + 2.0 ** -20 * q.abs().max()).all())
     want = K8.dequantise_reference(*K8.quantise_reference(x[:, hq + hk:].float()))
     assert torch.equal(K8.read_rows_e4m3(pool, slots, hk, d, page)[:, 1].float().cpu(), want)
+
+
+@pytest.mark.parametrize("rows", [1, 4, 100])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_huge_keys_across_huge_queries(cuda, rows, d):
+    """Keys and queries whose factors together pass f32's range, and whose products are 0: the mean of the values."""
+    hq, hk, page, l = 8, 2, 64, 300
+    g = torch.Generator().manual_seed(rows)
+    k, v = torch.randn(2, l, hk, d, generator=g)
+    k = torch.where(torch.arange(d) < d // 2, k * 2.0 ** 100, 0.0)
+    pool, table, kv = cache_of(k, v, page)
+    q = torch.where(torch.arange(d) < d // 2, 0.0, torch.randn(rows, hq, d, generator=g) * 2.0 ** 60).view(rows, -1).bfloat16().cuda()
+    ref, spread = attend64(q.cpu().view(rows, hq, d), kv, causal(rows, l), d ** -0.5)
+    for out in both_ways(q, pool, table, l, hq, hk, d, page):
+        close(out, ref, spread, WEIGHT["e4m3"])
