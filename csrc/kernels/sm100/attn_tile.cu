@@ -189,9 +189,8 @@ KERN_DEVICE void tile_body(const CUtensorMap* kv_map, const RowsArgs& a, const i
         const uint32_t word = scale_word(by, here);
         const int top = top_byte(word), vtop = which ? 0 : top_byte(scale_word(by + kT, here));
         // (a row of zeros has the byte -40 + 127)
-        if (top > kLeastScale + 20 && (__vcmpgtu4(word, 0u) & __vcmpltu4(word, (uint32_t)(top - 20) * 0x01010101u)) != 0 &&
-            rows_lost<D, 1>(src, 0, lane, word, top))
-          *wide_s = 1;
+        if (top > kLeastScale + 20 && (__vcmpgtu4(word, 0u) & __vcmpltu4(word, (uint32_t)(top - 20) * 0x01010101u)) != 0)
+          rows_lost<D, 1>(src, 0, lane, word, top, wide_s);
         uint8_t* dst = h_s + half * Cfg::kHalf;
         bool nan = false;
         // rows r0 + j * kStep: all in the same place of the swizzle and of their words of scale bytes

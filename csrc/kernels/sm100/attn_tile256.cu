@@ -172,9 +172,8 @@ KERN_DEVICE void tile256_body(const CUtensorMap* kv_map, const RowsArgs& a, cons
         const uint32_t word = scale_word(by), v_word = which ? 0u : scale_word(by + kKeys);
         const int top = top_byte(word), vtop = top_byte(v_word);
         // (a row of zeros has the byte -40 + 127)
-        if (top > kLeastScale + 20 && (__vcmpgtu4(word, 0u) & __vcmpltu4(word, (uint32_t)(top - 20) * 0x01010101u)) != 0 &&
-            rows_lost<128, 2>(src, kBlock, lane, word, top))
-          *wide_s = 1;
+        if (top > kLeastScale + 20 && (__vcmpgtu4(word, 0u) & __vcmpltu4(word, (uint32_t)(top - 20) * 0x01010101u)) != 0)
+          rows_lost<128, 2>(src, kBlock, lane, word, top, wide_s);
         // a lane: 8 codes of the row's first 128 and 8 of its second (a piece of 16-bit values each), in rows r0 + 8 j: all in the
         // same place of the swizzle and of their words of scale bytes
         constexpr int kLoads = kKeys / 8;

@@ -105,12 +105,12 @@ KERN_DEVICE float level_share(float& m, float& l) {
   return f;
 }
 
-// (8-bit) Whether one of this lane's four rows of a half, whose scale bytes are `word`, holds anything but zeros and is lost under the half's
-// largest scale (`top`; f16 has room for 2^20 below it). Asked for where there is such a scale, which in earnest is a row of zeros'.
-// Rows lie as they came: BLOCKS column blocks of BYTES to a row, in whatever order its pieces are. (A call: 14 registers where it is used,
-// none where it is not. In the loop that converts, 4 prompts took 395 us for 387.)
+// (8-bit) Sets wide_s if one of this lane's four rows of a half, whose scale bytes are `word`, holds anything but zeros and is lost under
+// the half's largest scale (`top`; f16 has room for 2^20 below it). Asked for where there is such a scale, which in earnest is a row of
+// zeros'. Rows lie as they came: BLOCKS column blocks of BYTES to a row, in whatever order its pieces are. A call that gives nothing
+// back, of 14 registers: 4 prompts take 388 us with it, 392 where it gave the answer back, and 395 with its loop among the conversions.
 template <int BYTES, int BLOCKS>
-__device__ __noinline__ bool rows_lost(uint32_t codes, uint32_t block_bytes, int lane, uint32_t word, int top) {
+__device__ __noinline__ void rows_lost(uint32_t codes, uint32_t block_bytes, int lane, uint32_t word, int top, volatile int* wide_s) {
   uint32_t any = 0;
 #pragma unroll 1
   for (int k = 0; k < 4; ++k) {
@@ -126,7 +126,7 @@ __device__ __noinline__ bool rows_lost(uint32_t codes, uint32_t block_bytes, int
       any |= v0 | v1 | v2 | v3;
     }
   }
-  return (any & 0x7f7f7f7fu) != 0;
+  if ((any & 0x7f7f7f7fu) != 0) *wide_s = 1;
 }
 
 // Block y of the call: (sequence, block of its rows) to found[0] and [1]; sequence -1 past the last. Blocks are counted through the
