@@ -220,14 +220,16 @@ KERN_DEVICE void put_back(const RowsArgs& a, const long long* mask, int seq, int
   }
 }
 
-// A block's rows over the 8-bit cache, a row to a warp in turn and one token at a time, for scales that have no common exponent, in a tile
-// or over the tiles.
+// A block's rows over the 8-bit cache, a row to a warp in turn and some tokens at a time, for scales that have no common exponent, in a tile
+// or over the tiles. Far slower than the products are: 4 prompts of up to 2048 rows on up to 6000 with such a row in every page take 97 ms, not
+// 0.4, and 16 trees of up to 64 nodes on up to 4096 19 ms, not 0.08 (176 and 69 with one token under way at a time).
 template <int D, bool TREE>
 __device__ __noinline__ void tile_wide(const RowsArgs& a, int seq, int row0, int tok_lo, int valid, int past, int from, int to, int shares,
                                        int warps) {
-  constexpr int kCols = D / 32;                               // of a lane
+  constexpr int kCols = D / 32, kAtOnce = D == 256 ? 4 : 8;   // columns of a lane; tokens
   const int G = a.hq / a.hk, kvh = blockIdx.x, lane = threadIdx.x & 31;
   const size_t codes = (size_t)2 * a.hk * a.page_size * D, page_bytes = codes + 2 * a.hk * a.page_size;
+  const size_t to_v = (size_t)a.hk * a.page_size;
   for (int r = threadIdx.x >> 5; r < valid; r += warps) {
     const int tk = tok_lo + r / G, head = kvh * G + r % G, stop = TREE ? to : min(to, past + tk + 1);
     const long long* mask = TREE ? a.masks + (size_t)(row0 + tk) * a.words : nullptr;
@@ -237,40 +239,83 @@ __device__ __noinline__ void tile_wide(const RowsArgs& a, int seq, int row0, int
       q[i] = __bfloat162float(a.q[(size_t)(row0 + tk) * a.q_stride + (size_t)head * D + lane * kCols + i]) * a.scale_log2;
       o[i] = 0.f;
     }
-    for (int j = from; j < stop; ++j) {
-      if (TREE && j >= past) {
+#pragma unroll 1
+    for (int j0 = from; j0 < stop; j0 += kAtOnce) {
+      // a lane to each token: whether the row sees it, where it lies, its scale bytes
+      const int j = j0 + lane % kAtOnce, in = min(j, stop - 1);
+      bool see = j < stop;
+      if (TREE && see && j >= past) {
         const int n = j - past;
-        if (n >> 6 >= a.words || !(mask[n >> 6] >> (n & 63) & 1)) continue;
+        see = n >> 6 < a.words && (mask[n >> 6] >> (n & 63) & 1);
       }
-      const int pi = j / a.page_size, off = j - pi * a.page_size;
+      const unsigned live = __ballot_sync(0xffffffffu, see) & ((1u << kAtOnce) - 1);
+      if (live == 0) continue;
+      const int pi = in / a.page_size, off = in - pi * a.page_size;
       int page = pi < a.max_pages ? a.block_table[(size_t)seq * a.max_pages + pi] : 0;
       if (page < 0 || page >= a.pool_pages) page = 0;         // (recorded by the walk before)
-      float kv[2][kCols], size[2];
+      const uint8_t* sizes = a.pool + (size_t)page * page_bytes + codes + (size_t)kvh * a.page_size + off;
+      const int k_size = sizes[0], v_size = sizes[to_v];
+      uint32_t w[kAtOnce][2][(kCols + 3) / 4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const size_t at = (size_t)(h * a.hk + kvh) * a.page_size + off;
-        const uint8_t* src = a.pool + (size_t)page * page_bytes;
-        size[h] = pow2i((int)src[codes + at] - 127);
+      for (int u = 0; u < kAtOnce; ++u) {
+        const uint8_t* src = a.pool + (size_t)__shfl_sync(0xffffffffu, page, u) * page_bytes +
+                             ((size_t)kvh * a.page_size + __shfl_sync(0xffffffffu, off, u)) * D + lane * kCols;
 #pragma unroll
-        for (int i = 0; i < kCols; i += 2) {
-          uint32_t lo, hi;
-          codes_f16x4(*reinterpret_cast<const uint16_t*>(src + at * D + lane * kCols + i), lo, hi);
-          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-          kv[h][i] = v.x;
-          kv[h][i + 1] = v.y;
+        for (int h = 0; h < 2; ++h) {
+          const uint8_t* at = src + h * to_v * D;
+          if constexpr (kCols == 2) {
+            w[u][h][0] = *reinterpret_cast<const uint16_t*>(at);
+          } else {
+#pragma unroll
+            for (int i = 0; i < kCols / 4; ++i) w[u][h][i] = reinterpret_cast<const uint32_t*>(at)[i];
+          }
         }
       }
-      float s = 0.f;
+      // the lane's values of k or v of token u
+      auto open = [&](int u, int h, float (&x)[kCols]) {
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) s = fmaf(q[i], kv[0][i], s);
+        for (int i = 0; i < kCols; i += 2) {
+          uint32_t two, none;
+          codes_f16x4(w[u][h][i / 4] >> (8 * (i & 2)), two, none);
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
+          x[i] = f.x;
+          x[i + 1] = f.y;
+        }
+      };
+      float s[kAtOnce], top = m;
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s *= size[0];
-      const float top = fmaxf(m, s), keep = exp2f(m - top), p = exp2f(s - top);
+      for (int u = 0; u < kAtOnce; ++u) {
+        float k[kCols];
+        open(u, 0, k);
+        s[u] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) s[u] = fmaf(q[i], k[i], s[u]);
+      }
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1)
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], x);
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        s[u] *= pow2i(__shfl_sync(0xffffffffu, k_size, u) - 127);
+        if (live >> u & 1) top = fmaxf(top, s[u]);
+      }
+      const float keep = exp2f(m - top);
       m = top;
-      l = fmaf(l, keep, p);
+      l *= keep;
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) o[i] = fmaf(o[i], keep, p * (kv[1][i] * size[1]));
+      for (int i = 0; i < kCols; ++i) o[i] *= keep;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const float size = pow2i(__shfl_sync(0xffffffffu, v_size, u) - 127);
+        if (!(live >> u & 1)) continue;                       // (uniform; what is not seen does not reach the row, whatever it is)
+        float v[kCols];
+        open(u, 1, v);
+        const float p = exp2f(s[u] - m);
+        l += p;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) o[i] = fmaf(p, v[i] * size, o[i]);
+      }
     }
     if (shares == 1) {
       const float inv = l == 0.f ? 0.f : 1.f / l;

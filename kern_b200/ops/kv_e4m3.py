@@ -61,6 +61,9 @@ def paged_attention_e4m3(q: torch.Tensor, pool: torch.Tensor, block_table: torch
     ``seq_lens[s]`` counts the context including this step's rows; rows of sequence s are ``cu_q[s]:cu_q[s+1]`` or
     ``s * rows_per_seq`` onward, and row i of R sees tokens 0 .. seq_lens[s] - R + i. ``max_rows``: the most rows of one sequence
     (all of q's unless given), ``max_len``: the longest context, which sets how it is shared out (the table's width unless given).
+    Calls of more than 16 query rows to a kv head keep their speed where the scales of a context's keys, and of its values, are within 2^20
+    of one another over 128 tokens (64 at head_dim 256; rows of zeros aside) and those of its values within 2^100 over all: 256 query
+    rows that meet others are computed token by token, some 200 times slower, and as exactly.
     A row that sees nothing gives zeros; rows of ``out`` behind the last sequence's stay as they are. Pages
     outside the pool, contexts longer than the table, rows outside ``q`` and sequences of more rows than ``max_rows`` (which are
     left out) set the device's error word. Returns ``out[rows, hq * d]``."""
