@@ -520,8 +520,13 @@ def _attention_e4m3(g, m, q, out, ws_o, ws_ml, kv, table, seq_lens, cu_q, masks,
         kk, vv = (dequantise_reference(codes[pages, i], scales[pages, i]).permute(0, 2, 1, 3).reshape(-1, hk, d)[:L].repeat_interleave(grp, 1) for i in (0, 1))
         qq = _f(torch.as_strided(q, (R, hq, d), (q_stride, d, 1), q.storage_offset() + r0 * q_stride))
         sc = torch.einsum("rhd,lhd->hrl", qq, kk) * (scale_log2 / 1.4426950408889634)
-        sc = sc.masked_fill(~(torch.arange(L)[None] <= torch.arange(L - R, L)[:, None])[None], float("-inf"))
-        o = torch.einsum("hrl,lhd->rhd", torch.softmax(sc, -1).nan_to_num(0.0), vv)
+        seen = torch.arange(L)[None] <= torch.arange(L - R, L)[:, None]
+        p = torch.softmax(sc.masked_fill(~seen[None], float("-inf")), -1)
+        # a row that sees nothing: zeros; values that are not numbers reach the rows that see them, and no others
+        bad = torch.isnan(vv)
+        o = torch.einsum("hrl,lhd->rhd", torch.where(seen.any(-1)[None, :, None], p, 0.0), vv.masked_fill(bad, 0.0))
+        if bad.any():
+            o = o.masked_fill(torch.einsum("rl,lhd->rhd", seen.float(), bad.float()) > 0, float("nan"))
         torch.as_strided(out, (R, hq * d), (out_stride, 1), out.storage_offset() + r0 * out_stride).copy_(o.reshape(R, hq * d).to(out.dtype))
 
 

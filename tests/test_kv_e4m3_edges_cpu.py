@@ -7,7 +7,7 @@ import types
 import pytest
 import torch
 
-from kern_b200 import _build
+from kern_b200 import _build, cpu
 from kern_b200.models import dense, moe, registry
 from kern_b200.ops import host, launcher
 from kern_b200.ops import kv_e4m3 as K8
@@ -83,6 +83,30 @@ def test_families_that_have_no_such_option(name, tmp_path):
     (tmp_path / "config.json").write_text("{}")
     with pytest.raises(ValueError, match="cache of its own"):
         registry.resolve(str(tmp_path), kv="e4m3")
+
+
+def test_the_host_statement_shows_nan_where_it_is_seen():
+    """A NaN among the keys, or the values, reaches the rows that see it and no others, as on the device; a row that sees nothing is zeros."""
+    hq, hk, d, page, rows = 2, 1, 16, 8, 5
+    g = torch.Generator().manual_seed(0)
+    for which, tokens in (("keys", 6), ("values", 6), ("none", 3)):
+        kv = torch.randn(8, 2, hk, d, generator=g)
+        if which != "none":
+            kv[4, int(which == "values"), 0, 7] = float("nan")
+        codes, scales = K8.quantise_reference(kv)
+        pool = torch.cat([codes.view(torch.uint8).permute(1, 2, 0, 3).reshape(-1), scales.permute(1, 2, 0).reshape(-1)])
+        q, out = torch.randn(rows * hq * d, generator=g).bfloat16(), torch.zeros(rows * hq * d, dtype=torch.bfloat16)
+        shape = types.SimpleNamespace(_head_dim=d, _vars_seqs=1)
+        cpu.CPU_KERNELS[f"kern_attn_tile_e4m3_causal_d{d}"](
+            (1,), shape, q, out, 0, 0, pool, torch.zeros(1, dtype=torch.int32), torch.tensor([tokens], dtype=torch.int32), 0, 0, 0, rows, hq, hk, hq * d, hq * d, 1, page,
+            1, 1, 1, rows, rows, rows, 0, 0.25 * 1.4426950408889634, torch.zeros(1, dtype=torch.int32))
+        nan = torch.isnan(out.view(rows, hq, d))
+        if which == "none":                                # (5 rows on 3 tokens: the first two see none)
+            assert not bool(nan.any()) and bool((out.view(rows, -1)[:2] == 0).all()) and bool((out.view(rows, -1)[2:] != 0).any())
+            continue
+        first = 4 - (tokens - rows)                        # the row that token 4 belongs to
+        assert not bool(nan[:first].any())
+        assert bool(nan[first:].all()) if which == "keys" else bool(nan[first:, :, 7].all()) and int(nan.sum()) == (rows - first) * hq
 
 
 # ---- what hangs on the host side's library ---------------------------------------------------------------------------------------
