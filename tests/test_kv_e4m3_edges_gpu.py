@@ -365,3 +365,33 @@ def test_huge_keys_across_huge_queries(cuda, rows, d):
     ref, spread = attend64(q.cpu().view(rows, hq, d), kv, causal(rows, l), d ** -0.5)
     for out in both_ways(q, pool, table, l, hq, hk, d, page):
         close(out, ref, spread, WEIGHT["e4m3"])
+
+
+@pytest.mark.parametrize("heads,hk,d", [(8, 1, 128), (4, 2, 64), (2, 1, 256)])
+def test_a_decoder_whose_padding_token_is_zeros(cuda, tmp_path, heads, hk, d):
+    """An embedding row of zeros, as checkpoints have it for padding: its queries, keys and values are zeros, in prompts and chunks."""
+    import dataclasses
+
+    from kern_b200.engine import Engine
+    from kern_b200.models import common, dense
+    from kern_b200.runtime import Runtime
+
+    cfg = dataclasses.replace(dense.TINY, kv="e4m3", heads=heads, kv_heads=hk, head_dim=d, max_context=512, max_tokens=512)
+    w = dense.random_weights(cfg, seed=0, std=0.05)
+    w["model.embed_tokens.weight"][3] = 0
+    common.write_safetensors(tmp_path / "model.safetensors", w)
+    rt = Runtime(dense.build_manifest(cfg), weights=tmp_path / "model.safetensors", tokens=cfg.page_size * 64)
+    rt.once()
+    eng, oracle = Engine(rt), dense.DenseOracle(cfg, w, device="cuda")
+    g = torch.Generator().manual_seed(3)
+    words = torch.randint(4, cfg.vocab, (60,), generator=g).tolist()
+    prompts = [[3] * 200, [3] * 150 + words[:40], [3]]
+    seqs, caches = [eng.open(len(p) + 40) for p in prompts], [oracle.new_cache() for _ in prompts]
+    for feeds in (prompts, [[3] * 30, words[40:], [3] * 9], [[3], [3], words[:1]]):
+        eng.step(list(zip(seqs, feeds)))
+        logits = rt.tensor("logits")[:3].float()
+        for f, c, lg in zip(feeds, caches, logits):
+            ref = oracle.forward(f, c)[-1]
+            # 1.3 % for codes that bf16 takes to their neighbours, as much for bf16 elsewhere; zeros exactly
+            assert float((lg - ref).norm()) <= 0.05 * float(ref.norm())
+    rt.check_error()
