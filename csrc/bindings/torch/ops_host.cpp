@@ -425,7 +425,7 @@ py::tuple tree_rows(const Tensor& parents, const Tensor& cu, const Tensor& base,
                lens = at::empty({seqs}, typed(parents, at::kInt));
   Host& h = host_of(gpu);
   Block b;
-  b.at(parents).at(cu).at(base).at(table).at(positions).at(slots).at(lens).at(masks).ints(nodes, words, table.size(1), page).put(h.err);
+  b.at(parents).at(cu).at(base).at(table).at(positions).at(slots).at(lens).at(masks).ints(nodes, most, words, table.size(1), page).put(h.err);
   launch(h, "tree", "kern_tree_rows", seqs, 1, 1, 256, b);
   return py::make_tuple(positions, slots, lens, masks);
 }
@@ -433,7 +433,7 @@ py::tuple tree_rows(const Tensor& parents, const Tensor& cu, const Tensor& base,
 py::tuple tree_keep(const Tensor& ids, const Tensor& parents, const Tensor& verify, const Tensor& cu, const Tensor& base, const Tensor& table,
                     const std::vector<Tensor>& pools, int64_t hk, int64_t d, int64_t page, std::optional<int64_t> max_rows) {
   heads(hk, hk, d, page, false);
-  glue(parents, cu, base, table, page, max_rows);
+  const int64_t most = glue(parents, cu, base, table, page, max_rows);
   const int64_t nodes = parents.size(0), seqs = table.size(0);
   numbers(ids, at::kLong, nodes, "ids");
   numbers(verify, at::kLong, nodes, "verify");
@@ -459,7 +459,7 @@ py::tuple tree_keep(const Tensor& ids, const Tensor& parents, const Tensor& veri
   const bool e4m3 = !pools.empty() && pools[0].scalar_type() == at::kByte;
   Block b;
   b.bytes(where, sizeof(where)).at(ids).at(parents).at(verify).at(cu).at(base).at(table).at(count).at(path).at(emitted);
-  b.ints(nodes, pools.size(), table.size(1), page, hk, d, e4m3, pages).put(h.err);
+  b.ints(nodes, most, pools.size(), table.size(1), page, hk, d, e4m3, pages).put(h.err);
   launch(h, "tree", "kern_tree_keep", seqs, std::max<int64_t>(1, pools.size()), 1, 128, b);
   return py::make_tuple(count, path, emitted);
 }

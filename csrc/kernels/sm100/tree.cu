@@ -45,11 +45,11 @@ KERN_DEVICE long long place_slot(long long place, const int* pages, int max_page
 
 }  // namespace kern
 
-// grid seqs, block 256. Nodes that no tree holds (of padding sequences, before the first sequence and behind the last, over the limit,
+// grid seqs, block 256; `most` nodes of a tree (up to 256, 64 to a word). Nodes that no tree holds (of padding sequences, before the first sequence and behind the last, over the limit,
 // between bounds that are none) get position 0, slot -1 and no mask.
 extern "C" __global__ void __launch_bounds__(256)
     kern_tree_rows(const int* parents, const int* cu, const long long* base, const int* block_table, long long* positions, long long* slots,
-                   int* seq_lens, long long* masks, int nodes, int words, int max_pages, int page_size, int* err) {
+                   int* seq_lens, long long* masks, int nodes, int most, int words, int max_pages, int page_size, int* err) {
   __shared__ unsigned long long mask_s[kMaxNodes][4];
   __shared__ int jump_s[kMaxNodes], depth_s[kMaxNodes];
   pdl_wait();
@@ -58,7 +58,7 @@ extern "C" __global__ void __launch_bounds__(256)
   const int row0 = mine.from, all = mine.lie ? mine.to - mine.from : 0;
   if (!mine.lie && i == 0) set_error(err, ERR_BOUNDS);
   const long long b = min(base[s], kFar);
-  const int n = b < 0 ? 0 : min(min(all, kMaxNodes), words * 64);
+  const int n = b < 0 ? 0 : min(all, most);
   auto none = [&](int from, int to) {
     for (int x = from + i; x < to; x += blockDim.x) {
       positions[x] = 0;
@@ -115,10 +115,10 @@ extern "C" __global__ void __launch_bounds__(256)
   }
 }
 
-// grid (seqs, layers), block 128
+// grid (seqs, layers), block 128; `most` as above
 extern "C" __global__ void __launch_bounds__(128)
     kern_tree_keep(const __grid_constant__ PoolTable pools, const long long* ids, const int* parents, const long long* verify, const int* cu,
-                   const long long* base, const int* block_table, int* count, int* path, long long* emitted, int nodes, int layers, int max_pages,
+                   const long long* base, const int* block_table, int* count, int* path, long long* emitted, int nodes, int most, int layers, int max_pages,
                    int page_size, int hk, int d, int e4m3, int pool_pages, int* err) {
   __shared__ int path_s[kMaxNodes];
   __shared__ long long slot_s[2][kMaxNodes];
@@ -128,7 +128,7 @@ extern "C" __global__ void __launch_bounds__(128)
   const Span mine = span_of(cu, s, nodes);
   const int row0 = mine.from, all = mine.lie ? mine.to - mine.from : 0;
   if (!mine.lie && t == 0) set_error(err, ERR_BOUNDS);
-  const int n = min(all, kMaxNodes);
+  const int n = min(all, most);
   const long long b = min(base[s], kFar);
   if (t < 32) {
     // lane holds nodes t, t + 32, ..: the edge into each, and whether the model agrees with it

@@ -50,7 +50,8 @@ def tree_keep(ids: torch.Tensor, parents: torch.Tensor, verify: torch.Tensor, cu
     ``verify`` along the path, the last of them new, as `spec.accept` counts them.
 
     In every pool of ``pools`` (all layers, one format, up to 128) the cache rows of path node i move from place base + path[i]
-    to base + i. Places outside the table or the pool set the error word and are not touched."""
+    to base + i. Places outside the table or the pool set the error word and are not touched; so do trees of more than ``max_rows``
+    (256) nodes, whose further nodes are not walked to, and bounds in ``cu`` that are none."""
     return _host.ops().tree_keep(ids, parents, verify, cu, base, block_table, pools, hk, d, page_size, max_rows)
 
 

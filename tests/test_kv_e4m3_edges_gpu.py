@@ -395,3 +395,19 @@ def test_a_decoder_whose_padding_token_is_zeros(cuda, tmp_path, heads, hk, d):
             # 1.3 % for codes that bf16 takes to their neighbours, as much for bf16 elsewhere; zeros exactly
             assert float((lg - ref).norm()) <= 0.05 * float(ref.norm())
     rt.check_error()
+
+
+@pytest.mark.parametrize("most", [0, 1, 30, 64, 70])
+def test_more_nodes_than_max_rows(cuda, most):
+    """A chain of 75 nodes, all agreed with: those from `most` on have no slot and are not walked to, and the error word says so."""
+    page, n = 16, 75
+    table = torch.arange(8, dtype=torch.int32, device=cuda)[None].contiguous()
+    par, ids = i32([i - 1 for i in range(n)]), torch.zeros(n, dtype=torch.int64, device=cuda)
+    cu, base = i32([0, n]), torch.tensor([3], device=cuda)
+    pos, slots, lens, masks = failed(lambda: TR.tree_rows(par, cu, base, table, page, max_rows=most))
+    assert slots.tolist() == [3 + i for i in range(most)] + [-1] * (n - most) and masks.shape[1] == max(1, -(-most // 64))
+    assert pos.tolist() == [3 + i for i in range(most)] + [0] * (n - most) and bool((masks[most:] == 0).all())
+    pool = torch.randint(0, 255, (8, K8.page_bytes(1, page, 64)), dtype=torch.uint8, device=cuda)
+    before = pool.clone()
+    count, path, _ = failed(lambda: TR.tree_keep(ids, par, ids, cu, base, table, [pool], 1, 64, page, max_rows=most))
+    assert count.tolist() == [most] and path.tolist() == list(range(most)) + [-1] * (n - most) and torch.equal(pool, before)
