@@ -29,7 +29,7 @@
 // rows see different tokens values that are not finite are taken out of the product and put back for the rows that see them (a
 // second pass of products over 0 / 1, only when there are any).
 //
-// Measured (8-bit, 8 kv heads, 32 heads of 128): single tokens of 64 sequences of up to 4096 tokens 54 us, 0.83 of the measured copy
+// Measured (8-bit, 8 kv heads, 32 heads of 128): single tokens of 64 sequences of up to 4096 tokens 51 us, 0.88 of the measured copy
 // bandwidth, of 128 sequences of up to 8000 168 us, 0.97; 2 sequences of 100,003 40 us, 0.74; one of 1001 8 us, which is launch,
 // one round to DRAM and the join.
 #include "attn_rows.cuh"

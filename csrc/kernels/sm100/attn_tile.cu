@@ -25,7 +25,7 @@
 // between the two warps that share the row; no pass over O but then). Registers are dealt by role, as a spill costs an L2 access
 // where shared memory has taken the L1's place.
 //
-// Measured (8 kv heads, 32 heads of 128): 4 prompts of up to 2048 rows on 8-bit contexts of up to 6000 384 us, 0.60 of the measured
+// Measured (8 kv heads, 32 heads of 128): 4 prompts of up to 2048 rows on 8-bit contexts of up to 6000 388 us, 0.60 of the measured
 // tensor peak; 18 trees of 128 nodes over 4000 tokens 1100 TFLOP/s (bf16) and 970 (8-bit); 64 trees of up to 32 nodes over bf16
 // contexts of up to 8192 210 us, 0.88 of the measured bandwidth.
 //
