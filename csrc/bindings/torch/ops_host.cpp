@@ -344,7 +344,7 @@ Tensor attend(const Tensor& q, const Tensor& pool, const Tensor& table, const Te
   const int64_t all = INT32_MAX, few = std::max<int64_t>(1, 8 / g);
   // one kernel over the sequences of lo .. hi rows
   auto run = [&](bool tiled, int64_t lo, int64_t hi) {
-    const int64_t most = std::max<int64_t>(1, std::min(max_rows, hi));       // (no rows, by the call's own word: the kernels see whether that is so)
+    const int64_t most = std::max<int64_t>(1, std::min(max_rows, hi));       // (max_rows 0: the kernels see whether that is so)
     int64_t toks, cluster = 1, shares, gx, gy;
     unsigned shared;
     std::string name;

@@ -45,8 +45,8 @@ KERN_DEVICE long long place_slot(long long place, const int* pages, int max_page
 
 }  // namespace kern
 
-// grid seqs, block 256; `most` nodes of a tree (up to 256, 64 to a word). Nodes that no tree holds (of padding sequences, before the first sequence and behind the last, over the limit,
-// between bounds that are none) get position 0, slot -1 and no mask.
+// grid seqs, block 256; `most` nodes of a tree (up to 256, 64 to a word). Nodes that no tree holds (of padding sequences, before the first
+// sequence and behind the last, over the limit, between bounds that are none) get position 0, slot -1 and no mask.
 extern "C" __global__ void __launch_bounds__(256)
     kern_tree_rows(const int* parents, const int* cu, const long long* base, const int* block_table, long long* positions, long long* slots,
                    int* seq_lens, long long* masks, int nodes, int most, int words, int max_pages, int page_size, int* err) {
@@ -118,8 +118,8 @@ extern "C" __global__ void __launch_bounds__(256)
 // grid (seqs, layers), block 128; `most` as above
 extern "C" __global__ void __launch_bounds__(128)
     kern_tree_keep(const __grid_constant__ PoolTable pools, const long long* ids, const int* parents, const long long* verify, const int* cu,
-                   const long long* base, const int* block_table, int* count, int* path, long long* emitted, int nodes, int most, int layers, int max_pages,
-                   int page_size, int hk, int d, int e4m3, int pool_pages, int* err) {
+                   const long long* base, const int* block_table, int* count, int* path, long long* emitted, int nodes, int most, int layers,
+                   int max_pages, int page_size, int hk, int d, int e4m3, int pool_pages, int* err) {
   __shared__ int path_s[kMaxNodes];
   __shared__ long long slot_s[2][kMaxNodes];
   __shared__ int len_s;

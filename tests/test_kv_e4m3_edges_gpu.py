@@ -411,3 +411,21 @@ def test_more_nodes_than_max_rows(cuda, most):
     before = pool.clone()
     count, path, _ = failed(lambda: TR.tree_keep(ids, par, ids, cu, base, table, [pool], 1, 64, page, max_rows=most))
     assert count.tolist() == [most] and path.tolist() == list(range(most)) + [-1] * (n - most) and torch.equal(pool, before)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_blocks_of_up_to_128_rows(cuda, d):
+    """The cases above in blocks that both tiles of the many-row kernel share, on alternate key tiles."""
+    rows = 30                                              # of 4 heads
+    for size in (0.0, 2.0 ** -30):
+        for query in (0.0, 1.0):
+            test_caches_of_zeros_or_next_to_nothing(cuda, rows, d, size, query)
+    test_a_pool_that_nobody_has_written_to(cuda, rows, d, 1.0)
+    for past in (100, 4000):
+        for swap in (False, True):
+            test_rows_that_nobody_has_written_to_beside_others(cuda, rows, past, d, swap)
+            for low, high in ((None, 100), (-30, 60), (-38, 118)):
+                test_value_tiles_far_apart(cuda, rows, past, d, low, high, swap)
+    for which in ("values", "keys"):
+        test_rows_under_the_smallest_scale_beside_ordinary_ones(cuda, rows, d, which)
+    test_huge_keys_across_huge_queries(cuda, rows, d)
