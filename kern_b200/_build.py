@@ -175,7 +175,11 @@ def _torch_here() -> tuple[str, bool]:
     spec = importlib.util.find_spec("torch")
     if spec is None or not spec.submodule_search_locations:
         return "", False
-    return importlib.metadata.version("torch"), (Path(spec.submodule_search_locations[0]) / "lib" / "libc10_cuda.so").exists()
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:     # (a tree of its own on the path)
+        version = "unknown"
+    return version, (Path(spec.submodule_search_locations[0]) / "lib" / "libc10_cuda.so").exists()
 
 
 def build_ops_host(force: bool = False, needed: bool = True) -> Path | None:
