@@ -683,7 +683,7 @@ KERN_DEVICE void rows_body(const CUtensorMap* kv_map, const RowsArgs& a) {
       y[4] += f * v.x; y[5] += f * v.y; y[6] += f * v.z; y[7] += f * v.w;
     }
     if (a.cluster == 1) {
-      if (whole || (int)blockIdx.z < shares) store(r, col, m, l, y, whole);
+      if ((int)blockIdx.z < shares) store(r, col, m, l, y, whole);         // (whole: the one share there is, not those that nobody has)
     } else {
       float4* dst = reinterpret_cast<float4*>(mo + r * kPad + col);       // (in place of what this thread has read)
       dst[0] = make_float4(y[0], y[1], y[2], y[3]);

@@ -7,7 +7,7 @@ pytestmark = pytest.mark.gpu
 from kern_b200.ops import kv_e4m3 as K8
 from kern_b200.ops import tree as TR
 from kern_b200.ops.launcher import Kernels
-from test_kv_e4m3_gpu import WEIGHT, attend64, close
+from test_kv_e4m3_gpu import WEIGHT, attend64, close, fill_cache
 
 
 @pytest.fixture(autouse=True)
@@ -429,3 +429,35 @@ def test_blocks_of_up_to_128_rows(cuda, d):
     for which in ("values", "keys"):
         test_rows_under_the_smallest_scale_beside_ordinary_ones(cuda, rows, d, which)
     test_huge_keys_across_huge_queries(cuda, rows, d)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("kind", ["e4m3", "bf16"])
+@pytest.mark.parametrize("rows", [1, 3])
+def test_short_contexts_under_a_long_limit(cuda, d, kind, rows):
+    """A limit that asks for many shares, each a block of its own, over contexts of one: the block that has it writes the rows, and no
+    other does. From idle with cold caches, and one behind the other."""
+    hq, hk, page, lens = 6, 2, 64, [3, 128, 40]
+    g = torch.Generator().manual_seed(d)
+    pool, table, kv = fill_cache(kind, lens, hk, d, page, g)
+    table = torch.cat([table, torch.zeros(3, 2000, dtype=torch.int32, device=cuda)], 1).contiguous()
+    cu, l = i32([0, rows, 2 * rows, 3 * rows]), i32(lens)
+    q = torch.randn(3 * rows, hq * d, generator=g).bfloat16().cuda()
+    chain = bits_of(torch.ones(rows, rows).tril().bool()).repeat(3, 1)
+    if kind == "e4m3":
+        call = lambda: K8.paged_attention_e4m3(q, pool, table, l, hq, hk, d, page, cu_q=cu, max_rows=rows)
+    else:
+        call = lambda: TR.tree_attention(q, pool, table, l, chain, cu, hq, hk, d, page, max_rows=rows)
+    out, wrong = call(), torch.zeros((), dtype=torch.int64, device=cuda)
+    cold = torch.empty(200 << 20, dtype=torch.uint8, device=cuda)
+    for i in range(300):
+        if i % 3 == 0:
+            cold.fill_(i & 255)
+        if i % 3 < 2:
+            torch.cuda.synchronize()
+        wrong += (call() != out).any()
+    assert int(wrong) == 0
+    for s in range(3):
+        ref, spread = attend64(q[s * rows:(s + 1) * rows].cpu().view(rows, hq, d), kv[s], causal(rows, lens[s]), d ** -0.5)
+        # bf16 weights are summed as rounded: 2^-8 of a weight, and of their sum
+        close(out[s * rows:(s + 1) * rows].view(rows, hq, d), ref, spread, WEIGHT[kind] * (2 if kind == "bf16" else 1))
