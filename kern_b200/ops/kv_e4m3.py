@@ -64,6 +64,8 @@ def paged_attention_e4m3(q: torch.Tensor, pool: torch.Tensor, block_table: torch
     Calls of more than 16 query rows to a kv head keep their speed where the scales of a context's keys, and of its values, are within 2^20
     of one another over 128 tokens (64 at head_dim 256; rows of zeros aside) and those of its values within 2^100 over all: 256 query
     rows that meet others are computed token by token, some 200 times slower, and as exactly.
+    Scores and sums are held in 32 bits, weights as f16: a token whose weight times its values' scale is under 2^-25 of the row's largest
+    adds nothing to the values, and its part of the sum alone.
     A row that sees nothing gives zeros; rows of ``out`` behind the last sequence's stay as they are. Pages
     outside the pool, contexts longer than the table, rows outside ``q`` and sequences of more rows than ``max_rows`` (which are
     left out) set the device's error word. Returns ``out[rows, hq * d]``."""
