@@ -187,7 +187,7 @@ def build_ops_host(force: bool = False, needed: bool = True) -> Path | None:
     PyTorch of this environment, and again when that changes. None beside a PyTorch without CUDA, which has no use for it. Not
     `needed` (an import of the package, most of which does without): a build that fails is a warning, once for the same sources."""
     out, src = ops_host_path(), CSRC / "bindings" / "torch" / "ops_host.cpp"
-    stamp = BUILD / "ops_host.torch"                    # the PyTorch that it was last built for
+    stamp = PKG / "_ops_host.torch"                     # beside it, where it travels with it: the PyTorch that it was last built for
     stale = _newer([src, *(CSRC / "runtime").glob("*.hpp")], stamp)
     version, cuda = _torch_here()
     if not cuda:
